@@ -113,6 +113,11 @@ int lut_read_device_error(int* flag);
 int mma_read_device_error(int* flag);
 int chain_read_device_error(int* flag);
 int glue_read_device_error(int* flag);
+namespace paged {
+int rope_read_device_error(int* flag);
+int cache_read_device_error(int* flag);
+int attend_read_device_error(int* flag);
+}  // namespace paged
 
 static bool x_ok(const void* x, int64_t m, int64_t k, int64_t ldx) {
     return (m == 0 || k == 0) || (x != nullptr && ldx >= k);
@@ -151,11 +156,22 @@ int epq_device_error(int* flag) {
     int glue = 0;
     rc = glue_read_device_error(&glue);
     if (rc) return rc;
+    int found[3] = {0, 0, 0};
+    rc = paged::rope_read_device_error(&found[0]);
+    if (rc) return rc;
+    rc = paged::cache_read_device_error(&found[1]);
+    if (rc) return rc;
+    rc = paged::attend_read_device_error(&found[2]);
+    if (rc) return rc;
+    const int paged_bad = found[0] | found[1] | found[2];
     // bit 0: LUT placement check; bit 1: a bounded wait gave up (GEMV, GEMM, backward or chain);
     // bit 2: the chain kernel's placement or grid check failed; bit 3: an embedding id was
     // outside the store's rows; bit 4: a decode position was at or past the KV cache's capacity
+    // (or, for the paged cache, a position, length or sequence outside it); bit 5: a page
+    // table named a page outside the pool
     *flag = (lut ? 1 : 0) | (((mma & 1) || tc || bwd || chain == 1) ? 2 : 0) | (chain == 2 ? 4 : 0) |
-            (emb ? 8 : 0) | ((glue || (mma & 2)) ? 16 : 0);
+            (emb ? 8 : 0) | ((glue || (mma & 2) || (paged_bad & 1)) ? 16 : 0) |
+            ((paged_bad & 2) ? 32 : 0);
     return EPQ_OK;
 }
 

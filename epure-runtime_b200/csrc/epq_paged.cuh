@@ -1,0 +1,129 @@
+// Shared by the rotary, paged-cache and paged-attention kernels: typed loads and
+// stores, the device form of the cache's description, and launches that may overlap
+// the end of the kernel before them.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "epq_common.cuh"
+#include "epq_paged.h"
+
+namespace epq {
+namespace paged {
+
+// What a kernel found wrong, kept in one word a file until epq_device_error reads it.
+constexpr int kBadPosition = 1;   // a position, length or sequence outside the cache or the rotary table
+constexpr int kBadPage = 2;       // a page outside the pool
+
+// Lets the next kernel of the stream start its launch, and waits for the one before.
+__device__ __forceinline__ void pdl_enter() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <typename... KArgs, typename... Args>
+int launch(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const char* what,
+           Args... args) {
+    if (smem > 48 * 1024) {
+        const int rc = set_smem_limit(reinterpret_cast<const void*>(kern), (int)smem, what);
+        if (rc != EPQ_OK) return rc;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+    return check_launch(what);
+}
+
+// float <-> T, rounded to nearest even.
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// V consecutive values; the address is aligned to their size (at most 16 bytes a load).
+template <int kBytes> struct Word;
+template <> struct Word<2> { using type = uint16_t; };
+template <> struct Word<4> { using type = uint32_t; };
+template <> struct Word<8> { using type = uint2; };
+template <> struct Word<16> { using type = uint4; };
+template <> struct Word<32> { struct type { uint4 a, b; }; };
+
+template <typename T, int V>
+__device__ __forceinline__ void load_v(float (&f)[V], const T* p) {
+    using W = typename Word<V * (int)sizeof(T)>::type;
+    union { W w; T t[V]; } u;
+    u.w = *reinterpret_cast<const W*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = to_f<T>(u.t[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T* p, const float (&f)[V]) {
+    using W = typename Word<V * (int)sizeof(T)>::type;
+    union { W w; T t[V]; } u;
+#pragma unroll
+    for (int i = 0; i < V; ++i) u.t[i] = from_f<T>(f[i]);
+    *reinterpret_cast<W*>(p) = u.w;
+}
+
+// One pair turned by (c, s): every product rounded, as elementwise float32 code does
+// it, so results equal x1 * c - x2 * s written with tensors bit for bit.
+__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+    const float x = a, y = b;
+    a = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
+    b = __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
+}
+
+// The device's side of epq_pages.
+struct PagesD {
+    uint8_t* k;
+    uint8_t* v;
+    float* k_scale;
+    float* v_scale;
+    const int32_t* table;
+    int64_t page_stride, scale_stride, table_stride, pages;
+    int seqs, max_pages, page_size, kv_heads, head_dim, format;
+};
+
+// Page and slot of token `pos` of sequence `s`, or false with *bad set.
+__device__ __forceinline__ bool find_slot(const PagesD& p, int s, int64_t pos, int64_t* page, int* slot, int* bad) {
+    if (s < 0 || s >= p.seqs || pos >= (int64_t)p.max_pages * p.page_size) {
+        *bad = kBadPosition;
+        return false;
+    }
+    const int t = (int)pos;                       // max_pages * page_size < 2^31 (checked on the host)
+    const int col = t / p.page_size;
+    const int64_t pg = p.table[s * p.table_stride + col];
+    if (pg < 0 || pg >= p.pages) {
+        *bad = kBadPage;
+        return false;
+    }
+    *page = pg;
+    *slot = t - col * p.page_size;
+    return true;
+}
+
+// Checks the description and copies it (k_paged_cache.cu).
+int make_pages(const epq_pages* in, PagesD* out, const char* who);
+// Whether rows of `v` can be read as `bytes`-byte words at every head and multiple of `bytes`.
+inline bool heads_aligned(const epq_heads& v, int elem, int bytes) {
+    return ((uintptr_t)v.data | (uintptr_t)(v.stride_row * elem) | (uintptr_t)(v.stride_head * elem)) % bytes == 0;
+}
+
+int rope_read_device_error(int* flag);
+int cache_read_device_error(int* flag);
+int attend_read_device_error(int* flag);
+
+}  // namespace paged
+}  // namespace epq

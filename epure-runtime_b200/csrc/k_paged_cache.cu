@@ -1,0 +1,440 @@
+// The paged key-value cache: rows written with the norm, the rotation and the 8-bit
+// quantisation of the step fused in (epq_paged_write), and read back (epq_paged_read).
+//
+//   a = max|x| over a head's row, scale = a * (1 / top), code = round(x * (top / a)),
+//   top = 127 (int8, rounded to even) or 448 (e4m3); read: code * scale.
+//
+// Bound: HBM.  A row is read once in its own type and written once in the cache's; the
+// arithmetic (one division a row, about ten operations a value) stays below that.
+//
+// Split: one warp takes (a share of) one token's rows -- q heads, k heads, v heads --
+// with 8 values a lane, so a row is 8, 16 or 32 lanes, its maximum and sum of squares a
+// few shuffles, and the token's page, cos and sin are found once.
+#include "epq_paged.cuh"
+
+namespace epq {
+namespace paged {
+namespace {
+
+__device__ int g_cache_error = 0;
+
+constexpr int kCacheThreads = 256;
+
+struct Rows {
+    const void* p;
+    int64_t row, head;   // strides, in elements
+};
+
+enum Turn { kNoTurn = 0, kHalfLanes = 1, kNeighbours = 2, kHalfLoads = 3 };
+
+struct WriteArgs {
+    PagesD pages;
+    Rows q, k, v;
+    void* q_out;
+    int64_t qo_row, qo_head;
+    const int32_t* seq;
+    const int64_t* pos;
+    const float* cos_t;
+    const float* sin_t;
+    int64_t m, max_len;
+    int heads, r, turn, qk_norm, splits, aligned, out_aligned;
+    float eps;
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(float (&x)[8], const T* p, int aligned) {
+    if (aligned) {
+        load_v<T, 8>(x, p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f<T>(p[i]);
+    }
+}
+
+// Eight values times `inv`, as codes.
+template <int kFormat>
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv, float scale) {
+    uint32_t b[8];
+    // A row whose maximum is so small that top / max overflows is divided instead.
+    const bool tiny = inv == INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        float y0 = x[i] * inv, y1 = x[i + 1] * inv;
+        if (tiny) {
+            y0 = scale > 0.f ? __fdiv_rn(x[i], scale) : 0.f;
+            y1 = scale > 0.f ? __fdiv_rn(x[i + 1], scale) : 0.f;
+        }
+        if (kFormat == EPQ_CACHE_INT8) {
+            b[i] = (uint32_t)max(-127, min(127, __float2int_rn(y0))) & 0xffu;
+            b[i + 1] = (uint32_t)max(-127, min(127, __float2int_rn(y1))) & 0xffu;
+        } else {
+            const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(y0, y1), __NV_SATFINITE, __NV_E4M3);
+            b[i] = two & 0xffu;
+            b[i + 1] = two >> 8;
+        }
+    }
+    return make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
+}
+
+template <typename T, int kFormat, int kLanes>
+__global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A) {
+    pdl_enter();
+    constexpr unsigned kAll = 0xffffffffu;
+    const int warp = blockIdx.x * (kCacheThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int64_t row = warp / A.splits;
+    if (row >= A.m) return;
+    const int split = warp - (int)row * A.splits;
+    const PagesD& P = A.pages;
+    const int hd = P.head_dim, KV = P.kv_heads;
+    const int sub = lane / kLanes, chunk = lane & (kLanes - 1), e0 = chunk * 8;
+    const bool in_row = e0 < hd;
+
+    const int64_t pos = A.pos[row];
+    int64_t page = 0;
+    int slot = 0, bad = 0;
+    bool live = pos >= 0;
+    if (live) {
+        live = find_slot(P, A.seq[row], pos, &page, &slot, &bad);
+        if (live && A.turn != kNoTurn && pos >= A.max_len) {
+            live = false;
+            bad = kBadPosition;
+        }
+        if (bad && lane == 0) atomicOr(&g_cache_error, bad);
+    }
+
+    // cos and the signed sin of this lane's 8 values: y = x c + partner s.
+    float c[8], s[8];
+    if (A.turn != kNoTurn && live) {
+        const int half = A.r >> 1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = e0 + i;
+            c[i] = 1.f;
+            s[i] = 0.f;
+            if (e < A.r) {
+                const bool second = A.turn == kNeighbours ? e & 1 : e >= half;
+                const int64_t at = pos * half + (A.turn == kNeighbours ? e >> 1 : second ? e - half : e);
+                c[i] = A.cos_t[at];
+                s[i] = second ? A.sin_t[at] : -A.sin_t[at];
+            }
+        }
+    }
+    constexpr int kFit = 32 / kLanes;
+    const int rows = A.heads + 2 * KV, passes = (rows + kFit - 1) / kFit;
+    const int p0 = (int)((int64_t)passes * split / A.splits), p1 = (int)((int64_t)passes * (split + 1) / A.splits);
+    for (int ps = p0; ps < p1; ++ps) {
+        const int j = ps * kFit + sub;
+        const bool is_q = j < A.heads, is_v = j >= A.heads + KV;
+        const int head = is_q ? j : is_v ? j - A.heads - KV : j - A.heads;
+        const bool on = j < rows && in_row && live;
+        const Rows src = is_q ? A.q : is_v ? A.v : A.k;
+        const T* x_at = static_cast<const T*>(src.p) + row * src.row + head * src.head;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        if (on) load8<T>(x, x_at + e0, A.aligned);
+        float gain = 1.f;
+        if (A.qk_norm) {                              // RMSNorm of a q or k head, rounded to T
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
+            if (!is_v) {
+                gain = rsqrtf(ss / (float)hd + A.eps);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = to_f<T>(from_f<T>(x[i] * gain));
+            }
+        }
+        if (A.turn != kNoTurn) {
+            float other[8];
+            if (A.turn == kHalfLanes) {               // rotary_dim a multiple of 16: the partner's lane
+                const int part = A.r >> 4;
+                const int from = sub * kLanes + (chunk < part ? chunk + part : chunk < 2 * part ? chunk - part : chunk);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(kAll, x[i], from);
+            } else if (A.turn == kNeighbours) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) other[i] = x[i ^ 1];
+            } else {
+                const int half = A.r >> 1;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int e = e0 + i;
+                    other[i] = 0.f;
+                    if (on && !is_v && e < A.r) {
+                        other[i] = to_f<T>(x_at[e < half ? e + half : e - half]);
+                        if (A.qk_norm) other[i] = to_f<T>(from_f<T>(other[i] * gain));
+                    }
+                }
+            }
+            if (!is_v && live) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (e0 + i < A.r)
+                        x[i] = to_f<T>(from_f<T>(__fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(other[i], s[i]))));
+            }
+        }
+        if (is_q) {
+            if (in_row) {                             // a padding row's q is zero
+                T* o = static_cast<T*>(A.q_out) + row * A.qo_row + head * A.qo_head + e0;
+                if (A.out_aligned) {
+                    store_v<T, 8>(o, x);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] = from_f<T>(x[i]);
+                }
+            }
+        }
+        const int64_t at = page * P.page_stride + ((int64_t)head * P.page_size + slot) * hd + e0;
+        if (kFormat == EPQ_CACHE_SAME) {
+            if (on && !is_q) store_v<T, 8>(reinterpret_cast<T*>(is_v ? P.v : P.k) + at, x);
+        } else {
+            // |x| compared as integers, so that a NaN is the largest
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kAll, top, o));
+            const float a = __uint_as_float(top);
+            constexpr float kTop = kFormat == EPQ_CACHE_INT8 ? 127.f : 448.f;
+            const float scale = __fmul_rn(a, 1.f / kTop), inv = a > 0.f ? __fdiv_rn(kTop, a) : 0.f;
+            if (on && !is_q) {
+                *reinterpret_cast<uint2*>((is_v ? P.v : P.k) + at) = codes8<kFormat>(x, inv, scale);
+                if (chunk == 0)
+                    (is_v ? P.v_scale : P.k_scale)[page * P.scale_stride + (int64_t)head * P.page_size + slot] = scale;
+            }
+        }
+    }
+}
+
+struct ReadArgs {
+    PagesD pages;
+    const int32_t* seq;
+    const int64_t* pos;
+    void* k_out;
+    void* v_out;
+    int64_t m;
+    int splits;
+};
+
+// 16 values an item: 16 bytes of codes, or two loads of a cache in T.
+template <typename T, int kFormat>
+__global__ void __launch_bounds__(kCacheThreads) read_kernel(const ReadArgs A) {
+    pdl_enter();
+    const int warp = blockIdx.x * (kCacheThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int64_t row = warp / A.splits;
+    if (row >= A.m) return;
+    const int split = warp - (int)row * A.splits;
+    const PagesD& P = A.pages;
+    const int hd = P.head_dim, KV = P.kv_heads, per_head = hd >> 4, items = 2 * KV * per_head;
+    const int64_t pos = A.pos[row];
+    int64_t page = 0;
+    int slot = 0, bad = 0;
+    const bool live = pos >= 0 && find_slot(P, A.seq[row], pos, &page, &slot, &bad);
+    if (bad && lane == 0) atomicOr(&g_cache_error, bad);
+    for (int it = split * 32 + lane; it < items; it += 32 * A.splits) {
+        const int j = it / per_head, e0 = (it - j * per_head) * 16;
+        const bool is_v = j >= KV;
+        const int head = is_v ? j - KV : j;
+        const int64_t slot_at = (int64_t)head * P.page_size + slot, at = page * P.page_stride + slot_at * hd + e0;
+        const uint8_t* from = is_v ? P.v : P.k;
+        T* to = static_cast<T*>(is_v ? A.v_out : A.k_out) + (row * KV + head) * hd + e0;
+        float f[2][8];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i >> 3][i & 7] = 0.f;
+        if (live) {
+            if (kFormat == EPQ_CACHE_SAME) {
+                load_v<T, 8>(f[0], reinterpret_cast<const T*>(from) + at);
+                load_v<T, 8>(f[1], reinterpret_cast<const T*>(from) + at + 8);
+            } else {
+                const uint4 w = *reinterpret_cast<const uint4*>(from + at);
+                const float scale = (is_v ? P.v_scale : P.k_scale)[page * P.scale_stride + slot_at];
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t b = u[i >> 2] >> (8 * (i & 3)) & 0xffu;
+                    float code;
+                    if (kFormat == EPQ_CACHE_INT8) {
+                        code = (float)(int8_t)b;
+                    } else {
+                        const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3);
+                        code = __half2float(__half(h));
+                    }
+                    f[i >> 3][i & 7] = code * scale;
+                }
+            }
+        }
+        store_v<T, 8>(to, f[0]);
+        store_v<T, 8>(to + 8, f[1]);
+    }
+}
+
+template <typename T, int kFormat>
+int launch_write(const WriteArgs& A, unsigned blocks, cudaStream_t st) {
+    const int hd = A.pages.head_dim;
+    const char* who = "epq_paged_write";
+    if (hd <= 64) return launch(write_kernel<T, kFormat, 8>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+    if (hd <= 128) return launch(write_kernel<T, kFormat, 16>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+    return launch(write_kernel<T, kFormat, 32>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+}
+template <typename T>
+int launch_write_t(const WriteArgs& A, unsigned blocks, cudaStream_t st) {
+    if (A.pages.format == EPQ_CACHE_SAME) return launch_write<T, EPQ_CACHE_SAME>(A, blocks, st);
+    if (A.pages.format == EPQ_CACHE_INT8) return launch_write<T, EPQ_CACHE_INT8>(A, blocks, st);
+    return launch_write<T, EPQ_CACHE_FP8>(A, blocks, st);
+}
+template <typename T>
+int launch_read_t(const ReadArgs& A, unsigned blocks, cudaStream_t st) {
+    const char* who = "epq_paged_read";
+    if (A.pages.format == EPQ_CACHE_SAME)
+        return launch(read_kernel<T, EPQ_CACHE_SAME>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+    if (A.pages.format == EPQ_CACHE_INT8)
+        return launch(read_kernel<T, EPQ_CACHE_INT8>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+    return launch(read_kernel<T, EPQ_CACHE_FP8>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+}
+
+// Warps a token: one, or as many as it has passes while there are too few tokens to give
+// every SM 16 warps.
+int share_out(int64_t m, int64_t passes) {
+    int64_t splits = cdiv((int64_t)device_sms() * 16, m);
+    return (int)(splits < passes ? splits : passes);
+}
+
+}  // namespace
+
+int make_pages(const epq_pages* in, PagesD* d, const char* who) {
+    if (!in) return set_error(EPQ_EINVAL, "%s: pages is NULL", who);
+    if (in->kv_heads <= 0 || in->page_size <= 0 || in->seqs <= 0 || in->max_pages <= 0 || in->pages <= 0)
+        return set_error(EPQ_EINVAL, "%s: kv_heads=%d, page_size=%d, seqs=%d, max_pages=%d, pages=%lld", who,
+                         in->kv_heads, in->page_size, in->seqs, in->max_pages, (long long)in->pages);
+    if (!in->k || !in->v || !in->table) return set_error(EPQ_EINVAL, "%s: k, v and table must be non-NULL", who);
+    if (in->head_dim < 16 || in->head_dim > 256 || in->head_dim % 16)
+        return set_error(EPQ_EUNSUPPORTED, "%s: head_dim=%d (a multiple of 16 up to 256)", who, in->head_dim);
+    if (in->format < EPQ_CACHE_SAME || in->format > EPQ_CACHE_FP8)
+        return set_error(EPQ_EINVAL, "%s: format=%d", who, in->format);
+    if (in->format != EPQ_CACHE_SAME && (!in->k_scale || !in->v_scale))
+        return set_error(EPQ_EINVAL, "%s: an 8-bit cache needs k_scale and v_scale", who);
+    if ((int64_t)in->max_pages * in->page_size > INT32_MAX)
+        return set_error(EPQ_EUNSUPPORTED, "%s: %d pages of %d tokens a sequence", who, in->max_pages, in->page_size);
+    const int64_t rows = (int64_t)in->kv_heads * in->page_size;
+    if (in->page_stride < rows * in->head_dim || in->table_stride < in->max_pages ||
+        (in->format != EPQ_CACHE_SAME && in->scale_stride < rows))
+        return set_error(EPQ_ESHAPE, "%s: strides of pages (%lld), scales (%lld) or table (%lld) are too small", who,
+                         (long long)in->page_stride, (long long)in->scale_stride, (long long)in->table_stride);
+    if (((uintptr_t)in->k | (uintptr_t)in->v) % 16 || in->page_stride % 16)
+        return set_error(EPQ_EALIGN, "%s: k, v and page_stride must be multiples of 16 bytes / values", who);
+    d->k = static_cast<uint8_t*>(in->k);
+    d->v = static_cast<uint8_t*>(in->v);
+    d->k_scale = in->k_scale;
+    d->v_scale = in->v_scale;
+    d->table = in->table;
+    d->page_stride = in->page_stride;
+    d->scale_stride = in->scale_stride;
+    d->table_stride = in->table_stride;
+    d->pages = in->pages;
+    d->seqs = in->seqs;
+    d->max_pages = in->max_pages;
+    d->page_size = in->page_size;
+    d->kv_heads = in->kv_heads;
+    d->head_dim = in->head_dim;
+    d->format = in->format;
+    return EPQ_OK;
+}
+
+int cache_read_device_error(int* flag) {
+    if (cudaMemcpyFromSymbol(flag, g_cache_error, sizeof(int)) != cudaSuccess)
+        return check_launch("read paged cache error flag");
+    return EPQ_OK;
+}
+
+}  // namespace paged
+}  // namespace epq
+
+using namespace epq;
+using namespace epq::paged;
+
+extern "C" {
+
+int epq_paged_write(const epq_pages* pages, const epq_heads* q, const epq_heads* q_out, const epq_heads* k,
+                    const epq_heads* v, const int32_t* seq, const int64_t* pos, int64_t m, const float* cos_tab,
+                    const float* sin_tab, int64_t max_len, int32_t rotary_dim, int32_t interleaved,
+                    int32_t qk_norm, float eps, int32_t dtype, void* stream) {
+    WriteArgs A = {};
+    const int rc = make_pages(pages, &A.pages, "epq_paged_write");
+    if (rc != EPQ_OK) return rc;
+    if (!k || !v || m < 0 || (!q) != (!q_out) || (!cos_tab) != (!sin_tab))
+        return set_error(EPQ_EINVAL, "epq_paged_write: bad arguments");
+    if (!dtype_ok(dtype)) return set_error(EPQ_EDTYPE, "epq_paged_write: dtype %d", dtype);
+    const int hd = A.pages.head_dim, KV = A.pages.kv_heads, elem = dtype_size(dtype);
+    if (k->heads != KV || v->heads != KV || (q && (q->heads <= 0 || q->heads != q_out->heads || q->heads > 65536)))
+        return set_error(EPQ_ESHAPE, "epq_paged_write: %d k heads and %d v heads for a cache of %d", k->heads,
+                         v->heads, KV);
+    if (cos_tab && (rotary_dim < 2 || rotary_dim > hd || rotary_dim % 2 || max_len <= 0))
+        return set_error(EPQ_EUNSUPPORTED, "epq_paged_write: rotary_dim=%d (even, 2..%d)", rotary_dim, hd);
+    if (m == 0) return EPQ_OK;
+    if (!seq || !pos || !k->data || !v->data || (q && (!q->data || !q_out->data)))
+        return set_error(EPQ_EINVAL, "epq_paged_write: NULL rows, seq or pos");
+    A.k = {k->data, k->stride_row, k->stride_head};
+    A.v = {v->data, v->stride_row, v->stride_head};
+    A.aligned = heads_aligned(*k, elem, 16) && heads_aligned(*v, elem, 16);
+    if (q) {
+        A.q = {q->data, q->stride_row, q->stride_head};
+        A.aligned = A.aligned && heads_aligned(*q, elem, 16);
+        A.q_out = q_out->data;
+        A.qo_row = q_out->stride_row;
+        A.qo_head = q_out->stride_head;
+        A.out_aligned = heads_aligned(*q_out, elem, 16);
+        A.heads = q->heads;
+    }
+    A.seq = seq;
+    A.pos = pos;
+    A.cos_t = cos_tab;
+    A.sin_t = sin_tab;
+    A.m = m;
+    A.max_len = max_len;
+    A.r = rotary_dim;
+    A.turn = !cos_tab ? kNoTurn : interleaved ? kNeighbours : rotary_dim % 16 == 0 ? kHalfLanes : kHalfLoads;
+    // In place, a lane's loads of its partner's values would race with that lane's store.
+    if (A.turn == kHalfLoads && q && q->data == q_out->data)
+        return set_error(EPQ_EUNSUPPORTED, "epq_paged_write: q in place needs rotary_dim %% 16 == 0 (got %d)", rotary_dim);
+    A.qk_norm = qk_norm != 0;
+    A.eps = eps;
+    const int fit = hd <= 64 ? 4 : hd <= 128 ? 2 : 1;
+    A.splits = share_out(m, cdiv(A.heads + 2 * KV, fit));
+    if (m * A.splits > (int64_t)1 << 30)
+        return set_error(EPQ_EUNSUPPORTED, "epq_paged_write: m=%lld rows", (long long)m);
+    const unsigned blocks = (unsigned)cdiv(m * A.splits * 32, kCacheThreads);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == EPQ_F32) return launch_write_t<float>(A, blocks, st);
+    if (dtype == EPQ_F16) return launch_write_t<__half>(A, blocks, st);
+    return launch_write_t<__nv_bfloat16>(A, blocks, st);
+}
+
+int epq_paged_read(const epq_pages* pages, const int32_t* seq, const int64_t* pos, int64_t m, void* k_out,
+                   void* v_out, int32_t dtype, void* stream) {
+    ReadArgs A = {};
+    const int rc = make_pages(pages, &A.pages, "epq_paged_read");
+    if (rc != EPQ_OK) return rc;
+    if (m < 0) return set_error(EPQ_EINVAL, "epq_paged_read: m=%lld", (long long)m);
+    if (!dtype_ok(dtype)) return set_error(EPQ_EDTYPE, "epq_paged_read: dtype %d", dtype);
+    if (m == 0) return EPQ_OK;
+    if (!seq || !pos || !k_out || !v_out) return set_error(EPQ_EINVAL, "epq_paged_read: NULL rows, seq or pos");
+    if (((uintptr_t)k_out | (uintptr_t)v_out) % 16)
+        return set_error(EPQ_EALIGN, "epq_paged_read: k_out and v_out must be 16-byte aligned");
+    A.seq = seq;
+    A.pos = pos;
+    A.k_out = k_out;
+    A.v_out = v_out;
+    A.m = m;
+    A.splits = share_out(m, cdiv(2 * A.pages.kv_heads * (A.pages.head_dim / 16), 32));
+    if (m * A.splits > (int64_t)1 << 30)
+        return set_error(EPQ_EUNSUPPORTED, "epq_paged_read: m=%lld rows", (long long)m);
+    const unsigned blocks = (unsigned)cdiv(m * A.splits * 32, kCacheThreads);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == EPQ_F32) return launch_read_t<float>(A, blocks, st);
+    if (dtype == EPQ_F16) return launch_read_t<__half>(A, blocks, st);
+    return launch_read_t<__nv_bfloat16>(A, blocks, st);
+}
+
+}  // extern "C"

@@ -126,7 +126,9 @@ const char* epq_last_error(void);
  * chain kernel's placement or grid check failed; bit 3 -- epq_embedding was
  * given an id outside the store's rows (that row of its output is zero); bit
  * 4 -- a decode-glue call (include/epq_decode.h) got a position outside its
- * KV cache (nothing was written to the cache).
+ * KV cache (nothing was written to the cache), or a paged one
+ * (include/epq_paged.h) a position, length or sequence outside it; bit 5 -- a
+ * page table named a page outside its pool.
  * *flag = 0 means no kernel has reported a failure. */
 int epq_device_error(int* flag);
 
