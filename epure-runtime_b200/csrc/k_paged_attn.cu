@@ -39,6 +39,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kBlock = 16;                 // tokens of a warp's block
 constexpr int kMinBlocks = 4;              // a CTA's run is at least this long
 constexpr int kMaxUnits = 65536;           // counters in the workspace
+constexpr int kMaxGrid = 512;              // CTAs of a launch
 constexpr float kSlack = 8.f;              // how far (log2) a score may pass the running maximum
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -54,6 +55,7 @@ struct AttendArgs {
     unsigned* counters;
     int64_t window;
     int batch, heads, group, chunks, dtype;
+    uint32_t page_mul, page_shift;         // t / page_size = (mulhi(t, page_mul) + t) >> page_shift
     float scale_log2;
 };
 
@@ -84,18 +86,18 @@ __device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t at) {
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 template <bool kIsBf16>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if (kIsBf16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                      "{%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                      "{%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -188,17 +190,24 @@ struct Shape {
     static constexpr int kRows = kBlock * kPitch;                        // one of K, V
     static constexpr int kScales = kBytes == 1 ? 2 * kBlock * 4 : 0;
     static constexpr int kStage = 2 * kRows + kScales;
-    static constexpr int kBudget = kDim == 256 && kBytes == 2 ? 48 * 1024 : 24 * 1024;   // a warp's ring
+    static constexpr int kCtas = kPitch > 256 ? 1 : kPitch == 256 || kCols == 2 ? 2 : 3;   // an SM
+    static constexpr int kMergePitch = kDim + 4;                         // floats; spreads a column's heads over the banks
+    static constexpr int kMergeRows = kWarps * 8 * kMergePitch * 4;
+    static constexpr int kMerge = kMergeRows > kMaxGrid * 8 * 4 ? kMergeRows : kMaxGrid * 8 * 4;
+    // a warp's ring: its share of what 228 KB leave a CTA (1 KB is the system's, 512 bytes are static)
+    static constexpr int kBudget = (228 * 1024 / kCtas - 1024 - 512 - kMerge) / kWarps;
     static constexpr int kFit = kBudget / kStage;
     static constexpr int kStages = kFit > 6 ? 6 : kFit;
     static constexpr int kRing = kStages * kStage;
-    static constexpr int kMergePitch = kDim + 4;                         // floats; spreads a column's heads over the banks
-    static constexpr int kMerge = kWarps * 8 * kMergePitch * 4;
     static constexpr int kSmem = kWarps * kRing + kMerge;
-    static constexpr int kCtas = kDim == 256 && kBytes == 2 ? 1 : 2;     // an SM
     static constexpr int kRecord = kCols * 8 * kMergePitch;              // floats: accumulators, then m, M, l in the padding
     static_assert(kStages >= 2, "ring");
 };
+
+// a / b of the dealt-out order: 32-bit wherever it is enough.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
 
 template <int kKind, int kDim, int kCols>
 __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) attend_kernel(const AttendArgs A) {
@@ -207,54 +216,75 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     constexpr bool kIsBf16 = kKind == kBf16;
     constexpr unsigned kAll = 0xffffffffu;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float wm[kWarps][8 * kCols], wM[kWarps][8 * kCols], wl[kWarps][8 * kCols];
+    __shared__ float4 joined[8];                       // (m, M, l) of a joined unit's heads
     __shared__ uint32_t seen[kWarps][S::kStages];     // bit r: row r of the stage is a token of the span
-    __shared__ int64_t sums[kWarps];
-    __shared__ int start_b;
-    __shared__ int64_t start_at;
+    __shared__ int64_t sums[2][kWarps];
+    __shared__ int start_b, start_u, start_i;
     __shared__ bool last;
     pdl_enter();
 
     const PagesD& P = A.pages;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int hd = P.head_dim, KV = P.kv_heads, units = KV * A.chunks;
+    const int hd = P.head_dim, units = P.kv_heads * A.chunks;
     const int hd_chunks = hd * S::kBytes / 16;
 
-    // ---- this CTA's run of blocks [f0, f1)
+    // ---- this CTA's run of blocks
     const int per = (A.batch + kThreads - 1) / kThreads;
     const int b0 = min(A.batch, tid * per), b1 = min(A.batch, b0 + per);
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += span_of(A, b, blockIdx.x == 0).blocks;
-    int64_t before = mine;                             // inclusive scan over the threads
+    const int first_blocks = b0 < b1 ? span_of(A, b0, blockIdx.x == 0).blocks : 0;
+    int64_t mine = first_blocks;
+    for (int b = b0 + 1; b < b1; ++b) mine += span_of(A, b, blockIdx.x == 0).blocks;
+    // inclusive scan over the threads
+    auto scan = [&](int64_t v, int which, int64_t* total) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(kAll, before, o);
-        if (lane >= o) before += v;
-    }
-    if (lane == 31) sums[warp] = before;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += sums[w];
-        total += sums[w];
-    }
-    before -= mine;
-    total *= units;
-    int64_t run = (total + gridDim.x - 1) / gridDim.x;
-    if (run < kMinBlocks) run = kMinBlocks;
-    const int64_t f0 = min(total, blockIdx.x * run), f1 = min(total, f0 + run);
-    if (f0 < f1 && f0 >= before * units && f0 < (before + mine) * units) {
-        int64_t at = f0 - before * units;
-        int b = b0;
-        for (;;) {
-            const int64_t here = (int64_t)span_of(A, b, false).blocks * units;
-            if (at < here) break;
-            at -= here;
-            ++b;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(kAll, v, o);
+            if (lane >= o) v += u;
         }
-        start_b = b;
-        start_at = at;
+        if (lane == 31) sums[which][warp] = v;
+        __syncthreads();
+        *total = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) v += sums[which][w];
+            *total += sums[which][w];
+        }
+        return v;
+    };
+    int64_t total;
+    const int64_t upto = scan(mine, 0, &total);
+    total *= units;
+    int64_t run = quotient(total + gridDim.x - 1, gridDim.x);
+    if (run < kMinBlocks) run = kMinBlocks;
+    // Where cutting every unit into pieces of at most `run` blocks makes no more pieces
+    // than there are CTAs, each CTA takes one piece; else runs go over unit boundaries.
+    int64_t pieces = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int blocks = b == b0 ? first_blocks : span_of(A, b, false).blocks;
+        pieces += quotient(blocks + run - 1, run);
+    }
+    int64_t all_pieces;
+    const int64_t pieces_upto = scan(pieces, 1, &all_pieces);
+    const bool one_each = all_pieces * units <= gridDim.x;
+    const int64_t f0 = one_each ? blockIdx.x : blockIdx.x * run;       // piece, or block of the dealt-out order
+    const int64_t limit = one_each ? all_pieces * units : total;
+    {
+        const int64_t lo = (one_each ? pieces_upto - pieces : upto - mine) * units;
+        const int64_t hi = (one_each ? pieces_upto : upto) * units;
+        if (f0 >= lo && f0 < hi) {
+            int64_t at = f0 - lo;
+            for (int b = b0;; ++b) {
+                const int blocks = b == b0 ? first_blocks : span_of(A, b, false).blocks;
+                const int64_t each = one_each ? quotient(blocks + run - 1, run) : blocks;
+                if (at < each * units) {
+                    start_b = b;
+                    start_u = (int)quotient(at, each);
+                    start_i = (int)(at - start_u * each);
+                    break;
+                }
+                at -= each * units;
+            }
+        }
     }
     // sequences without a token
     for (int b = blockIdx.x; b < A.batch; b += gridDim.x) {
@@ -269,66 +299,106 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     if (hd < kDim)                                     // chunks past the head's end stay zero
         for (int e = lane; e < S::kRing / 16; e += 32) reinterpret_cast<uint4*>(ring)[e] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (f0 >= f1) return;
+    if (f0 >= limit) return;
 
     Cursor unit;                                       // of the unit that the CTA is at
     unit.units = units;
     unit.b = start_b;
+    unit.u = start_u;
+    unit.i = start_i;
     unit.s = span_of(A, start_b, false);
-    unit.u = (int)(start_at / unit.s.blocks);
-    unit.i = (int)(start_at - (int64_t)unit.u * unit.s.blocks);
+    int count, piece = 0, piece_count = 1;             // blocks of this CTA; its place among its unit's pieces
+    if (one_each) {
+        piece = start_i;
+        piece_count = (int)quotient(unit.s.blocks + run - 1, run);
+        unit.i = (int)((int64_t)unit.s.blocks * piece / piece_count);
+        count = (int)((int64_t)unit.s.blocks * (piece + 1) / piece_count) - unit.i;
+    } else {
+        count = (int)min(run, total - f0);
+    }
 
     // ---- loads, kStages - 1 blocks ahead
+    const bool linear = P.page_size % kBlock == 0;     // a block is in one page, its rows side by side
     Cursor ahead = unit;
-    int64_t f_load = f0 + warp;
-    int next_page = 0;                                 // table entry of row `lane & 15` of the next block to load
-    bool next_on = false;                              // whether that row is a token (the entry may still be on its way)
+    int f_load = warp;                                 // blocks are counted from the run's start
+    int next_page = 0, next_slot = 0;                  // table entry and slot of the next block to load (its row `lane & 15`)
+    bool next_on = false;                              // whether that is a token (the entry may still be on its way)
     auto look_up = [&]() {
-        const int t = ahead.s.lo16 + ahead.i * kBlock + (lane & 15);
-        next_on = t >= ahead.s.lo && t < ahead.s.n;
+        const int t0 = ahead.s.lo16 + ahead.i * kBlock, t = linear ? t0 : t0 + (lane & 15);
+        next_on = linear || (t >= ahead.s.lo && t < ahead.s.n);
         if (next_on) {
+            const int col = (int)((__umulhi((uint32_t)t, A.page_mul) + (uint32_t)t) >> A.page_shift);
             const int s = A.seq ? A.seq[ahead.b] : ahead.b;
-            next_page = P.table[(int64_t)s * P.table_stride + t / P.page_size];
+            next_slot = t - col * P.page_size;
+            next_page = P.table[(int64_t)s * P.table_stride + col];
         }
     };
-    if (f_load < f1) {
+    if (f_load < count) {
         ahead.advance(A, warp);
         look_up();
     }
+    constexpr int kChunks = S::kPitch / 16;            // of a row
+    constexpr int kCopies = kBlock * kChunks / 32;     // chunks a lane
+    const int my_row = lane / kChunks, my_ch = lane % kChunks;     // a lane's chunks: rows my_row, my_row + 32 / kChunks, ...
+    // its place in a stage: 512 bytes further each time, with bit 6 turned (see swizzled)
+    const uint32_t my_at = swizzled<S::kPitch>(my_row, my_ch);
     int load_stage = 0;
     auto load = [&]() {
-        if (f_load < f1) {
-            const int t = ahead.s.lo16 + ahead.i * kBlock + (lane & 15);
-            const int head = ahead.u / A.chunks;
+        if (f_load < count) {
             if (next_on && (next_page < 0 || next_page >= P.pages)) {
                 atomicOr(&g_attend_error, kBadPage);
                 next_on = false;
             }
-            const int slot = t - t / P.page_size * P.page_size;
-            const int64_t slot_at = (int64_t)head * P.page_size + slot;
-            const int64_t at = next_on ? next_page * P.page_stride + slot_at * hd : -1;
+            const int head = A.chunks == 1 ? ahead.u : ahead.u / A.chunks;
+            const int64_t slot_at = (int64_t)head * P.page_size + next_slot;
+            const int64_t at = next_page * P.page_stride + slot_at * hd;
             const uint32_t k_at = ring_at + load_stage * S::kStage, v_at = k_at + S::kRows;
-            const uint32_t mask = __ballot_sync(kAll, next_on) & 0xffffu;
-            if (lane == 0) seen[warp][load_stage] = mask;
-            constexpr int kChunks = S::kPitch / 16;
+            if (linear) {
+                const int t0 = ahead.s.lo16 + ahead.i * kBlock;
+                const int r0 = max(0, ahead.s.lo - t0), r1 = next_on ? min(kBlock, ahead.s.n - t0) : 0;   // rows that are tokens
+                if (lane == 0) seen[warp][load_stage] = r1 > r0 ? (0xffffu >> (kBlock - r1)) & (0xffffu << r0) : 0u;
+                const int64_t off = next_on ? (at + my_row * hd) * S::kBytes + my_ch * 16 : 0;
+                const uint8_t* k_from = P.k + off;
+                const uint8_t* v_from = P.v + off;
+                const int step = next_on ? 32 / kChunks * hd * S::kBytes : 0;
+                if (my_ch < hd_chunks) {
 #pragma unroll
-            for (int e = 0; e < kBlock * kChunks / 32; ++e) {
-                const int idx = e * 32 + lane, row = idx / kChunks, ch = idx % kChunks;
-                const int64_t from = __shfl_sync(kAll, at, row);
-                if (ch < hd_chunks) {
-                    const int64_t off = from < 0 ? 0 : (from * S::kBytes + ch * 16);
-                    const int bytes = from < 0 ? 0 : 16;
-                    cp16(k_at + swizzled<S::kPitch>(row, ch), P.k + off, bytes);
-                    cp16(v_at + swizzled<S::kPitch>(row, ch), P.v + off, bytes);
+                    for (int e = 0; e < kCopies; ++e) {
+                        const int row = my_row + e * (32 / kChunks);
+                        const int bytes = row >= r0 && row < r1 ? 16 : 0;
+                        const uint32_t to = (my_at ^ (e & 1) * 64) + e * 512;
+                        cp16(k_at + to, k_from + e * step, bytes);
+                        cp16(v_at + to, v_from + e * step, bytes);
+                    }
+                }
+                if (kQuant) {                          // lanes 0-15: key scales, 16-31: value scales
+                    const int row = lane & 15;
+                    const bool on = row >= r0 && row < r1;
+                    const float* sc = lane < 16 ? P.k_scale : P.v_scale;
+                    cp4(v_at + S::kRows + lane * 4, sc + (on ? next_page * P.scale_stride + slot_at + row : 0), on ? 4 : 0);
+                }
+            } else {
+                const uint32_t mask = __ballot_sync(kAll, next_on) & 0xffffu;
+                if (lane == 0) seen[warp][load_stage] = mask;
+#pragma unroll
+                for (int e = 0; e < kCopies; ++e) {
+                    const int row = my_row + e * (32 / kChunks);
+                    const int64_t from = __shfl_sync(kAll, at, row);
+                    const bool on = mask >> row & 1;
+                    if (my_ch < hd_chunks) {
+                        const int64_t off = on ? from * S::kBytes + my_ch * 16 : 0;
+                        const uint32_t to = (my_at ^ (e & 1) * 64) + e * 512;
+                        cp16(k_at + to, P.k + off, on ? 16 : 0);
+                        cp16(v_at + to, P.v + off, on ? 16 : 0);
+                    }
+                }
+                if (kQuant) {
+                    const float* sc = lane < 16 ? P.k_scale : P.v_scale;
+                    cp4(v_at + S::kRows + lane * 4, sc + (next_on ? next_page * P.scale_stride + slot_at : 0), next_on ? 4 : 0);
                 }
             }
-            if (kQuant) {                              // lanes 0-15: key scales, 16-31: value scales
-                const float* sc = lane < 16 ? P.k_scale : P.v_scale;
-                const int64_t off = next_on ? next_page * P.scale_stride + slot_at : 0;
-                cp4(v_at + S::kRows + lane * 4, sc + off, next_on ? 4 : 0);
-            }
             f_load += kWarps;
-            if (f_load < f1) {
+            if (f_load < count) {
                 ahead.advance(A, kWarps);
                 look_up();
             }
@@ -341,32 +411,40 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
 
     // ---- units
     const int g = lane >> 2, c = lane & 3;             // row and column pair of the tensor fragments
-    int64_t f = f0 + warp;
-    int stage = 0;
-    for (int64_t at = f0; at < f1;) {
-        const int64_t unit_start = at - unit.i, unit_end = unit_start + unit.s.blocks;
-        const int64_t end = min(f1, unit_end);
-        const int head = unit.u / A.chunks, chunk = unit.u - head * A.chunks;
-        const int h_first = head * A.group + chunk * 8 * kCols;               // query heads of this unit
-        const int h_count = min(8 * kCols, A.group - chunk * 8 * kCols);
-
-        // q as B fragments: column g is head h_first + 8 n + g
-        uint32_t qf[kCols][kDim / 16][2];
-        float q_gain[kCols][2];                        // what scores of heads 2c, 2c + 1 are multiplied by
+    // q as B fragments: column g is the unit's query head 8 n + g.  16-bit caches: dims 2c, 2c+1
+    // and 2c+8, 2c+9 of every 16; 8-bit ones: 4c .. 4c+3
+    uint32_t qf[kCols][kDim / 16][2];
+    auto load_q = [&](const Cursor& u) {
+        const int head = A.chunks == 1 ? u.u : u.u / A.chunks, chunk = u.u - head * A.chunks;
+        const int h0 = head * A.group + chunk * 8 * kCols, n_heads = min(8 * kCols, A.group - chunk * 8 * kCols);
 #pragma unroll
         for (int n = 0; n < kCols; ++n) {
-            const bool on = 8 * n + g < h_count;
-            const uint16_t* q = static_cast<const uint16_t*>(A.q) + unit.b * A.q_row + (h_first + 8 * n + g) * A.q_head;
+            const bool on = 8 * n + g < n_heads;
+            const uint16_t* q = static_cast<const uint16_t*>(A.q) + u.b * A.q_row + (h0 + 8 * n + g) * A.q_head;
 #pragma unroll
             for (int k = 0; k < kDim / 16; ++k) {
-                // 16-bit caches: dims 2c, 2c+1 and 2c+8, 2c+9; 8-bit ones: 4c .. 4c+3
                 const int d0 = 16 * k + (kQuant ? 4 * c : 2 * c), d1 = d0 + (kQuant ? 2 : 8);
                 const bool there = on && 16 * k < hd;
                 qf[n][k][0] = there ? *reinterpret_cast<const uint32_t*>(q + d0) : 0u;
                 qf[n][k][1] = there ? *reinterpret_cast<const uint32_t*>(q + d1) : 0u;
             }
+        }
+    };
+    load_q(unit);
+    int f = warp, stage = 0;
+    for (int at = 0; at < count;) {
+        const int unit_start = at - unit.i, unit_end = unit_start + unit.s.blocks;   // unit_start < 0: begun before this run
+        const int end = min(count, unit_end);
+        const int head = A.chunks == 1 ? unit.u : unit.u / A.chunks, chunk = unit.u - head * A.chunks;
+        const int h_first = head * A.group + chunk * 8 * kCols;               // query heads of this unit
+        const int h_count = min(8 * kCols, A.group - chunk * 8 * kCols);
+        const int seq_b = unit.b, unit_index = unit.b * units + unit.u;
+
+        float q_gain[kCols][2];                        // what scores of heads 2c, 2c + 1 are multiplied by
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
             q_gain[n][0] = q_gain[n][1] = A.scale_log2;
-            if (kQuant) {                              // to f16, times a power of two
+            if (kQuant) {                              // q to f16, times a power of two
                 const bool bf = A.dtype == EPQ_BF16;
                 auto value = [&](uint32_t two, int hi) {
                     const uint16_t h = hi ? two >> 16 : two & 0xffff;
@@ -415,44 +493,54 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
             load();                                    // into the stage of the block before this one
             const uint32_t k_at = ring_at + stage * S::kStage, v_at = k_at + S::kRows;
             const uint32_t mask = seen[warp][stage];
+            constexpr int kLoads = kDim * S::kBytes / 32;          // ldmatrix a block and operand
+            constexpr int kBatch = kLoads < 8 ? kLoads : 8;        // of which so many are in registers
 
-            // scores
-            float sc[kCols][4];
+            // scores: even and odd steps into accumulators of their own
+            float sc[kCols][4], sc2[kCols][4];
 #pragma unroll
             for (int n = 0; n < kCols; ++n)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sc[n][r] = 0.f;
-            if (!kQuant) {
+                for (int r = 0; r < 4; ++r) sc[n][r] = sc2[n][r] = 0.f;
 #pragma unroll
-                for (int k = 0; k < kDim / 16; ++k) {
-                    if (16 * k < hd) {
-                        uint32_t a[4];
-                        ldsm(a, k_at + swizzled<S::kPitch>(lane & 15, 2 * k + (lane >> 4)));
+            for (int k0 = 0; k0 < kLoads; k0 += kBatch) {
+                uint32_t x[kBatch][4];
 #pragma unroll
-                        for (int n = 0; n < kCols; ++n) mma<kIsBf16>(sc[n], a, qf[n][k][0], qf[n][k][1]);
-                    }
-                }
-            } else {
+                for (int k = 0; k < kBatch; ++k)
+                    ldsm(x[k], k_at + (kQuant ? swizzled<S::kPitch>((lane >> 3 & 1) * 8 + (lane & 7), 2 * (k0 + k) + (lane >> 4))
+                                              : swizzled<S::kPitch>(lane & 15, 2 * (k0 + k) + (lane >> 4))));
 #pragma unroll
-                for (int k = 0; k < kDim / 32; ++k) {
-                    if (32 * k < hd) {
-                        uint32_t x[4];
-                        ldsm(x, k_at + swizzled<S::kPitch>((lane >> 3 & 1) * 8 + (lane & 7), 2 * k + (lane >> 4)));
+                for (int k = 0; k < kBatch; ++k) {
+                    if (!kQuant) {
+#pragma unroll
+                        for (int n = 0; n < kCols; ++n)
+                            mma<kIsBf16>(k & 1 ? sc2[n] : sc[n], x[k], qf[n][k0 + k][0], qf[n][k0 + k][1]);
+                    } else {
                         if (kKind == kInt8) {
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) x[r] ^= 0x80808080u;
+                            for (int r = 0; r < 4; ++r) x[k][r] ^= 0x80808080u;
                         }
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const uint32_t a[4] = {codes_f16<kKind, 0x4140>(x[2 * r]), codes_f16<kKind, 0x4140>(x[2 * r + 1]),
-                                                   codes_f16<kKind, 0x4342>(x[2 * r]), codes_f16<kKind, 0x4342>(x[2 * r + 1])};
+                            const uint32_t a[4] = {
+                                codes_f16<kKind, 0x4140>(x[k][2 * r]), codes_f16<kKind, 0x4140>(x[k][2 * r + 1]),
+                                codes_f16<kKind, 0x4342>(x[k][2 * r]), codes_f16<kKind, 0x4342>(x[k][2 * r + 1])};
 #pragma unroll
                             for (int n = 0; n < kCols; ++n)
-                                mma<false>(sc[n], a, qf[n][2 * k + r][0], qf[n][2 * k + r][1]);
+                                mma<false>(r ? sc2[n] : sc[n], a, qf[n][2 * (k0 + k) + r][0], qf[n][2 * (k0 + k) + r][1]);
                         }
                     }
                 }
             }
+            // the first values are on their way while the weights are formed
+            uint32_t y[kBatch][4];
+            auto load_values = [&](int d0) {
+#pragma unroll
+                for (int d = 0; d < kBatch; ++d)
+                    ldsm_t(y[d], v_at + (kQuant ? swizzled<S::kPitch>((lane >> 3 & 1) * 8 + (lane & 7), 2 * (d0 + d) + (lane >> 4))
+                                                : swizzled<S::kPitch>((lane >> 4) * 8 + (lane & 7), 2 * (d0 + d) + (lane >> 3 & 1))));
+            };
+            load_values(0);
             float ks[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};
             if (kQuant) {
                 const float* scales = reinterpret_cast<const float*>(ring + stage * S::kStage + 2 * S::kRows);
@@ -469,7 +557,8 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {          // r: token g + 8 (r >> 1), head 2c + (r & 1)
                     const bool on = mask >> (g + 8 * (r >> 1)) & 1;
-                    sc[n][r] = on ? sc[n][r] * (kQuant ? q_gain[n][r & 1] * ks[r >> 1] : q_gain[n][r & 1]) : -INFINITY;
+                    const float s = sc[n][r] + sc2[n][r];
+                    sc[n][r] = on ? s * (kQuant ? q_gain[n][r & 1] * ks[r >> 1] : q_gain[n][r & 1]) : -INFINITY;
                     rise |= sc[n][r] > m[n][r & 1] + kSlack;
                     if (kQuant) rise |= sc[n][r] + lv[r >> 1] > M[n][r & 1] + kSlack;
                 }
@@ -522,32 +611,26 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                 pf[n][1] = transpose8x8(pack<kIsBf16>(w[2], w[3]));
             }
             // O^T += V^T P^T
-            if (!kQuant) {
 #pragma unroll
-                for (int d = 0; d < kDim / 16; ++d) {
-                    if (16 * d < hd) {
-                        uint32_t a[4];
-                        ldsm_t(a, v_at + swizzled<S::kPitch>((lane >> 4) * 8 + (lane & 7), 2 * d + (lane >> 3 & 1)));
+            for (int d0 = 0; d0 < kLoads; d0 += kBatch) {
+                if (d0) load_values(d0);
 #pragma unroll
-                        for (int n = 0; n < kCols; ++n) mma<kIsBf16>(acc[n][d], a, pf[n][0], pf[n][1]);
-                    }
-                }
-            } else {
+                for (int d = 0; d < kBatch; ++d) {
+                    if (!kQuant) {
 #pragma unroll
-                for (int d = 0; d < kDim / 32; ++d) {
-                    if (32 * d < hd) {
-                        uint32_t x[4];
-                        ldsm_t(x, v_at + swizzled<S::kPitch>((lane >> 3 & 1) * 8 + (lane & 7), 2 * d + (lane >> 4)));
+                        for (int n = 0; n < kCols; ++n) mma<kIsBf16>(acc[n][d0 + d], y[d], pf[n][0], pf[n][1]);
+                    } else {
                         if (kKind == kInt8) {
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) x[r] ^= 0x80808080u;
+                            for (int r = 0; r < 4; ++r) y[d][r] ^= 0x80808080u;
                         }
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {  // rows 0-7: the even dims of 16, rows 8-15: the odd ones
-                            const uint32_t a[4] = {codes_f16<kKind, 0x4240>(x[2 * r]), codes_f16<kKind, 0x4341>(x[2 * r]),
-                                                   codes_f16<kKind, 0x4240>(x[2 * r + 1]), codes_f16<kKind, 0x4341>(x[2 * r + 1])};
+                            const uint32_t a[4] = {
+                                codes_f16<kKind, 0x4240>(y[d][2 * r]), codes_f16<kKind, 0x4341>(y[d][2 * r]),
+                                codes_f16<kKind, 0x4240>(y[d][2 * r + 1]), codes_f16<kKind, 0x4341>(y[d][2 * r + 1])};
 #pragma unroll
-                            for (int n = 0; n < kCols; ++n) mma<false>(acc[n][2 * d + r], a, pf[n][0], pf[n][1]);
+                            for (int n = 0; n < kCols; ++n) mma<false>(acc[n][2 * (d0 + d) + r], a, pf[n][0], pf[n][1]);
                         }
                     }
                 }
@@ -556,145 +639,162 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         }
 
         // ---- the unit's piece: the four warps' states to one
+        const bool cut_before = unit_start < 0, cut = cut_before || unit_end > count;
+        at = end;
+        if (at < count) {                              // the next unit's q is on its way meanwhile
+            unit.advance(A, unit.s.blocks - unit.i);
+            load_q(unit);
+        }
         float* const merge = reinterpret_cast<float*>(smem + kWarps * S::kRing);
-        const bool whole = at == unit_start && end == unit_end;
-        float* const record = A.records + ((int64_t)blockIdx.x * 2 + (unit_start < f0 ? 0 : 1)) * S::kRecord;
-        const int unit_index = unit.b * units + unit.u;
-
-        // m, M and l of a warp to shared memory (l summed over the lanes of a column)
-        auto put_sums = [&](const float (&m_)[kCols][2], const float (&M_)[kCols][2], const float (&l_)[kCols][2]) {
-#pragma unroll
-            for (int n = 0; n < kCols; ++n)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    float s = l_[n][r];
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) s += __shfl_xor_sync(kAll, s, o);
-                    if (lane < 4) {
-                        wm[warp][8 * n + 2 * c + r] = m_[n][r];
-                        wM[warp][8 * n + 2 * c + r] = kQuant ? M_[n][r] : m_[n][r];
-                        wl[warp][8 * n + 2 * c + r] = s;
-                    }
-                }
-        };
-        // Joins the warps' states of column n and hands (head in unit, dim, value, m, M, l) on.
-        auto join = [&](int n, bool final) {
-            for (int e = tid; e < 8 * hd; e += kThreads) {
-                const int j = e / hd, d = e - j * hd, h = 8 * n + j;
-                if (h >= h_count) break;
-                float mx = -INFINITY, Mx = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    mx = fmaxf(mx, wm[w][h]);
-                    Mx = fmaxf(Mx, wM[w][h]);
-                }
-                float sum = 0.f, val = 0.f;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    // a warp that saw nothing has l = 0 and zeros; NaN must pass through
-                    sum += wm[w][h] == -INFINITY ? wl[w][h] : wl[w][h] * ex2(wm[w][h] - mx);
-                    const float a = merge[(w * 8 + j) * S::kMergePitch + d];
-                    val += wM[w][h] == -INFINITY ? a : a * ex2(wM[w][h] - Mx);
-                }
-                if (final) {
-                    // l = 0: every score was -inf.  2^(M - m) is 1 for 16-bit caches.
-                    float o = sum == 0.f ? 0.f : val / sum;
-                    if (kQuant && Mx != -INFINITY) o *= ex2(Mx - mx);
-                    const int64_t to = ((int64_t)unit.b * A.heads + h_first + h) * hd + d;
-                    if (A.dtype == EPQ_BF16) static_cast<__nv_bfloat16*>(A.out)[to] = __float2bfloat16_rn(o);
-                    else static_cast<__half*>(A.out)[to] = __float2half_rn(o);
-                    if (A.lse && d == 0)
-                        A.lse[(int64_t)unit.b * A.heads + h_first + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
-                } else {
-                    float* rec = record + (int64_t)h * S::kMergePitch;
-                    rec[d] = val;
-                    if (d == 0) {
-                        rec[kDim] = mx;
-                        rec[kDim + 1] = Mx;
-                        rec[kDim + 2] = sum;
-                    }
-                }
+        constexpr int kQuads = kDim / 4;               // of a head's dims
+        auto emit = [&](int h, int d, const float (&val)[4], float mx, float Mx, float sum) {
+            // sum = 0: every score was -inf.  2^(M - m) is 1 for 16-bit caches.
+            float gain = sum == 0.f ? 0.f : 1.f / sum;
+            if (kQuant && Mx != -INFINITY) gain *= ex2(Mx - mx);
+            uint2 o;
+            if (A.dtype == EPQ_BF16) {
+                o = make_uint2(pack<true>(val[0] * gain, val[1] * gain), pack<true>(val[2] * gain, val[3] * gain));
+            } else {
+                o = make_uint2(pack<false>(val[0] * gain, val[1] * gain), pack<false>(val[2] * gain, val[3] * gain));
             }
+            const int64_t to = (int64_t)seq_b * A.heads + h_first + h;
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(A.out) + to * hd + d) = o;
+            if (A.lse && d == 0) A.lse[to] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
         };
-        put_sums(m, M, l);
+        // none where the unit is whole; else where the piece's record goes
+        float* const record = !cut ? nullptr
+                                   : A.records + ((int64_t)blockIdx.x * 2 + (cut_before && !one_each ? 0 : 1)) * S::kRecord;
 #pragma unroll
         for (int n = 0; n < kCols; ++n) {
             if (8 * n < h_count) {
 #pragma unroll
-                for (int d = 0; d < kDim / 16; ++d)
+                for (int d = 0; d < kDim / 16; ++d) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int dim = 16 * d + (kQuant ? 2 * g + (r >> 1) : g + 8 * (r >> 1));
                         merge[(warp * 8 + 2 * c + (r & 1)) * S::kMergePitch + dim] = acc[n][d][r];
                     }
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {          // (m, M, l) behind the head's accumulators
+                    float s = l[n][r];
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) s += __shfl_xor_sync(kAll, s, o);
+                    if (lane < 4)
+                        *reinterpret_cast<float4*>(merge + (warp * 8 + 2 * c + r) * S::kMergePitch + kDim) =
+                            make_float4(m[n][r], kQuant ? M[n][r] : m[n][r], s, 0.f);
+                }
                 __syncthreads();
-                join(n, whole);
+                for (int e = tid; e < 8 * kQuads; e += kThreads) {
+                    const int j = e / kQuads, d = e % kQuads * 4, h = 8 * n + j;
+                    if (h >= h_count) break;
+                    if (d >= hd) continue;
+                    float4 of[kWarps];
+                    float mx = -INFINITY, Mx = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) {
+                        of[w] = *reinterpret_cast<const float4*>(merge + (w * 8 + j) * S::kMergePitch + kDim);
+                        mx = fmaxf(mx, of[w].x);
+                        Mx = fmaxf(Mx, of[w].y);
+                    }
+                    float sum = 0.f, val[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) {
+                        // a warp that saw nothing has l = 0 and zeros; NaN must pass through
+                        const float fl = of[w].x == -INFINITY ? 1.f : ex2(of[w].x - mx);
+                        const float fa = !kQuant ? fl : of[w].y == -INFINITY ? 1.f : ex2(of[w].y - Mx);
+                        const float4 a = *reinterpret_cast<const float4*>(merge + (w * 8 + j) * S::kMergePitch + d);
+                        sum += of[w].z * fl;
+                        val[0] += a.x * fa;
+                        val[1] += a.y * fa;
+                        val[2] += a.z * fa;
+                        val[3] += a.w * fa;
+                    }
+                    if (!record) {
+                        emit(h, d, val, mx, Mx, sum);
+                    } else {
+                        float* rec = record + h * S::kMergePitch;
+                        *reinterpret_cast<float4*>(rec + d) = make_float4(val[0], val[1], val[2], val[3]);
+                        if (d == 0) *reinterpret_cast<float4*>(rec + kDim) = make_float4(mx, Mx, sum, 0.f);
+                    }
+                }
                 __syncthreads();
             }
         }
 
         // ---- a unit cut over several CTAs: the last of them joins the records
-        if (!whole) {
-            __threadfence();
-            __syncthreads();
-            const int first = (int)(unit_start / run), pieces = (int)((unit_end - 1) / run) - first + 1;
-            if (tid == 0) last = atomicAdd(&A.counters[unit_index], 1u) == (unsigned)pieces - 1;
+        if (record) {
+            int first, parts;
+            if (one_each) {
+                first = (int)blockIdx.x - piece;
+                parts = piece_count;
+            } else {
+                first = (int)quotient(f0 + unit_start, run);
+                parts = (int)quotient(f0 + unit_end - 1, run) - first + 1;
+            }
+            if (tid == 0) {
+                __threadfence();                       // orders the CTA's records (the barrier above) before the count
+                last = atomicAdd(&A.counters[unit_index], 1u) == (unsigned)parts - 1;
+                if (last) {
+                    __threadfence();
+                    A.counters[unit_index] = 0u;
+                }
+            }
             __syncthreads();
             if (last) {
-                __threadfence();
+                // where runs go over boundaries, only the first part is its CTA's last piece
                 auto record_of = [&](int p) {
-                    return A.records + ((int64_t)(first + p) * 2 + (unit_start < (first + p) * run ? 0 : 1)) * S::kRecord;
+                    return A.records + ((int64_t)(first + p) * 2 + (one_each || p == 0 ? 1 : 0)) * S::kRecord;
                 };
-                constexpr int kPer = kDim / 32;        // dims a lane
 #pragma unroll
                 for (int n = 0; n < kCols; ++n) {
                     if (8 * n < h_count) {
-                        for (int j = 0; j < 8 && 8 * n + j < h_count; ++j) {
-                            const int64_t off = (int64_t)(8 * n + j) * S::kMergePitch;
+                        // warp w: maxima, sum and every part's factor of heads w, w + 4 of the column
+                        for (int j = warp; j < 8 && 8 * n + j < h_count; j += kWarps) {
+                            const int off = (8 * n + j) * S::kMergePitch + kDim;
                             float mx = -INFINITY, Mx = -INFINITY;
-                            for (int p = warp + kWarps * lane; p < pieces; p += kWarps * 32) {
-                                const float* rec = record_of(p) + off;
-                                mx = fmaxf(mx, __ldcg(rec + kDim));
-                                Mx = fmaxf(Mx, __ldcg(rec + kDim + 1));
+                            for (int p = lane; p < parts; p += 32) {
+                                const float4 t = __ldcg(reinterpret_cast<const float4*>(record_of(p) + off));
+                                mx = fmaxf(mx, t.x);
+                                Mx = fmaxf(Mx, t.y);
                             }
 #pragma unroll
                             for (int o = 16; o > 0; o >>= 1) {
                                 mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
                                 Mx = fmaxf(Mx, __shfl_xor_sync(kAll, Mx, o));
                             }
-                            float sum = 0.f, val[kPer];
-#pragma unroll
-                            for (int i = 0; i < kPer; ++i) val[i] = 0.f;
-#pragma unroll 4
-                            for (int p = warp; p < pieces; p += kWarps) {
-                                const float* rec = record_of(p) + off;
-                                const float pm = __ldcg(rec + kDim), pM = __ldcg(rec + kDim + 1);
-                                const float fl = pm == -INFINITY ? 1.f : ex2(pm - mx);
-                                const float fa = pM == -INFINITY ? 1.f : ex2(pM - Mx);
-                                sum += __ldcg(rec + kDim + 2) * fl;
-#pragma unroll
-                                for (int i = 0; i < kPer; ++i)
-                                    if (i * 32 + lane < hd) val[i] += __ldcg(rec + i * 32 + lane) * fa;
+                            float sum = 0.f;
+                            for (int p = lane; p < parts; p += 32) {
+                                const float4 t = __ldcg(reinterpret_cast<const float4*>(record_of(p) + off));
+                                sum += t.x == -INFINITY ? t.z : t.z * ex2(t.x - mx);
+                                merge[p * 8 + j] = t.y == -INFINITY ? 1.f : ex2(t.y - Mx);
                             }
 #pragma unroll
-                            for (int i = 0; i < kPer; ++i)
-                                merge[(warp * 8 + j) * S::kMergePitch + i * 32 + lane] = val[i];
-                            if (lane == 0) {
-                                wm[warp][8 * n + j] = mx;
-                                wM[warp][8 * n + j] = Mx;
-                                wl[warp][8 * n + j] = sum;
-                            }
+                            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+                            if (lane == 0) joined[j] = make_float4(mx, Mx, sum, 0.f);
                         }
                         __syncthreads();
-                        join(n, true);
+                        for (int e = tid; e < 8 * kQuads; e += kThreads) {
+                            const int j = e / kQuads, d = e % kQuads * 4, h = 8 * n + j;
+                            if (h >= h_count) break;
+                            if (d >= hd) continue;
+                            float val[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+                            for (int p = 0; p < parts; ++p) {
+                                const float4 a = __ldcg(reinterpret_cast<const float4*>(record_of(p) + h * S::kMergePitch + d));
+                                const float fa = merge[p * 8 + j];
+                                val[0] += a.x * fa;
+                                val[1] += a.y * fa;
+                                val[2] += a.z * fa;
+                                val[3] += a.w * fa;
+                            }
+                            emit(h, d, val, joined[j].x, joined[j].y, joined[j].z);
+                        }
                         __syncthreads();
                     }
                 }
-                if (tid == 0) A.counters[unit_index] = 0u;
             }
         }
-        at = end;
-        if (at < f1) unit.advance(A, unit.s.blocks - unit.i);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -702,7 +802,8 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
 template <int kKind, int kDim, int kCols>
 int launch_attend(const AttendArgs& A, cudaStream_t st) {
     using S = Shape<kKind, kDim, kCols>;
-    return launch(attend_kernel<kKind, kDim, kCols>, dim3((unsigned)(device_sms() * S::kCtas)), dim3(kThreads),
+    const int grid = device_sms() * S::kCtas;
+    return launch(attend_kernel<kKind, kDim, kCols>, dim3((unsigned)(grid < kMaxGrid ? grid : kMaxGrid)), dim3(kThreads),
                   (size_t)S::kSmem, st, "epq_paged_attend", A);
 }
 template <int kKind, int kDim>
@@ -722,7 +823,7 @@ int cols_of(int group) { return group <= 8 ? 1 : 2; }
 
 int64_t records_bytes(int hd, int group) {
     const int dim = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-    return (int64_t)device_sms() * 2 * 2 * cols_of(group) * 8 * (dim + 4) * 4;
+    return (int64_t)kMaxGrid * 2 * cols_of(group) * 8 * (dim + 4) * 4;
 }
 
 }  // namespace
@@ -774,8 +875,8 @@ int epq_paged_attend(const epq_pages* pages, const epq_heads* q, const int32_t* 
                          A.pages.seqs);
     if (batch == 0) return EPQ_OK;
     if (!q->data || !lengths || !out) return set_error(EPQ_EINVAL, "epq_paged_attend: NULL q, lengths or out");
-    if (!heads_aligned(*q, 2, 4))
-        return set_error(EPQ_EALIGN, "epq_paged_attend: q must be 4-byte aligned with even strides");
+    if (!heads_aligned(*q, 2, 4) || (uintptr_t)out % 16)
+        return set_error(EPQ_EALIGN, "epq_paged_attend: q must be 4-byte aligned with even strides, out 16-byte aligned");
     const int64_t need = epq_paged_attend_workspace_bytes(pages, batch, q->heads);
     if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256)
         return set_error(EPQ_EWORKSPACE, "epq_paged_attend: workspace of %lld bytes (need %lld, 256-aligned)",
@@ -794,6 +895,9 @@ int epq_paged_attend(const epq_pages* pages, const epq_heads* q, const int32_t* 
     A.heads = q->heads;
     A.dtype = dtype;
     A.scale_log2 = scale * kLog2e;
+    // division by page_size as a product: exact for all t < 2^31
+    while ((1u << A.page_shift) < (uint32_t)A.pages.page_size) ++A.page_shift;
+    A.page_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << A.page_shift) - A.pages.page_size)) / A.pages.page_size + 1);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (A.pages.format) {
         case EPQ_CACHE_INT8: return launch_attend_k<kInt8>(A, cols, st);
