@@ -26,6 +26,8 @@
 // largest); the key's scale multiplies the score, and the value's scale enters the
 // weight as 2^(s + log2 scale - M) with a running maximum M of its own, so that neither
 // large nor small scales leave f16's range.
+#include <cfloat>
+
 #include "epq_paged.cuh"
 
 namespace epq {
@@ -66,6 +68,9 @@ template <int kKind> constexpr int kind_bytes() { return kKind <= kF16 ? 2 : 1; 
 
 // ---------------------------------------------------------------- PTX
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {   // bytes 0: zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -76,13 +81,13 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N> __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+template <int kOffset> __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at), "n"(kOffset) : "memory");
 }
-__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+template <int kOffset> __device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at), "n"(kOffset) : "memory");
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
@@ -104,7 +109,7 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
 }
 __device__ __forceinline__ float ex2(float x) {
     float r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 template <bool kIsBf16> __device__ __forceinline__ uint32_t pack(float lo, float hi) {
@@ -361,7 +366,14 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                 const uint8_t* k_from = P.k + off;
                 const uint8_t* v_from = P.v + off;
                 const int step = next_on ? 32 / kChunks * hd * S::kBytes : 0;
-                if (my_ch < hd_chunks) {
+                if (hd == kDim && r1 - r0 == kBlock) {             // the ordinary block: nothing to leave out
+#pragma unroll
+                    for (int e = 0; e < kCopies; ++e) {
+                        const uint32_t to = (my_at ^ (e & 1) * 64) + e * 512;
+                        cp16(k_at + to, k_from + e * 512);
+                        cp16(v_at + to, v_from + e * 512);
+                    }
+                } else if (my_ch < hd_chunks) {
 #pragma unroll
                     for (int e = 0; e < kCopies; ++e) {
                         const int row = my_row + e * (32 / kChunks);
@@ -478,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         for (int n = 0; n < kCols; ++n) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                m[n][r] = M[n][r] = -INFINITY;
+                m[n][r] = M[n][r] = -FLT_MAX;
                 l[n][r] = 0.f;
             }
 #pragma unroll
@@ -491,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
             cp_wait<S::kStages - 2>();
             __syncwarp();
             load();                                    // into the stage of the block before this one
-            const uint32_t k_at = ring_at + stage * S::kStage, v_at = k_at + S::kRows;
+            const uint32_t k_at = ring_at + stage * S::kStage;
             const uint32_t mask = seen[warp][stage];
             constexpr int kLoads = kDim * S::kBytes / 32;          // ldmatrix a block and operand
             constexpr int kBatch = kLoads < 8 ? kLoads : 8;        // of which so many are in registers
@@ -502,13 +514,12 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
             for (int n = 0; n < kCols; ++n)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sc[n][r] = sc2[n][r] = 0.f;
+            // rows 0-15, 16-byte chunks 2 k and 2 k + 1 of them: the four 8 x 8 parts lie tokens first
 #pragma unroll
             for (int k0 = 0; k0 < kLoads; k0 += kBatch) {
                 uint32_t x[kBatch][4];
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k)
-                    ldsm(x[k], k_at + (kQuant ? swizzled<S::kPitch>((lane >> 3 & 1) * 8 + (lane & 7), 2 * (k0 + k) + (lane >> 4))
-                                              : swizzled<S::kPitch>(lane & 15, 2 * (k0 + k) + (lane >> 4))));
+                for (int k = 0; k < kBatch; ++k) ldsm<0>(x[k], k_at + swizzled<S::kPitch>(lane & 15, 2 * (k0 + k) + (lane >> 4)));
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
                     if (!kQuant) {
@@ -537,8 +548,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
             auto load_values = [&](int d0) {
 #pragma unroll
                 for (int d = 0; d < kBatch; ++d)
-                    ldsm_t(y[d], v_at + (kQuant ? swizzled<S::kPitch>((lane >> 3 & 1) * 8 + (lane & 7), 2 * (d0 + d) + (lane >> 4))
-                                                : swizzled<S::kPitch>((lane >> 4) * 8 + (lane & 7), 2 * (d0 + d) + (lane >> 3 & 1))));
+                    ldsm_t<S::kRows>(y[d], k_at + swizzled<S::kPitch>(lane & 15, 2 * (d0 + d) + (lane >> 4)));
             };
             load_values(0);
             float ks[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};
@@ -550,25 +560,33 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                     lv[r] = __log2f(scales[16 + g + 8 * r]);
                 }
             }
-            // weights
-            bool rise = false;
+            // weights; r: token g + 8 (r >> 1), head 2c + (r & 1)
 #pragma unroll
             for (int n = 0; n < kCols; ++n)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {          // r: token g + 8 (r >> 1), head 2c + (r & 1)
-                    const bool on = mask >> (g + 8 * (r >> 1)) & 1;
-                    const float s = sc[n][r] + sc2[n][r];
-                    sc[n][r] = on ? s * (kQuant ? q_gain[n][r & 1] * ks[r >> 1] : q_gain[n][r & 1]) : -INFINITY;
-                    rise |= sc[n][r] > m[n][r & 1] + kSlack;
-                    if (kQuant) rise |= sc[n][r] + lv[r >> 1] > M[n][r & 1] + kSlack;
+                for (int r = 0; r < 4; ++r)
+                    sc[n][r] = (sc[n][r] + sc2[n][r]) * (kQuant ? q_gain[n][r & 1] * ks[r >> 1] : q_gain[n][r & 1]);
+            if (mask != 0xffffu) {
+#pragma unroll
+                for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!(mask >> (g + 8 * (r >> 1)) & 1)) sc[n][r] = -INFINITY;
+            }
+            float over = -INFINITY;                    // fmaxf passes over NaN, which reaches the sums through the weights
+#pragma unroll
+            for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    over = fmaxf(over, sc[n][r] - m[n][r & 1]);
+                    if (kQuant) over = fmaxf(over, sc[n][r] + (lv[r >> 1] - M[n][r & 1]));
                 }
-            if (__any_sync(kAll, rise)) {
+            if (__any_sync(kAll, over > kSlack)) {
 #pragma unroll
                 for (int n = 0; n < kCols; ++n) {
                     float turn_acc[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        // fmaxf passes over NaN, which then reaches the sums through the weights
                         float top = fmaxf(sc[n][r], sc[n][r + 2]);
                         float topM = kQuant ? fmaxf(sc[n][r] + lv[0], sc[n][r + 2] + lv[1]) : 0.f;
 #pragma unroll
@@ -599,13 +617,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                 float w[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float p = sc[n][r] == -INFINITY ? 0.f : ex2(sc[n][r] - m[n][r & 1]);
-                    l[n][r & 1] += p;
-                    w[r] = p;
-                    if (kQuant) {
-                        const float x = sc[n][r] + lv[r >> 1];
-                        w[r] = x == -INFINITY ? 0.f : ex2(x - M[n][r & 1]);
-                    }
+                    w[r] = ex2(sc[n][r] - m[n][r & 1]);
+                    l[n][r & 1] += w[r];
+                    if (kQuant) w[r] = ex2(sc[n][r] + (lv[r >> 1] - M[n][r & 1]));
                 }
                 pf[n][0] = transpose8x8(pack<kIsBf16>(w[0], w[1]));
                 pf[n][1] = transpose8x8(pack<kIsBf16>(w[2], w[3]));
@@ -618,7 +632,10 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                 for (int d = 0; d < kBatch; ++d) {
                     if (!kQuant) {
 #pragma unroll
-                        for (int n = 0; n < kCols; ++n) mma<kIsBf16>(acc[n][d0 + d], y[d], pf[n][0], pf[n][1]);
+                        for (int n = 0; n < kCols; ++n) {
+                            const uint32_t a[4] = {y[d][0], y[d][2], y[d][1], y[d][3]};
+                            mma<kIsBf16>(acc[n][d0 + d], a, pf[n][0], pf[n][1]);
+                        }
                     } else {
                         if (kKind == kInt8) {
 #pragma unroll
@@ -650,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         auto emit = [&](int h, int d, const float (&val)[4], float mx, float Mx, float sum) {
             // sum = 0: every score was -inf.  2^(M - m) is 1 for 16-bit caches.
             float gain = sum == 0.f ? 0.f : 1.f / sum;
-            if (kQuant && Mx != -INFINITY) gain *= ex2(Mx - mx);
+            if (kQuant) gain *= ex2(Mx - mx);
             uint2 o;
             if (A.dtype == EPQ_BF16) {
                 o = make_uint2(pack<true>(val[0] * gain, val[1] * gain), pack<true>(val[2] * gain, val[3] * gain));
@@ -690,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                     if (h >= h_count) break;
                     if (d >= hd) continue;
                     float4 of[kWarps];
-                    float mx = -INFINITY, Mx = -INFINITY;
+                    float mx = -FLT_MAX, Mx = -FLT_MAX;
 #pragma unroll
                     for (int w = 0; w < kWarps; ++w) {
                         of[w] = *reinterpret_cast<const float4*>(merge + (w * 8 + j) * S::kMergePitch + kDim);
@@ -700,9 +717,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                     float sum = 0.f, val[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int w = 0; w < kWarps; ++w) {
-                        // a warp that saw nothing has l = 0 and zeros; NaN must pass through
-                        const float fl = of[w].x == -INFINITY ? 1.f : ex2(of[w].x - mx);
-                        const float fa = !kQuant ? fl : of[w].y == -INFINITY ? 1.f : ex2(of[w].y - Mx);
+                        // a warp that saw nothing has m = M = -FLT_MAX and zeros; NaN passes through
+                        const float fl = ex2(of[w].x - mx);
+                        const float fa = kQuant ? ex2(of[w].y - Mx) : fl;
                         const float4 a = *reinterpret_cast<const float4*>(merge + (w * 8 + j) * S::kMergePitch + d);
                         sum += of[w].z * fl;
                         val[0] += a.x * fa;
@@ -752,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                         // warp w: maxima, sum and every part's factor of heads w, w + 4 of the column
                         for (int j = warp; j < 8 && 8 * n + j < h_count; j += kWarps) {
                             const int off = (8 * n + j) * S::kMergePitch + kDim;
-                            float mx = -INFINITY, Mx = -INFINITY;
+                            float mx = -FLT_MAX, Mx = -FLT_MAX;
                             for (int p = lane; p < parts; p += 32) {
                                 const float4 t = __ldcg(reinterpret_cast<const float4*>(record_of(p) + off));
                                 mx = fmaxf(mx, t.x);
@@ -766,8 +783,8 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                             float sum = 0.f;
                             for (int p = lane; p < parts; p += 32) {
                                 const float4 t = __ldcg(reinterpret_cast<const float4*>(record_of(p) + off));
-                                sum += t.x == -INFINITY ? t.z : t.z * ex2(t.x - mx);
-                                merge[p * 8 + j] = t.y == -INFINITY ? 1.f : ex2(t.y - Mx);
+                                sum += t.z * ex2(t.x - mx);
+                                merge[p * 8 + j] = ex2(t.y - Mx);
                             }
 #pragma unroll
                             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
