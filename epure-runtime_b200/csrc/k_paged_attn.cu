@@ -38,7 +38,7 @@ __device__ int g_attend_error = 0;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kBlock = 16;                 // tokens of a warp's block
+constexpr int kTile = 16;                  // tokens of a tensor-core tile; a warp's block is one or two
 constexpr int kMinBlocks = 4;              // a CTA's run is at least this long
 constexpr int kMaxUnits = 65536;           // counters in the workspace
 constexpr int kMaxGrid = 512;              // CTAs of a launch
@@ -81,13 +81,13 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N> __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-template <int kOffset> __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at), "n"(kOffset) : "memory");
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
-template <int kOffset> __device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at), "n"(kOffset) : "memory");
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
@@ -121,20 +121,23 @@ template <bool kIsBf16> __device__ __forceinline__ uint32_t pack(float lo, float
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Two f16 values from the 8-bit codes that `sel` picks from x (bytes of an int8 pair
-// come with 0x64 above them: 1024 + (code ^ 0x80), so 1152 is taken off).
-template <int kKind, uint32_t kSel> __device__ __forceinline__ uint32_t codes_f16(uint32_t x) {
+// The four 8-bit codes of x as two pairs of f16: its bytes (0, 1) and (2, 3), or with
+// kAcross (0, 2) and (1, 3).  An int8 byte comes with 0x64 above it, 1024 + (code ^ 0x80),
+// and 1152 is taken off; e4m3 has an instruction of its own.
+template <int kKind, bool kAcross> __device__ __forceinline__ void codes_f16(uint32_t x, uint32_t& p0, uint32_t& p1) {
     if (kKind == kInt8) {
-        const uint32_t u = __byte_perm(x, 0x64646464u, kSel);
-        const uint32_t off = 0x64806480u;
-        const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&off));
-        return *reinterpret_cast<const uint32_t*>(&v);
+        const uint32_t u = x ^ 0x80808080u, off = 0x64806480u;
+        const uint32_t u0 = __byte_perm(u, 0x64646464u, kAcross ? 0x4240 : 0x4140);
+        const uint32_t u1 = __byte_perm(u, 0x64646464u, kAcross ? 0x4341 : 0x4342);
+        const __half2 v0 = __hsub2(*reinterpret_cast<const __half2*>(&u0), *reinterpret_cast<const __half2*>(&off));
+        const __half2 v1 = __hsub2(*reinterpret_cast<const __half2*>(&u1), *reinterpret_cast<const __half2*>(&off));
+        p0 = *reinterpret_cast<const uint32_t*>(&v0);
+        p1 = *reinterpret_cast<const uint32_t*>(&v1);
+    } else {
+        const uint32_t u = kAcross ? __byte_perm(x, 0u, 0x3120) : x;
+        asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %2;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n cvt.rn.f16x2.e4m3x2 %1, hi;\n}\n"
+            : "=r"(p0), "=r"(p1) : "r"(u));
     }
-    constexpr uint32_t kPair = (kSel & 0xf) | (kSel >> 4 & 0xf0);   // the two codes' bytes side by side
-    const uint32_t two = __byte_perm(x, 0u, kPair);
-    uint32_t r;
-    asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(r) : "r"(two));
-    return r;
 }
 
 // Byte offset of 16-byte chunk `ch` of row `row` in a stage of rows of kPitch bytes: the
@@ -147,10 +150,10 @@ template <int kPitch> __device__ __forceinline__ uint32_t swizzled(int row, int 
 
 // ---------------------------------------------------------------- units and blocks
 struct Span {
-    int lo, lo16, n, blocks;   // tokens [lo, n) in blocks from lo16 on
+    int lo, first, n, blocks;   // tokens [lo, n) in blocks of kTok from `first` on
 };
 
-__device__ __forceinline__ Span span_of(const AttendArgs& A, int b, bool report) {
+template <int kTok> __device__ __forceinline__ Span span_of(const AttendArgs& A, int b, bool report) {
     const int64_t cap = (int64_t)A.pages.max_pages * A.pages.page_size;
     int64_t n = A.lengths[b];
     bool bad = n < 0 || n > cap;
@@ -162,19 +165,19 @@ __device__ __forceinline__ Span span_of(const AttendArgs& A, int b, bool report)
     Span s;
     s.n = (int)n;
     s.lo = A.window > 0 && n > A.window ? (int)(n - A.window) : 0;
-    s.lo16 = s.lo & ~(kBlock - 1);
-    s.blocks = (s.n - s.lo16 + kBlock - 1) / kBlock;
+    s.first = s.lo & ~(kTok - 1);
+    s.blocks = (s.n - s.first + kTok - 1) / kTok;
     return s;
 }
 
 // A place in the dealt-out order: block i of unit u of sequence b.
-struct Cursor {
+template <int kTok> struct Cursor {
     int b, u, i, units;
     Span s;
     __device__ __forceinline__ void next_sequence(const AttendArgs& A) {
         do {
             ++b;
-            s = span_of(A, b, false);
+            s = span_of<kTok>(A, b, false);
         } while (s.blocks == 0);
         u = 0;
     }
@@ -192,10 +195,14 @@ template <int kKind, int kDim, int kCols>
 struct Shape {
     static constexpr int kBytes = kind_bytes<kKind>();
     static constexpr int kPitch = kDim * kBytes;
-    static constexpr int kRows = kBlock * kPitch;                        // one of K, V
-    static constexpr int kScales = kBytes == 1 ? 2 * kBlock * 4 : 0;
+    // Two tiles a block where a tile is at most 2 KB and its accumulators leave the registers
+    // for them: the block's control flow then counts half (64 x 8k fp8: 119 us with one).
+    static constexpr int kTiles = kPitch <= 128 && kDim * kCols <= 128 ? 2 : 1;
+    static constexpr int kTok = kTiles * kTile;
+    static constexpr int kRows = kTok * kPitch;                          // one of K, V
+    static constexpr int kScales = kBytes == 1 ? 2 * kTok * 4 : 0;
     static constexpr int kStage = 2 * kRows + kScales;
-    static constexpr int kCtas = kPitch > 256 ? 1 : kPitch == 256 || kCols == 2 ? 2 : 3;   // an SM
+    static constexpr int kCtas = kPitch > 256 ? 1 : kPitch == 64 && kCols == 1 ? 3 : 2;       // an SM
     static constexpr int kMergePitch = kDim + 4;                         // floats; spreads a column's heads over the banks
     static constexpr int kMergeRows = kWarps * 8 * kMergePitch * 4;
     static constexpr int kMerge = kMergeRows > kMaxGrid * 8 * 4 ? kMergeRows : kMaxGrid * 8 * 4;
@@ -219,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     using S = Shape<kKind, kDim, kCols>;
     constexpr bool kQuant = kKind >= kInt8;
     constexpr bool kIsBf16 = kKind == kBf16;
+    constexpr int kTok = S::kTok, kTiles = S::kTiles;
     constexpr unsigned kAll = 0xffffffffu;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float4 joined[8];                       // (m, M, l) of a joined unit's heads
@@ -236,9 +244,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     // ---- this CTA's run of blocks
     const int per = (A.batch + kThreads - 1) / kThreads;
     const int b0 = min(A.batch, tid * per), b1 = min(A.batch, b0 + per);
-    const int first_blocks = b0 < b1 ? span_of(A, b0, blockIdx.x == 0).blocks : 0;
+    const int first_blocks = b0 < b1 ? span_of<kTok>(A, b0, blockIdx.x == 0).blocks : 0;
     int64_t mine = first_blocks;
-    for (int b = b0 + 1; b < b1; ++b) mine += span_of(A, b, blockIdx.x == 0).blocks;
+    for (int b = b0 + 1; b < b1; ++b) mine += span_of<kTok>(A, b, blockIdx.x == 0).blocks;
     // inclusive scan over the threads
     auto scan = [&](int64_t v, int which, int64_t* total) {
 #pragma unroll
@@ -265,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     // than there are CTAs, each CTA takes one piece; else runs go over unit boundaries.
     int64_t pieces = 0;
     for (int b = b0; b < b1; ++b) {
-        const int blocks = b == b0 ? first_blocks : span_of(A, b, false).blocks;
+        const int blocks = b == b0 ? first_blocks : span_of<kTok>(A, b, false).blocks;
         pieces += quotient(blocks + run - 1, run);
     }
     int64_t all_pieces;
@@ -279,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         if (f0 >= lo && f0 < hi) {
             int64_t at = f0 - lo;
             for (int b = b0;; ++b) {
-                const int blocks = b == b0 ? first_blocks : span_of(A, b, false).blocks;
+                const int blocks = b == b0 ? first_blocks : span_of<kTok>(A, b, false).blocks;
                 const int64_t each = one_each ? quotient(blocks + run - 1, run) : blocks;
                 if (at < each * units) {
                     start_b = b;
@@ -293,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     }
     // sequences without a token
     for (int b = blockIdx.x; b < A.batch; b += gridDim.x) {
-        if (span_of(A, b, false).blocks) continue;
+        if (span_of<kTok>(A, b, false).blocks) continue;
         for (int e = tid; e < A.heads * hd; e += kThreads)
             static_cast<uint16_t*>(A.out)[(int64_t)b * A.heads * hd + e] = 0;
         if (A.lse)
@@ -306,12 +314,12 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     __syncthreads();
     if (f0 >= limit) return;
 
-    Cursor unit;                                       // of the unit that the CTA is at
+    Cursor<kTok> unit;                                       // of the unit that the CTA is at
     unit.units = units;
     unit.b = start_b;
     unit.u = start_u;
     unit.i = start_i;
-    unit.s = span_of(A, start_b, false);
+    unit.s = span_of<kTok>(A, start_b, false);
     int count, piece = 0, piece_count = 1;             // blocks of this CTA; its place among its unit's pieces
     if (one_each) {
         piece = start_i;
@@ -323,14 +331,15 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     }
 
     // ---- loads, kStages - 1 blocks ahead
-    const bool linear = P.page_size % kBlock == 0;     // a block is in one page, its rows side by side
-    Cursor ahead = unit;
+    const bool straight = P.page_size % kTile == 0 && hd == kDim;      // a tile's rows lie side by side in one page
+    Cursor<kTok> ahead = unit;
     int f_load = warp;                                 // blocks are counted from the run's start
-    int next_page = 0, next_slot = 0;                  // table entry and slot of the next block to load (its row `lane & 15`)
-    bool next_on = false;                              // whether that is a token (the entry may still be on its way)
+    // of the next block's row `lane & (kTok - 1)`: table entry, slot, whether it is a token
+    int next_page = 0, next_slot = 0;
+    bool next_on = false;                              // (the entry may still be on its way)
     auto look_up = [&]() {
-        const int t0 = ahead.s.lo16 + ahead.i * kBlock, t = linear ? t0 : t0 + (lane & 15);
-        next_on = linear || (t >= ahead.s.lo && t < ahead.s.n);
+        const int t = ahead.s.first + ahead.i * kTok + (lane & (kTok - 1));
+        next_on = t >= ahead.s.lo && t < ahead.s.n;
         if (next_on) {
             const int col = (int)((__umulhi((uint32_t)t, A.page_mul) + (uint32_t)t) >> A.page_shift);
             const int s = A.seq ? A.seq[ahead.b] : ahead.b;
@@ -343,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         look_up();
     }
     constexpr int kChunks = S::kPitch / 16;            // of a row
-    constexpr int kCopies = kBlock * kChunks / 32;     // chunks a lane
+    constexpr int kCopies = kTile * kChunks / 32;      // chunks a lane and tile
     const int my_row = lane / kChunks, my_ch = lane % kChunks;     // a lane's chunks: rows my_row, my_row + 32 / kChunks, ...
     // its place in a stage: 512 bytes further each time, with bit 6 turned (see swizzled)
     const uint32_t my_at = swizzled<S::kPitch>(my_row, my_ch);
@@ -355,58 +364,46 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                 next_on = false;
             }
             const int head = A.chunks == 1 ? ahead.u : ahead.u / A.chunks;
-            const int64_t slot_at = (int64_t)head * P.page_size + next_slot;
-            const int64_t at = next_page * P.page_stride + slot_at * hd;
+            const int slot_at = head * P.page_size + next_slot;
+            const int64_t at = (next_page * P.page_stride + (int64_t)slot_at * hd) * S::kBytes;
             const uint32_t k_at = ring_at + load_stage * S::kStage, v_at = k_at + S::kRows;
-            if (linear) {
-                const int t0 = ahead.s.lo16 + ahead.i * kBlock;
-                const int r0 = max(0, ahead.s.lo - t0), r1 = next_on ? min(kBlock, ahead.s.n - t0) : 0;   // rows that are tokens
-                if (lane == 0) seen[warp][load_stage] = r1 > r0 ? (0xffffu >> (kBlock - r1)) & (0xffffu << r0) : 0u;
-                const int64_t off = next_on ? (at + my_row * hd) * S::kBytes + my_ch * 16 : 0;
-                const uint8_t* k_from = P.k + off;
-                const uint8_t* v_from = P.v + off;
-                const int step = next_on ? 32 / kChunks * hd * S::kBytes : 0;
-                if (hd == kDim && r1 - r0 == kBlock) {             // the ordinary block: nothing to leave out
+            const uint32_t mask = __ballot_sync(kAll, next_on);
+            if (lane == 0) seen[warp][load_stage] = mask;
+            if (straight && mask == kAll) {            // the ordinary block: every row is a token (with 16 rows, lanes repeat)
+#pragma unroll
+                for (int tile = 0; tile < kTiles; ++tile) {
+                    const int64_t off = __shfl_sync(kAll, at, tile * kTile) + lane * 16;
+                    const uint8_t* k_from = P.k + off;
+                    const uint8_t* v_from = P.v + off;
 #pragma unroll
                     for (int e = 0; e < kCopies; ++e) {
-                        const uint32_t to = (my_at ^ (e & 1) * 64) + e * 512;
+                        const uint32_t to = tile * kTile * S::kPitch + (my_at ^ (e & 1) * 64) + e * 512;
                         cp16(k_at + to, k_from + e * 512);
                         cp16(v_at + to, v_from + e * 512);
                     }
-                } else if (my_ch < hd_chunks) {
-#pragma unroll
-                    for (int e = 0; e < kCopies; ++e) {
-                        const int row = my_row + e * (32 / kChunks);
-                        const int bytes = row >= r0 && row < r1 ? 16 : 0;
-                        const uint32_t to = (my_at ^ (e & 1) * 64) + e * 512;
-                        cp16(k_at + to, k_from + e * step, bytes);
-                        cp16(v_at + to, v_from + e * step, bytes);
-                    }
-                }
-                if (kQuant) {                          // lanes 0-15: key scales, 16-31: value scales
-                    const int row = lane & 15;
-                    const bool on = row >= r0 && row < r1;
-                    const float* sc = lane < 16 ? P.k_scale : P.v_scale;
-                    cp4(v_at + S::kRows + lane * 4, sc + (on ? next_page * P.scale_stride + slot_at + row : 0), on ? 4 : 0);
                 }
             } else {
-                const uint32_t mask = __ballot_sync(kAll, next_on) & 0xffffu;
-                if (lane == 0) seen[warp][load_stage] = mask;
 #pragma unroll
-                for (int e = 0; e < kCopies; ++e) {
+                for (int e = 0; e < kTiles * kCopies; ++e) {
                     const int row = my_row + e * (32 / kChunks);
                     const int64_t from = __shfl_sync(kAll, at, row);
                     const bool on = mask >> row & 1;
                     if (my_ch < hd_chunks) {
-                        const int64_t off = on ? from * S::kBytes + my_ch * 16 : 0;
+                        const int64_t off = on ? from + my_ch * 16 : 0;
                         const uint32_t to = (my_at ^ (e & 1) * 64) + e * 512;
                         cp16(k_at + to, P.k + off, on ? 16 : 0);
                         cp16(v_at + to, P.v + off, on ? 16 : 0);
                     }
                 }
-                if (kQuant) {
-                    const float* sc = lane < 16 ? P.k_scale : P.v_scale;
-                    cp4(v_at + S::kRows + lane * 4, sc + (next_on ? next_page * P.scale_stride + slot_at : 0), next_on ? 4 : 0);
+            }
+            if (kQuant) {
+                const int64_t off = next_on ? next_page * P.scale_stride + slot_at : 0;
+                const int bytes = next_on ? 4 : 0;
+                if (kTiles == 2) {
+                    cp4(v_at + S::kRows + lane * 4, P.k_scale + off, bytes);
+                    cp4(v_at + S::kRows + kTok * 4 + lane * 4, P.v_scale + off, bytes);
+                } else {                               // lanes 0-15: key scales, 16-31: value scales
+                    cp4(v_at + S::kRows + lane * 4, (lane < 16 ? P.k_scale : P.v_scale) + off, bytes);
                 }
             }
             f_load += kWarps;
@@ -426,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     // q as B fragments: column g is the unit's query head 8 n + g.  16-bit caches: dims 2c, 2c+1
     // and 2c+8, 2c+9 of every 16; 8-bit ones: 4c .. 4c+3
     uint32_t qf[kCols][kDim / 16][2];
-    auto load_q = [&](const Cursor& u) {
+    auto load_q = [&](const Cursor<kTok>& u) {
         const int head = A.chunks == 1 ? u.u : u.u / A.chunks, chunk = u.u - head * A.chunks;
         const int h0 = head * A.group + chunk * 8 * kCols, n_heads = min(8 * kCols, A.group - chunk * 8 * kCols);
 #pragma unroll
@@ -509,86 +506,108 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
             constexpr int kBatch = kLoads < 8 ? kLoads : 8;        // of which so many are in registers
 
             // scores: even and odd steps into accumulators of their own
-            float sc[kCols][4], sc2[kCols][4];
+            float sc[kTiles][kCols][4];
 #pragma unroll
-            for (int n = 0; n < kCols; ++n)
+            for (int tile = 0; tile < kTiles; ++tile) {
+                float sc2[kCols][4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sc[n][r] = sc2[n][r] = 0.f;
-            // rows 0-15, 16-byte chunks 2 k and 2 k + 1 of them: the four 8 x 8 parts lie tokens first
+                for (int n = 0; n < kCols; ++n)
 #pragma unroll
-            for (int k0 = 0; k0 < kLoads; k0 += kBatch) {
-                uint32_t x[kBatch][4];
+                    for (int r = 0; r < 4; ++r) sc[tile][n][r] = sc2[n][r] = 0.f;
+                // rows 0-15, 16-byte chunks 2 k and 2 k + 1 of them: the four 8 x 8 parts lie tokens first
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k) ldsm<0>(x[k], k_at + swizzled<S::kPitch>(lane & 15, 2 * (k0 + k) + (lane >> 4)));
+                for (int k0 = 0; k0 < kLoads; k0 += kBatch) {
+                    uint32_t x[kBatch][4];
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
-                    if (!kQuant) {
+                    for (int k = 0; k < kBatch; ++k)
+                        ldsm(x[k], k_at + tile * kTile * S::kPitch + swizzled<S::kPitch>(lane & 15, 2 * (k0 + k) + (lane >> 4)));
 #pragma unroll
-                        for (int n = 0; n < kCols; ++n)
-                            mma<kIsBf16>(k & 1 ? sc2[n] : sc[n], x[k], qf[n][k0 + k][0], qf[n][k0 + k][1]);
-                    } else {
-                        if (kKind == kInt8) {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) x[k][r] ^= 0x80808080u;
-                        }
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const uint32_t a[4] = {
-                                codes_f16<kKind, 0x4140>(x[k][2 * r]), codes_f16<kKind, 0x4140>(x[k][2 * r + 1]),
-                                codes_f16<kKind, 0x4342>(x[k][2 * r]), codes_f16<kKind, 0x4342>(x[k][2 * r + 1])};
+                    for (int k = 0; k < kBatch; ++k) {
+                        if (!kQuant) {
 #pragma unroll
                             for (int n = 0; n < kCols; ++n)
-                                mma<false>(r ? sc2[n] : sc[n], a, qf[n][2 * (k0 + k) + r][0], qf[n][2 * (k0 + k) + r][1]);
+                                mma<kIsBf16>(k & 1 ? sc2[n] : sc[tile][n], x[k], qf[n][k0 + k][0], qf[n][k0 + k][1]);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                uint32_t a[4];
+                                codes_f16<kKind, false>(x[k][2 * r], a[0], a[2]);
+                                codes_f16<kKind, false>(x[k][2 * r + 1], a[1], a[3]);
+#pragma unroll
+                                for (int n = 0; n < kCols; ++n)
+                                    mma<false>(r ? sc2[n] : sc[tile][n], a, qf[n][2 * (k0 + k) + r][0], qf[n][2 * (k0 + k) + r][1]);
+                            }
                         }
                     }
                 }
+#pragma unroll
+                for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sc[tile][n][r] += sc2[n][r];
             }
             // the first values are on their way while the weights are formed
-            uint32_t y[kBatch][4];
-            auto load_values = [&](int d0) {
+            uint32_t y[kTiles][kBatch][4];
+            auto load_values = [&](int tile, int d0) {
 #pragma unroll
-                for (int d = 0; d < kBatch; ++d)
-                    ldsm_t<S::kRows>(y[d], k_at + swizzled<S::kPitch>(lane & 15, 2 * (d0 + d) + (lane >> 4)));
+                for (int d = 0; d < kBatch; ++d) {
+                    // 16-bit: chunks first, the order of the fragment; 8-bit: tokens first, the codes are paired below
+                    const int row = kQuant ? lane & 15 : (lane >> 4) * 8 + (lane & 7);
+                    const int ch = 2 * (d0 + d) + (kQuant ? lane >> 4 : lane >> 3 & 1);
+                    ldsm_t(y[tile][d], k_at + S::kRows + tile * kTile * S::kPitch + swizzled<S::kPitch>(row, ch));
+                }
             };
-            load_values(0);
-            float ks[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) load_values(tile, 0);
+            float ks[kTiles][2], lv[kTiles][2];
             if (kQuant) {
                 const float* scales = reinterpret_cast<const float*>(ring + stage * S::kStage + 2 * S::kRows);
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    ks[r] = scales[g + 8 * r];
-                    lv[r] = __log2f(scales[16 + g + 8 * r]);
-                }
+                for (int tile = 0; tile < kTiles; ++tile)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        ks[tile][r] = scales[tile * kTile + g + 8 * r];
+                        lv[tile][r] = __log2f(scales[kTok + tile * kTile + g + 8 * r]);
+                    }
             }
-            // weights; r: token g + 8 (r >> 1), head 2c + (r & 1)
+            // weights; r: token g + 8 (r >> 1) of the tile, head 2c + (r & 1)
 #pragma unroll
-            for (int n = 0; n < kCols; ++n)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    sc[n][r] = (sc[n][r] + sc2[n][r]) * (kQuant ? q_gain[n][r & 1] * ks[r >> 1] : q_gain[n][r & 1]);
-            if (mask != 0xffffu) {
+            for (int tile = 0; tile < kTiles; ++tile)
 #pragma unroll
                 for (int n = 0; n < kCols; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (!(mask >> (g + 8 * (r >> 1)) & 1)) sc[n][r] = -INFINITY;
+                        sc[tile][n][r] *= kQuant ? q_gain[n][r & 1] * ks[tile][r >> 1] : q_gain[n][r & 1];
+            if (mask != kAll) {
+#pragma unroll
+                for (int tile = 0; tile < kTiles; ++tile)
+#pragma unroll
+                    for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (!(mask >> (tile * kTile + g + 8 * (r >> 1)) & 1)) sc[tile][n][r] = -INFINITY;
             }
             float over = -INFINITY;                    // fmaxf passes over NaN, which reaches the sums through the weights
 #pragma unroll
-            for (int n = 0; n < kCols; ++n)
+            for (int tile = 0; tile < kTiles; ++tile)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    over = fmaxf(over, sc[n][r] - m[n][r & 1]);
-                    if (kQuant) over = fmaxf(over, sc[n][r] + (lv[r >> 1] - M[n][r & 1]));
-                }
+                for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        over = fmaxf(over, sc[tile][n][r] - m[n][r & 1]);
+                        if (kQuant) over = fmaxf(over, sc[tile][n][r] + (lv[tile][r >> 1] - M[n][r & 1]));
+                    }
             if (__any_sync(kAll, over > kSlack)) {
 #pragma unroll
                 for (int n = 0; n < kCols; ++n) {
                     float turn_acc[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        float top = fmaxf(sc[n][r], sc[n][r + 2]);
-                        float topM = kQuant ? fmaxf(sc[n][r] + lv[0], sc[n][r + 2] + lv[1]) : 0.f;
+                        float top = -FLT_MAX, topM = -FLT_MAX;
+#pragma unroll
+                        for (int tile = 0; tile < kTiles; ++tile) {
+                            top = fmaxf(top, fmaxf(sc[tile][n][r], sc[tile][n][r + 2]));
+                            if (kQuant) topM = fmaxf(topM, fmaxf(sc[tile][n][r] + lv[tile][0], sc[tile][n][r + 2] + lv[tile][1]));
+                        }
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) {
                             top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
@@ -611,47 +630,46 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                         for (int r = 0; r < 4; ++r) acc[n][d][r] *= turn_acc[r & 1];
                 }
             }
-            uint32_t pf[kCols][2];
+            uint32_t pf[kTiles][kCols][2];
 #pragma unroll
-            for (int n = 0; n < kCols; ++n) {
-                float w[4];
+            for (int tile = 0; tile < kTiles; ++tile)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    w[r] = ex2(sc[n][r] - m[n][r & 1]);
-                    l[n][r & 1] += w[r];
-                    if (kQuant) w[r] = ex2(sc[n][r] + (lv[r >> 1] - M[n][r & 1]));
+                for (int n = 0; n < kCols; ++n) {
+                    float w[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        w[r] = ex2(sc[tile][n][r] - m[n][r & 1]);
+                        l[n][r & 1] += w[r];
+                        if (kQuant) w[r] = ex2(sc[tile][n][r] + (lv[tile][r >> 1] - M[n][r & 1]));
+                    }
+                    pf[tile][n][0] = transpose8x8(pack<kIsBf16>(w[0], w[1]));
+                    pf[tile][n][1] = transpose8x8(pack<kIsBf16>(w[2], w[3]));
                 }
-                pf[n][0] = transpose8x8(pack<kIsBf16>(w[0], w[1]));
-                pf[n][1] = transpose8x8(pack<kIsBf16>(w[2], w[3]));
-            }
             // O^T += V^T P^T
 #pragma unroll
-            for (int d0 = 0; d0 < kLoads; d0 += kBatch) {
-                if (d0) load_values(d0);
+            for (int d0 = 0; d0 < kLoads; d0 += kBatch)
 #pragma unroll
-                for (int d = 0; d < kBatch; ++d) {
-                    if (!kQuant) {
+                for (int tile = 0; tile < kTiles; ++tile) {
+                    if (d0) load_values(tile, d0);
 #pragma unroll
-                        for (int n = 0; n < kCols; ++n) {
-                            const uint32_t a[4] = {y[d][0], y[d][2], y[d][1], y[d][3]};
-                            mma<kIsBf16>(acc[n][d0 + d], a, pf[n][0], pf[n][1]);
-                        }
-                    } else {
-                        if (kKind == kInt8) {
+                    for (int d = 0; d < kBatch; ++d) {
+                        const uint32_t (&v)[4] = y[tile][d];
+                        if (!kQuant) {
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) y[d][r] ^= 0x80808080u;
-                        }
+                            for (int n = 0; n < kCols; ++n) mma<kIsBf16>(acc[n][d0 + d], v, pf[tile][n][0], pf[tile][n][1]);
+                        } else {
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {  // rows 0-7: the even dims of 16, rows 8-15: the odd ones
-                            const uint32_t a[4] = {
-                                codes_f16<kKind, 0x4240>(y[d][2 * r]), codes_f16<kKind, 0x4341>(y[d][2 * r]),
-                                codes_f16<kKind, 0x4240>(y[d][2 * r + 1]), codes_f16<kKind, 0x4341>(y[d][2 * r + 1])};
+                            for (int r = 0; r < 2; ++r) {  // rows 0-7: the even dims of 16, rows 8-15: the odd ones
+                                uint32_t a[4];
+                                codes_f16<kKind, true>(v[2 * r], a[0], a[1]);
+                                codes_f16<kKind, true>(v[2 * r + 1], a[2], a[3]);
 #pragma unroll
-                            for (int n = 0; n < kCols; ++n) mma<false>(acc[n][2 * (d0 + d) + r], a, pf[n][0], pf[n][1]);
+                                for (int n = 0; n < kCols; ++n)
+                                    mma<false>(acc[n][2 * (d0 + d) + r], a, pf[tile][n][0], pf[tile][n][1]);
+                            }
                         }
                     }
                 }
-            }
             if (++stage == S::kStages) stage = 0;
         }
 
