@@ -40,6 +40,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16;                  // tokens of a tensor-core tile; a warp's block is one or two
 constexpr int kMinBlocks = 4;              // a CTA's run is at least this long
+constexpr int kUnitCost = 4;               // what a unit costs besides its blocks, in blocks
 constexpr int kMaxUnits = 65536;           // counters in the workspace
 constexpr int kMaxGrid = 512;              // CTAs of a launch
 constexpr float kSlack = 8.f;              // how far (log2) a score may pass the running maximum
@@ -204,8 +205,7 @@ struct Shape {
     static constexpr int kStage = 2 * kRows + kScales;
     static constexpr int kCtas = kPitch > 256 ? 1 : kPitch == 64 && kCols == 1 ? 3 : 2;       // an SM
     static constexpr int kMergePitch = kDim + 4;                         // floats; spreads a column's heads over the banks
-    static constexpr int kMergeRows = kWarps * 8 * kMergePitch * 4;
-    static constexpr int kMerge = kMergeRows > kMaxGrid * 8 * 4 ? kMergeRows : kMaxGrid * 8 * 4;
+    static constexpr int kMerge = kWarps * 8 * kMergePitch * 4;
     // a warp's ring: its share of what 228 KB leave a CTA (1 KB is the system's, 512 bytes are static)
     static constexpr int kBudget = (228 * 1024 / kCtas - 1024 - 512 - kMerge) / kWarps;
     static constexpr int kFit = kBudget / kStage;
@@ -229,10 +229,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     constexpr int kTok = S::kTok, kTiles = S::kTiles;
     constexpr unsigned kAll = 0xffffffffu;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float4 joined[8];                       // (m, M, l) of a joined unit's heads
     __shared__ uint32_t seen[kWarps][S::kStages];     // bit r: row r of the stage is a token of the span
-    __shared__ int64_t sums[2][kWarps];
-    __shared__ int start_b, start_u, start_i;
     __shared__ bool last;
     pdl_enter();
 
@@ -241,64 +238,33 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     const int hd = P.head_dim, units = P.kv_heads * A.chunks;
     const int hd_chunks = hd * S::kBytes / 16;
 
-    // ---- this CTA's run of blocks
-    const int per = (A.batch + kThreads - 1) / kThreads;
-    const int b0 = min(A.batch, tid * per), b1 = min(A.batch, b0 + per);
-    const int first_blocks = b0 < b1 ? span_of<kTok>(A, b0, blockIdx.x == 0).blocks : 0;
-    int64_t mine = first_blocks;
-    for (int b = b0 + 1; b < b1; ++b) mine += span_of<kTok>(A, b, blockIdx.x == 0).blocks;
-    // inclusive scan over the threads
-    auto scan = [&](int64_t v, int which, int64_t* total) {
+    // ---- this CTA's run of blocks.  Every warp works it out for itself: lane i looks at the
+    // sequences [i per, (i + 1) per)
+    const int per = (A.batch + 31) / 32;
+    const int b0 = min(A.batch, lane * per), b1 = min(A.batch, b0 + per);
+    auto weight = [&](int blocks) { return blocks ? blocks + kUnitCost : 0; };
+    auto scan = [&](int v) {                           // inclusive, over the lanes
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t u = __shfl_up_sync(kAll, v, o);
+            const int u = __shfl_up_sync(kAll, v, o);
             if (lane >= o) v += u;
-        }
-        if (lane == 31) sums[which][warp] = v;
-        __syncthreads();
-        *total = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) v += sums[which][w];
-            *total += sums[which][w];
         }
         return v;
     };
-    int64_t total;
-    const int64_t upto = scan(mine, 0, &total);
-    total *= units;
-    int64_t run = quotient(total + gridDim.x - 1, gridDim.x);
-    if (run < kMinBlocks) run = kMinBlocks;
+    const int first_blocks = b0 < b1 ? span_of<kTok>(A, b0, blockIdx.x == 0).blocks : 0;
+    int mine = weight(first_blocks);
+    for (int b = b0 + 1; b < b1; ++b) mine += weight(span_of<kTok>(A, b, blockIdx.x == 0).blocks);
+    const int upto = scan(mine);
+    const int64_t total = (int64_t)__shfl_sync(kAll, upto, 31) * units;
+    const int run = max(kMinBlocks, (int)quotient(total + gridDim.x - 1, gridDim.x));
     // Where cutting every unit into pieces of at most `run` blocks makes no more pieces
     // than there are CTAs, each CTA takes one piece; else runs go over unit boundaries.
-    int64_t pieces = 0;
-    for (int b = b0; b < b1; ++b) {
-        const int blocks = b == b0 ? first_blocks : span_of<kTok>(A, b, false).blocks;
-        pieces += quotient(blocks + run - 1, run);
-    }
-    int64_t all_pieces;
-    const int64_t pieces_upto = scan(pieces, 1, &all_pieces);
-    const bool one_each = all_pieces * units <= gridDim.x;
-    const int64_t f0 = one_each ? blockIdx.x : blockIdx.x * run;       // piece, or block of the dealt-out order
-    const int64_t limit = one_each ? all_pieces * units : total;
-    {
-        const int64_t lo = (one_each ? pieces_upto - pieces : upto - mine) * units;
-        const int64_t hi = (one_each ? pieces_upto : upto) * units;
-        if (f0 >= lo && f0 < hi) {
-            int64_t at = f0 - lo;
-            for (int b = b0;; ++b) {
-                const int blocks = b == b0 ? first_blocks : span_of<kTok>(A, b, false).blocks;
-                const int64_t each = one_each ? quotient(blocks + run - 1, run) : blocks;
-                if (at < each * units) {
-                    start_b = b;
-                    start_u = (int)quotient(at, each);
-                    start_i = (int)(at - start_u * each);
-                    break;
-                }
-                at -= each * units;
-            }
-        }
-    }
+    int pieces = (first_blocks + run - 1) / run;
+    for (int b = b0 + 1; b < b1; ++b) pieces += (span_of<kTok>(A, b, false).blocks + run - 1) / run;
+    const int pieces_upto = scan(pieces);
+    const int64_t all_pieces = (int64_t)__shfl_sync(kAll, pieces_upto, 31) * units;
+    const bool one_each = all_pieces <= gridDim.x;
+    const int64_t f0 = one_each ? blockIdx.x : blockIdx.x * (int64_t)run;    // piece, or place in the dealt-out order
     // sequences without a token
     for (int b = blockIdx.x; b < A.batch; b += gridDim.x) {
         if (span_of<kTok>(A, b, false).blocks) continue;
@@ -307,27 +273,68 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         if (A.lse)
             for (int h = tid; h < A.heads; h += kThreads) A.lse[(int64_t)b * A.heads + h] = -INFINITY;
     }
-    uint8_t* ring = smem + warp * S::kRing;
-    const uint32_t ring_at = smem_u32(ring);
-    if (hd < kDim)                                     // chunks past the head's end stay zero
-        for (int e = lane; e < S::kRing / 16; e += 32) reinterpret_cast<uint4*>(ring)[e] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    if (f0 >= limit) return;
-
-    Cursor<kTok> unit;                                       // of the unit that the CTA is at
+    if (f0 >= (one_each ? all_pieces : total)) return;
+    Cursor<kTok> unit;                                 // of the unit that the CTA is at
     unit.units = units;
-    unit.b = start_b;
-    unit.u = start_u;
-    unit.i = start_i;
-    unit.s = span_of<kTok>(A, start_b, false);
+    {
+        const int64_t lo = (int64_t)(one_each ? pieces_upto - pieces : upto - mine) * units;
+        const int64_t hi = (int64_t)(one_each ? pieces_upto : upto) * units;
+        const bool here = f0 >= lo && f0 < hi;
+        int at_b = 0, at_u = 0, at_i = 0;
+        if (here) {
+            int64_t at = f0 - lo;
+            for (int b = b0;; ++b) {
+                const int blocks = b == b0 ? first_blocks : span_of<kTok>(A, b, false).blocks;
+                const int each = one_each ? (blocks + run - 1) / run : weight(blocks);
+                if (at < (int64_t)each * units) {
+                    at_b = b;
+                    at_u = (int)quotient(at, each);
+                    at_i = (int)(at - (int64_t)at_u * each);
+                    break;
+                }
+                at -= (int64_t)each * units;
+            }
+        }
+        const int from = __ffs(__ballot_sync(kAll, here)) - 1;
+        unit.b = __shfl_sync(kAll, at_b, from);
+        unit.u = __shfl_sync(kAll, at_u, from);
+        unit.i = __shfl_sync(kAll, at_i, from);
+    }
+    unit.s = span_of<kTok>(A, unit.b, false);
     int count, piece = 0, piece_count = 1;             // blocks of this CTA; its place among its unit's pieces
+    int64_t unit_at = f0 - unit.i;                     // where the unit begins in the dealt-out order
     if (one_each) {
-        piece = start_i;
-        piece_count = (int)quotient(unit.s.blocks + run - 1, run);
+        piece = unit.i;
+        piece_count = (unit.s.blocks + run - 1) / run;
         unit.i = (int)((int64_t)unit.s.blocks * piece / piece_count);
         count = (int)((int64_t)unit.s.blocks * (piece + 1) / piece_count) - unit.i;
     } else {
-        count = (int)min(run, total - f0);
+        // a unit's first kUnitCost places stand for its own cost, the others are its blocks
+        const int at = unit.i;
+        unit.i = max(0, at - kUnitCost);
+        count = 0;
+        int left = (int)min((int64_t)run, total - f0), begun = at;
+        Cursor<kTok> to = unit;
+        for (;;) {
+            const int all = weight(to.s.blocks), take = min(left, all - begun);
+            count += max(0, begun + take - kUnitCost) - max(0, begun - kUnitCost);
+            left -= take;
+            if (left == 0) break;
+            const int same = min(units - 1 - to.u, left / all);    // whole units of the same sequence
+            count += same * to.s.blocks;
+            left -= same * all;
+            if (left == 0) break;
+            to.u += same;
+            begun = 0;
+            if (++to.u == units) to.next_sequence(A);
+        }
+        if (count == 0) return;
+    }
+    uint8_t* ring = smem + warp * S::kRing;
+    const uint32_t ring_at = smem_u32(ring);
+    if (hd < kDim) {                                   // chunks past the head's end stay zero
+        for (int e = lane; e < S::kRing / 16; e += 32) reinterpret_cast<uint4*>(ring)[e] = make_uint4(0, 0, 0, 0);
+        __syncwarp();
     }
 
     // ---- loads, kStages - 1 blocks ahead
@@ -675,8 +682,10 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
 
         // ---- the unit's piece: the four warps' states to one
         const bool cut_before = unit_start < 0, cut = cut_before || unit_end > count;
+        const int64_t unit_from = unit_at + kUnitCost, unit_to = unit_from + unit.s.blocks;
         at = end;
         if (at < count) {                              // the next unit's q is on its way meanwhile
+            unit_at = unit_to;
             unit.advance(A, unit.s.blocks - unit.i);
             load_q(unit);
         }
@@ -764,69 +773,61 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                 first = (int)blockIdx.x - piece;
                 parts = piece_count;
             } else {
-                first = (int)quotient(f0 + unit_start, run);
-                parts = (int)quotient(f0 + unit_end - 1, run) - first + 1;
+                first = (int)quotient(unit_from, run);
+                parts = (int)quotient(unit_to - 1, run) - first + 1;
             }
             if (tid == 0) {
-                __threadfence();                       // orders the CTA's records (the barrier above) before the count
-                last = atomicAdd(&A.counters[unit_index], 1u) == (unsigned)parts - 1;
-                if (last) {
-                    __threadfence();
-                    A.counters[unit_index] = 0u;
-                }
+                // releases the CTA's record (complete at the barrier above), acquires the others'
+                unsigned before;
+                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
+                             : "=r"(before) : "l"(A.counters + unit_index) : "memory");
+                last = before == (unsigned)parts - 1;
+                if (last) A.counters[unit_index] = 0u;
             }
             __syncthreads();
             if (last) {
-                // where runs go over boundaries, only the first part is its CTA's last piece
-                auto record_of = [&](int p) {
-                    return A.records + ((int64_t)(first + p) * 2 + (one_each || p == 0 ? 1 : 0)) * S::kRecord;
-                };
+                for (int e = tid; e < 8 * kCols * kQuads; e += kThreads) {
+                    const int h = e / kQuads, d = e % kQuads * 4;
+                    if (h >= h_count) break;
+                    if (d >= hd) continue;
+                    float mx = -FLT_MAX, Mx = -FLT_MAX, sum = 0.f, val[4] = {0.f, 0.f, 0.f, 0.f};
+                    constexpr int kAtOnce = 8;
+                    for (int p0 = 0; p0 < parts; p0 += kAtOnce) {
+                        float4 of[kAtOnce], a[kAtOnce];
 #pragma unroll
-                for (int n = 0; n < kCols; ++n) {
-                    if (8 * n < h_count) {
-                        // warp w: maxima, sum and every part's factor of heads w, w + 4 of the column
-                        for (int j = warp; j < 8 && 8 * n + j < h_count; j += kWarps) {
-                            const int off = (8 * n + j) * S::kMergePitch + kDim;
-                            float mx = -FLT_MAX, Mx = -FLT_MAX;
-                            for (int p = lane; p < parts; p += 32) {
-                                const float4 t = __ldcg(reinterpret_cast<const float4*>(record_of(p) + off));
-                                mx = fmaxf(mx, t.x);
-                                Mx = fmaxf(Mx, t.y);
-                            }
-#pragma unroll
-                            for (int o = 16; o > 0; o >>= 1) {
-                                mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
-                                Mx = fmaxf(Mx, __shfl_xor_sync(kAll, Mx, o));
-                            }
-                            float sum = 0.f;
-                            for (int p = lane; p < parts; p += 32) {
-                                const float4 t = __ldcg(reinterpret_cast<const float4*>(record_of(p) + off));
-                                sum += t.z * ex2(t.x - mx);
-                                merge[p * 8 + j] = ex2(t.y - Mx);
-                            }
-#pragma unroll
-                            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
-                            if (lane == 0) joined[j] = make_float4(mx, Mx, sum, 0.f);
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            const int p = min(p0 + i, parts - 1);
+                            // where runs go over boundaries, only the first part is its CTA's last piece
+                            const float* rec = A.records + ((int64_t)(first + p) * 2 + (one_each || p == 0 ? 1 : 0)) * S::kRecord +
+                                               h * S::kMergePitch;
+                            of[i] = __ldcg(reinterpret_cast<const float4*>(rec + kDim));
+                            a[i] = __ldcg(reinterpret_cast<const float4*>(rec + d));
                         }
-                        __syncthreads();
-                        for (int e = tid; e < 8 * kQuads; e += kThreads) {
-                            const int j = e / kQuads, d = e % kQuads * 4, h = 8 * n + j;
-                            if (h >= h_count) break;
-                            if (d >= hd) continue;
-                            float val[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-                            for (int p = 0; p < parts; ++p) {
-                                const float4 a = __ldcg(reinterpret_cast<const float4*>(record_of(p) + h * S::kMergePitch + d));
-                                const float fa = merge[p * 8 + j];
-                                val[0] += a.x * fa;
-                                val[1] += a.y * fa;
-                                val[2] += a.z * fa;
-                                val[3] += a.w * fa;
-                            }
-                            emit(h, d, val, joined[j].x, joined[j].y, joined[j].z);
+                        float mn = mx, Mn = Mx;
+#pragma unroll
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            mn = fmaxf(mn, of[i].x);
+                            Mn = fmaxf(Mn, of[i].y);
                         }
-                        __syncthreads();
+                        const float fl = mn == mx ? 1.f : ex2(mx - mn), fa = Mn == Mx ? 1.f : ex2(Mx - Mn);
+                        sum *= fl;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) val[i] *= fa;
+#pragma unroll
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            if (p0 + i < parts) {
+                                const float w = ex2(of[i].y - Mn);
+                                sum += of[i].z * ex2(of[i].x - mn);
+                                val[0] += a[i].x * w;
+                                val[1] += a[i].y * w;
+                                val[2] += a[i].z * w;
+                                val[3] += a[i].w * w;
+                            }
+                        }
+                        mx = mn;
+                        Mx = Mn;
                     }
+                    emit(h, d, val, mx, Mx, sum);
                 }
             }
         }
@@ -908,6 +909,9 @@ int epq_paged_attend(const epq_pages* pages, const epq_heads* q, const int32_t* 
     if (!seq && batch > A.pages.seqs)
         return set_error(EPQ_ESHAPE, "epq_paged_attend: batch=%lld of a table of %d sequences", (long long)batch,
                          A.pages.seqs);
+    if (batch * ((int64_t)A.pages.max_pages * A.pages.page_size / kTile + 1 + kUnitCost) > INT32_MAX)
+        return set_error(EPQ_EUNSUPPORTED, "epq_paged_attend: batch=%lld of up to %lld tokens each", (long long)batch,
+                         (long long)A.pages.max_pages * A.pages.page_size);
     if (batch == 0) return EPQ_OK;
     if (!q->data || !lengths || !out) return set_error(EPQ_EINVAL, "epq_paged_attend: NULL q, lengths or out");
     if (!heads_aligned(*q, 2, 4) || (uintptr_t)out % 16)
