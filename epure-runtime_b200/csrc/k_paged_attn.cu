@@ -40,7 +40,10 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16;                  // tokens of a tensor-core tile; a warp's block is one or two
 constexpr int kMinBlocks = 4;              // a CTA's run is at least this long
-constexpr int kUnitCost = 4;               // what a unit costs besides its blocks, in blocks
+constexpr int kWhole = 12;                 // and a unit of at most this many is not cut for latency
+// What a unit costs besides its blocks (its q, joining its warps), in blocks: 64 x 8k fp8
+// took 104 us with 2, 101 with 4, 97 with 8 to 16.
+constexpr int kUnitCost = 12;
 constexpr int kMaxUnits = 65536;           // counters in the workspace
 constexpr int kMaxGrid = 512;              // CTAs of a launch
 constexpr float kSlack = 8.f;              // how far (log2) a score may pass the running maximum
@@ -257,10 +260,11 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     const int upto = scan(mine);
     const int64_t total = (int64_t)__shfl_sync(kAll, upto, 31) * units;
     const int run = max(kMinBlocks, (int)quotient(total + gridDim.x - 1, gridDim.x));
-    // Where cutting every unit into pieces of at most `run` blocks makes no more pieces
+    // Where cutting every long unit into pieces of at most `run` blocks makes no more pieces
     // than there are CTAs, each CTA takes one piece; else runs go over unit boundaries.
-    int pieces = (first_blocks + run - 1) / run;
-    for (int b = b0 + 1; b < b1; ++b) pieces += (span_of<kTok>(A, b, false).blocks + run - 1) / run;
+    auto pieces_of = [&](int blocks) { return blocks > kWhole ? (blocks + run - 1) / run : blocks > 0; };
+    int pieces = pieces_of(first_blocks);
+    for (int b = b0 + 1; b < b1; ++b) pieces += pieces_of(span_of<kTok>(A, b, false).blocks);
     const int pieces_upto = scan(pieces);
     const int64_t all_pieces = (int64_t)__shfl_sync(kAll, pieces_upto, 31) * units;
     const bool one_each = all_pieces <= gridDim.x;
@@ -285,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
             int64_t at = f0 - lo;
             for (int b = b0;; ++b) {
                 const int blocks = b == b0 ? first_blocks : span_of<kTok>(A, b, false).blocks;
-                const int each = one_each ? (blocks + run - 1) / run : weight(blocks);
+                const int each = one_each ? pieces_of(blocks) : weight(blocks);
                 if (at < (int64_t)each * units) {
                     at_b = b;
                     at_u = (int)quotient(at, each);
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     int64_t unit_at = f0 - unit.i;                     // where the unit begins in the dealt-out order
     if (one_each) {
         piece = unit.i;
-        piece_count = (unit.s.blocks + run - 1) / run;
+        piece_count = pieces_of(unit.s.blocks);
         unit.i = (int)((int64_t)unit.s.blocks * piece / piece_count);
         count = (int)((int64_t)unit.s.blocks * (piece + 1) / piece_count) - unit.i;
     } else {
