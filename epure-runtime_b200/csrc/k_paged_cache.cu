@@ -18,13 +18,19 @@ namespace {
 
 __device__ int g_cache_error = 0;
 
-constexpr int kCacheThreads = 256;
+constexpr int kCacheThreads = 128;
 
 struct Rows {
     const void* p;
     int64_t row, head;   // strides, in elements
 };
 
+template <int N> struct Const {
+    static constexpr int value = N;
+};
+
+// How a lane comes by the values that its own turn with: from the lane that holds them,
+// from its own, or from memory (where neither fits).
 enum Turn { kNoTurn = 0, kHalfLanes = 1, kNeighbours = 2, kHalfLoads = 3 };
 
 struct WriteArgs {
@@ -41,45 +47,43 @@ struct WriteArgs {
     float eps;
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const T* p, int aligned) {
-    if (aligned) {
-        load_v<T, 8>(x, p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f<T>(p[i]);
-    }
-}
+template <int kFormat> constexpr float kTop = kFormat == EPQ_CACHE_INT8 ? 127.f : 448.f;    // the largest code
 
-// Eight values times `inv`, as codes.
+// Eight values times `inv` (= top / max, at most top (1 + 2^-23) in magnitude), as codes.
 template <int kFormat>
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv, float scale) {
-    uint32_t b[8];
-    // A row whose maximum is so small that top / max overflows is divided instead.
-    const bool tiny = inv == INFINITY;
+    float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        float y0 = x[i] * inv, y1 = x[i + 1] * inv;
-        if (tiny) {
-            y0 = scale > 0.f ? __fdiv_rn(x[i], scale) : 0.f;
-            y1 = scale > 0.f ? __fdiv_rn(x[i + 1], scale) : 0.f;
-        }
-        if (kFormat == EPQ_CACHE_INT8) {
-            b[i] = (uint32_t)max(-127, min(127, __float2int_rn(y0))) & 0xffu;
-            b[i + 1] = (uint32_t)max(-127, min(127, __float2int_rn(y1))) & 0xffu;
-        } else {
-            const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(y0, y1), __NV_SATFINITE, __NV_E4M3);
-            b[i] = two & 0xffu;
-            b[i + 1] = two >> 8;
-        }
+    for (int i = 0; i < 8; i += 2) mul2(y[i], y[i + 1], x[i], x[i + 1], inv, inv);
+    if (inv == INFINITY) {          // a row whose maximum is so small that top / max overflows is divided instead
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            y[i] = scale > 0.f ? fmaxf(-kTop<kFormat>, fminf(kTop<kFormat>, __fdiv_rn(x[i], scale))) : 0.f;
     }
-    return make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
+    uint32_t b[8];
+    if (kFormat == EPQ_CACHE_INT8) {
+        // 1.5 2^23 + y: float32 rounds to the integer (ties to even), which is its low byte
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(__fadd_rn(y[i], 12582912.f));
+        return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                          __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            b[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i], y[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+        return make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+    }
 }
 
-template <typename T, int kFormat, int kLanes>
+constexpr int kAtOnce = 2;          // rows of a lane in flight
+
+// kGeneral: any alignment and any turn; else 16-byte loads and stores, and a turn (if any)
+// whose partners are whole lanes.
+template <typename T, int kFormat, int kLanes, bool kGeneral>
 __global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A) {
     pdl_enter();
     constexpr unsigned kAll = 0xffffffffu;
+    constexpr int kFit = 32 / kLanes, kStep = kFit * kAtOnce;      // heads of a warp side by side, and a pass
     const int warp = blockIdx.x * (kCacheThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int64_t row = warp / A.splits;
     if (row >= A.m) return;
@@ -88,6 +92,25 @@ __global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A)
     const int hd = P.head_dim, KV = P.kv_heads;
     const int sub = lane / kLanes, chunk = lane & (kLanes - 1), e0 = chunk * 8;
     const bool in_row = e0 < hd;
+    const bool aligned = !kGeneral || A.aligned, out_aligned = !kGeneral || A.out_aligned;
+
+    // A pass is kStep heads of q, k or v; this warp's are [p0, p1).  A pass's rows are
+    // fetched while the one before it (first: the token's place) is worked on.  Lanes past
+    // the last head or value fetch what another lane does.
+    const int of_q = (A.heads + kStep - 1) / kStep, of_kv = (KV + kStep - 1) / kStep, passes = of_q + 2 * of_kv;
+    const int p0 = passes * split / A.splits, p1 = passes * (split + 1) / A.splits;
+    Eight<T> next[kAtOnce];
+    auto fetch = [&](const Rows& src, int heads, int h0) {
+        const T* const from = static_cast<const T*>(src.p) + row * src.row + (in_row ? e0 : 0);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) next[i].load(from + min(h0 + sub + i * kFit, heads - 1) * src.head, aligned);
+    };
+    auto fetch_pass = [&](int p) {
+        if (p < of_q) fetch(A.q, A.heads, p * kStep);
+        else if (p < of_q + of_kv) fetch(A.k, KV, (p - of_q) * kStep);
+        else fetch(A.v, KV, (p - of_q - of_kv) * kStep);
+    };
+    if (p0 < p1) fetch_pass(p0);
 
     const int64_t pos = A.pos[row];
     int64_t page = 0;
@@ -104,107 +127,133 @@ __global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A)
 
     // cos and the signed sin of this lane's 8 values: y = x c + partner s.
     float c[8], s[8];
-    if (A.turn != kNoTurn && live) {
+    int partner = lane;                                // kHalfLanes: the lane that holds the other halves
+    const bool turned = A.turn != kNoTurn && live;
+    if (turned) {
         const int half = A.r >> 1;
+        if (!kGeneral || A.turn == kHalfLanes) {
+            const int part = half >> 3;
+            const bool second = chunk >= part;
+            if (e0 < A.r) {
+                partner = second ? lane - part : lane + part;
+                const int64_t at = pos * half + (second ? e0 - half : e0);
+                load_v<float, 8>(c, A.cos_t + at);
+                load_v<float, 8>(s, A.sin_t + at);
+                if (!second) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int e = e0 + i;
-            c[i] = 1.f;
-            s[i] = 0.f;
-            if (e < A.r) {
-                const bool second = A.turn == kNeighbours ? e & 1 : e >= half;
-                const int64_t at = pos * half + (A.turn == kNeighbours ? e >> 1 : second ? e - half : e);
-                c[i] = A.cos_t[at];
-                s[i] = second ? A.sin_t[at] : -A.sin_t[at];
+                    for (int i = 0; i < 8; ++i) s[i] = -s[i];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = e0 + i;
+                if (e < A.r) {
+                    const bool second = A.turn == kNeighbours ? e & 1 : e >= half;
+                    const int64_t at = pos * half + (A.turn == kNeighbours ? e >> 1 : second ? e - half : e);
+                    c[i] = A.cos_t[at];
+                    s[i] = second ? A.sin_t[at] : -A.sin_t[at];
+                }
             }
         }
     }
-    constexpr int kFit = 32 / kLanes;
-    const int rows = A.heads + 2 * KV, passes = (rows + kFit - 1) / kFit;
-    const int p0 = (int)((int64_t)passes * split / A.splits), p1 = (int)((int64_t)passes * (split + 1) / A.splits);
-    for (int ps = p0; ps < p1; ++ps) {
-        const int j = ps * kFit + sub;
-        const bool is_q = j < A.heads, is_v = j >= A.heads + KV;
-        const int head = is_q ? j : is_v ? j - A.heads - KV : j - A.heads;
-        const bool on = j < rows && in_row && live;
-        const Rows src = is_q ? A.q : is_v ? A.v : A.k;
-        const T* x_at = static_cast<const T*>(src.p) + row * src.row + head * src.head;
-        float x[8];
+
+    // Works on the pass's rows x: heads h0 + sub, h0 + sub + kFit, ... of q (kWhich = 0), k (1) or v (2)
+    auto work = [&](auto which, int h0, Eight<T> (&x)[kAtOnce]) {
+        constexpr int kWhich = decltype(which)::value;
+        const int heads = kWhich == 0 ? A.heads : KV;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        if (on) load8<T>(x, x_at + e0, A.aligned);
-        float gain = 1.f;
-        if (A.qk_norm) {                              // RMSNorm of a q or k head, rounded to T
-            float ss = 0.f;
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int h = h0 + sub + i * kFit;
+            const bool on = in_row && h < heads;
+            if (!in_row) x[i].clear();
+            if (kWhich < 2) {
+                float f[8], gain = 1.f;
+                if (A.qk_norm) {                       // RMSNorm of the head, rounded to T
+                    x[i].get(f);
+                    float ss = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+                    for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
 #pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
-            if (!is_v) {
-                gain = rsqrtf(ss / (float)hd + A.eps);
+                    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
+                    gain = rsqrtf(ss / (float)hd + A.eps);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = to_f<T>(from_f<T>(x[i] * gain));
-            }
-        }
-        if (A.turn != kNoTurn) {
-            float other[8];
-            if (A.turn == kHalfLanes) {               // rotary_dim a multiple of 16: the partner's lane
-                const int part = A.r >> 4;
-                const int from = sub * kLanes + (chunk < part ? chunk + part : chunk < 2 * part ? chunk - part : chunk);
+                    for (int j = 0; j < 8; ++j) f[j] *= gain;
+                    x[i].set(f);
+                }
+                if (turned) {
+                    float other[8];
+                    x[i].get(f);
+                    if (!kGeneral || A.turn == kHalfLanes) {
+                        x[i].from_lane(partner).get(other);
+                        if (e0 < A.r) {                // (rotary_dim is a multiple of 16: all 8 or none)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(kAll, x[i], from);
-            } else if (A.turn == kNeighbours) {
+                            for (int j = 0; j < 8; j += 2) {
+                                mul2(f[j], f[j + 1], f[j], f[j + 1], c[j], c[j + 1]);
+                                mul2(other[j], other[j + 1], other[j], other[j + 1], s[j], s[j + 1]);
+                            }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) other[i] = x[i ^ 1];
-            } else {
-                const int half = A.r >> 1;
+                            for (int j = 0; j < 8; ++j) f[j] = __fadd_rn(f[j], other[j]);
+                            x[i].set(f);
+                        }
+                    } else {
+                        if (A.turn == kNeighbours) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int e = e0 + i;
-                    other[i] = 0.f;
-                    if (on && !is_v && e < A.r) {
-                        other[i] = to_f<T>(x_at[e < half ? e + half : e - half]);
-                        if (A.qk_norm) other[i] = to_f<T>(from_f<T>(other[i] * gain));
+                            for (int j = 0; j < 8; ++j) other[j] = f[j ^ 1];
+                        } else {
+                            const Rows& src = kWhich == 0 ? A.q : A.k;
+                            const T* const from = static_cast<const T*>(src.p) + row * src.row + h * src.head + e0;
+                            const int half = A.r >> 1;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const int e = e0 + j;
+                                other[j] = 0.f;
+                                if (on && e < A.r) {
+                                    other[j] = to_f<T>(from[(e < half ? half : -half) + j]);
+                                    if (A.qk_norm) other[j] = to_f<T>(from_f<T>(other[j] * gain));
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (e0 + j < A.r) f[j] = __fadd_rn(__fmul_rn(f[j], c[j]), __fmul_rn(other[j], s[j]));
+                        x[i].set(f);
                     }
                 }
             }
-            if (!is_v && live) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (e0 + i < A.r)
-                        x[i] = to_f<T>(from_f<T>(__fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(other[i], s[i]))));
-            }
-        }
-        if (is_q) {
-            if (in_row) {                             // a padding row's q is zero
-                T* o = static_cast<T*>(A.q_out) + row * A.qo_row + head * A.qo_head + e0;
-                if (A.out_aligned) {
-                    store_v<T, 8>(o, x);
+            if (kWhich == 0) {
+                if (on) {
+                    if (!live) x[i].clear();           // a padding row's q is zero
+                    x[i].store(static_cast<T*>(A.q_out) + row * A.qo_row + h * A.qo_head + e0, out_aligned);
+                }
+            } else {
+                const int64_t slot_at = (int64_t)h * P.page_size + slot;
+                uint8_t* const pool = kWhich == 1 ? P.k : P.v;
+                if (kFormat == EPQ_CACHE_SAME) {
+                    if (on && live) x[i].store(reinterpret_cast<T*>(pool) + page * P.page_stride + slot_at * hd + e0, true);
                 } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = from_f<T>(x[i]);
+                    const float a = x[i].template largest<kLanes>();
+                    // (a row that is not finite reads back as NaN, whatever its codes are)
+                    const float scale = a < INFINITY ? __fmul_rn(a, 1.f / kTop<kFormat>) : NAN;
+                    const float inv = a > 0.f ? __fdiv_rn(kTop<kFormat>, a) : 0.f;
+                    if (on && live) {
+                        float f[8];
+                        x[i].get(f);
+                        *reinterpret_cast<uint2*>(pool + page * P.page_stride + slot_at * hd + e0) = codes8<kFormat>(f, inv, scale);
+                        if (chunk == 0) (kWhich == 1 ? P.k_scale : P.v_scale)[page * P.scale_stride + slot_at] = scale;
+                    }
                 }
             }
         }
-        const int64_t at = page * P.page_stride + ((int64_t)head * P.page_size + slot) * hd + e0;
-        if (kFormat == EPQ_CACHE_SAME) {
-            if (on && !is_q) store_v<T, 8>(reinterpret_cast<T*>(is_v ? P.v : P.k) + at, x);
-        } else {
-            // |x| compared as integers, so that a NaN is the largest
-            uint32_t top = 0;
+    };
+    for (int p = p0; p < p1; ++p) {
+        Eight<T> x[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-#pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kAll, top, o));
-            const float a = __uint_as_float(top);
-            constexpr float kTop = kFormat == EPQ_CACHE_INT8 ? 127.f : 448.f;
-            const float scale = __fmul_rn(a, 1.f / kTop), inv = a > 0.f ? __fdiv_rn(kTop, a) : 0.f;
-            if (on && !is_q) {
-                *reinterpret_cast<uint2*>((is_v ? P.v : P.k) + at) = codes8<kFormat>(x, inv, scale);
-                if (chunk == 0)
-                    (is_v ? P.v_scale : P.k_scale)[page * P.scale_stride + (int64_t)head * P.page_size + slot] = scale;
-            }
-        }
+        for (int i = 0; i < kAtOnce; ++i) x[i] = next[i];
+        if (p + 1 < p1) fetch_pass(p + 1);
+        if (p < of_q) work(Const<0>(), p * kStep, x);
+        else if (p < of_q + of_kv) work(Const<1>(), (p - of_q) * kStep, x);
+        else work(Const<2>(), (p - of_q - of_kv) * kStep, x);
     }
 }
 
@@ -256,7 +305,8 @@ __global__ void __launch_bounds__(kCacheThreads) read_kernel(const ReadArgs A) {
                     const uint32_t b = u[i >> 2] >> (8 * (i & 3)) & 0xffu;
                     float code;
                     if (kFormat == EPQ_CACHE_INT8) {
-                        code = (float)(int8_t)b;
+                        // 2^23 + (b ^ 0x80) as bits, less 2^23 + 128
+                        code = __uint_as_float(0x4b000000u | (b ^ 0x80u)) - 8388736.f;
                     } else {
                         const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3);
                         code = __half2float(__half(h));
@@ -270,13 +320,18 @@ __global__ void __launch_bounds__(kCacheThreads) read_kernel(const ReadArgs A) {
     }
 }
 
-template <typename T, int kFormat>
-int launch_write(const WriteArgs& A, unsigned blocks, cudaStream_t st) {
+template <typename T, int kFormat, bool kGeneral>
+int launch_write_g(const WriteArgs& A, unsigned blocks, cudaStream_t st) {
     const int hd = A.pages.head_dim;
     const char* who = "epq_paged_write";
-    if (hd <= 64) return launch(write_kernel<T, kFormat, 8>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
-    if (hd <= 128) return launch(write_kernel<T, kFormat, 16>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
-    return launch(write_kernel<T, kFormat, 32>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+    if (hd <= 64) return launch(write_kernel<T, kFormat, 8, kGeneral>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+    if (hd <= 128) return launch(write_kernel<T, kFormat, 16, kGeneral>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+    return launch(write_kernel<T, kFormat, 32, kGeneral>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+}
+template <typename T, int kFormat>
+int launch_write(const WriteArgs& A, unsigned blocks, cudaStream_t st) {
+    const bool plain = A.aligned && (A.heads == 0 || A.out_aligned) && (A.turn == kNoTurn || A.turn == kHalfLanes);
+    return plain ? launch_write_g<T, kFormat, false>(A, blocks, st) : launch_write_g<T, kFormat, true>(A, blocks, st);
 }
 template <typename T>
 int launch_write_t(const WriteArgs& A, unsigned blocks, cudaStream_t st) {
@@ -295,9 +350,9 @@ int launch_read_t(const ReadArgs& A, unsigned blocks, cudaStream_t st) {
 }
 
 // Warps a token: one, or as many as it has passes while there are too few tokens to give
-// every SM 16 warps.
+// every SM 32 warps.
 int share_out(int64_t m, int64_t passes) {
-    int64_t splits = cdiv((int64_t)device_sms() * 16, m);
+    int64_t splits = cdiv((int64_t)device_sms() * 32, m);
     return (int)(splits < passes ? splits : passes);
 }
 
@@ -394,14 +449,16 @@ int epq_paged_write(const epq_pages* pages, const epq_heads* q, const epq_heads*
     A.m = m;
     A.max_len = max_len;
     A.r = rotary_dim;
-    A.turn = !cos_tab ? kNoTurn : interleaved ? kNeighbours : rotary_dim % 16 == 0 ? kHalfLanes : kHalfLoads;
+    const bool whole = rotary_dim % 16 == 0 && ((uintptr_t)cos_tab | (uintptr_t)sin_tab) % 16 == 0;
+    A.turn = !cos_tab ? kNoTurn : interleaved ? kNeighbours : whole ? kHalfLanes : kHalfLoads;
     // In place, a lane's loads of its partner's values would race with that lane's store.
     if (A.turn == kHalfLoads && q && q->data == q_out->data)
-        return set_error(EPQ_EUNSUPPORTED, "epq_paged_write: q in place needs rotary_dim %% 16 == 0 (got %d)", rotary_dim);
+        return set_error(EPQ_EUNSUPPORTED, "epq_paged_write: q in place needs rotary_dim %% 16 == 0 (got %d) and aligned tables",
+                         rotary_dim);
     A.qk_norm = qk_norm != 0;
     A.eps = eps;
     const int fit = hd <= 64 ? 4 : hd <= 128 ? 2 : 1;
-    A.splits = share_out(m, cdiv(A.heads + 2 * KV, fit));
+    A.splits = share_out(m, cdiv(A.heads, fit * kAtOnce) + 2 * cdiv(KV, fit * kAtOnce));
     if (m * A.splits > (int64_t)1 << 30)
         return set_error(EPQ_EUNSUPPORTED, "epq_paged_write: m=%lld rows", (long long)m);
     const unsigned blocks = (unsigned)cdiv(m * A.splits * 32, kCacheThreads);

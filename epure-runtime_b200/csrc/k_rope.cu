@@ -29,28 +29,29 @@ struct RopeArgs {
     int hd, r, splits, inverse;
 };
 
-constexpr int kRopeThreads = 256;
-constexpr int kRopeHeads = 4;   // heads of one lane in flight
+constexpr int kRopeThreads = 128;
+constexpr int kRopeHeads = 2;   // heads of one lane in flight
 
 // V: values a load (V = 1: any alignment and size).  An item holds V pairs (half
-// layout) or max(V, 2) neighbouring values (interleaved, and every copied item).
+// layout) or max(V, 2) neighbouring values (interleaved), or is V copied values.
 template <typename T, int V, bool kInterleaved>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs A) {
     pdl_enter();
-    constexpr int kCopy = V;                                // values of a copied item
     constexpr int kNear = V > 1 ? V : 2;                    // values of an interleaved item
+    constexpr int kPairs = kInterleaved ? kNear / 2 : V;
+    using W = typename Word<V * (int)sizeof(T)>::type;
     const int warp = blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int64_t row = warp / A.splits;
     if (row >= A.m) return;
     const int split = warp - (int)row * A.splits;
     const int half = A.r >> 1;
     const int turns = kInterleaved ? A.r / kNear : half / V;
-    const int items = turns + (A.hd - A.r) / kCopy;
+    const int items = turns + (A.hd - A.r) / V;
     const int fit = items < 32 ? 32 / items : 1;            // heads side by side in the warp
     const int sub = items < 32 ? lane / items : 0;
     const int first = items < 32 ? lane - sub * items : lane;
-    const int total = A.heads[0] + A.heads[1];
-    const int groups = (total + fit - 1) / fit;             // this split's share of the head groups
+    // this split's share [g0, g1) of the two tensors' groups of `fit` heads
+    const int groups0 = (A.heads[0] + fit - 1) / fit, groups = groups0 + (A.heads[1] + fit - 1) / fit;
     const int g0 = (int)((int64_t)groups * split / A.splits), g1 = (int)((int64_t)groups * (split + 1) / A.splits);
     const int64_t p = A.pos[row];
     const bool inside = p >= 0 && p < A.max_len;
@@ -58,79 +59,56 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs A) {
     if (sub >= fit) return;
     for (int it = first; it < items; it += 32) {
         const bool copied = it >= turns;
-        const int a0 = copied ? A.r + (it - turns) * kCopy : kInterleaved ? it * kNear : it * V;
-        float c[V], s[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) c[i] = s[i] = 0.f;
+        const int a0 = copied ? A.r + (it - turns) * V : kInterleaved ? it * kNear : it * V;
+        // the second value or word of a pair that is not side by side with the first
+        const int apart = copied ? 0 : kInterleaved ? (V > 1 ? 0 : 1) : half;
+        float c[kPairs], s[kPairs];
         if (inside && !copied) {
             const int64_t at = p * half + (kInterleaved ? a0 >> 1 : a0);
-            constexpr int kPairs = kInterleaved ? kNear / 2 : V;
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) {
                 c[i] = A.cos_t[at + i];
                 s[i] = A.inverse ? -A.sin_t[at + i] : A.sin_t[at + i];
             }
         }
-        for (int h0 = g0 * fit + sub; h0 < g1 * fit && h0 < total; h0 += kRopeHeads * fit) {
-            float u[kRopeHeads][kNear], w[kRopeHeads][V];
 #pragma unroll
-            for (int e = 0; e < kRopeHeads; ++e) {
-                const int h = h0 + e * fit;
-                if (h < g1 * fit && h < total) {
-                    const int which = h >= A.heads[0];
-                    const T* x = static_cast<const T*>(A.x[which]) + row * A.xr[which] +
-                                 (h - which * A.heads[0]) * A.xh[which] + a0;
-                    if (copied || !kInterleaved) {
-                        float t[V];
-                        load_v<T, V>(t, x);
+        for (int t = 0; t < 2; ++t) {
+            const int from = (t ? max(g0 - groups0, 0) : g0) * fit + sub;
+            const int to = min(A.heads[t], (t ? g1 - groups0 : min(g1, groups0)) * fit);
+            const T* x = static_cast<const T*>(A.x[t]) + row * A.xr[t] + a0;
+            T* y = static_cast<T*>(A.y[t]) + row * A.yr[t] + a0;
+            for (int h0 = from; h0 < to; h0 += kRopeHeads * fit) {
+                W u[kRopeHeads], w[kRopeHeads];
 #pragma unroll
-                        for (int i = 0; i < V; ++i) u[e][i] = t[i];
-                        if (!copied) load_v<T, V>(w[e], x + half);
-                    } else if (V > 1) {
-                        load_v<T, kNear>(u[e], x);
-                    } else {
-                        u[e][0] = to_f<T>(x[0]);
-                        u[e][1] = to_f<T>(x[1]);
-                    }
+                for (int e = 0; e < kRopeHeads; ++e) {
+                    const T* at = x + min(h0 + e * fit, to - 1) * A.xh[t];      // past the end: some head again
+                    u[e] = *reinterpret_cast<const W*>(at);
+                    if (apart) w[e] = *reinterpret_cast<const W*>(at + apart);
                 }
-            }
 #pragma unroll
-            for (int e = 0; e < kRopeHeads; ++e) {
-                const int h = h0 + e * fit;
-                if (h < g1 * fit && h < total) {
-                    const int which = h >= A.heads[0];
-                    T* y = static_cast<T*>(A.y[which]) + row * A.yr[which] +
-                           (h - which * A.heads[0]) * A.yh[which] + a0;
+                for (int e = 0; e < kRopeHeads; ++e) {
+                    const int h = h0 + e * fit;
+                    if (h >= to) break;
+                    T* at = y + h * A.yh[t];
                     if (!inside) {
+                        u[e] = W{};
+                        w[e] = W{};
+                    } else if (!copied) {
+                        float a[V], b[V];
+                        load_v<T, V>(a, reinterpret_cast<const T*>(&u[e]));
+                        if (apart) load_v<T, V>(b, reinterpret_cast<const T*>(&w[e]));
+                        if (!kInterleaved || V == 1) {
 #pragma unroll
-                        for (int i = 0; i < kNear; ++i) u[e][i] = 0.f;
-#pragma unroll
-                        for (int i = 0; i < V; ++i) w[e][i] = 0.f;
-                    }
-                    if (copied || !kInterleaved) {
-                        float t[V];
-#pragma unroll
-                        for (int i = 0; i < V; ++i) t[i] = u[e][i];
-                        if (!copied) {
-                            if (inside) {
-#pragma unroll
-                                for (int i = 0; i < V; ++i) turn(t[i], w[e][i], c[i], s[i]);
-                            }
-                            store_v<T, V>(y + half, w[e]);
-                        }
-                        store_v<T, V>(y, t);
-                    } else {
-                        if (inside) {
-#pragma unroll
-                            for (int i = 0; i < kNear / 2; ++i) turn(u[e][2 * i], u[e][2 * i + 1], c[i], s[i]);
-                        }
-                        if (V > 1) {
-                            store_v<T, kNear>(y, u[e]);
+                            for (int i = 0; i < V; ++i) turn(a[i], b[i], c[i], s[i]);
                         } else {
-                            y[0] = from_f<T>(u[e][0]);
-                            y[1] = from_f<T>(u[e][1]);
+#pragma unroll
+                            for (int i = 0; i < V / 2; ++i) turn(a[2 * i], a[2 * i + 1], c[i], s[i]);
                         }
+                        store_v<T, V>(reinterpret_cast<T*>(&u[e]), a);
+                        if (apart) store_v<T, V>(reinterpret_cast<T*>(&w[e]), b);
                     }
+                    *reinterpret_cast<W*>(at) = u[e];
+                    if (apart) *reinterpret_cast<W*>(at + apart) = w[e];
                 }
             }
         }
@@ -207,7 +185,8 @@ extern "C" int epq_rope(const epq_heads* x, const epq_heads* y, int32_t count, c
     const int v = fits(wide) ? wide : fits(2) ? 2 : 1;
     const int turns = interleaved ? rotary_dim / (v > 1 ? v : 2) : rotary_dim / 2 / v;
     const int items = turns + (head_dim - rotary_dim) / v;
-    const int64_t groups = items < 32 ? cdiv(heads, 32 / items) : heads;
+    const int fit = items < 32 ? 32 / items : 1;
+    const int64_t groups = cdiv(A.heads[0], fit) + cdiv(A.heads[1], fit);
     // A token's heads are shared out to several warps while there are too few tokens to
     // give every SM 16 warps.
     int64_t splits = cdiv((int64_t)device_sms() * 16, m);
