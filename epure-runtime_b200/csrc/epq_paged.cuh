@@ -227,6 +227,19 @@ __device__ __forceinline__ void mul2(float& r0, float& r1, float a0, float a1, f
         : "=f"(r0), "=f"(r1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
 
+// Two pairs (a_i, b_i) turned.
+__device__ __forceinline__ void turn2(float& a0, float& a1, float& b0, float& b1, float c0, float c1, float s0, float s1) {
+    float ac0, ac1, bs0, bs1, bc0, bc1, as0, as1;
+    mul2(ac0, ac1, a0, a1, c0, c1);
+    mul2(bs0, bs1, b0, b1, s0, s1);
+    mul2(bc0, bc1, b0, b1, c0, c1);
+    mul2(as0, as1, a0, a1, s0, s1);
+    a0 = __fsub_rn(ac0, bs0);
+    a1 = __fsub_rn(ac1, bs1);
+    b0 = __fadd_rn(bc0, as0);
+    b1 = __fadd_rn(bc1, as1);
+}
+
 // The device's side of epq_pages.
 struct PagesD {
     uint8_t* k;
