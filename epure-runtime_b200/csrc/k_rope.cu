@@ -212,7 +212,7 @@ extern "C" int epq_rope(const epq_heads* x, const epq_heads* y, int32_t count, c
     // Lanes a head: each has one item of it, or up to 4, where that leaves fewer of the
     // warp's lanes without work (20 items: 2 a lane of 3 heads at once, 60 of 64 places).
     double best = 0;
-    for (int n = 1; n <= 4 || (items + n - 1) / n > 32; ++n) {
+    for (int n = 1; n <= 4 || A.lanes == 0; ++n) {
         const int lanes = (items + n - 1) / n;
         if (lanes > 32) continue;
         const double used = (double)items * (32 / lanes) / (32.0 * n);
