@@ -6,7 +6,8 @@ Compiles every csrc/*.cu with nvcc into epure/libepq.so next to the Python
 package, so the library travels with the source tree.  Object files go to
 csrc/_build/.  A source is recompiled only when it or a header is newer than
 its object.  The CPU kernel (csrc_cpu/epq_cpu.cpp, include/epq_cpu.h) is built
-with g++/OpenMP into epure/libepq_cpu.so.
+with g++/OpenMP into epure/libepq_cpu.so, and the tensor binding of the paged calls
+(csrc_torch/epq_torch.cpp) against the installed torch into epure/_epq_torch.so.
 """
 import argparse
 import glob
@@ -20,6 +21,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "_build")
 OUT = os.path.join(HERE, "epure", "libepq.so")
 CPU_SRC = os.path.join(HERE, "csrc_cpu", "epq_cpu.cpp")
+TORCH_SRC = os.path.join(HERE, "csrc_torch", "epq_torch.cpp")
+TORCH_OUT = os.path.join(HERE, "epure", "_epq_torch.so")
 CPU_OUT = os.path.join(HERE, "epure", "libepq_cpu.so")
 INCLUDE = os.path.join(ROOT, "include")
 
@@ -62,6 +65,7 @@ def build(verbose_ptxas=False, force=False, quiet=False):
                *objs, "-o", OUT, "-lcudart_static", "-lrt", "-ldl", "-lpthread"]
         subprocess.check_call(cmd)
     build_cpu(force=force, quiet=quiet)
+    build_torch(force=force, quiet=quiet)
     return OUT
 
 
@@ -86,6 +90,32 @@ def build_cpu(force=False, quiet=False):
         print(" ".join(os.path.relpath(c, ROOT) if c.startswith(ROOT) else c for c in cmd), flush=True)
     subprocess.check_call(cmd)
     return CPU_OUT
+
+
+def build_torch(force=False, quiet=False):
+    """_epq_torch.so: a CPython module over torch's headers and libraries."""
+    headers = [os.path.join(INCLUDE, h) for h in ("epq.h", "epq_paged.h")]
+    newest = max(os.path.getmtime(f) for f in [TORCH_SRC, *headers])
+    if not force and os.path.exists(TORCH_OUT) and os.path.getmtime(TORCH_OUT) >= newest:
+        return TORCH_OUT
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
+    if not os.path.isdir(cuda):
+        cuda = "/usr/local/cuda/include"
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-I", INCLUDE, "-I", cuda, "-I", sysconfig.get_paths()["include"],
+           *[f for d in cpp_extension.include_paths() for f in ("-isystem", d)],
+           TORCH_SRC, "-o", TORCH_OUT, "-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           f"-Wl,-rpath,{lib}", "-ldl"]
+    if not quiet:
+        print(" ".join(os.path.relpath(c, ROOT) if c.startswith(ROOT) else c for c in cmd), flush=True)
+    subprocess.check_call(cmd)
+    return TORCH_OUT
 
 
 if __name__ == "__main__":

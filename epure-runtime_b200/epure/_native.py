@@ -591,199 +591,52 @@ class DecodeProgram:
 
 
 # -- rotary positions, the paged cache and its attention (include/epq_paged.h) ---------------
+# The calls of a batched decode step: module _epq_torch (csrc_torch/epq_torch.cpp) checks the
+# tensors and makes the C calls, because a call through ctypes costs more host time than the
+# kernels of a small step take.
 
-CACHE_SAME, CACHE_INT8, CACHE_FP8 = 0, 1, 2
-_CACHE_FORMATS = {torch.int8: CACHE_INT8, torch.float8_e4m3fn: CACHE_FP8,
-                  torch.bfloat16: CACHE_SAME, torch.float16: CACHE_SAME, torch.float32: CACHE_SAME}
-
-
-def _heads(t):
-    """The C ``epq_heads`` of a strided tensor [rows, heads, head_dim]."""
-    return EpqHeads(t.data_ptr(), t.stride(0), t.stride(1), t.shape[1], 0)
+_tensor_calls = None
 
 
-def _rows3(t, what, device, dtype, heads=None, head_dim=None, rows=None):
-    """Raises unless ``t`` is [rows, heads, head_dim] on the device, values of a head contiguous."""
-    if t.dim() != 3 or t.device != device or t.dtype != dtype:
-        raise RuntimeError(f"epure: {what} must be [rows, heads, head_dim], {dtype} on {device}; got "
-                           f"{tuple(t.shape)}, {t.dtype} on {t.device}")
-    if (heads is not None and t.shape[1] != heads) or (head_dim is not None and t.shape[2] != head_dim) or \
-            (rows is not None and t.shape[0] != rows):
-        raise RuntimeError(f"epure: {what} is {tuple(t.shape)}; expected "
-                           f"[{rows if rows is not None else 'rows'}, {heads if heads is not None else 'heads'}, "
-                           f"{head_dim if head_dim is not None else 'head_dim'}]")
-    if t.numel() and t.stride(2) != 1:
-        raise RuntimeError(f"epure: the values of a head of {what} must be contiguous (stride {t.stride(2)})")
+def _load_tensor_calls():
+    """The binding module, bound to the libepq.so of ``load_library``.  Raises if it is absent."""
+    global _tensor_calls
+    load_library()
+    with _lock:
+        if _tensor_calls is None:
+            try:
+                from . import _epq_torch
+            except ImportError as exc:
+                raise RuntimeError("epure: the tensor binding _epq_torch.so is not built or does not load here; run "
+                                   f"`python epure-runtime_b200/build_native.py` ({exc})") from exc
+            _epq_torch.bind(LIB_PATH, torch.OutOfMemoryError)
+            _tensor_calls = _epq_torch
+    return _tensor_calls
 
 
-def _index(t, what, device, dtype, n):
-    if t.dtype != dtype or t.device != device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise RuntimeError(f"epure: {what} must be {n} contiguous {dtype} on {device}; got {tuple(t.shape)}, "
-                           f"{t.dtype} on {t.device}")
+def rope(q, k, pos, cos, sin, interleaved=False, inverse=False, q_out=None, k_out=None):
+    """Turns q and k (or q alone: k None) [rows, heads, head_dim] by the positions ``pos`` [rows] in one launch
+    (epq_rope); ``inverse`` turns back, which is the gradient.  Returns (q', k') or q'."""
+    return (_tensor_calls or _load_tensor_calls()).rope(q, k, pos, cos, sin, interleaved, inverse, q_out, k_out)
 
 
-def _rotary_tables(cos, sin, device, head_dim):
-    """(max_len, rotary_dim) of a pair of rotary tables."""
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 or \
-            cos.device != device or sin.device != device or not cos.is_contiguous() or not sin.is_contiguous():
-        raise RuntimeError("epure: cos and sin must be contiguous float32 [max_len, rotary_dim / 2] tables on the "
-                           "tensors' device")
-    if not 1 <= cos.shape[1] <= head_dim // 2 or cos.shape[0] < 1:
-        raise RuntimeError(f"epure: rotary tables of {tuple(cos.shape)} for a head of {head_dim}")
-    return cos.shape[0], 2 * cos.shape[1]
+def paged_write(pages, k, v, seq, pos, q=None, q_out=None, cos=None, sin=None, interleaved=False, qk_norm=False,
+                eps=1e-6):
+    """Rows k, v [m, kv_heads, head_dim] into the cache ``pages`` (k, v, table, k_scale, v_scale) as tokens ``pos``
+    of sequences ``seq`` (epq_paged_write); returns the normed and rotated q, or None."""
+    return (_tensor_calls or _load_tensor_calls()).write(*pages, k, v, seq, pos, q, q_out, cos, sin, interleaved,
+                                                         qk_norm, eps)
 
 
-def rope(xs, pos, cos, sin, interleaved=False, inverse=False, outs=None):
-    """Turns every tensor of ``xs`` (one or two [rows, heads, head_dim]) by the positions ``pos`` [rows] in one
-    launch (epq_rope); ``inverse`` turns back, which is the gradient.  Returns the outputs (``outs`` may be
-    ``xs``: in place)."""
-    lib = load_library()
-    x0 = xs[0]
-    if not x0.is_cuda:
-        raise RuntimeError("epure: rope needs CUDA tensors")
-    if not 1 <= len(xs) <= 2 or (outs is not None and len(outs) != len(xs)):
-        raise RuntimeError(f"epure: rope takes one or two tensors and as many outputs (got {len(xs)})")
-    dev, dt, hd, m = x0.device, x0.dtype, x0.shape[-1], x0.shape[0]
-    code = dtype_code(dt)
-    if outs is None:
-        outs = [torch.empty(x.shape, dtype=dt, device=dev) for x in xs]
-    for x, y in zip(xs, outs):
-        _rows3(x, "a rope input", dev, dt, None, hd, m)
-        _rows3(y, "a rope output", dev, dt, x.shape[1], hd, m)
-    _index(pos, "pos", dev, torch.int64, m)
-    max_len, r = _rotary_tables(cos, sin, dev, hd)
-    n = len(xs)
-    ins = (EpqHeads * n)(*[_heads(x) for x in xs])
-    to = (EpqHeads * n)(*[_heads(y) for y in outs])
-    with torch.cuda.device(dev):
-        _check(lib.epq_rope(ins, to, n, pos.data_ptr(), m, hd, r, cos.data_ptr(), sin.data_ptr(), max_len,
-                            int(interleaved), int(inverse), code, _stream_ptr(dev)), "epq_rope")
-    return outs
+def paged_read(pages, seq, pos, dtype=None):
+    """(k, v) [rows, kv_heads, head_dim] of the cached tokens ``pos`` of sequences ``seq`` (epq_paged_read), in
+    ``dtype`` (default: the pool's own type, bfloat16 for 8-bit pools)."""
+    code = None if dtype is None else dtype_code(dtype)
+    return (_tensor_calls or _load_tensor_calls()).read(*pages, seq, pos, code)
 
 
-def describe_pages(k, v, table, k_scale=None, v_scale=None):
-    """The C ``epq_pages`` of pools k, v [pages, kv_heads, page_size, head_dim] (the last three dims contiguous),
-    scales [pages, kv_heads, page_size] (8-bit pools) and the int32 page table [seqs, max_pages]."""
-    try:
-        fmt = _CACHE_FORMATS[k.dtype]
-    except KeyError:
-        raise TypeError(f"epure: a cache of {k.dtype} is not supported") from None
-    dev = k.device
-    if not k.is_cuda:
-        raise RuntimeError("epure: the paged cache needs CUDA tensors")
-    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or v.device != dev or v.stride() != k.stride():
-        raise RuntimeError("epure: k and v must be alike, [pages, kv_heads, page_size, head_dim]")
-    _, kv, ps, hd = k.shape
-    if k.stride()[1:] != (ps * hd, hd, 1):
-        raise RuntimeError(f"epure: the heads, slots and values of a page must be contiguous (strides {k.stride()})")
-    if table.dim() != 2 or table.dtype != torch.int32 or table.device != dev or table.stride(1) != 1:
-        raise RuntimeError("epure: the page table must be int32 [seqs, max_pages] on the cache's device")
-    stride = 0
-    if fmt != CACHE_SAME:
-        if k_scale is None or v_scale is None:
-            raise RuntimeError("epure: an 8-bit cache needs k_scale and v_scale")
-        for s in (k_scale, v_scale):
-            if s.shape != k.shape[:3] or s.dtype != torch.float32 or s.device != dev or \
-                    s.stride()[1:] != (ps, 1) or s.stride(0) != k_scale.stride(0):
-                raise RuntimeError("epure: scales must be float32 [pages, kv_heads, page_size], pages contiguous")
-        stride = k_scale.stride(0)
-    elif k_scale is not None or v_scale is not None:
-        raise RuntimeError(f"epure: a cache of {k.dtype} has no scales")
-    return EpqPages(k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), k.stride(0), stride,
-                    table.stride(0), k.shape[0], table.shape[0], table.shape[1], ps, kv, hd, fmt)
-
-
-def paged_write(desc, cache_dtype, k, v, seq, pos, q=None, q_out=None, cos=None, sin=None, interleaved=False,
-                qk_norm=False, eps=1e-6):
-    """Rows k, v [m, kv_heads, head_dim] into the cache as tokens ``pos`` of sequences ``seq`` (epq_paged_write);
-    returns the normed and rotated q, or None."""
-    lib = load_library()
-    dev, dt, m, hd = k.device, k.dtype, k.shape[0], desc.head_dim
-    code = dtype_code(dt)
-    if desc.format == CACHE_SAME and cache_dtype != dt:
-        raise RuntimeError(f"epure: rows of {dt} for a cache of {cache_dtype}")
-    _rows3(k, "k", dev, dt, desc.kv_heads, hd, None)
-    _rows3(v, "v", dev, dt, desc.kv_heads, hd, m)
-    _index(seq, "seq", dev, torch.int32, m)
-    _index(pos, "pos", dev, torch.int64, m)
-    max_len, r = (0, 0) if cos is None else _rotary_tables(cos, sin, dev, hd)
-    qh = qo = None
-    if q is not None:
-        _rows3(q, "q", dev, dt, None, hd, m)
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=dt, device=dev)
-        _rows3(q_out, "q_out", dev, dt, q.shape[1], hd, m)
-        qh, qo = ctypes.byref(_heads(q)), ctypes.byref(_heads(q_out))
-    with torch.cuda.device(dev):
-        _check(lib.epq_paged_write(ctypes.byref(desc), qh, qo, ctypes.byref(_heads(k)), ctypes.byref(_heads(v)),
-                                   seq.data_ptr(), pos.data_ptr(), m, _ptr(cos), _ptr(sin), max_len, r,
-                                   int(interleaved), int(qk_norm), float(eps), code, _stream_ptr(dev)),
-               "epq_paged_write")
-    return q_out if q is not None else None
-
-
-def paged_read(desc, cache_dtype, device, seq, pos, dtype):
-    """(k, v) [rows, kv_heads, head_dim] of the cached tokens ``pos`` of sequences ``seq`` (epq_paged_read)."""
-    lib = load_library()
-    if desc.format == CACHE_SAME and cache_dtype != dtype:
-        raise RuntimeError(f"epure: a cache of {cache_dtype} is read as {cache_dtype}, not {dtype}")
-    m = pos.shape[0]
-    _index(seq, "seq", device, torch.int32, m)
-    _index(pos, "pos", device, torch.int64, m)
-    code = dtype_code(dtype)
-    k = torch.empty((m, desc.kv_heads, desc.head_dim), dtype=dtype, device=device)
-    v = torch.empty_like(k)
-    with torch.cuda.device(device):
-        _check(lib.epq_paged_read(ctypes.byref(desc), seq.data_ptr(), pos.data_ptr(), m, k.data_ptr(), v.data_ptr(),
-                                  code, _stream_ptr(device)), "epq_paged_read")
-    return k, v
-
-
-_attend_workspaces = {}
-
-
-def attend_workspace(device, stream_ptr, nbytes):
-    """The zeroed workspace of paged_attend for a stream, grown on demand."""
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream_ptr)
-    buf = _attend_workspaces.get(key)
-    if buf is None or buf.numel() < nbytes:
-        buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-        _attend_workspaces[key] = buf
-    return buf
-
-
-def paged_attend(desc, cache_dtype, q, lengths, seq=None, scale=None, window=0, out=None, return_lse=False):
+def paged_attend(pages, q, lengths, seq=None, scale=None, window=0, out=None, return_lse=False):
     """Attention of one new token a sequence (epq_paged_attend): q [batch, heads, head_dim] over the first
     ``lengths`` [batch] (int64) cached tokens of sequences ``seq`` (default 0..batch-1), the last ``window`` of
     them where window > 0.  Returns out, or (out, lse [batch, heads] float32)."""
-    lib = load_library()
-    dev, dt, hd = q.device, q.dtype, desc.head_dim
-    if dt not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"epure: paged attention takes float16 or bfloat16 queries, not {dt}")
-    if desc.format == CACHE_SAME and cache_dtype != dt:
-        raise RuntimeError(f"epure: queries of {dt} for a cache of {cache_dtype}")
-    _rows3(q, "q", dev, dt, None, hd, None)
-    B, H = q.shape[0], q.shape[1]
-    _index(lengths, "lengths", dev, torch.int64, B)
-    if seq is not None:
-        _index(seq, "seq", dev, torch.int32, B)
-    if (q.data_ptr() | 2 * q.stride(0) | 2 * q.stride(1)) % 4:
-        q = q.contiguous()
-        if q.data_ptr() % 4:
-            q = q.clone()
-    if out is None:
-        out = torch.empty((B, H, hd), dtype=dt, device=dev)
-    elif out.shape != (B, H, hd) or out.dtype != dt or out.device != dev or not out.is_contiguous():
-        raise RuntimeError(f"epure: out must be contiguous [{B}, {H}, {hd}], {dt} on {dev}")
-    lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
-    with torch.cuda.device(dev):
-        need = lib.epq_paged_attend_workspace_bytes(ctypes.byref(desc), B, H)
-        if need < 0:
-            _check(need, "epq_paged_attend_workspace_bytes")
-        stream = _stream_ptr(dev)
-        ws = attend_workspace(dev, stream, need)
-        _check(lib.epq_paged_attend(ctypes.byref(desc), ctypes.byref(_heads(q)), _ptr(seq), lengths.data_ptr(), B,
-                                    1.0 / hd ** 0.5 if scale is None else float(scale), int(window), out.data_ptr(),
-                                    _ptr(lse), dtype_code(dt), ws.data_ptr(), ws.numel(), stream),
-               "epq_paged_attend")
-    return (out, lse) if return_lse else out
+    return (_tensor_calls or _load_tensor_calls()).attend(*pages, q, lengths, seq, scale, window, out, return_lse)

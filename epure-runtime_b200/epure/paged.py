@@ -26,9 +26,6 @@ class KVPages(NamedTuple):
     k_scale: Optional[torch.Tensor] = None
     v_scale: Optional[torch.Tensor] = None
 
-    def describe(self):
-        return _native.describe_pages(self.k, self.v, self.table, self.k_scale, self.v_scale)
-
 
 def write(pages, k, v, seq, pos, q=None, q_out=None, cos=None, sin=None, interleaved=False, qk_norm=False, eps=1e-6):
     """Writes rows ``k``, ``v`` [m, kv_heads, head_dim] as tokens ``pos`` (int64 [m]) of sequences ``seq`` (int32
@@ -38,16 +35,13 @@ def write(pages, k, v, seq, pos, q=None, q_out=None, cos=None, sin=None, interle
     (epure.rotary) q and k are rotated by ``pos``.  Returns q so treated (``q_out``, a new tensor, or q itself
     given as q_out), or None without q.  A row with a negative position is padding.  No two rows may name the
     same token."""
-    return _native.paged_write(pages.describe(), pages.k.dtype, k, v, seq, pos, q, q_out, cos, sin, interleaved,
-                               qk_norm, eps)
+    return _native.paged_write(pages, k, v, seq, pos, q, q_out, cos, sin, interleaved, qk_norm, eps)
 
 
 def read(pages, seq, pos, dtype=None):
     """``(k, v)`` [m, kv_heads, head_dim] of cached tokens, in ``dtype`` (default: the pool's own type, bfloat16
     for 8-bit pools)."""
-    if dtype is None:
-        dtype = torch.bfloat16 if pages.k.dtype.itemsize == 1 else pages.k.dtype
-    return _native.paged_read(pages.describe(), pages.k.dtype, pages.k.device, seq, pos, dtype)
+    return _native.paged_read(pages, seq, pos, dtype)
 
 
 def attend(pages, q, lengths, seq=None, scale=None, window=0, out=None, return_lse=False):
@@ -56,7 +50,7 @@ def attend(pages, q, lengths, seq=None, scale=None, window=0, out=None, return_l
     ``scale`` defaults to head_dim ** -0.5.  Query head h reads key head h // (heads / kv_heads).  A length of 0
     gives zeros.  Returns out, or ``(out, lse)`` with the float32 log-sum-exp [batch, heads] of the scores
     (-inf for an empty row), with which results over disjoint sets of tokens can be joined."""
-    return _native.paged_attend(pages.describe(), pages.k.dtype, q, lengths, seq, scale, window, out, return_lse)
+    return _native.paged_attend(pages, q, lengths, seq, scale, window, out, return_lse)
 
 
 class PagedKVCache:

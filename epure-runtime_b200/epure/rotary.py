@@ -67,18 +67,20 @@ class _RopeFn(torch.autograd.Function):
     """The gradient of a rotation is the rotation back: dx = R^T dy."""
 
     @staticmethod
-    def forward(ctx, pos, cos, sin, interleaved, inverse, *xs):
+    def forward(ctx, pos, cos, sin, interleaved, inverse, q, k):
         ctx.save_for_backward(pos, cos, sin)
         ctx.how = (interleaved, inverse)
-        return tuple(_native.rope(xs, pos, cos, sin, interleaved, inverse))
+        return _native.rope(q, k, pos, cos, sin, interleaved, inverse)
 
     @staticmethod
-    def backward(ctx, *dys):
+    def backward(ctx, dq, dk=None):
         pos, cos, sin = ctx.saved_tensors
         interleaved, inverse = ctx.how
-        dys = [dy if dy.stride(-1) == 1 else dy.contiguous() for dy in dys]
-        dxs = _native.rope(dys, pos, cos, sin, interleaved, not inverse)
-        return (None,) * 5 + tuple(dxs)
+        dq = dq if dq.stride(-1) == 1 else dq.contiguous()
+        if dk is None:
+            return (None,) * 5 + (_native.rope(dq, None, pos, cos, sin, interleaved, not inverse), None)
+        dk = dk if dk.stride(-1) == 1 else dk.contiguous()
+        return (None,) * 5 + _native.rope(dq, dk, pos, cos, sin, interleaved, not inverse)
 
 
 def rope(q, k, pos, cos, sin, interleaved=False, inverse=False, out=None):
@@ -89,11 +91,9 @@ def rope(q, k, pos, cos, sin, interleaved=False, inverse=False, out=None):
     may be strided.  ``inverse`` turns back (for a gradient: ``dq, dk = rope(dy_q, dy_k, ..., inverse=True)``);
     autograd does so by itself.  ``out=(q_out, k_out)`` writes there, in place where they are q and k (no
     autograd).  Returns ``(q', k')``, or ``q'`` alone without k."""
-    xs = (q,) if k is None else (q, k)
     if out is not None:
-        got = _native.rope(xs, pos, cos, sin, interleaved, inverse, (out,) if k is None and torch.is_tensor(out) else out)
-    elif torch.is_grad_enabled() and any(x.requires_grad for x in xs):
-        got = _RopeFn.apply(pos, cos, sin, interleaved, inverse, *xs)
-    else:
-        got = _native.rope(xs, pos, cos, sin, interleaved, inverse)
-    return got[0] if k is None else (got[0], got[1])
+        q_out, k_out = out if k is not None else (out if torch.is_tensor(out) else out[0], None)
+        return _native.rope(q, k, pos, cos, sin, interleaved, inverse, q_out, k_out)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RopeFn.apply(pos, cos, sin, interleaved, inverse, q, k)
+    return _native.rope(q, k, pos, cos, sin, interleaved, inverse)
