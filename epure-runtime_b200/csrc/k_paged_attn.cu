@@ -116,13 +116,10 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+template <bool kIsBf16> struct Half { using type = __half; };
+template <> struct Half<true> { using type = __nv_bfloat16; };
 template <bool kIsBf16> __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    if (kIsBf16) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t*>(&v);
-    }
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
+    return pack2<typename Half<kIsBf16>::type>(lo, hi);
 }
 
 // The four 8-bit codes of x as two pairs of f16: its bytes (0, 1) and (2, 3), or with
@@ -641,7 +638,11 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                         for (int r = 0; r < 4; ++r) acc[n][d][r] *= turn_acc[r & 1];
                 }
             }
-            uint32_t pf[kTiles][kCols][2];
+            // 16-bit caches: a weight is the sum of two values of the type, since one rounding of it
+            // alone would be as large as the result's.  8-bit ones: f16 weights, whose rounding
+            // is an eighth of bf16's and the conversions are what their kernel is short of.
+            constexpr int kParts = kQuant ? 1 : 2;
+            uint32_t pf[kTiles][kCols][kParts][2];
 #pragma unroll
             for (int tile = 0; tile < kTiles; ++tile)
 #pragma unroll
@@ -653,8 +654,19 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                         l[n][r & 1] += w[r];
                         if (kQuant) w[r] = ex2(sc[tile][n][r] + (lv[tile][r >> 1] - M[n][r & 1]));
                     }
-                    pf[tile][n][0] = transpose8x8(pack<kIsBf16>(w[0], w[1]));
-                    pf[tile][n][1] = transpose8x8(pack<kIsBf16>(w[2], w[3]));
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const uint32_t two = pack<kIsBf16>(w[2 * r], w[2 * r + 1]);
+                            pf[tile][n][part][r] = transpose8x8(two);
+                            if (part + 1 < kParts) {
+                                const float2 back = unpack2<typename Half<kIsBf16>::type>(two);
+                                w[2 * r] -= back.x;
+                                w[2 * r + 1] -= back.y;
+                            }
+                        }
+                    }
                 }
             // O^T += V^T P^T
 #pragma unroll
@@ -667,7 +679,10 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                         const uint32_t (&v)[4] = y[tile][d];
                         if (!kQuant) {
 #pragma unroll
-                            for (int n = 0; n < kCols; ++n) mma<kIsBf16>(acc[n][d0 + d], v, pf[tile][n][0], pf[tile][n][1]);
+                            for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                                for (int part = 0; part < kParts; ++part)
+                                    mma<kIsBf16>(acc[n][d0 + d], v, pf[tile][n][part][0], pf[tile][n][part][1]);
                         } else {
 #pragma unroll
                             for (int r = 0; r < 2; ++r) {  // rows 0-7: the even dims of 16, rows 8-15: the odd ones
@@ -676,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                                 codes_f16<kKind, true>(v[2 * r + 1], a[2], a[3]);
 #pragma unroll
                                 for (int n = 0; n < kCols; ++n)
-                                    mma<false>(acc[n][2 * (d0 + d) + r], a, pf[tile][n][0], pf[tile][n][1]);
+                                    mma<false>(acc[n][2 * (d0 + d) + r], a, pf[tile][n][0][0], pf[tile][n][0][1]);
                             }
                         }
                     }
