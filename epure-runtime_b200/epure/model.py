@@ -36,6 +36,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _native
+from .rotary import rope
 from .synthetic import LinearStack
 
 _ROPE_THETA = {"qwen3-1.7b": 1.0e6, "llama3-8b": 5.0e5, "llama3-70b": 5.0e5}
@@ -346,13 +347,15 @@ class PackedCausalLM(torch.nn.Module):
     compressed-state backward (dX, dscale, dcb; dW never formed).
     ``linear_mode="reference"`` instead differentiates the reference's fallback
     ``F.linear(x, materialize(bf16))`` (runtime.py:78-89, 123-124) with torch
-    ops, the formulation the gradients are checked against.
+    ops, the formulation the gradients are checked against.  ``fused_rope=True``
+    rotates q and k by epure.rotary.rope, one launch forward and one backward with
+    the torch formulation's results bit for bit (GPU only).
 
     ``forward(input_ids [B, T], labels=None)`` returns an object with ``.loss``
     (labels default to the inputs, shifted by one inside), so ``ScaleTuner``
     can drive it."""
 
-    def __init__(self, decoder, linear_mode="ours"):
+    def __init__(self, decoder, linear_mode="ours", fused_rope=False):
         super().__init__()
         import types
         from .runtime import PackedLinear
@@ -361,6 +364,7 @@ class PackedCausalLM(torch.nn.Module):
         self._types = types
         self.shapes = decoder.shapes
         self.mode = linear_mode
+        self.fused_rope = fused_rope
         self.eps = decoder.eps
         self.qk_norm = decoder.qk_norm
         self.cos, self.sin = decoder.cos, decoder.sin
@@ -399,6 +403,7 @@ class PackedCausalLM(torch.nn.Module):
         if T > self.cos.shape[0]:
             raise ValueError(f"epure: sequence of {T} tokens exceeds the rotary table ({self.cos.shape[0]})")
         x = F.embedding(input_ids, self.embed_w)                              # [B, T, hidden] bf16
+        pos = torch.arange(T, device=x.device).repeat(B) if self.fused_rope else None
         for blk in self.layers:
             h = self._rms(x)
             q = self._lin(blk.q_proj, h).view(B, T, H, hd)
@@ -406,7 +411,11 @@ class PackedCausalLM(torch.nn.Module):
             v = self._lin(blk.v_proj, h).view(B, T, KV, hd)
             if self.qk_norm:
                 q, k = self._rms(q), self._rms(k)
-            q, k = self._rope(q), self._rope(k)
+            if self.fused_rope:
+                q, k = (t.view(B, T, -1, hd) for t in rope(q.view(B * T, H, hd), k.view(B * T, KV, hd), pos, self.cos,
+                                                           self.sin))
+            else:
+                q, k = self._rope(q), self._rope(k)
             att = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
                                                  is_causal=True, scale=1.0 / math.sqrt(hd), enable_gqa=True)
             att = att.transpose(1, 2).reshape(B, T, H * hd)
