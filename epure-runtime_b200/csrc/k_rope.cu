@@ -43,13 +43,20 @@ template <int N> __device__ __forceinline__ void load_table(float (&f)[N], const
 }
 
 constexpr int kRopeThreads = 128;
-constexpr int kRopeHeads = 2;   // heads of one lane in flight
+
+// Heads of one lane in flight: as many as keep about 64 bytes of it under way.  (Half
+// layout in bf16, 16384 tokens: 83 us with 1, 70 with 2 and 4; interleaved 77 with 2, 68
+// with 4; single values, 8192 tokens: 139 with 2, 105 with 4.)
+template <typename T, int V, bool kInterleaved> constexpr int rope_heads() {
+    return V <= 2 ? 8 : kInterleaved && sizeof(T) == 2 ? 4 : 2;
+}
 
 // V: values a load (V = 1: any alignment and size).  An item holds V pairs (half
 // layout) or max(V, 2) neighbouring values (interleaved), or is V copied values.
 template <typename T, int V, bool kInterleaved>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs A) {
     pdl_enter();
+    constexpr int kRopeHeads = rope_heads<T, V, kInterleaved>();
     constexpr int kNear = V > 1 ? V : 2;                    // values of an interleaved item
     constexpr int kPairs = kInterleaved ? kNear / 2 : V;
     using W = typename Word<V * (int)sizeof(T)>::type;
@@ -139,10 +146,22 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs A) {
     }
 }
 
-template <typename T, int V>
-int launch_rope_v(const RopeArgs& A, bool interleaved, unsigned blocks, cudaStream_t st) {
-    return interleaved ? launch(rope_kernel<T, V, true>, dim3(blocks), dim3(kRopeThreads), 0, st, "epq_rope", A)
-                       : launch(rope_kernel<T, V, false>, dim3(blocks), dim3(kRopeThreads), 0, st, "epq_rope", A);
+template <typename T, int V, bool kInterleaved>
+int launch_rope_l(RopeArgs A, cudaStream_t st) {
+    const int step = rope_heads<T, V, kInterleaved>() * (32 / A.lanes);
+    const int64_t passes = cdiv(A.heads[0], step) + cdiv(A.heads[1], step);
+    // A token's heads are shared out to several warps while there are too few tokens to
+    // give every SM 32 warps.
+    int64_t splits = cdiv((int64_t)device_sms() * 32, A.m);
+    if (splits > passes) splits = passes;
+    A.splits = (int)splits;
+    if (A.m * splits > (int64_t)1 << 30)
+        return set_error(EPQ_EUNSUPPORTED, "epq_rope: m=%lld rows", (long long)A.m);
+    const unsigned blocks = (unsigned)cdiv(A.m * splits * 32, kRopeThreads);
+    return launch(rope_kernel<T, V, kInterleaved>, dim3(blocks), dim3(kRopeThreads), 0, st, "epq_rope", A);
+}
+template <typename T, int V> int launch_rope_v(const RopeArgs& A, bool interleaved, cudaStream_t st) {
+    return interleaved ? launch_rope_l<T, V, true>(A, st) : launch_rope_l<T, V, false>(A, st);
 }
 
 }  // namespace
@@ -221,28 +240,19 @@ extern "C" int epq_rope(const epq_heads* x, const epq_heads* y, int32_t count, c
             A.lanes = lanes;
         }
     }
-    const int step = kRopeHeads * (32 / A.lanes);
-    const int64_t passes = cdiv(A.heads[0], step) + cdiv(A.heads[1], step);
     const int pairs = interleaved ? (v > 1 ? v / 2 : 1) : v;
     A.wide_table = ((uintptr_t)cos_tab | (uintptr_t)sin_tab) % 16 == 0 && rotary_dim / 2 % (pairs < 4 ? pairs : 4) == 0;
-    // A token's heads are shared out to several warps while there are too few tokens to
-    // give every SM 32 warps.
-    int64_t splits = cdiv((int64_t)device_sms() * 32, m);
-    if (splits > passes) splits = passes;
-    A.splits = (int)splits;
-    if (m * splits > (int64_t)1 << 30) return set_error(EPQ_EUNSUPPORTED, "epq_rope: m=%lld rows", (long long)m);
-    const unsigned blocks = (unsigned)cdiv(m * splits * 32, kRopeThreads);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool il = interleaved != 0;
     if (dtype == EPQ_F32) {
-        if (v == 4) return launch_rope_v<float, 4>(A, il, blocks, st);
-        return v == 2 ? launch_rope_v<float, 2>(A, il, blocks, st) : launch_rope_v<float, 1>(A, il, blocks, st);
+        if (v == 4) return launch_rope_v<float, 4>(A, il, st);
+        return v == 2 ? launch_rope_v<float, 2>(A, il, st) : launch_rope_v<float, 1>(A, il, st);
     }
     if (dtype == EPQ_F16) {
-        if (v == 8) return launch_rope_v<__half, 8>(A, il, blocks, st);
-        return v == 2 ? launch_rope_v<__half, 2>(A, il, blocks, st) : launch_rope_v<__half, 1>(A, il, blocks, st);
+        if (v == 8) return launch_rope_v<__half, 8>(A, il, st);
+        return v == 2 ? launch_rope_v<__half, 2>(A, il, st) : launch_rope_v<__half, 1>(A, il, st);
     }
-    if (v == 8) return launch_rope_v<__nv_bfloat16, 8>(A, il, blocks, st);
-    return v == 2 ? launch_rope_v<__nv_bfloat16, 2>(A, il, blocks, st)
-                  : launch_rope_v<__nv_bfloat16, 1>(A, il, blocks, st);
+    if (v == 8) return launch_rope_v<__nv_bfloat16, 8>(A, il, st);
+    return v == 2 ? launch_rope_v<__nv_bfloat16, 2>(A, il, st)
+                  : launch_rope_v<__nv_bfloat16, 1>(A, il, st);
 }
