@@ -370,9 +370,11 @@ int make_pages(const epq_pages* in, PagesD* d, const char* who) {
         return set_error(EPQ_EINVAL, "%s: format=%d", who, in->format);
     if (in->format != EPQ_CACHE_SAME && (!in->k_scale || !in->v_scale))
         return set_error(EPQ_EINVAL, "%s: an 8-bit cache needs k_scale and v_scale", who);
-    if ((int64_t)in->max_pages * in->page_size > INT32_MAX)
-        return set_error(EPQ_EUNSUPPORTED, "%s: %d pages of %d tokens a sequence", who, in->max_pages, in->page_size);
+    // positions and a page's rows are 32-bit in the kernels, with room for a block past the end
     const int64_t rows = (int64_t)in->kv_heads * in->page_size;
+    if ((int64_t)in->max_pages * in->page_size > INT32_MAX - 64 || rows > INT32_MAX - 64 || in->kv_heads > 65536)
+        return set_error(EPQ_EUNSUPPORTED, "%s: %d pages of %d tokens a sequence, %d kv heads", who, in->max_pages,
+                         in->page_size, in->kv_heads);
     if (in->page_stride < rows * in->head_dim || in->table_stride < in->max_pages ||
         (in->format != EPQ_CACHE_SAME && in->scale_stride < rows))
         return set_error(EPQ_ESHAPE, "%s: strides of pages (%lld), scales (%lld) or table (%lld) are too small", who,

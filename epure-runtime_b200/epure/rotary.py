@@ -74,13 +74,13 @@ class _RopeFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk=None):
+        # by rope() itself, so that a gradient's gradient is one too
         pos, cos, sin = ctx.saved_tensors
         interleaved, inverse = ctx.how
         dq = dq if dq.stride(-1) == 1 else dq.contiguous()
-        if dk is None:
-            return (None,) * 5 + (_native.rope(dq, None, pos, cos, sin, interleaved, not inverse), None)
-        dk = dk if dk.stride(-1) == 1 else dk.contiguous()
-        return (None,) * 5 + _native.rope(dq, dk, pos, cos, sin, interleaved, not inverse)
+        dk = dk if dk is None or dk.stride(-1) == 1 else dk.contiguous()
+        got = rope(dq, dk, pos, cos, sin, interleaved, not inverse)
+        return (None,) * 5 + ((got, None) if dk is None else got)
 
 
 def rope(q, k, pos, cos, sin, interleaved=False, inverse=False, out=None):

@@ -135,6 +135,22 @@ def test_gradient_of_one_used_output():
     assert not k.grad.any()
 
 
+@pytest.mark.parametrize("with_k", [True, False])
+def test_gradient_of_a_gradient(with_k):
+    """d/dq of w . (R^T R q) is R^T R w: two rotations, each with three float32 roundings of values below
+    3 max|w| (the gain of these tables is under 1.2), the first's error turned by the second."""
+    from epure import rotary
+    (q, k), pos, cos, sin = _inputs(5, 3, 2, 16, 8, torch.float32)
+    q = q.clone().requires_grad_(True)
+    y = rotary.rope(q, k if with_k else None, pos, cos, sin)
+    y = y[0] if with_k else y
+    (dq,) = torch.autograd.grad((y * y).sum() / 2, q, create_graph=True)        # R^T R q
+    w = torch.randn(q.shape, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV)
+    (d2,) = torch.autograd.grad((dq * w).sum(), q)                              # R^T R w
+    want = _exact(_exact(w, pos, cos, sin, False), pos, cos, -sin, False)
+    assert float((d2.double() - want).abs().max()) <= 3 * 2.0 ** -24 * 3 * float(w.abs().max()) * (1 + 2)
+
+
 def test_graph_replays_at_new_positions():
     from epure import rotary
     (q, k), pos, cos, sin = _inputs(16, 8, 2, 64, 64, torch.bfloat16, fused=False)

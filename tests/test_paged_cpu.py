@@ -95,7 +95,8 @@ def _heads(heads=2, **kw):
 
 BAD_PAGES = [("k", None, -1), ("kv_heads", 0, -1), ("page_size", 0, -1), ("pages", 0, -1), ("head_dim", 24, -8),
              ("head_dim", 512, -8), ("format", 3, -1), ("format", 1, -1), ("page_stride", 64, -2),
-             ("table_stride", 3, -2), ("k", 4104, -4), ("max_pages", 2 ** 28, -8), ("table", None, -1)]
+             ("table_stride", 3, -2), ("k", 4104, -4), ("max_pages", 2 ** 28, -8), ("table", None, -1),
+             ("kv_heads", 70000, -8)]
 
 
 @pytest.mark.parametrize("field,value,code", BAD_PAGES)
