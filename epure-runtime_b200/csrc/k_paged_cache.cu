@@ -77,10 +77,16 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv, float sc
 
 constexpr int kAtOnce = 2;          // rows of a lane in flight
 
-// kGeneral: any alignment and any turn; else 16-byte loads and stores, and a turn (if any)
-// whose partners are whole lanes.
-template <typename T, int kFormat, int kLanes, bool kGeneral>
-__global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A) {
+// What a kernel takes for granted.  kExact: heads fill their lanes and passes, the whole
+// head turns (or none of it); kLanesOnly: partners are whole lanes; both: 16-byte loads
+// and stores.  kAny: nothing.
+enum Class { kExact = 0, kLanesOnly = 1, kAny = 2 };
+
+// Registers for 7 CTAs (28 warps) an SM: 64k rows of 48 heads took 376 us (with their
+// reading back) at the 88 registers that the compiler would use, 340 at 72, 337 at 64.
+template <typename T, int kFormat, int kLanes, int kClass>
+__global__ void __launch_bounds__(kCacheThreads, sizeof(T) == 2 && kClass != kAny ? 7 : 1)
+    write_kernel(const WriteArgs A) {
     pdl_enter();
     constexpr unsigned kAll = 0xffffffffu;
     constexpr int kFit = 32 / kLanes, kStep = kFit * kAtOnce;      // heads of a warp side by side, and a pass
@@ -89,10 +95,10 @@ __global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A)
     if (row >= A.m) return;
     const int split = warp - (int)row * A.splits;
     const PagesD& P = A.pages;
-    const int hd = P.head_dim, KV = P.kv_heads;
+    const int hd = kClass == kExact ? kLanes * 8 : P.head_dim, KV = P.kv_heads;
     const int sub = lane / kLanes, chunk = lane & (kLanes - 1), e0 = chunk * 8;
-    const bool in_row = e0 < hd;
-    const bool aligned = !kGeneral || A.aligned, out_aligned = !kGeneral || A.out_aligned;
+    const bool in_row = kClass == kExact || e0 < hd;
+    const bool aligned = kClass != kAny || A.aligned, out_aligned = kClass != kAny || A.out_aligned;
 
     // A pass is kStep heads of q, k or v; this warp's are [p0, p1).  A pass's rows are
     // fetched while the one before it (first: the token's place) is worked on.  Lanes past
@@ -103,7 +109,10 @@ __global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A)
     auto fetch = [&](const Rows& src, int heads, int h0) {
         const T* const from = static_cast<const T*>(src.p) + row * src.row + (in_row ? e0 : 0);
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) next[i].load(from + min(h0 + sub + i * kFit, heads - 1) * src.head, aligned);
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int h = h0 + sub + i * kFit;
+            next[i].load(from + (kClass == kExact ? h : min(h, heads - 1)) * src.head, aligned);
+        }
     };
     auto fetch_pass = [&](int p) {
         if (p < of_q) fetch(A.q, A.heads, p * kStep);
@@ -124,17 +133,25 @@ __global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A)
         }
         if (bad && lane == 0) atomicOr(&g_cache_error, bad);
     }
+    T* const q_to = static_cast<T*>(A.q_out) + row * A.qo_row + e0;
+    if (!live) {                                       // a padding row's q is zero
+        for (int h = p0 * kStep + sub; h < min(p1 * kStep, A.heads); h += kFit) {
+            Eight<T> zero;
+            zero.clear();
+            if (in_row) zero.store(q_to + h * A.qo_head, out_aligned);
+        }
+        return;
+    }
 
     // cos and the signed sin of this lane's 8 values: y = x c + partner s.
     float c[8], s[8];
     int partner = lane;                                // kHalfLanes: the lane that holds the other halves
-    const bool turned = A.turn != kNoTurn && live;
-    if (turned) {
+    if (A.turn != kNoTurn) {
         const int half = A.r >> 1;
-        if (!kGeneral || A.turn == kHalfLanes) {
+        if (kClass != kAny || A.turn == kHalfLanes) {
             const int part = half >> 3;
             const bool second = chunk >= part;
-            if (e0 < A.r) {
+            if (kClass == kExact || e0 < A.r) {
                 partner = second ? lane - part : lane + part;
                 const int64_t at = pos * half + (second ? e0 - half : e0);
                 load_v<float, 8>(c, A.cos_t + at);
@@ -157,6 +174,8 @@ __global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A)
             }
         }
     }
+    const int64_t cached = page * P.page_stride + (int64_t)slot * hd + e0, scaled = page * P.scale_stride + slot;
+    const int64_t head_step = (int64_t)P.page_size * hd;
 
     // Works on the pass's rows x: heads h0 + sub, h0 + sub + kFit, ... of q (kWhich = 0), k (1) or v (2)
     auto work = [&](auto which, int h0, Eight<T> (&x)[kAtOnce]) {
@@ -165,8 +184,8 @@ __global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A)
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
             const int h = h0 + sub + i * kFit;
-            const bool on = in_row && h < heads;
-            if (!in_row) x[i].clear();
+            const bool on = kClass == kExact || (in_row && h < heads);
+            if (kClass != kExact && !in_row) x[i].clear();
             if (kWhich < 2) {
                 float f[8], gain = 1.f;
                 if (A.qk_norm) {                       // RMSNorm of the head, rounded to T
@@ -181,12 +200,12 @@ __global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A)
                     for (int j = 0; j < 8; ++j) f[j] *= gain;
                     x[i].set(f);
                 }
-                if (turned) {
+                if (A.turn != kNoTurn) {
                     float other[8];
                     x[i].get(f);
-                    if (!kGeneral || A.turn == kHalfLanes) {
+                    if (kClass != kAny || A.turn == kHalfLanes) {
                         x[i].from_lane(partner).get(other);
-                        if (e0 < A.r) {                // (rotary_dim is a multiple of 16: all 8 or none)
+                        if (kClass == kExact || e0 < A.r) {        // (rotary_dim is a multiple of 16: all 8 or none)
 #pragma unroll
                             for (int j = 0; j < 8; j += 2) {
                                 mul2(f[j], f[j + 1], f[j], f[j + 1], c[j], c[j + 1]);
@@ -222,25 +241,22 @@ __global__ void __launch_bounds__(kCacheThreads) write_kernel(const WriteArgs A)
                 }
             }
             if (kWhich == 0) {
-                if (on) {
-                    if (!live) x[i].clear();           // a padding row's q is zero
-                    x[i].store(static_cast<T*>(A.q_out) + row * A.qo_row + h * A.qo_head + e0, out_aligned);
-                }
+                if (on) x[i].store(q_to + h * A.qo_head, out_aligned);
             } else {
-                const int64_t slot_at = (int64_t)h * P.page_size + slot;
                 uint8_t* const pool = kWhich == 1 ? P.k : P.v;
+                const int64_t at = cached + h * head_step;
                 if (kFormat == EPQ_CACHE_SAME) {
-                    if (on && live) x[i].store(reinterpret_cast<T*>(pool) + page * P.page_stride + slot_at * hd + e0, true);
+                    if (on) x[i].store(reinterpret_cast<T*>(pool) + at, true);
                 } else {
                     const float a = x[i].template largest<kLanes>();
                     // (a row that is not finite reads back as NaN, whatever its codes are)
                     const float scale = a < INFINITY ? __fmul_rn(a, 1.f / kTop<kFormat>) : NAN;
                     const float inv = a > 0.f ? __fdiv_rn(kTop<kFormat>, a) : 0.f;
-                    if (on && live) {
+                    if (on) {
                         float f[8];
                         x[i].get(f);
-                        *reinterpret_cast<uint2*>(pool + page * P.page_stride + slot_at * hd + e0) = codes8<kFormat>(f, inv, scale);
-                        if (chunk == 0) (kWhich == 1 ? P.k_scale : P.v_scale)[page * P.scale_stride + slot_at] = scale;
+                        *reinterpret_cast<uint2*>(pool + at) = codes8<kFormat>(f, inv, scale);
+                        if (chunk == 0) (kWhich == 1 ? P.k_scale : P.v_scale)[scaled + (int64_t)h * P.page_size] = scale;
                     }
                 }
             }
@@ -320,18 +336,23 @@ __global__ void __launch_bounds__(kCacheThreads) read_kernel(const ReadArgs A) {
     }
 }
 
-template <typename T, int kFormat, bool kGeneral>
-int launch_write_g(const WriteArgs& A, unsigned blocks, cudaStream_t st) {
+template <typename T, int kFormat, int kLanes>
+int launch_write_l(const WriteArgs& A, unsigned blocks, cudaStream_t st) {
+    constexpr int kStep = 32 / kLanes * kAtOnce;
     const int hd = A.pages.head_dim;
+    const bool plain = A.aligned && (A.heads == 0 || A.out_aligned) && (A.turn == kNoTurn || A.turn == kHalfLanes);
+    const bool exact = plain && hd == kLanes * 8 && A.heads % kStep == 0 && A.pages.kv_heads % kStep == 0 &&
+                       (A.turn == kNoTurn || A.r == hd);
     const char* who = "epq_paged_write";
-    if (hd <= 64) return launch(write_kernel<T, kFormat, 8, kGeneral>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
-    if (hd <= 128) return launch(write_kernel<T, kFormat, 16, kGeneral>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
-    return launch(write_kernel<T, kFormat, 32, kGeneral>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+    if (exact) return launch(write_kernel<T, kFormat, kLanes, kExact>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+    if (plain) return launch(write_kernel<T, kFormat, kLanes, kLanesOnly>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
+    return launch(write_kernel<T, kFormat, kLanes, kAny>, dim3(blocks), dim3(kCacheThreads), 0, st, who, A);
 }
 template <typename T, int kFormat>
 int launch_write(const WriteArgs& A, unsigned blocks, cudaStream_t st) {
-    const bool plain = A.aligned && (A.heads == 0 || A.out_aligned) && (A.turn == kNoTurn || A.turn == kHalfLanes);
-    return plain ? launch_write_g<T, kFormat, false>(A, blocks, st) : launch_write_g<T, kFormat, true>(A, blocks, st);
+    const int hd = A.pages.head_dim;
+    if (hd <= 64) return launch_write_l<T, kFormat, 8>(A, blocks, st);
+    return hd <= 128 ? launch_write_l<T, kFormat, 16>(A, blocks, st) : launch_write_l<T, kFormat, 32>(A, blocks, st);
 }
 template <typename T>
 int launch_write_t(const WriteArgs& A, unsigned blocks, cudaStream_t st) {
