@@ -110,7 +110,7 @@ def build_torch(force=False, quiet=False):
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            "-I", INCLUDE, "-I", cuda, "-I", sysconfig.get_paths()["include"],
            *[f for d in cpp_extension.include_paths() for f in ("-isystem", d)],
-           TORCH_SRC, "-o", TORCH_OUT, "-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           TORCH_SRC, "-o", TORCH_OUT, "-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
            f"-Wl,-rpath,{lib}", "-ldl"]
     if not quiet:
         print(" ".join(os.path.relpath(c, ROOT) if c.startswith(ROOT) else c for c in cmd), flush=True)

@@ -11,6 +11,7 @@
 #include <dlfcn.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -185,7 +186,8 @@ struct OnDevice {
 cudaStream_t stream_of(const at::Device& dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
 Tensor empty(at::IntArrayRef sizes, at::ScalarType dtype, const at::Device& dev) {
-    return at::empty(sizes, at::TensorOptions().dtype(dtype).device(dev));
+    // at::empty's own function for CUDA: outputs need no dispatch (about 0.4 us each)
+    return at::detail::empty_cuda(sizes, dtype, dev, std::nullopt);
 }
 
 PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
