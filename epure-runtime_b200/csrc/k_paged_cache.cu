@@ -317,17 +317,24 @@ __global__ void __launch_bounds__(kCacheThreads) read_kernel(const ReadArgs A) {
                 const float scale = (is_v ? P.v_scale : P.k_scale)[page * P.scale_stride + slot_at];
                 const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t b = u[i >> 2] >> (8 * (i & 3)) & 0xffu;
-                    float code;
+                for (int i = 0; i < 4; ++i) {
+                    float(&g)[8] = f[i >> 1];
+                    const int j = 4 * (i & 1);
                     if (kFormat == EPQ_CACHE_INT8) {
-                        // 2^23 + (b ^ 0x80) as bits, less 2^23 + 128
-                        code = __uint_as_float(0x4b000000u | (b ^ 0x80u)) - 8388736.f;
+                        // a byte b = code + 128 below 2^23 as bits, less 2^23 + 128
+                        const uint32_t v = u[i] ^ 0x80808080u;
+                        g[j] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7650)) - 8388736.f;
+                        g[j + 1] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7651)) - 8388736.f;
+                        g[j + 2] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7652)) - 8388736.f;
+                        g[j + 3] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7653)) - 8388736.f;
                     } else {
-                        const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3);
-                        code = __half2float(__half(h));
+                        const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u[i] & 0xffffu), __NV_E4M3);
+                        const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u[i] >> 16), __NV_E4M3);
+                        const float2 a = __half22float2(__half2(lo)), b = __half22float2(__half2(hi));
+                        g[j] = a.x, g[j + 1] = a.y, g[j + 2] = b.x, g[j + 3] = b.y;
                     }
-                    f[i >> 3][i & 7] = code * scale;
+                    mul2(g[j], g[j + 1], g[j], g[j + 1], scale, scale);
+                    mul2(g[j + 2], g[j + 3], g[j + 2], g[j + 3], scale, scale);
                 }
             }
         }
