@@ -6,20 +6,27 @@
 // The work is to keep enough loads in flight on every SM, whatever the lengths are.
 //
 // Split.  A unit is (sequence, key head, up to 8 or 16 of its query heads); its tokens
-// are cut into blocks of 16.  The blocks of all units, in order, are dealt out to the
-// CTAs in equal runs, so ragged lengths load every SM alike; a unit that a run's ends
-// cut is joined from (maximum, sum, accumulator) records by the last of its CTAs to
-// finish, in the order of the CTAs, which keeps results independent of timing.  Within
-// a CTA warp w takes the blocks w, w + 4, ... of the run; each warp has its own ring of
+// are cut into blocks of 16 or 32.  The blocks of all units, in order, are dealt out to
+// the CTAs in equal runs, each unit counting for its own cost too, so ragged lengths load
+// every SM alike; where there are few units each CTA takes one piece of one instead.  A
+// unit that is cut is joined from (m, M, l, accumulator) records by the last of its CTAs
+// to finish, in the order of the CTAs, so results do not depend on timing.  Within a CTA
+// warp w takes the blocks w, w + 4, ... of the run; each warp has its own ring of
 // shared-memory stages filled by 16-byte asynchronous copies that run ahead over unit
-// boundaries.
+// boundaries, 64 to 130 KB in flight an SM.
 //
-// Mathematics of a block: S^T = K Q^T as m16n8k16 products with the 16 tokens as rows
-// and the query heads as the 8 columns, so a group of up to 8 heads fills the tile (with
+// Mathematics of a block: S^T = K Q^T as m16n8k16 products with 16 tokens as rows and
+// the query heads as the 8 columns, so a group of up to 8 heads fills the tile (with
 // heads as rows half of it or more would be padding); O^T = V^T P^T likewise, with the
-// head's dims as rows.  At one column of 8 heads tcgen05's 128-row tiles would be
-// 15/16 padding, and the tensor pipe is not what limits this kernel.  The running
-// maximum moves only when a score passes it by 2^8; sums are float32.
+// head's dims as rows.  tcgen05's tiles have 128 rows and at most 8 columns would be
+// used; the tensor pipe is not what limits this kernel.  The running maximum moves only
+// when a score passes it by 2^8; sums are float32.
+//
+// Measured (B200, device time in a graph of calls): 1 x 131072 tokens, 32 / 8 heads of
+// 128, bf16: 90 us, 5.9 TB/s (92% of the measured copy rate); 64 sequences of up to 8192,
+// 64 / 8 heads, e4m3: 98 us, 5.8 TB/s; 16 of up to 4096, 32 / 8 heads, int8: 21 us, of
+// which 3 are the plan and first loads and 4 the last joins; 1 x 145: 6.5 us, a chain of
+// five dependent memory accesses and one join of warps.
 //
 // 8-bit caches: codes are converted to f16 (exact: int8 and e4m3 fit its 11 bits); a
 // head's q is brought to f16 by a power of two (exact but for values below 2^-38 of the

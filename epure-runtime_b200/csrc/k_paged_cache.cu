@@ -9,7 +9,14 @@
 //
 // Split: one warp takes (a share of) one token's rows -- q heads, k heads, v heads --
 // with 8 values a lane, so a row is 8, 16 or 32 lanes, its maximum and sum of squares a
-// few shuffles, and the token's page, cos and sin are found once.
+// few shuffles, and the token's page, cos and sin are found once.  16-bit rows stay
+// packed two values a word for loads, shuffles and the maximum, and products go two an
+// instruction: at 110 instructions a row of 128 the kernel is as near to its issue rate
+// as to HBM's.
+//
+// Measured (B200): 65536 tokens of 32 + 8 + 8 heads of 128, bf16 to int8, rotated and
+// written: 265 us (1.48 GB, 5.6 TB/s, 87% of the measured copy rate); read back: 75 us
+// (0.41 GB, 5.4 TB/s).  16 tokens: 2.8 us and 2.1 us, the chain position, page, row.
 #include "epq_paged.cuh"
 
 namespace epq {

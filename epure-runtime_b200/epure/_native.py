@@ -4,7 +4,8 @@ This is the only module that touches the native library.  It turns torch
 tensors into the plain pointers and sizes of the C ABI, owns the per-stream
 workspaces the batch-1 kernel needs, and raises ``RuntimeError`` with the
 library's own message whenever a call returns a non-zero status.  There is no
-fallback: if the library is missing, every GPU call raises.
+fallback: if the library is missing, every GPU call raises.  The calls of
+include/epq_paged.h go through the binding module ``_epq_torch`` instead of ctypes.
 """
 import ctypes
 import os
