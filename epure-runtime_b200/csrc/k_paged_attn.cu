@@ -259,22 +259,26 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         return v;
     };
     const int first_blocks = b0 < b1 ? span_of<kTok>(A, b0, blockIdx.x == 0).blocks : 0;
-    int mine = weight(first_blocks);
-    for (int b = b0 + 1; b < b1; ++b) mine += weight(span_of<kTok>(A, b, blockIdx.x == 0).blocks);
-    const int upto = scan(mine);
-    const int64_t total = (int64_t)__shfl_sync(kAll, upto, 31) * units;
+    int mine = weight(first_blocks), some_empty = b0 < b1 && first_blocks == 0;
+    for (int b = b0 + 1; b < b1; ++b) {
+        const int blocks = span_of<kTok>(A, b, blockIdx.x == 0).blocks;
+        mine += weight(blocks);
+        some_empty |= blocks == 0;
+    }
+    const int64_t total = (int64_t)__reduce_add_sync(kAll, mine) * units;
     const int run = max(kMinBlocks, (int)quotient(total + gridDim.x - 1, gridDim.x));
     // Where cutting every long unit into pieces of at most `run` blocks makes no more pieces
     // than there are CTAs, each CTA takes one piece; else runs go over unit boundaries.
     auto pieces_of = [&](int blocks) { return blocks > kWhole ? (blocks + run - 1) / run : blocks > 0; };
     int pieces = pieces_of(first_blocks);
     for (int b = b0 + 1; b < b1; ++b) pieces += pieces_of(span_of<kTok>(A, b, false).blocks);
-    const int pieces_upto = scan(pieces);
-    const int64_t all_pieces = (int64_t)__shfl_sync(kAll, pieces_upto, 31) * units;
+    const int64_t all_pieces = (int64_t)__reduce_add_sync(kAll, pieces) * units;
     const bool one_each = all_pieces <= gridDim.x;
+    const int share = one_each ? pieces : mine, upto = scan(share);    // of the lane's sequences, and up to them
     const int64_t f0 = one_each ? blockIdx.x : blockIdx.x * (int64_t)run;    // piece, or place in the dealt-out order
     // sequences without a token
-    for (int b = blockIdx.x; b < A.batch; b += gridDim.x) {
+    some_empty = __any_sync(kAll, some_empty);
+    for (int b = blockIdx.x; some_empty && b < A.batch; b += gridDim.x) {
         if (span_of<kTok>(A, b, false).blocks) continue;
         for (int e = tid; e < A.heads * hd; e += kThreads)
             static_cast<uint16_t*>(A.out)[(int64_t)b * A.heads * hd + e] = 0;
@@ -285,8 +289,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     Cursor<kTok> unit;                                 // of the unit that the CTA is at
     unit.units = units;
     {
-        const int64_t lo = (int64_t)(one_each ? pieces_upto - pieces : upto - mine) * units;
-        const int64_t hi = (int64_t)(one_each ? pieces_upto : upto) * units;
+        const int64_t lo = (int64_t)(upto - share) * units, hi = (int64_t)upto * units;
         const bool here = f0 >= lo && f0 < hi;
         int at_b = 0, at_u = 0, at_i = 0;
         if (here) {
@@ -366,6 +369,27 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         ahead.advance(A, warp);
         look_up();
     }
+    const int g = lane >> 2, c = lane & 3;             // row and column pair of the tensor fragments
+    // q as B fragments: column g is the unit's query head 8 n + g.  16-bit caches: dims 2c, 2c+1
+    // and 2c+8, 2c+9 of every 16; 8-bit ones: 4c .. 4c+3
+    uint32_t qf[kCols][kDim / 16][2];
+    auto load_q = [&](const Cursor<kTok>& u) {
+        const int head = A.chunks == 1 ? u.u : u.u / A.chunks, chunk = u.u - head * A.chunks;
+        const int h0 = head * A.group + chunk * 8 * kCols, n_heads = min(8 * kCols, A.group - chunk * 8 * kCols);
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+            const bool on = 8 * n + g < n_heads;
+            const uint16_t* q = static_cast<const uint16_t*>(A.q) + u.b * A.q_row + (h0 + 8 * n + g) * A.q_head;
+#pragma unroll
+            for (int k = 0; k < kDim / 16; ++k) {
+                const int d0 = 16 * k + (kQuant ? 4 * c : 2 * c), d1 = d0 + (kQuant ? 2 : 8);
+                const bool there = on && 16 * k < hd;
+                qf[n][k][0] = there ? *reinterpret_cast<const uint32_t*>(q + d0) : 0u;
+                qf[n][k][1] = there ? *reinterpret_cast<const uint32_t*>(q + d1) : 0u;
+            }
+        }
+    };
+    load_q(unit);                                      // (on its way with the first table entry)
     constexpr int kChunks = S::kPitch / 16;            // of a row
     constexpr int kCopies = kTile * kChunks / 32;      // chunks a lane and tile
     const int my_row = lane / kChunks, my_ch = lane % kChunks;     // a lane's chunks: rows my_row, my_row + 32 / kChunks, ...
@@ -434,27 +458,6 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     for (int e = 0; e < S::kStages - 1; ++e) load();
 
     // ---- units
-    const int g = lane >> 2, c = lane & 3;             // row and column pair of the tensor fragments
-    // q as B fragments: column g is the unit's query head 8 n + g.  16-bit caches: dims 2c, 2c+1
-    // and 2c+8, 2c+9 of every 16; 8-bit ones: 4c .. 4c+3
-    uint32_t qf[kCols][kDim / 16][2];
-    auto load_q = [&](const Cursor<kTok>& u) {
-        const int head = A.chunks == 1 ? u.u : u.u / A.chunks, chunk = u.u - head * A.chunks;
-        const int h0 = head * A.group + chunk * 8 * kCols, n_heads = min(8 * kCols, A.group - chunk * 8 * kCols);
-#pragma unroll
-        for (int n = 0; n < kCols; ++n) {
-            const bool on = 8 * n + g < n_heads;
-            const uint16_t* q = static_cast<const uint16_t*>(A.q) + u.b * A.q_row + (h0 + 8 * n + g) * A.q_head;
-#pragma unroll
-            for (int k = 0; k < kDim / 16; ++k) {
-                const int d0 = 16 * k + (kQuant ? 4 * c : 2 * c), d1 = d0 + (kQuant ? 2 : 8);
-                const bool there = on && 16 * k < hd;
-                qf[n][k][0] = there ? *reinterpret_cast<const uint32_t*>(q + d0) : 0u;
-                qf[n][k][1] = there ? *reinterpret_cast<const uint32_t*>(q + d1) : 0u;
-            }
-        }
-    };
-    load_q(unit);
     int f = warp, stage = 0;
     for (int at = 0; at < count;) {
         const int unit_start = at - unit.i, unit_end = unit_start + unit.s.blocks;   // unit_start < 0: begun before this run

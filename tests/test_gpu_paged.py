@@ -197,6 +197,28 @@ def test_not_finite_tiny_and_large_rows():
             assert float((k[i].double() - x[i].double()).abs().max()) <= float(step * 1.001 + 2.0 ** -149 * TOP[fmt] * 1.5)
 
 
+@pytest.mark.parametrize("fmt", ["same", "int8"])
+def test_pools_side_by_side_and_a_wider_table(fmt):
+    """Keys and values as the two halves of one pool's pages (a page stride of two), and a table that is a part of
+    a wider one."""
+    from epure import paged
+    lengths = [37, 90]
+    plain = _pages(lengths, 2, 64, 16, fmt, torch.bfloat16)
+    both = torch.stack((plain.k.view(torch.int8), plain.v.view(torch.int8)), 1).view(plain.k.dtype)
+    scales = (None, None) if fmt == "same" else torch.stack((plain.k_scale, plain.v_scale), 1).unbind(1)
+    wide = torch.full((2, 40), 10 ** 6, dtype=torch.int32, device=DEV)
+    wide[:, 3:3 + plain.table.shape[1]] = plain.table
+    pages = paged.KVPages(both[:, 0], both[:, 1], wide[:, 3:3 + plain.table.shape[1]], *scales)
+    assert pages.k.stride(0) == 2 * 2 * 16 * 64
+    got = _fill(pages, lengths, torch.bfloat16)
+    want = _fill(plain, lengths, torch.bfloat16)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q = torch.randn(2, 8, 64, generator=_gen(23), device=DEV).to(torch.bfloat16)
+    n = torch.tensor(lengths, device=DEV)
+    assert torch.equal(paged.attend(pages, q, n), paged.attend(plain, q, n))
+    _check(pages, q, lengths, *got)
+
+
 def test_unaligned_rows():
     from epure import paged
     pages = _pages([6], 2, 32, 16, "same", torch.bfloat16)
