@@ -183,11 +183,16 @@ template <int kTok> struct Cursor {
     int b, u, i, units;
     Span s;
     __device__ __forceinline__ void next_sequence(const AttendArgs& A) {
+        u = 0;
         do {
+            if (b + 1 >= A.batch) {                    // never, unless lengths change under the kernel: nothing more is read
+                s.n = 0;
+                s.blocks = 1 << 28;
+                return;
+            }
             ++b;
             s = span_of<kTok>(A, b, false);
         } while (s.blocks == 0);
-        u = 0;
     }
     // Moves on by `step` blocks; the caller knows that they exist.
     __device__ __forceinline__ void advance(const AttendArgs& A, int step) {
@@ -294,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         int at_b = 0, at_u = 0, at_i = 0;
         if (here) {
             int64_t at = f0 - lo;
-            for (int b = b0;; ++b) {
+            for (int b = b0; b < b1; ++b) {
                 const int blocks = b == b0 ? first_blocks : span_of<kTok>(A, b, false).blocks;
                 const int each = one_each ? pieces_of(blocks) : weight(blocks);
                 if (at < (int64_t)each * units) {
