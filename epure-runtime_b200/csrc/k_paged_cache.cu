@@ -129,11 +129,45 @@ __global__ void __launch_bounds__(kCacheThreads, sizeof(T) == 2 && kClass != kAn
     if (p0 < p1) fetch_pass(p0);
 
     const int64_t pos = A.pos[row];
+    const int seq = A.seq[row];
+    // cos and the signed sin of this lane's 8 values, y = x c + partner s, on their way with
+    // the page's number (of some position of the table, where the row's is outside it)
+    float c[8], s[8];
+    int partner = lane;                                // kHalfLanes: the lane that holds the other halves
+    if (A.turn != kNoTurn) {
+        const int half = A.r >> 1;
+        const int64_t at_row = (pos < 0 ? 0 : pos < A.max_len ? pos : A.max_len - 1) * half;
+        if (kClass != kAny || A.turn == kHalfLanes) {
+            const int part = half >> 3;
+            const bool second = chunk >= part;
+            if (kClass == kExact || e0 < A.r) {
+                partner = second ? lane - part : lane + part;
+                const int64_t at = at_row + (second ? e0 - half : e0);
+                load_v<float, 8>(c, A.cos_t + at);
+                load_v<float, 8>(s, A.sin_t + at);
+                if (!second) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s[i] = -s[i];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = e0 + i;
+                if (e < A.r) {
+                    const bool second = A.turn == kNeighbours ? e & 1 : e >= half;
+                    const int64_t at = at_row + (A.turn == kNeighbours ? e >> 1 : second ? e - half : e);
+                    c[i] = A.cos_t[at];
+                    s[i] = second ? A.sin_t[at] : -A.sin_t[at];
+                }
+            }
+        }
+    }
     int64_t page = 0;
     int slot = 0, bad = 0;
     bool live = pos >= 0;
     if (live) {
-        live = find_slot(P, A.seq[row], pos, &page, &slot, &bad);
+        live = find_slot(P, seq, pos, &page, &slot, &bad);
         if (live && A.turn != kNoTurn && pos >= A.max_len) {
             live = false;
             bad = kBadPosition;
@@ -150,37 +184,6 @@ __global__ void __launch_bounds__(kCacheThreads, sizeof(T) == 2 && kClass != kAn
         return;
     }
 
-    // cos and the signed sin of this lane's 8 values: y = x c + partner s.
-    float c[8], s[8];
-    int partner = lane;                                // kHalfLanes: the lane that holds the other halves
-    if (A.turn != kNoTurn) {
-        const int half = A.r >> 1;
-        if (kClass != kAny || A.turn == kHalfLanes) {
-            const int part = half >> 3;
-            const bool second = chunk >= part;
-            if (kClass == kExact || e0 < A.r) {
-                partner = second ? lane - part : lane + part;
-                const int64_t at = pos * half + (second ? e0 - half : e0);
-                load_v<float, 8>(c, A.cos_t + at);
-                load_v<float, 8>(s, A.sin_t + at);
-                if (!second) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) s[i] = -s[i];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int e = e0 + i;
-                if (e < A.r) {
-                    const bool second = A.turn == kNeighbours ? e & 1 : e >= half;
-                    const int64_t at = pos * half + (A.turn == kNeighbours ? e >> 1 : second ? e - half : e);
-                    c[i] = A.cos_t[at];
-                    s[i] = second ? A.sin_t[at] : -A.sin_t[at];
-                }
-            }
-        }
-    }
     const int64_t cached = page * P.page_stride + (int64_t)slot * hd + e0, scaled = page * P.scale_stride + slot;
     const int64_t head_step = (int64_t)P.page_size * hd;
 
