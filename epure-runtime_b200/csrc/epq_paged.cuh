@@ -249,6 +249,12 @@ struct PagesD {
     const int32_t* table;
     int64_t page_stride, scale_stride, table_stride, pages;
     int seqs, max_pages, page_size, kv_heads, head_dim, format;
+    uint32_t page_mul, page_shift;
+
+    // t / page_size for 0 <= t < 2^31 as a product (the constants: make_pages)
+    __device__ __forceinline__ int page_of(int t) const {
+        return (int)((__umulhi((uint32_t)t, page_mul) + (uint32_t)t) >> page_shift);
+    }
 };
 
 // Page and slot of token `pos` of sequence `s`, or false with *bad set.
@@ -258,7 +264,7 @@ __device__ __forceinline__ bool find_slot(const PagesD& p, int s, int64_t pos, i
         return false;
     }
     const int t = (int)pos;                       // max_pages * page_size < 2^31 (checked on the host)
-    const int col = t / p.page_size;
+    const int col = p.page_of(t);
     const int64_t pg = p.table[s * p.table_stride + col];
     if (pg < 0 || pg >= p.pages) {
         *bad = kBadPage;

@@ -68,7 +68,6 @@ struct AttendArgs {
     unsigned* counters;
     int64_t window;
     int batch, heads, group, chunks, dtype;
-    uint32_t page_mul, page_shift;         // t / page_size = (mulhi(t, page_mul) + t) >> page_shift
     float scale_log2;
 };
 
@@ -364,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         const int t = ahead.s.first + ahead.i * kTok + (lane & (kTok - 1));
         next_on = t >= ahead.s.lo && t < ahead.s.n;
         if (next_on) {
-            const int col = (int)((__umulhi((uint32_t)t, A.page_mul) + (uint32_t)t) >> A.page_shift);
+            const int col = P.page_of(t);
             const int s = A.seq ? A.seq[ahead.b] : ahead.b;
             next_slot = t - col * P.page_size;
             next_page = P.table[(int64_t)s * P.table_stride + col];
@@ -968,9 +967,6 @@ int epq_paged_attend(const epq_pages* pages, const epq_heads* q, const int32_t* 
     A.heads = q->heads;
     A.dtype = dtype;
     A.scale_log2 = scale * kLog2e;
-    // division by page_size as a product: exact for all t < 2^31
-    while ((1u << A.page_shift) < (uint32_t)A.pages.page_size) ++A.page_shift;
-    A.page_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << A.page_shift) - A.pages.page_size)) / A.pages.page_size + 1);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (A.pages.format) {
         case EPQ_CACHE_INT8: return launch_attend_k<kInt8>(A, cols, st);

@@ -434,6 +434,10 @@ int make_pages(const epq_pages* in, PagesD* d, const char* who) {
     d->kv_heads = in->kv_heads;
     d->head_dim = in->head_dim;
     d->format = in->format;
+    // t / page_size = (mulhi(t, page_mul) + t) >> page_shift, exact for all t < 2^31
+    d->page_shift = 0;
+    while ((1u << d->page_shift) < (uint32_t)in->page_size) ++d->page_shift;
+    d->page_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << d->page_shift) - in->page_size)) / in->page_size + 1);
     return EPQ_OK;
 }
 
