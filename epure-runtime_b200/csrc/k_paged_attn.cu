@@ -23,9 +23,9 @@
 // when a score passes it by 2^8; sums are float32.
 //
 // Measured (B200, device time in a graph of calls): 1 x 131072 tokens, 32 / 8 heads of
-// 128, bf16: 90 us, 5.9 TB/s (92% of the measured copy rate); 64 sequences of up to 8192,
-// 64 / 8 heads, e4m3: 98 us, 5.8 TB/s; 16 of up to 4096, 32 / 8 heads, int8: 21 us, of
-// which 3 are the plan and first loads and 4 the last joins; 1 x 145: 6.5 us, a chain of
+// 128, bf16: 90 us, 6.0 TB/s (93% of the measured copy rate); 64 sequences of up to 8192,
+// 64 / 8 heads, e4m3: 98 us, 5.8 TB/s; 16 of up to 4096, 32 / 8 heads, int8: 20 us, of
+// which 3 are the plan and first loads and 4 the last joins; 1 x 145: 6.4 us, a chain of
 // five dependent memory accesses and one join of warps.
 //
 // 8-bit caches: codes are converted to f16 (exact: int8 and e4m3 fit its 11 bits); a

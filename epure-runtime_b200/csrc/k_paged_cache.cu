@@ -15,8 +15,8 @@
 // as to HBM's.
 //
 // Measured (B200): 65536 tokens of 32 + 8 + 8 heads of 128, bf16 to int8, rotated and
-// written: 265 us (1.48 GB, 5.6 TB/s, 87% of the measured copy rate); read back: 75 us
-// (0.41 GB, 5.4 TB/s).  16 tokens: 2.8 us and 2.1 us, the chain position, page, row.
+// written: 258 us (1.48 GB, 5.7 TB/s, 89% of the measured copy rate); read back: 75 us
+// (0.41 GB, 5.4 TB/s).  16 tokens: 2.6 us and 2.0 us, the chain position, page, row.
 #include "epq_paged.cuh"
 
 namespace epq {
