@@ -11,7 +11,7 @@
 // visits, so its cos / sin stay in registers and the table is read once a token.  The
 // rows of the next heads are fetched while the last ones are turned, the first while the
 // position and the table are on their way: 16384 tokens of 24 heads in bf16, forward and
-// gradient, take 71 us (404 MB, 88% of the copy rate; 94 us without fetching ahead).
+// gradient, take 70 us (404 MB, 89% of the copy rate; 94 us without fetching ahead).
 #include "epq_paged.cuh"
 
 namespace epq {

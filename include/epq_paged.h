@@ -47,8 +47,9 @@ int epq_rope(const epq_heads* x, const epq_heads* y, int32_t count, const int64_
 
 /* How a cache holds its values: in the activations' type, or as one 8-bit code a
  * value with one float32 scale a token and head (value = code * scale):
- *   INT8  scale = max|x| / 127, code = x * (127 / max|x|) rounded to even
- *   FP8   scale = max|x| / 448, code = x * (448 / max|x|) rounded to e4m3
+ *   INT8  scale = max|x| * (1 / 127), code = x * (127 / max|x|) rounded to even
+ *   FP8   scale = max|x| * (1 / 448), code = x * (448 / max|x|) rounded to e4m3
+ * (every operation in float32, rounded by itself).
  * A row of zeros has scale 0; a row that holds an infinity or NaN reads back as NaN. */
 enum epq_cache_format { EPQ_CACHE_SAME = 0, EPQ_CACHE_INT8 = 1, EPQ_CACHE_FP8 = 2 };
 
