@@ -14,6 +14,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -289,14 +290,15 @@ PyObject* write(PyObject* const* a) {
     return wrap(y);
 }
 
-// read(k_pool, v_pool, table, k_scale, v_scale, seq, pos, dtype code | None)
+// read(k_pool, v_pool, table, k_scale, v_scale, seq, pos, dtype | None)
 PyObject* read(PyObject* const* a) {
     const Cache c = cache_of(a);
     at::ScalarType dt = c.p.format == EPQ_CACHE_SAME ? c.dtype : at::kBFloat16;
     if (a[7] != Py_None) {
-        const int64_t code = integer(a[7]);
-        dt = code == EPQ_F32 ? at::kFloat : code == EPQ_F16 ? at::kHalf : at::kBFloat16;
+        if (!THPDtype_Check(a[7])) throw TypeProblem("epure: dtype must be a torch.dtype");
+        dt = reinterpret_cast<THPDtype*>(a[7])->scalar_type;
     }
+    const int code = dtype_code(dt);
     if (c.p.format == EPQ_CACHE_SAME && c.dtype != dt) refuse("a cache of ", c.dtype, " is read as ", c.dtype, ", not ", dt);
     OnDevice on(c.device);
     const Tensor& pos = tensor(a[6], "pos");
@@ -305,7 +307,7 @@ PyObject* read(PyObject* const* a) {
     const Tensor& seq = index_of(tensor(a[5], "seq"), "seq", c.device, at::kInt, m);
     const Tensor k = empty({m, c.p.kv_heads, c.p.head_dim}, dt, c.device), v = empty({m, c.p.kv_heads, c.p.head_dim}, dt, c.device);
     check(lib.read(&c.p, seq.const_data_ptr<int32_t>(), pos.const_data_ptr<int64_t>(), m, k.data_ptr(), v.data_ptr(),
-                   dtype_code(dt), stream_of(c.device)),
+                   code, stream_of(c.device)),
           "epq_paged_read");
     return wrap2(k, v);
 }

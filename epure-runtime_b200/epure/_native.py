@@ -594,50 +594,22 @@ class DecodeProgram:
 # -- rotary positions, the paged cache and its attention (include/epq_paged.h) ---------------
 # The calls of a batched decode step: module _epq_torch (csrc_torch/epq_torch.cpp) checks the
 # tensors and makes the C calls, because a call through ctypes costs more host time than the
-# kernels of a small step take.
+# kernels of a small step take.  epure.rotary and epure.paged are its callers.
 
-_tensor_calls = None
+tensor_calls = None
 
 
-def _load_tensor_calls():
+def load_tensor_calls():
     """The binding module, bound to the libepq.so of ``load_library``.  Raises if it is absent."""
-    global _tensor_calls
+    global tensor_calls
     load_library()
     with _lock:
-        if _tensor_calls is None:
+        if tensor_calls is None:
             try:
                 from . import _epq_torch
             except ImportError as exc:
                 raise RuntimeError("epure: the tensor binding _epq_torch.so is not built or does not load here; run "
                                    f"`python epure-runtime_b200/build_native.py` ({exc})") from exc
             _epq_torch.bind(LIB_PATH, torch.OutOfMemoryError)
-            _tensor_calls = _epq_torch
-    return _tensor_calls
-
-
-def rope(q, k, pos, cos, sin, interleaved=False, inverse=False, q_out=None, k_out=None):
-    """Turns q and k (or q alone: k None) [rows, heads, head_dim] by the positions ``pos`` [rows] in one launch
-    (epq_rope); ``inverse`` turns back, which is the gradient.  Returns (q', k') or q'."""
-    return (_tensor_calls or _load_tensor_calls()).rope(q, k, pos, cos, sin, interleaved, inverse, q_out, k_out)
-
-
-def paged_write(pages, k, v, seq, pos, q=None, q_out=None, cos=None, sin=None, interleaved=False, qk_norm=False,
-                eps=1e-6):
-    """Rows k, v [m, kv_heads, head_dim] into the cache ``pages`` (k, v, table, k_scale, v_scale) as tokens ``pos``
-    of sequences ``seq`` (epq_paged_write); returns the normed and rotated q, or None."""
-    return (_tensor_calls or _load_tensor_calls()).write(*pages, k, v, seq, pos, q, q_out, cos, sin, interleaved,
-                                                         qk_norm, eps)
-
-
-def paged_read(pages, seq, pos, dtype=None):
-    """(k, v) [rows, kv_heads, head_dim] of the cached tokens ``pos`` of sequences ``seq`` (epq_paged_read), in
-    ``dtype`` (default: the pool's own type, bfloat16 for 8-bit pools)."""
-    code = None if dtype is None else dtype_code(dtype)
-    return (_tensor_calls or _load_tensor_calls()).read(*pages, seq, pos, code)
-
-
-def paged_attend(pages, q, lengths, seq=None, scale=None, window=0, out=None, return_lse=False):
-    """Attention of one new token a sequence (epq_paged_attend): q [batch, heads, head_dim] over the first
-    ``lengths`` [batch] (int64) cached tokens of sequences ``seq`` (default 0..batch-1), the last ``window`` of
-    them where window > 0.  Returns out, or (out, lse [batch, heads] float32)."""
-    return (_tensor_calls or _load_tensor_calls()).attend(*pages, q, lengths, seq, scale, window, out, return_lse)
+            tensor_calls = _epq_torch
+    return tensor_calls

@@ -35,13 +35,14 @@ def write(pages, k, v, seq, pos, q=None, q_out=None, cos=None, sin=None, interle
     (epure.rotary) q and k are rotated by ``pos``.  Returns q so treated (``q_out``, a new tensor, or q itself
     given as q_out), or None without q.  A row with a negative position is padding.  No two rows may name the
     same token."""
-    return _native.paged_write(pages, k, v, seq, pos, q, q_out, cos, sin, interleaved, qk_norm, eps)
+    return (_native.tensor_calls or _native.load_tensor_calls()).write(*pages, k, v, seq, pos, q, q_out, cos, sin,
+                                                                       interleaved, qk_norm, eps)
 
 
 def read(pages, seq, pos, dtype=None):
     """``(k, v)`` [m, kv_heads, head_dim] of cached tokens, in ``dtype`` (default: the pool's own type, bfloat16
     for 8-bit pools)."""
-    return _native.paged_read(pages, seq, pos, dtype)
+    return (_native.tensor_calls or _native.load_tensor_calls()).read(*pages, seq, pos, dtype)
 
 
 def attend(pages, q, lengths, seq=None, scale=None, window=0, out=None, return_lse=False):
@@ -50,7 +51,8 @@ def attend(pages, q, lengths, seq=None, scale=None, window=0, out=None, return_l
     ``scale`` defaults to head_dim ** -0.5.  Query head h reads key head h // (heads / kv_heads).  A length of 0
     gives zeros.  Returns out, or ``(out, lse)`` with the float32 log-sum-exp [batch, heads] of the scores
     (-inf for an empty row), with which results over disjoint sets of tokens can be joined."""
-    return _native.paged_attend(pages, q, lengths, seq, scale, window, out, return_lse)
+    return (_native.tensor_calls or _native.load_tensor_calls()).attend(*pages, q, lengths, seq, scale, window, out,
+                                                                        return_lse)
 
 
 class PagedKVCache:

@@ -63,6 +63,10 @@ def rope_tables(rotary_dim, max_len, device="cuda", **kw):
     return (gain * angle.cos()).float(), (gain * angle.sin()).float()
 
 
+def _calls():
+    return _native.tensor_calls or _native.load_tensor_calls()
+
+
 class _RopeFn(torch.autograd.Function):
     """The gradient of a rotation is the rotation back: dx = R^T dy."""
 
@@ -70,7 +74,7 @@ class _RopeFn(torch.autograd.Function):
     def forward(ctx, pos, cos, sin, interleaved, inverse, q, k):
         ctx.save_for_backward(pos, cos, sin)
         ctx.how = (interleaved, inverse)
-        return _native.rope(q, k, pos, cos, sin, interleaved, inverse)
+        return _calls().rope(q, k, pos, cos, sin, interleaved, inverse, None, None)
 
     @staticmethod
     def backward(ctx, dq, dk=None):
@@ -93,7 +97,7 @@ def rope(q, k, pos, cos, sin, interleaved=False, inverse=False, out=None):
     autograd).  Returns ``(q', k')``, or ``q'`` alone without k."""
     if out is not None:
         q_out, k_out = out if k is not None else (out if torch.is_tensor(out) else out[0], None)
-        return _native.rope(q, k, pos, cos, sin, interleaved, inverse, q_out, k_out)
+        return _calls().rope(q, k, pos, cos, sin, interleaved, inverse, q_out, k_out)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RopeFn.apply(pos, cos, sin, interleaved, inverse, q, k)
-    return _native.rope(q, k, pos, cos, sin, interleaved, inverse)
+    return _calls().rope(q, k, pos, cos, sin, interleaved, inverse, None, None)
