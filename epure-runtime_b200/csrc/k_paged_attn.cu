@@ -29,8 +29,8 @@
 // five dependent memory accesses and one join of warps.
 //
 // 8-bit caches: codes are converted to f16 (exact: int8 and e4m3 fit its 11 bits); a
-// head's q is brought to f16 by a power of two (exact but for values below 2^-38 of the
-// largest); the key's scale multiplies the score, and the value's scale enters the
+// head's q is brought to f16 by a power of two (f16 queries and bf16 values down to 2^-31 of
+// the largest exactly, smaller ones to 2^-39 of the largest's power of two); the key's scale multiplies the score, and the value's scale enters the
 // weight as 2^(s + log2 scale - M) with a running maximum M of its own, so that neither
 // large nor small scales leave f16's range.
 #include <cfloat>
@@ -54,6 +54,9 @@ constexpr int kUnitCost = 12;
 constexpr int kMaxUnits = 65536;           // counters in the workspace
 constexpr int kMaxGrid = 512;              // CTAs of a launch
 constexpr float kSlack = 8.f;              // how far (log2) a score may pass the running maximum
+// Weights in f16 are 2^kLift of those that the maximum stands for, which is as high as f16
+// goes (2^(8 + 7)): what is below 2^-32 of the maximum is lost, not what is below 2^-25.
+constexpr float kLift = 7.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendArgs {
@@ -238,6 +241,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     constexpr bool kQuant = kKind >= kInt8;
     constexpr bool kIsBf16 = kKind == kBf16;
     constexpr int kTok = S::kTok, kTiles = S::kTiles;
+    constexpr float kSumLift = kKind == kF16 ? kLift : 0.f;      // 8-bit caches lift the values' weights alone
     constexpr unsigned kAll = 0xffffffffu;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t seen[kWarps][S::kStages];     // bit r: row r of the stage is a token of the span
@@ -664,9 +668,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
                     float w[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        w[r] = ex2(sc[tile][n][r] - m[n][r & 1]);
+                        w[r] = ex2(sc[tile][n][r] - (m[n][r & 1] - kSumLift));
                         l[n][r & 1] += w[r];
-                        if (kQuant) w[r] = ex2(sc[tile][n][r] + (lv[tile][r >> 1] - M[n][r & 1]));
+                        if (kQuant) w[r] = ex2(sc[tile][n][r] + (lv[tile][r >> 1] - (M[n][r & 1] - kLift)));
                     }
 #pragma unroll
                     for (int part = 0; part < kParts; ++part) {
@@ -725,9 +729,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         float* const merge = reinterpret_cast<float*>(smem + kWarps * S::kRing);
         constexpr int kQuads = kDim / 4;               // of a head's dims
         auto emit = [&](int h, int d, const float (&val)[4], float mx, float Mx, float sum) {
-            // sum = 0: every score was -inf.  2^(M - m) is 1 for 16-bit caches.
+            // sum = 0: every score was -inf.  16-bit caches: M = m, and sum is lifted as the weights are.
             float gain = sum == 0.f ? 0.f : 1.f / sum;
-            if (kQuant) gain *= ex2(Mx - mx);
+            if (kQuant) gain *= ex2(Mx - kLift - mx);
             uint2 o;
             if (A.dtype == EPQ_BF16) {
                 o = make_uint2(pack<true>(val[0] * gain, val[1] * gain), pack<true>(val[2] * gain, val[3] * gain));
@@ -736,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
             }
             const int64_t to = (int64_t)seq_b * A.heads + h_first + h;
             *reinterpret_cast<uint2*>(static_cast<uint16_t*>(A.out) + to * hd + d) = o;
-            if (A.lse && d == 0) A.lse[to] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
+            if (A.lse && d == 0) A.lse[to] = sum == 0.f ? -INFINITY : (mx - kSumLift + log2f(sum)) / kLog2e;
         };
         // none where the unit is whole; else where the piece's record goes
         float* const record = !cut ? nullptr
