@@ -35,3 +35,30 @@ def test_many_small_weights_beside_a_peak(fmt, dtype, n, peak):
     assert float((out[..., 1].double() - want).abs().max()) <= bound
     assert float((out[..., 0].double() - 64 / total).abs().max()) <= 64 * (UNIT[dtype] + 2.0 ** -11)
     assert float((lse.double() - 17.5 - math.log(total)).abs().max()) <= 2.0 ** -18
+
+
+@pytest.mark.parametrize("fmt", ["same", "int8", "fp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_weights_are_held_in_two_parts(fmt, dtype):
+    """Values of +-1 whose weighted sums cancel: one rounding of a weight to 16 bits would show.
+
+    Bounds: a weight is two values of the tensor cores' type, so it is off by its unit roundoff squared (bf16 for
+    bf16 caches, else f16); twice its score's error (numerator and sum) and 2^-18 of exp2, log2 and the sums; all
+    of the weighted |v|; the result's rounding (2^-25: f16's smallest step)."""
+    from epure import paged
+    lengths = [5 + i % 8 for i in range(64)]
+    pages = _pages(lengths, 1, 16, 16, fmt, dtype)
+    seq, pos = _tokens(lengths)
+    g = _gen(31)
+    k = (torch.rand(len(pos), 1, 16, generator=g, device=DEV) - 0.5).to(dtype)
+    v = (torch.randint(0, 2, (len(pos), 1, 16), generator=g, device=DEV) * 2 - 1).to(dtype)
+    paged.write(pages, k, v, seq, pos)
+    if fmt != "same":
+        k, v = paged.read(pages, seq, pos, torch.float32)
+    q = torch.randn(64, 8, 16, generator=g, device=DEV).to(dtype)
+    out = paged.attend(pages, q, torch.tensor(lengths, device=DEV))
+    want, _, mag, err = _reference(q, k.double(), v.double(), lengths, 0, 0.25)
+    unit = UNIT[dtype if fmt == "same" else torch.float16]
+    bound = UNIT[dtype] * want.abs() + (unit ** 2 + 2 * err[..., None] + 2.0 ** -18) * 1.01 * mag + 2.0 ** -25
+    off = (out.double() - want).abs()
+    assert bool((off <= bound).all()), (float((off / bound).max()), int((off > bound).sum()))
