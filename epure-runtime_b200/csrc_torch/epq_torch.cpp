@@ -12,12 +12,14 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <map>
 #include <sstream>
 #include <stdexcept>
@@ -90,6 +92,23 @@ int dtype_code(at::ScalarType t) {
     if (t == at::kHalf) return EPQ_F16;
     if (t == at::kBFloat16) return EPQ_BF16;
     throw TypeProblem(text("dtype ", t, " is not supported by the CUDA kernels"));
+}
+
+// These calls record nothing for autograd: a tensor whose derivative they would drop is refused, as torch's own
+// out= functions refuse it.  (rope's gradient is _RopeFn's, whose calls come without grad mode.)
+struct Named {
+    const Tensor* t;
+    const char* name;
+};
+void no_gradient(const char* call, std::initializer_list<Named> tensors) {
+    const bool grads = c10::GradMode::is_enabled();
+    for (const Named& n : tensors) {
+        if (!n.t) continue;
+        if (grads && n.t->requires_grad())
+            refuse(n.name, " requires a gradient, which ", call, " does not pass on; detach it or call under torch.no_grad()");
+        if (n.t->_fw_grad(0).defined())
+            refuse(n.name, " has a forward-mode tangent, which ", call, " does not pass on");
+    }
 }
 
 // A strided tensor [rows, heads, head_dim]; negative sizes are not checked.
@@ -236,6 +255,8 @@ PyObject* rope(PyObject* const* a) {
     const Tensor* k = maybe(a[1], "k");
     const Tensor *qo = maybe(a[7], "q_out"), *ko = maybe(a[8], "k_out");
     if (!q.is_cuda()) refuse("rope needs CUDA tensors");
+    no_gradient(qo || ko ? "rope with out" : "rope", {{&q, "q"}, {k, "k"}, {&tensor(a[3], "cos"), "cos"}, {&tensor(a[4], "sin"), "sin"},
+                                                      {qo, "out"}, {ko, "out"}});
     if (q.dim() != 3) refuse("a rope input must be [rows, heads, head_dim]; got ", q.sizes());
     const at::Device dev = q.device();
     const at::ScalarType dt = q.scalar_type();
@@ -264,6 +285,8 @@ PyObject* write(PyObject* const* a) {
     const Cache c = cache_of(a);
     const Tensor &k = tensor(a[5], "k"), &v = tensor(a[6], "v");
     const Tensor *q = maybe(a[9], "q"), *qo = maybe(a[10], "q_out"), *cs = maybe(a[11], "cos"), *sn = maybe(a[12], "sin");
+    no_gradient("write", {{&tensor(a[0], "k"), "the k pool"}, {&tensor(a[1], "v"), "the v pool"}, {maybe(a[3], "k_scale"), "k_scale"},
+                          {maybe(a[4], "v_scale"), "v_scale"}, {&k, "k"}, {&v, "v"}, {q, "q"}, {qo, "q_out"}, {cs, "cos"}, {sn, "sin"}});
     const at::ScalarType dt = k.scalar_type();
     const int code = dtype_code(dt);
     if (c.p.format == EPQ_CACHE_SAME && c.dtype != dt) refuse("rows of ", dt, " for a cache of ", c.dtype);
@@ -293,6 +316,8 @@ PyObject* write(PyObject* const* a) {
 // read(k_pool, v_pool, table, k_scale, v_scale, seq, pos, dtype | None)
 PyObject* read(PyObject* const* a) {
     const Cache c = cache_of(a);
+    no_gradient("read", {{&tensor(a[0], "k"), "the k pool"}, {&tensor(a[1], "v"), "the v pool"}, {maybe(a[3], "k_scale"), "k_scale"},
+                         {maybe(a[4], "v_scale"), "v_scale"}});
     at::ScalarType dt = c.p.format == EPQ_CACHE_SAME ? c.dtype : at::kBFloat16;
     if (a[7] != Py_None) {
         if (!THPDtype_Check(a[7])) throw TypeProblem("epure: dtype must be a torch.dtype");
@@ -318,6 +343,8 @@ PyObject* attend(PyObject* const* a) {
     Tensor q = tensor(a[5], "q");
     const Tensor& lengths = tensor(a[6], "lengths");
     const Tensor *seq = maybe(a[7], "seq"), *to = maybe(a[10], "out");
+    no_gradient("attend", {{&tensor(a[0], "k"), "the k pool"}, {&tensor(a[1], "v"), "the v pool"}, {maybe(a[3], "k_scale"), "k_scale"},
+                           {maybe(a[4], "v_scale"), "v_scale"}, {&q, "q"}, {to, "out"}});
     const at::ScalarType dt = q.scalar_type();
     if (dt != at::kBFloat16 && dt != at::kHalf)
         throw TypeProblem(text("paged attention takes float16 or bfloat16 queries, not ", dt));

@@ -7,7 +7,8 @@ page ``table[s, t // page_size]``.  A pool holds the activations' type, int8 or 
 float32 scale a token and head.
 
 ``KVPages`` names the tensors of one layer; ``write``, ``read`` and ``attend`` are the operators on it.
-``PagedKVCache`` owns the pools of all layers and hands pages out."""
+``PagedKVCache`` owns the pools of all layers and hands pages out.  The operators have no gradient: with grad mode
+on they refuse tensors that require one."""
 from typing import NamedTuple, Optional
 
 import torch

@@ -93,11 +93,14 @@ def rope(q, k, pos, cos, sin, interleaved=False, inverse=False, out=None):
     The first ``rotary_dim`` values of every head (the tables' width times two) turn, pairs ``(j, j + r / 2)``, or
     ``(2j, 2j + 1)`` with ``interleaved``; the others are copied.  float32, float16 or bfloat16; rows and heads
     may be strided.  ``inverse`` turns back (for a gradient: ``dq, dk = rope(dy_q, dy_k, ..., inverse=True)``);
-    autograd does so by itself.  ``out=(q_out, k_out)`` writes there, in place where they are q and k (no
-    autograd).  Returns ``(q', k')``, or ``q'`` alone without k."""
+    autograd does so by itself (for q and k; tables that require a gradient are refused, and so are tensors with
+    a forward-mode tangent).  ``out=(q_out, k_out)`` writes there, in place where they are q and k; it records
+    nothing for autograd, so with grad mode on, tensors that require a gradient are refused.  Returns ``(q', k')``, or ``q'`` alone without k."""
     if out is not None:
         q_out, k_out = out if k is not None else (out if torch.is_tensor(out) else out[0], None)
         return _calls().rope(q, k, pos, cos, sin, interleaved, inverse, q_out, k_out)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if cos.requires_grad or sin.requires_grad:
+            raise RuntimeError("epure: rope has no gradient with respect to cos and sin; detach them")
         return _RopeFn.apply(pos, cos, sin, interleaved, inverse, q, k)
     return _calls().rope(q, k, pos, cos, sin, interleaved, inverse, None, None)
