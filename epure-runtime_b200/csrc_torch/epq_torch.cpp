@@ -111,6 +111,12 @@ void no_gradient(const char* call, std::initializer_list<Named> tensors) {
     }
 }
 
+// Counts a write into a tensor that the caller gave, so that a backward which saved its old values finds out.
+// (Inference tensors have no count.)
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // A strided tensor [rows, heads, head_dim]; negative sizes are not checked.
 epq_heads heads_of(const Tensor& t, const char* what, const at::Device& dev, at::ScalarType dtype, int64_t rows,
                    int64_t heads, int64_t head_dim) {
@@ -276,6 +282,8 @@ PyObject* rope(PyObject* const* a) {
     check(lib.rope(in, out, k ? 2 : 1, pos.const_data_ptr<int64_t>(), m, (int32_t)hd, t.rotary_dim, t.cos, t.sin, t.max_len,
                    truth(a[5]), truth(a[6]), code, stream_of(dev)),
           "epq_rope");
+    if (qo) written(*qo);
+    if (k && ko) written(*ko);
     return k ? wrap2(y, z) : wrap(y);
 }
 
@@ -309,6 +317,9 @@ PyObject* write(PyObject* const* a) {
                     pos.const_data_ptr<int64_t>(), m, t.cos, t.sin, t.max_len, t.rotary_dim, truth(a[13]), truth(a[14]),
                     (float)number(a[15]), code, stream_of(c.device)),
           "epq_paged_write");
+    for (int i : {0, 1, 3, 4})
+        if (const Tensor* t = maybe(a[i], "a pool")) written(*t);
+    if (q && qo) written(*qo);
     if (!q) Py_RETURN_NONE;
     return wrap(y);
 }
@@ -374,6 +385,7 @@ PyObject* attend(PyObject* const* a) {
                      window, out.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr, dtype_code(dt), ws.data_ptr(), ws.numel(),
                      st),
           "epq_paged_attend");
+    if (to) written(*to);
     return with_lse ? wrap2(out, lse) : wrap(out);
 }
 

@@ -74,3 +74,49 @@ def test_forward_mode_tangents_are_refused():
             with pytest.raises(RuntimeError, match="tangent"):
                 call()
         assert torch.isfinite(rotary.rope(q, None, pos, cos, sin).float()).all()
+
+
+def test_writes_are_counted():
+    """A tensor that an earlier operation saved for its backward, overwritten in place: torch's own error."""
+    from epure import paged, rotary
+    pages, seq, pos = _cache()
+    cos, sin = rotary.rope_tables(64, 8, DEV)
+    q, k, v = _rows(4, 2, 2)
+    n = torch.tensor([4], device=DEV)
+
+    def versions():
+        return [t._version for t in (q, k, pages.k, pages.v)]
+
+    before = versions()
+    rotary.rope(q, k, pos, cos, sin)
+    paged.read(pages, seq, pos)
+    assert versions() == before
+    rotary.rope(q, k, pos, cos, sin, out=(q, k))
+    assert versions() == [before[0] + 1, before[1] + 1, before[2], before[3]]
+    paged.write(pages, k, v, seq, pos, q=q, q_out=q)
+    assert versions() == [before[0] + 2, before[1] + 1, before[2] + 1, before[3] + 1]
+    out = torch.empty_like(q[:1])
+    paged.attend(pages, q[:1], n, out=out)
+    assert out._version == 1 and versions()[0] == before[0] + 2
+    q8 = _pages([4], 2, 64, 16, "int8", torch.bfloat16)
+    scale = q8.k_scale._version
+    paged.write(q8, k, v, seq, pos)
+    assert q8.k_scale._version == scale + 1
+    w = torch.randn(64, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    for overwrite in (lambda t: rotary.rope(t, None, pos, cos, sin, out=t),
+                      lambda t: paged.write(pages, k, v, seq, pos, q=t, q_out=t)):
+        x = torch.randn(4, 4, 64, device=DEV, dtype=torch.bfloat16)
+        y = x @ w                                      # saves x
+        overwrite(x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
+def test_inference_tensors_are_taken():
+    from epure import paged
+    with torch.inference_mode():
+        pages, seq, pos = _cache()
+        _, k, v = _rows(4, 2, 2)
+    paged.write(pages, k, v, seq, pos)
+    got = paged.read(pages, seq, pos)
+    assert torch.equal(got[0], k) and torch.equal(got[1], v)
