@@ -282,6 +282,24 @@ inline bool heads_aligned(const epq_heads& v, int elem, int bytes) {
     return ((uintptr_t)v.data | (uintptr_t)(v.stride_row * elem) | (uintptr_t)(v.stride_head * elem)) % bytes == 0;
 }
 
+// Whether two heads of the view [m, heads, head_dim] have a value in common (an expanded tensor, say).
+inline bool heads_overlap(const epq_heads& v, int64_t m, int64_t hd) {
+    const int64_t H = v.heads;
+    const int64_t sr = v.stride_row < 0 ? -v.stride_row : v.stride_row;
+    const int64_t sh = v.stride_head < 0 ? -v.stride_head : v.stride_head;
+    if ((m > 1 && sr < hd) || (H > 1 && sh < hd)) return true;
+    if (m <= 1 || H <= 1 || sr / H >= sh || sh / m >= sr) return false;    // the ordinary orders: rows of heads, heads of rows
+    for (int64_t h = 1; h < H; ++h) {
+        const int64_t r = h * sh / sr, past = h * sh - r * sr;             // head h of row 0 begins `past` behind row r
+        if ((r < m && past < hd) || (r + 1 < m && sr - past < hd)) return true;
+    }
+    return false;
+}
+// Whether y is written where x is read, but not value for value.
+inline bool moved_in_place(const epq_heads& x, const epq_heads& y, int64_t m) {
+    return x.data == y.data && ((m > 1 && x.stride_row != y.stride_row) || (x.heads > 1 && x.stride_head != y.stride_head));
+}
+
 int rope_read_device_error(int* flag);
 int cache_read_device_error(int* flag);
 int attend_read_device_error(int* flag);

@@ -474,6 +474,9 @@ int epq_paged_write(const epq_pages* pages, const epq_heads* q, const epq_heads*
     if (m == 0) return EPQ_OK;
     if (!seq || !pos || !k->data || !v->data || (q && (!q->data || !q_out->data)))
         return set_error(EPQ_EINVAL, "epq_paged_write: NULL rows, seq or pos");
+    if (q && (heads_overlap(*q_out, m, hd) || moved_in_place(*q, *q_out, m)))
+        return set_error(EPQ_ESHAPE, "epq_paged_write: rows or heads of q_out overlap (strides %lld, %lld)",
+                         (long long)q_out->stride_row, (long long)q_out->stride_head);
     A.k = {k->data, k->stride_row, k->stride_head};
     A.v = {v->data, v->stride_row, v->stride_head};
     A.aligned = heads_aligned(*k, elem, 16) && heads_aligned(*v, elem, 16);

@@ -207,6 +207,10 @@ extern "C" int epq_rope(const epq_heads* x, const epq_heads* y, int32_t count, c
     }
     if (heads > 65536) return set_error(EPQ_EUNSUPPORTED, "epq_rope: %lld heads > 65536", (long long)heads);
     if (m == 0 || heads == 0) return EPQ_OK;
+    for (int i = 0; i < count; ++i)
+        if (heads_overlap(y[i], m, head_dim) || moved_in_place(x[i], y[i], m))
+            return set_error(EPQ_ESHAPE, "epq_rope: rows or heads of output %d overlap (strides %lld, %lld)", i,
+                             (long long)y[i].stride_row, (long long)y[i].stride_head);
     A.pos = pos;
     A.cos_t = cos_tab;
     A.sin_t = sin_tab;

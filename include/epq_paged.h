@@ -39,7 +39,8 @@ typedef struct epq_heads {
  *     y_a = x_a c - x_b s,   y_b = x_b c + x_a s,
  * computed in float32 and rounded once; values past rotary_dim are copied.
  * inverse != 0 turns by -s: the gradient of the call with respect to x.  y[i] may be
- * x[i] (in place), and may not overlap it otherwise.  A position outside
+ * x[i] (in place, with its strides), and may not overlap it otherwise; no two heads of
+ * y[i] may overlap (EPQ_ESHAPE).  A position outside
  * [0, max_len) writes zeros.  rotary_dim even, 2..head_dim; head_dim <= 1024. */
 int epq_rope(const epq_heads* x, const epq_heads* y, int32_t count, const int64_t* pos, int64_t m,
              int32_t head_dim, int32_t rotary_dim, const float* cos_tab, const float* sin_tab, int64_t max_len,
@@ -81,7 +82,7 @@ typedef struct epq_pages {
  * seq[r].  qk_norm != 0 first normalises every head of q and k (RMSNorm, weight 1);
  * with cos_tab / sin_tab (NULL: none) q and k are then rotated as by epq_rope.  Both
  * results are rounded to dtype, as the tensors of a model are, before k is quantised.
- * q [m, heads, head_dim] may be NULL; q_out receives it (q_out may be q).  A row with
+ * q [m, heads, head_dim] may be NULL; q_out receives it (q_out may be q, as in epq_rope).  A row with
  * a negative position is padding: nothing is written to the cache, zeros to q_out.  No
  * two rows may name the same token. */
 int epq_paged_write(const epq_pages* pages, const epq_heads* q, const epq_heads* q_out, const epq_heads* k,
