@@ -949,7 +949,9 @@ int epq_paged_attend(const epq_pages* pages, const epq_heads* q, const int32_t* 
     if (!seq && batch > A.pages.seqs)
         return set_error(EPQ_ESHAPE, "epq_paged_attend: batch=%lld of a table of %d sequences", (long long)batch,
                          A.pages.seqs);
-    if (batch * ((int64_t)A.pages.max_pages * A.pages.page_size / kTile + 1 + kUnitCost) > INT32_MAX)
+    // a batch's blocks are counted in 32 bits, and a CTA's run of all units' blocks too (at least 64 CTAs share them)
+    const int64_t most = batch * ((int64_t)A.pages.max_pages * A.pages.page_size / kTile + 1 + kUnitCost);
+    if (most > INT32_MAX || most * KV * A.chunks > (int64_t)INT32_MAX * 64)
         return set_error(EPQ_EUNSUPPORTED, "epq_paged_attend: batch=%lld of up to %lld tokens each", (long long)batch,
                          (long long)A.pages.max_pages * A.pages.page_size);
     if (batch == 0) return EPQ_OK;

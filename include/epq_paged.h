@@ -107,8 +107,8 @@ int epq_paged_read(const epq_pages* pages, const int32_t* seq, const int64_t* po
  * 16-byte aligned.  The workspace
  * (256-byte aligned) has to be zeroed once before its first use and is left ready for
  * the next call; calls that share one must not overlap.
- * batch * kv_heads * ceil(heads / kv_heads / 16) <= 65536, and batch * (max_pages *
- * page_size / 16 + 13) < 2^31. */
+ * units = kv_heads * ceil(heads / kv_heads / 16): batch * units <= 65536, and with
+ * blocks = batch * (max_pages * page_size / 16 + 13), blocks < 2^31 and blocks * units < 2^37. */
 int64_t epq_paged_attend_workspace_bytes(const epq_pages* pages, int64_t batch, int32_t heads);
 int epq_paged_attend(const epq_pages* pages, const epq_heads* q, const int32_t* seq, const int64_t* lengths,
                      int64_t batch, float scale, int64_t window, void* out, float* lse, int32_t dtype,
