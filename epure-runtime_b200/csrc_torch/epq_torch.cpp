@@ -117,6 +117,9 @@ void written(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// The stride of a dimension, or `alone` where it has one element and its stride says nothing.
+int64_t step(const Tensor& t, int d, int64_t alone) { return t.size(d) > 1 ? t.stride(d) : alone; }
+
 // A strided tensor [rows, heads, head_dim]; negative sizes are not checked.
 epq_heads heads_of(const Tensor& t, const char* what, const at::Device& dev, at::ScalarType dtype, int64_t rows,
                    int64_t heads, int64_t head_dim) {
@@ -127,7 +130,7 @@ epq_heads heads_of(const Tensor& t, const char* what, const at::Device& dev, at:
         refuse(what, " is ", t.sizes(), "; expected [", rows, ", ", heads, ", ", head_dim, "] (-1: any)");
     if (t.size(1) > INT32_MAX) refuse(what, " has ", t.size(1), " heads");
     if (t.numel() && t.stride(2) != 1) refuse("the values of a head of ", what, " must be contiguous (stride ", t.stride(2), ")");
-    return {t.data_ptr(), t.stride(0), t.stride(1), (int32_t)t.size(1), 0};
+    return {t.data_ptr(), step(t, 0, 0), step(t, 1, 0), (int32_t)t.size(1), 0};
 }
 
 const Tensor& index_of(const Tensor& t, const char* what, const at::Device& dev, at::ScalarType dtype, int64_t n) {
@@ -170,12 +173,14 @@ Cache cache_of(PyObject* const* a) {
     else if (c.dtype == at::kBFloat16 || c.dtype == at::kHalf || c.dtype == at::kFloat) fmt = EPQ_CACHE_SAME;
     else throw TypeProblem(text("a cache of ", c.dtype, " is not supported"));
     if (!k.is_cuda()) refuse("the paged cache needs CUDA tensors");
-    if (k.dim() != 4 || v.sizes() != k.sizes() || v.scalar_type() != c.dtype || v.device() != c.device || v.strides() != k.strides())
+    if (k.dim() != 4 || v.sizes() != k.sizes() || v.scalar_type() != c.dtype || v.device() != c.device)
         refuse("k and v must be alike, [pages, kv_heads, page_size, head_dim]");
-    const int64_t kv = k.size(1), ps = k.size(2), hd = k.size(3);
-    if (k.stride(3) != 1 || k.stride(2) != hd || k.stride(1) != ps * hd)
-        refuse("the heads, slots and values of a page must be contiguous (strides ", k.strides(), ")");
-    if (table.dim() != 2 || table.scalar_type() != at::kInt || table.device() != c.device || table.stride(1) != 1)
+    const int64_t kv = k.size(1), ps = k.size(2), hd = k.size(3), page = step(k, 0, kv * ps * hd);
+    for (const Tensor* t : {&k, &v})
+        if (step(*t, 3, 1) != 1 || step(*t, 2, hd) != hd || step(*t, 1, ps * hd) != ps * hd)
+            refuse("the heads, slots and values of a page must be contiguous (strides ", t->strides(), ")");
+    if (step(v, 0, page) != page) refuse("k and v must be alike: pages ", page, " and ", v.stride(0), " values apart");
+    if (table.dim() != 2 || table.scalar_type() != at::kInt || table.device() != c.device || step(table, 1, 1) != 1)
         refuse("the page table must be int32 [seqs, max_pages] on the cache's device");
     if (std::max({kv, ps, hd, table.size(0), table.size(1)}) > INT32_MAX) refuse("a size of the cache is past 2^31");
     int64_t stride = 0;
@@ -183,14 +188,15 @@ Cache cache_of(PyObject* const* a) {
         if (!ks || !vs) refuse("an 8-bit cache needs k_scale and v_scale");
         for (const Tensor* s : {ks, vs})
             if (s->dim() != 3 || s->size(0) != k.size(0) || s->size(1) != kv || s->size(2) != ps || s->scalar_type() != at::kFloat ||
-                s->device() != c.device || s->stride(2) != 1 || s->stride(1) != ps || s->stride(0) != ks->stride(0))
+                s->device() != c.device || step(*s, 2, 1) != 1 || step(*s, 1, ps) != ps ||
+                step(*s, 0, kv * ps) != step(*ks, 0, kv * ps))
                 refuse("scales must be float32 [pages, kv_heads, page_size], pages contiguous");
-        stride = ks->stride(0);
+        stride = step(*ks, 0, kv * ps);
     } else if (ks || vs) {
         refuse("a cache of ", c.dtype, " has no scales");
     }
     c.p = {k.data_ptr(), v.data_ptr(), ks ? ks->data_ptr<float>() : nullptr, vs ? vs->data_ptr<float>() : nullptr,
-           table.const_data_ptr<int32_t>(), k.stride(0), stride, table.stride(0), k.size(0), (int32_t)table.size(0),
+           table.const_data_ptr<int32_t>(), page, stride, step(table, 0, table.size(1)), k.size(0), (int32_t)table.size(0),
            (int32_t)table.size(1), (int32_t)ps, (int32_t)kv, (int32_t)hd, fmt};
     return c;
 }

@@ -47,3 +47,46 @@ def test_outputs_whose_rows_are_one_are_refused():
     # inputs may be expanded
     same = rotary.rope(q[:1].expand(6, 4, 64), None, pos, cos, sin)
     assert torch.equal(same, rotary.rope(q[:1].expand(6, 4, 64).contiguous(), None, pos, cos, sin))
+
+
+@pytest.mark.parametrize("fmt", ["same", "int8"])
+def test_strides_of_single_elements_say_nothing(fmt):
+    """One page, one key head, slot, table column, row or head, with strides that no dense tensor has."""
+    from epure import paged
+    g = torch.Generator(device=DEV).manual_seed(52)
+
+    def odd(t, dim, stride=7):
+        assert t.shape[dim] == 1
+        return t.as_strided(t.shape, [stride if d == dim else s for d, s in enumerate(t.stride())])
+
+    for pages, kv, ps, seqs in ((1, 2, 16, 1), (3, 1, 16, 3), (3, 2, 1, 3)):
+        plain = _pages([min(ps, 5)] * seqs, kv, 64, ps, fmt, torch.bfloat16, spare=pages - seqs)
+        dim = 0 if pages == 1 else 1 if kv == 1 else 2
+        strange = [t if t is None else odd(t, dim) for t in (plain.k, plain.v, plain.k_scale, plain.v_scale)]
+        table = odd(plain.table, 1 if seqs > 1 else 0)
+        assert table.shape == plain.table.shape and table.stride() != plain.table.stride()
+        cache = paged.KVPages(strange[0], strange[1], table, *strange[2:])
+        m = seqs
+        seq, pos = torch.arange(m, dtype=torch.int32, device=DEV), torch.zeros(m, dtype=torch.long, device=DEV)
+        x = torch.randn(m, 2, kv, 64, generator=g, device=DEV).to(torch.bfloat16)
+        q = torch.randn(m, 2 * kv, 64, generator=g, device=DEV).to(torch.bfloat16)
+        rows = (x[:, 0], x[:, 1]) if m > 1 else (odd(x[:, 0], 0), odd(x[:, 1], 0))
+        got = [paged.write(c, *rows, seq, pos, q=q if m > 1 else odd(q, 0)) for c in (plain, cache)]
+        assert torch.equal(got[0], got[1]) and torch.equal(got[0], q)
+        n = torch.ones(m, dtype=torch.long, device=DEV)
+        for a, b in zip(paged.read(plain, seq, pos), paged.read(cache, seq, pos)):
+            assert torch.equal(a, b)
+        assert torch.equal(paged.attend(plain, q, n), paged.attend(cache, q if m > 1 else odd(q, 0), n))
+
+
+def test_real_strides_are_still_refused():
+    from epure import paged
+    pages, seq, pos, q, k, v, cos, sin = _inputs()
+    two = _pages([20, 20], 2, 64, 16, "int8", torch.bfloat16)
+    for bad in (pages._replace(v=pages.v[:, :, ::2]), pages._replace(k=pages.k.transpose(1, 2), v=pages.v.transpose(1, 2)),
+                pages._replace(v=torch.empty(3, 2, 2, 16, 64, dtype=q.dtype, device=DEV)[:, 0]),
+                two._replace(table=two.table.t().contiguous().t()),
+                two._replace(v_scale=torch.empty(*two.v_scale.shape[:2], 32, device=DEV)[..., ::2])):
+        assert bad.k.shape[0] > 1
+        with pytest.raises(RuntimeError, match="alike|contiguous|page table"):
+            paged.read(bad, seq, pos)
