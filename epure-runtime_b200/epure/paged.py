@@ -94,10 +94,13 @@ class PagedKVCache:
     def free_pages(self):
         return len(self._free)
 
-    def reserve(self, seq, tokens):
-        """Makes room for the first ``tokens`` tokens of sequence ``seq``."""
+    def _check(self, seq):
         if not 0 <= seq < self.seqs:
             raise IndexError(f"epure: sequence {seq} of a cache of {self.seqs}")
+
+    def reserve(self, seq, tokens):
+        """Makes room for the first ``tokens`` tokens of sequence ``seq``."""
+        self._check(seq)
         if tokens > self.max_tokens:
             raise ValueError(f"epure: {tokens} tokens; this cache holds max_tokens={self.max_tokens} a sequence")
         held = self._held[seq]
@@ -113,6 +116,7 @@ class PagedKVCache:
 
     def release(self, seq):
         """Gives sequence ``seq``'s pages back."""
+        self._check(seq)
         self._free += reversed(self._held[seq])
         self._held[seq] = []
         self.table[seq].fill_(-1)
