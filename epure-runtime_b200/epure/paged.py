@@ -109,10 +109,11 @@ class PagedKVCache:
             return
         if more > len(self._free):
             raise RuntimeError(f"epure: the cache is full ({len(self._free)} pages free, {more} needed)")
-        got = [self._free.pop() for _ in range(more)]
+        got = self._free[:-more - 1:-1]
         first = len(held)
-        held += got
         self.table[seq, first:first + more] = torch.tensor(got, dtype=torch.int32).to(self.device)
+        held += got                                    # behind the copy: where it raises, no page is lost
+        del self._free[-more:]
 
     def release(self, seq):
         """Gives sequence ``seq``'s pages back."""

@@ -24,3 +24,25 @@ def test_release_refuses_sequences_that_are_not():
     c.release(2)
     c.release(2)                                       # nothing held: nothing happens
     assert c.free_pages() == 6 and not any(_held(c))
+
+
+def test_a_failed_copy_takes_no_pages():
+    """The table cannot be written (inside a capture, say): the pages stay free."""
+    class Refusing:
+        def __setitem__(self, at, value):
+            raise RuntimeError("no copy")
+
+    c = _cache()
+    c.reserve(0, 17)
+    table, c.table = c.table, Refusing()
+    with pytest.raises(RuntimeError, match="no copy"):
+        c.reserve(0, 64)
+    with pytest.raises(RuntimeError, match="no copy"):
+        c.reserve(1, 1)
+    assert c.free_pages() == 4
+    c.table = table
+    c.reserve(1, 64)
+    assert _held(c) == [[0, 1], [2, 3, 4, 5], []] and c.free_pages() == 0
+    c.release(0)
+    c.release(1)
+    assert c.free_pages() == 6
