@@ -1,4 +1,6 @@
 """The paged cache hands its pages out once each, and takes them back from the sequence that is named."""
+import random
+
 import pytest
 
 from epure.paged import PagedKVCache
@@ -46,3 +48,33 @@ def test_a_failed_copy_takes_no_pages():
     c.release(0)
     c.release(1)
     assert c.free_pages() == 6
+
+
+def test_no_page_is_held_twice():
+    """Random reserves and releases: every page is free or held by one sequence, the table names just those held,
+    and a sequence keeps the pages it had."""
+    rng = random.Random(3)
+    c = _cache(pages=9, seqs=4, max_tokens=80)
+    want = [[] for _ in range(4)]
+    refused = 0
+    for _ in range(600):
+        seq = rng.randrange(4)
+        if rng.random() < 0.3:
+            c.release(seq)
+            want[seq] = []
+        else:
+            tokens = rng.randint(0, 80)
+            need = -(-tokens // 16) - len(want[seq])
+            if need > 9 - sum(map(len, want)):
+                with pytest.raises(RuntimeError, match="full"):
+                    c.reserve(seq, tokens)
+                refused += 1
+            else:
+                c.reserve(seq, tokens)
+                got = _held(c)[seq]
+                assert got[:len(want[seq])] == want[seq] and len(got) == len(want[seq]) + max(0, need)
+                want[seq] = got
+        held = [p for row in _held(c) for p in row]
+        assert _held(c) == want and len(set(held)) == len(held) and all(0 <= p < 9 for p in held)
+        assert c.free_pages() == 9 - len(held)
+    assert refused > 20
