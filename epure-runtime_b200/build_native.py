@@ -11,9 +11,12 @@ with g++/OpenMP into epure/libepq_cpu.so, and the tensor binding of the paged ca
 """
 import argparse
 import glob
+import importlib.metadata
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -93,13 +96,17 @@ def build_cpu(force=False, quiet=False):
 
 
 def build_torch(force=False, quiet=False):
-    """_epq_torch.so: a CPython module over torch's headers and libraries."""
+    """_epq_torch.so: a CPython module over torch's headers and libraries; built again for another torch or Python,
+    whose binary interface may be another."""
     headers = [os.path.join(INCLUDE, h) for h in ("epq.h", "epq_paged.h")]
     newest = max(os.path.getmtime(f) for f in [TORCH_SRC, *headers])
-    if not force and os.path.exists(TORCH_OUT) and os.path.getmtime(TORCH_OUT) >= newest:
-        return TORCH_OUT
-    import sysconfig
-
+    against = "\n".join((importlib.metadata.version("torch"), importlib.util.find_spec("torch").origin,
+                         sysconfig.get_config_var("EXT_SUFFIX")))
+    stamp = os.path.join(OBJ, "_epq_torch.built")
+    if not force and os.path.exists(TORCH_OUT) and os.path.getmtime(TORCH_OUT) >= newest and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == against:
+                return TORCH_OUT
     import torch
     from torch.utils import cpp_extension
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
@@ -115,6 +122,9 @@ def build_torch(force=False, quiet=False):
     if not quiet:
         print(" ".join(os.path.relpath(c, ROOT) if c.startswith(ROOT) else c for c in cmd), flush=True)
     subprocess.check_call(cmd)
+    os.makedirs(OBJ, exist_ok=True)
+    with open(stamp, "w") as f:
+        f.write(against)
     return TORCH_OUT
 
 
