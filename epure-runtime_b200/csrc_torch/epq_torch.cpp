@@ -35,6 +35,9 @@ struct TypeProblem : std::runtime_error {
     using std::runtime_error::runtime_error;
 };
 
+// An exception that Python has already set.
+struct PythonError {};
+
 template <typename... A> std::string text(const A&... a) {
     std::ostringstream o;
     o << "epure: ";
@@ -85,7 +88,11 @@ double number(PyObject* o) {
     }
     return v;
 }
-bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw PythonError();
+    return v == 1;
+}
 
 int dtype_code(at::ScalarType t) {
     if (t == at::kFloat) return EPQ_F32;
@@ -424,6 +431,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (n != N) throw TypeProblem(text(N, " arguments are expected, ", n, " were given"));
         if (F != bind && !lib.last_error) refuse("libepq.so is not bound");
         return F(args);
+    } catch (const PythonError&) {
     } catch (const TypeProblem& e) {
         PyErr_SetString(PyExc_TypeError, e.what());
     } catch (const c10::OutOfMemoryError& e) {

@@ -1,4 +1,5 @@
-"""Layouts of the paged and rotary calls' tensors: outputs in other orders, strides that say nothing."""
+"""Layouts of the paged and rotary calls' tensors (outputs in other orders, strides that say nothing), and flags that
+have no truth value."""
 import pytest
 import torch
 from test_gpu_paged import DEV, _gpu, _pages, _tokens  # noqa: F401 (_gpu: a fixture)
@@ -90,3 +91,23 @@ def test_real_strides_are_still_refused():
         assert bad.k.shape[0] > 1
         with pytest.raises(RuntimeError, match="alike|contiguous|page table"):
             paged.read(bad, seq, pos)
+
+
+def test_flags_without_a_truth_value():
+    """The flag's own exception, and nothing is written."""
+    from epure import paged, rotary
+    pages, seq, pos, q, k, v, cos, sin = _inputs()
+    paged.write(pages, k, v, seq, pos)
+    before = pages.k.clone().nan_to_num_(9.0)
+    out = torch.zeros_like(q)
+    both = torch.tensor([True, False])
+    for call in (lambda: rotary.rope(q, None, pos, cos, sin, interleaved=both, out=out),
+                 lambda: rotary.rope(q, None, pos, cos, sin, inverse=both, out=out),
+                 lambda: paged.write(pages, v, k, seq, pos, cos=cos, sin=sin, interleaved=both),
+                 lambda: paged.write(pages, v, k, seq, pos, qk_norm=both),
+                 lambda: paged.attend(pages, q[:1], pos[1:2], return_lse=both)):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            call()
+    assert not out.any() and torch.equal(pages.k.nan_to_num(9.0), before)
+    assert torch.equal(rotary.rope(q, None, pos, cos, sin, interleaved=torch.tensor(True)),
+                       rotary.rope(q, None, pos, cos, sin, interleaved=True))
