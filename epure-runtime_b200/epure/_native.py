@@ -92,17 +92,16 @@ EXPORTS = (
 )
 
 _lib = None
-_lib_path = None
 _lock = threading.Lock()
 
 
 def load_library(path=None):
     """Load libepq.so (once) and declare its signatures.  Raises if it is absent."""
-    global _lib, _lib_path
+    global _lib
     with _lock:
         if _lib is not None:
             return _lib
-        path = os.path.abspath(path or LIB_PATH)
+        path = path or LIB_PATH
         if not os.path.exists(path):
             raise RuntimeError(
                 f"epure: the CUDA library {path} is not built; run "
@@ -163,7 +162,7 @@ def load_library(path=None):
             getattr(lib, name)          # every declared entry point must be exported
         if lib.epq_abi_version() != 1:
             raise RuntimeError(f"epure: {path} has ABI {lib.epq_abi_version()}, expected 1")
-        _lib, _lib_path = lib, path
+        _lib = lib
         return lib
 
 
@@ -611,6 +610,6 @@ def load_tensor_calls():
             except ImportError as exc:
                 raise RuntimeError("epure: the tensor binding _epq_torch.so is not built or does not load here; run "
                                    f"`python epure-runtime_b200/build_native.py` ({exc})") from exc
-            _epq_torch.bind(_lib_path, torch.OutOfMemoryError)
+            _epq_torch.bind(LIB_PATH, torch.OutOfMemoryError)
             tensor_calls = _epq_torch
     return tensor_calls
