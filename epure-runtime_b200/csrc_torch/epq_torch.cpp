@@ -318,6 +318,7 @@ PyObject* write(PyObject* const* a) {
     const Tensor& seq = index_of(tensor(a[7], "seq"), "seq", c.device, at::kInt, m);
     const Tensor& pos = index_of(tensor(a[8], "pos"), "pos", c.device, at::kLong, m);
     if (!cs != !sn) refuse("cos and sin come together");
+    if (qo && !q) refuse("q_out needs q");
     const Tables t = cs ? tables_of(*cs, *sn, c.device, c.p.head_dim) : Tables();
     epq_heads qh, oh;
     Tensor y;

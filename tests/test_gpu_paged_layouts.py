@@ -111,3 +111,10 @@ def test_flags_without_a_truth_value():
     assert not out.any() and torch.equal(pages.k.nan_to_num(9.0), before)
     assert torch.equal(rotary.rope(q, None, pos, cos, sin, interleaved=torch.tensor(True)),
                        rotary.rope(q, None, pos, cos, sin, interleaved=True))
+
+
+def test_an_output_without_its_input_is_refused():
+    from epure import paged
+    pages, seq, pos, q, k, v, cos, sin = _inputs()
+    with pytest.raises(RuntimeError, match="q_out needs q"):
+        paged.write(pages, k, v, seq, pos, q_out=torch.empty_like(q))
