@@ -1145,6 +1145,25 @@ bool mma_eligible(const StoreD& s, int64_t m, int x_dtype) {
            s.k > 0 && s.k < (1 << 30);
 }
 
+// Shared bytes of a fused GEMV of m rows: `fixed` below the staged activations,
+// requested as if the dynamic block started at window address 0 (it starts a little
+// above, so the request always covers the layout), and `xbytes` of these.
+static void fused_bytes(int64_t m, int64_t kpad, int parts, int& fixed, int64_t& xbytes) {
+    fixed = (int)kHighWin + kSlots * parts * kConsumerWarps * 16 * (int)m * 4;
+    xbytes = m * kpad * 2;
+}
+static bool fused_stages_x(int fixed, int64_t xbytes) { return xbytes <= kMaxXSmem && fixed + xbytes <= kMaxSmem; }
+// The most rows whose call fits; the prologue works on staged activations only.
+static int fused_max_rows(int64_t k, int prologue, int epilogue) {
+    int rows = 0, fixed;
+    int64_t xbytes;
+    for (int m = 1; m <= 16; ++m) {
+        fused_bytes(m, cdiv(k, 128) * 128, epilogue == EPQ_EPI_SILU_MUL ? 2 : 1, fixed, xbytes);
+        if (fixed <= kMaxSmem && (prologue != EPQ_PRO_RMSNORM || fused_stages_x(fixed, xbytes))) rows = m;
+    }
+    return rows;
+}
+
 // Checks a fused GEMV and fills its parameters (everything but x_off); `fixed`
 // = shared bytes below the staged activations, `xbytes` = their size.
 static int build_mma_params(const StoreD* s, int count, const void* x, int x_dtype, int64_t m, int64_t ldx,
@@ -1165,11 +1184,8 @@ static int build_mma_params(const StoreD* s, int count, const void* x, int x_dty
     if (epilogue != EPQ_EPI_STORE && out_dtype != x_dtype)
         return set_error(EPQ_EDTYPE, "decode linear: fused epilogues write the activation dtype");
     const int64_t kpad = s[0].ng * 128;
-    xbytes = m * kpad * 2;
     const int slot_floats = parts * kConsumerWarps * 16 * (int)m;
-    // Requested as if the dynamic block started at window address 0 (it starts a
-    // little above, so the request always covers the layout).
-    fixed = (int)kHighWin + kSlots * slot_floats * 4;
+    fused_bytes(m, kpad, parts, fixed, xbytes);
     P = MmaParams{};
     P.count = count;
     P.x = x;
@@ -1225,12 +1241,10 @@ int launch_linear_mma_fused(const StoreD* s, int count, const void* x, int x_dty
         if (rc != EPQ_OK) return rc;
     }
     const bool sf32 = s[0].scale_dtype == EPQ_F32;
-    const bool xsm = xbytes <= kMaxXSmem && fixed + xbytes <= kMaxSmem;
-    if (prologue == EPQ_PRO_RMSNORM && !xsm)
-        return set_error(EPQ_EUNSUPPORTED, "decode linear: RMSNorm prologue needs m*k*2 <= %d bytes", kMaxXSmem);
-    if (fixed > kMaxSmem)
-        return set_error(EPQ_EUNSUPPORTED, "decode linear: m=%lld needs %d bytes of shared memory", (long long)m,
-                         fixed);
+    const bool xsm = fused_stages_x(fixed, xbytes);
+    if (fixed > kMaxSmem || (prologue == EPQ_PRO_RMSNORM && !xsm))
+        return set_error(EPQ_EUNSUPPORTED, "decode linear: m=%lld rows of k=%lld (at most %d with this prologue and epilogue)",
+                         (long long)m, (long long)s[0].k, fused_max_rows(s[0].k, prologue, epilogue));
     const int smem = fixed + (xsm ? (int)xbytes : 0);
     P.x_off = fixed;
     const int variant = (bf ? 1 : 0) + (nt == 2 ? 2 : 0) + (sf32 ? 4 : 0) + (xsm ? 8 : 0);
@@ -1276,6 +1290,13 @@ int launch_linear_mma(const StoreD* s, int count, const void* x, int x_dtype, in
 }  // namespace epq
 
 using namespace epq;
+
+extern "C" int32_t epq_decode_linear_max_rows(int64_t k, int32_t prologue, int32_t epilogue) {
+    if (k <= 0 || k >= (int64_t)1 << 30 || (prologue != EPQ_PRO_NONE && prologue != EPQ_PRO_RMSNORM) ||
+        (epilogue != EPQ_EPI_STORE && epilogue != EPQ_EPI_RESIDUAL && epilogue != EPQ_EPI_SILU_MUL))
+        return set_error(EPQ_EINVAL, "epq_decode_linear_max_rows: bad arguments");
+    return fused_max_rows(k, prologue, epilogue);
+}
 
 extern "C" int epq_decode_linear(const epq_store* stores, int32_t count, const void* x, int32_t x_dtype,
                                  int64_t m, int64_t ldx, int32_t prologue, float eps, void* const* outs,

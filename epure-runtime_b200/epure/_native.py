@@ -85,7 +85,7 @@ EXPORTS = (
     "epq_chain_workspace_bytes", "epq_chain_prepare", "epq_chain_run", "epq_chain_set_tp",
     "epq_add_rmsnorm", "epq_rope_kv", "epq_attn_decode", "epq_attn_decode_workspace_bytes",
     "epq_silu_mul", "epq_argmax", "epq_argmax_workspace_bytes", "epq_attn_rope_decode",
-    "epq_embedding", "epq_decode_linear", "epq_program_create", "epq_program_add_linear",
+    "epq_embedding", "epq_decode_linear", "epq_decode_linear_max_rows", "epq_program_create", "epq_program_add_linear",
     "epq_program_add_attention", "epq_program_workspace_bytes", "epq_program_finalize", "epq_program_run",
     "epq_program_destroy", "epq_rope", "epq_paged_write", "epq_paged_read", "epq_paged_attend",
     "epq_paged_attend_workspace_bytes",
@@ -141,6 +141,7 @@ def load_library(path=None):
         lib.epq_argmax_workspace_bytes.restype = I64
         lib.epq_argmax_workspace_bytes.argtypes = []
         lib.epq_silu_mul.argtypes = [P, P, P, I64, I32, P]
+        lib.epq_decode_linear_max_rows.argtypes = [I64, I32, I32]
         lib.epq_decode_linear.argtypes = [SP, I32, P, I32, I64, I64, I32, F32, P, P, I32, P]
         lib.epq_program_create.argtypes = [ctypes.POINTER(P)]
         lib.epq_program_add_linear.argtypes = [P, SP, I32, P, I64, I32, F32, P, P, I32]
@@ -488,10 +489,18 @@ PRO_NONE, PRO_RMSNORM = 0, 1
 EPI_STORE, EPI_RESIDUAL, EPI_SILU_MUL = 0, 1, 2
 
 
+def decode_linear_max_rows(k, prologue=PRO_NONE, epilogue=EPI_STORE):
+    """The most rows of k features that ``decode_linear`` takes with this prologue and epilogue (0: none)."""
+    rows = load_library().epq_decode_linear_max_rows(k, int(prologue), int(epilogue))
+    if rows < 0:
+        _check(rows, "epq_decode_linear_max_rows")
+    return rows
+
+
 def decode_linear(x, stores, prologue=PRO_NONE, epilogue=EPI_STORE, outs=None, eps=1e-6):
     """A decode-step packed linear with the block glue fused in (epq_decode_linear).
 
-    ``x`` [m, k] bf16/f16 (m <= 16).  ``prologue=PRO_RMSNORM`` normalises x first;
+    ``x`` [m, k] bf16/f16 (m <= 16, or what ``decode_linear_max_rows`` says).  ``prologue=PRO_RMSNORM`` normalises x first;
     ``epilogue=EPI_RESIDUAL`` adds the result into ``outs[0]`` (a residual stream,
     updated in place); ``EPI_SILU_MUL`` (stores = [gate, up]) returns
     silu(gate(x)) * up(x).  Returns the list of written outputs."""

@@ -34,6 +34,12 @@ class BatchDecoder:
         self.cache = paged.PagedKVCache(decoder.layers, pages or seqs * per_seq, page_size, sh.kv_heads, sh.head_dim,
                                         seqs, decoder.max_len, format, decoder.dtype, decoder.device)
         self._layers = [self.cache.layer(i) for i in range(decoder.layers)]
+        # rows that the fused linears of a block take; larger batches go through linear_multi and separate glue
+        rms, none = _native.PRO_RMSNORM, _native.PRO_NONE
+        self._fused_rows = min(_native.decode_linear_max_rows(*call) for call in (
+            (sh.hidden, rms, _native.EPI_STORE), (sh.hidden, rms, _native.EPI_SILU_MUL),
+            (sh.heads * sh.head_dim, none, _native.EPI_RESIDUAL), (sh.intermediate, none, _native.EPI_RESIDUAL)
+        )) if decoder._fusable else 0
         self._graphs = {}
 
     def _logits(self, h):
@@ -62,7 +68,7 @@ class BatchDecoder:
         B, scale = tokens.shape[0], 1.0 / math.sqrt(sh.head_dim)
         lengths = pos + 1
         h = d.embed[tokens]                                            # residual stream [B, hidden]
-        fused = d._fusable and B <= 16 and B * sh.hidden * 2 <= 65536  # limits of epq_decode_linear's prologue
+        fused = B <= self._fused_rows
         y = None if fused else _native.add_rmsnorm(h, eps=d.eps)
         for pages, b in zip(self._layers, d.stack.blocks):
             qkv = [b["q_proj"], b["k_proj"], b["v_proj"]]

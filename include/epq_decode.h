@@ -87,7 +87,7 @@ enum epq_epilogue { EPQ_EPI_STORE = 0, EPQ_EPI_RESIDUAL = 1, EPQ_EPI_SILU_MUL = 
  * as dtype(dtype(cb[idx]) * dtype(scale)), the reference's materialize rounding)
  * with
  *   prologue EPQ_PRO_RMSNORM: x is replaced by RMSNorm(x) (weight 1, eps) per
- *            row while it is staged (m * k * 2 <= 64 KiB);
+ *            row while it is staged in shared memory;
  *   epilogue EPQ_EPI_STORE:    outs[i] = x @ W_i^T (rounded to x_dtype);
  *            EPQ_EPI_RESIDUAL: one store; outs[0] is a residual stream updated
  *                              in place: h = h + dtype(x @ W^T);
@@ -96,7 +96,11 @@ enum epq_epilogue { EPQ_EPI_STORE = 0, EPQ_EPI_RESIDUAL = 1, EPQ_EPI_SILU_MUL = 
  *                              (outs[1] is not written).
  * The reference's block (epure/runtime.py:98-126 PackedLinear inside a Llama /
  * Qwen3 decoder layer) rounds at exactly these points.  No workspace; the launch
- * may overlap the previous kernel on the stream (programmatic dependent launch). */
+ * may overlap the previous kernel on the stream (programmatic dependent launch).
+ * Shared memory bounds the rows below 16 for long prologues and for the SiLU
+ * epilogue: epq_decode_linear_max_rows gives the most rows of k features that a call
+ * takes (0: none; negative: bad arguments). */
+int32_t epq_decode_linear_max_rows(int64_t k, int32_t prologue, int32_t epilogue);
 int epq_decode_linear(const epq_store* stores, int32_t count, const void* x, int32_t x_dtype, int64_t m,
                       int64_t ldx, int32_t prologue, float eps, void* const* outs, const int64_t* ldo,
                       int32_t epilogue, void* stream);

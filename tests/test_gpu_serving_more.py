@@ -1,4 +1,4 @@
-"""Batched decoding: a sequence's logits do not depend on what its neighbours hold."""
+"""Batched decoding: a sequence's logits do not depend on what its neighbours hold; batches of every size."""
 import pytest
 import torch
 from test_gpu_serving import DEV, TOLERANCE, _decoder, _gpu, _prompts  # noqa: F401 (_gpu: a fixture)
@@ -55,3 +55,36 @@ def test_rotation_has_the_tensor_formulas_gradient_bit_for_bit():
     want = torch.autograd.grad((formula(q), formula(k)), (q, k), (dq, dk))
     got = torch.autograd.grad(rotary.rope(q, k, pos, cos, sin), (q, k), (dq, dk))
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("hidden,batch", [(512, 11), (512, 12), (512, 16), (2048, 8), (2048, 9), (2048, 16), (2048, 17)])
+def test_batches_around_the_fused_limit(hidden, batch):
+    """The fused linears take 8 rows of 2048 features or 11 of 512; larger batches step all the same."""
+    dec = _decoder(hidden=hidden)
+    lengths = [2 + 3 * (i % 5) for i in range(batch)]
+    prompts, feed = _prompts(lengths), (torch.arange(2 * batch).view(2, batch) * 53) % 1000
+    got = _steps(dec, "same", prompts, feed)
+    f32 = dec.share_weights("fp32")
+    for i in (0, batch // 2, batch - 1):
+        f32.prefill(prompts[i])
+        for t in range(2):
+            want = f32.step(feed[t, i:i + 1].to(DEV), torch.tensor([lengths[i] + t], device=DEV))
+            assert float((got[t, i] - want).abs().max() / want.abs().max()) <= TOLERANCE["same"]
+
+
+@pytest.mark.parametrize("k", [512, 2048])
+def test_most_rows_of_the_fused_linears(k):
+    """What decode_linear_max_rows says is taken, and one row more is refused."""
+    from epure import _native, synthetic
+    st = [synthetic.make_store(64, k, device=torch.device(DEV), seed=s, gpu_layout="mma16") for s in (1, 2)]
+    for epilogue, stores in ((_native.EPI_STORE, st), (_native.EPI_SILU_MUL, st)):
+        rows = _native.decode_linear_max_rows(k, _native.PRO_RMSNORM, epilogue)
+        assert 1 <= rows <= 16
+        x = torch.randn(16, k, device=DEV).to(torch.bfloat16)
+        got = _native.decode_linear(x[:rows], stores, prologue=_native.PRO_RMSNORM, epilogue=epilogue)
+        one = _native.decode_linear(x[:1], stores, prologue=_native.PRO_RMSNORM, epilogue=epilogue)
+        for a, b in zip(got, one):
+            assert float((a[0] - b[0]).abs().max()) <= 2.0 ** -7 * float(b.abs().max())
+        if rows < 16:
+            with pytest.raises(RuntimeError, match=f"at most {rows} "):
+                _native.decode_linear(x[:rows + 1], stores, prologue=_native.PRO_RMSNORM, epilogue=epilogue)
