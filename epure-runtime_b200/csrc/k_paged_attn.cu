@@ -24,7 +24,7 @@
 //
 // Measured (B200, device time in a graph of calls): 1 x 131072 tokens, 32 / 8 heads of
 // 128, bf16: 90 us, 6.0 TB/s (93% of the measured copy rate); 64 sequences of up to 8192,
-// 64 / 8 heads, e4m3: 98 us, 5.8 TB/s; 16 of up to 4096, 32 / 8 heads, int8: 20 us, of
+// 64 / 8 heads, e4m3: 98 us, 5.7 TB/s; 16 of up to 4096, 32 / 8 heads, int8: 21 us, of
 // which 3 are the plan and first loads and 4 the last joins; 1 x 145: 6.4 us, a chain of
 // five dependent memory accesses and one join of warps.
 //
@@ -217,6 +217,8 @@ struct Shape {
     static constexpr int kRows = kTok * kPitch;                          // one of K, V
     static constexpr int kScales = kBytes == 1 ? 2 * kTok * 4 : 0;
     static constexpr int kStage = 2 * kRows + kScales;
+    // (Two columns of heads of 256 spill 216 to 448 bytes at 255 registers: 24 / 2 heads over
+    // 32 sequences of up to 8192 tokens take 80 us in bf16, where 16 / 2 heads, which do not, take 64.)
     static constexpr int kCtas = kPitch > 256 ? 1 : kPitch == 64 && kCols == 1 ? 3 : 2;       // an SM
     static constexpr int kMergePitch = kDim + 4;                         // floats; spreads a column's heads over the banks
     static constexpr int kMerge = kWarps * 8 * kMergePitch * 4;

@@ -86,7 +86,8 @@ constexpr int kAtOnce = 2;          // rows of a lane in flight
 
 // What a kernel takes for granted.  kExact: heads fill their lanes and passes, the whole
 // head turns (or none of it); kLanesOnly: partners are whole lanes; both: 16-byte loads
-// and stores.  kAny: nothing.
+// and stores.  kAny: nothing.  (8192 tokens of 32 + 8 + 8 heads of 128 to int8, us: kExact
+// 36 in bf16 and 64 in float32; kAny, bf16, interleaved 46, unaligned 58, 50 values turned 84.)
 enum Class { kExact = 0, kLanesOnly = 1, kAny = 2 };
 
 // Registers for 7 CTAs (28 warps) an SM: 64k rows of 48 heads took 376 us (with their
@@ -388,7 +389,8 @@ int launch_read_t(const ReadArgs& A, unsigned blocks, cudaStream_t st) {
 }
 
 // Warps a token: one, or as many as it has passes while there are too few tokens to give
-// every SM 32 warps.
+// every SM 32 warps.  (The bounded write kernels hold 28 of them, so some sizes end with a
+// round of their own: 2048 tokens of 16 + 8 + 8 heads have 3 warps each, 1.5 rounds.)
 int share_out(int64_t m, int64_t passes) {
     int64_t splits = cdiv((int64_t)device_sms() * 32, m);
     return (int)(splits < passes ? splits : passes);

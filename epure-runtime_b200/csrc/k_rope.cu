@@ -44,7 +44,8 @@ template <int N> __device__ __forceinline__ void load_table(float (&f)[N], const
 
 constexpr int kRopeThreads = 128;
 
-// Heads of one lane in flight: as many as keep about 64 bytes of it under way.  (Half
+// Heads of one lane in flight: as many as keep about 64 bytes of it under way, and 32 of
+// single 16-bit values and of interleaved float32.  (Half
 // layout in bf16, 16384 tokens: 83 us with 1, 70 with 2 and 4; interleaved 77 with 2, 68
 // with 4; single values, 8192 tokens: 139 with 2, 105 with 4.)
 template <typename T, int V, bool kInterleaved> constexpr int rope_heads() {

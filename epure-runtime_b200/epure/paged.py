@@ -59,7 +59,8 @@ def attend(pages, q, lengths, seq=None, scale=None, window=0, out=None, return_l
 class PagedKVCache:
     """The pools of every layer over one page table, and which pages are free.
 
-    ``format``: "same" (the activations' ``dtype``), "int8" or "fp8".  Pages are handed out by ``reserve(seq,
+    ``format``: "same" (the activations' ``dtype``; a float32 cache can be written and read, but not attended
+    over), "int8" or "fp8".  Pages are handed out by ``reserve(seq,
     tokens)`` and given back by ``release(seq)``; both change the table on the device in the current stream's
     order, so a captured step sees them at its next replay."""
 
