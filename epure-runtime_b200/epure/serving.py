@@ -66,7 +66,7 @@ class BatchDecoder:
         (``cache.reserve``).  Static shapes: capturable."""
         d, sh = self.decoder, self.shapes
         B, scale = tokens.shape[0], 1.0 / math.sqrt(sh.head_dim)
-        lengths = pos + 1
+        lengths = (pos + 1).clamp_(min=0)                              # idle rows have no tokens
         h = d.embed[tokens]                                            # residual stream [B, hidden]
         fused = B <= self._fused_rows
         y = None if fused else _native.add_rmsnorm(h, eps=d.eps)

@@ -88,3 +88,17 @@ def test_most_rows_of_the_fused_linears(k):
         if rows < 16:
             with pytest.raises(RuntimeError, match=f"at most {rows} "):
                 _native.decode_linear(x[:rows + 1], stores, prologue=_native.PRO_RMSNORM, epilogue=epilogue)
+
+
+def test_idle_rows_at_any_negative_position():
+    """They are no error, and leave the other rows as they are."""
+    from epure import _native
+    from epure.serving import BatchDecoder
+    b = BatchDecoder(_decoder(), seqs=3, format="int8", page_size=16)
+    b.prefill(1, _prompts([5])[0])
+    b.cache.reserve(1, 6)
+    tok, seq = torch.tensor([3, 4, 5], device=DEV), torch.arange(3, dtype=torch.int32, device=DEV)
+    want = b.step(tok, seq, torch.tensor([-1, 5, -1], device=DEV))
+    got = b.step(tok, seq, torch.tensor([-4, 5, -2 ** 40], device=DEV))
+    assert _native.device_error() == 0
+    assert torch.equal(got, want) and torch.isfinite(got).all()
