@@ -104,7 +104,8 @@ int epq_paged_read(const epq_pages* pages, const int32_t* seq, const int64_t* po
  * gives zeros and -inf, and so does a row whose every score is -inf.  q
  * [batch, heads, head_dim] is f16 or bf16 (4-byte aligned, even strides), and so is an
  * EPQ_CACHE_SAME cache; out [batch, heads, head_dim] is contiguous and
- * 16-byte aligned.  The workspace
+ * 16-byte aligned.  lengths and seq must not change while the call runs: its CTAs
+ * read them one by one, and share the work by them.  The workspace
  * (256-byte aligned) has to be zeroed once before its first use and is left ready for
  * the next call; calls that share one must not overlap.
  * units = kv_heads * ceil(heads / kv_heads / 16): batch * units <= 65536, and with
