@@ -98,7 +98,7 @@ def build_cpu(force=False, quiet=False):
 def build_torch(force=False, quiet=False):
     """_epq_torch.so: a CPython module over torch's headers and libraries; built again for another torch or Python,
     whose binary interface may be another."""
-    headers = [os.path.join(INCLUDE, h) for h in ("epq.h", "epq_paged.h")]
+    headers = [os.path.join(INCLUDE, h) for h in ("epq.h", "epq_paged.h", "epq_sampling.h")]
     newest = max(os.path.getmtime(f) for f in [TORCH_SRC, *headers])
     against = "\n".join((importlib.metadata.version("torch"), importlib.util.find_spec("torch").origin,
                          sysconfig.get_config_var("EXT_SUFFIX")))

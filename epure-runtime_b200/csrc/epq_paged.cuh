@@ -303,6 +303,9 @@ inline bool moved_in_place(const epq_heads& x, const epq_heads& y, int64_t m) {
 int rope_read_device_error(int* flag);
 int cache_read_device_error(int* flag);
 int attend_read_device_error(int* flag);
+int attend_blocks_read_device_error(int* flag);
+int shared_read_device_error(int* flag);
+int sparse_read_device_error(int* flag);
 
 }  // namespace paged
 }  // namespace epq

@@ -1,4 +1,4 @@
-// The Python binding of include/epq_paged.h: module epure._epq_torch.
+// The Python binding of include/epq_paged.h and include/epq_sampling.h: module epure._epq_torch.
 //
 // The calls of a decode step are a few microseconds of GPU work each, so what a call
 // costs on the host is what a small step costs.  These functions take tensors straight
@@ -26,6 +26,7 @@
 #include <string>
 
 #include "epq_paged.h"
+#include "epq_sampling.h"
 
 namespace {
 
@@ -54,6 +55,13 @@ struct Library {
     decltype(&epq_paged_read) read = nullptr;
     decltype(&epq_paged_attend) attend = nullptr;
     decltype(&epq_paged_attend_workspace_bytes) attend_bytes = nullptr;
+    decltype(&epq_paged_attend_blocks) attend_blocks = nullptr;
+    decltype(&epq_paged_attend_shared) attend_shared = nullptr;
+    decltype(&epq_paged_attend_shared_workspace_bytes) shared_bytes = nullptr;
+    decltype(&epq_paged_bounds) bounds = nullptr;
+    decltype(&epq_paged_select) select = nullptr;
+    decltype(&epq_paged_select_workspace_bytes) select_bytes = nullptr;
+    decltype(&epq_verify_drafts) verify = nullptr;
 } lib;
 
 template <typename F> void find(void* h, const char* name, F& f) {
@@ -362,45 +370,197 @@ PyObject* read(PyObject* const* a) {
     return wrap2(k, v);
 }
 
-// attend(k_pool, v_pool, table, k_scale, v_scale, q, lengths, seq | None, scale | None, window, out | None, return_lse)
-PyObject* attend(PyObject* const* a) {
-    const Cache c = cache_of(a);
-    Tensor q = tensor(a[5], "q");
-    const Tensor& lengths = tensor(a[6], "lengths");
-    const Tensor *seq = maybe(a[7], "seq"), *to = maybe(a[10], "out");
-    no_gradient("attend", {{&tensor(a[0], "k"), "the k pool"}, {&tensor(a[1], "v"), "the v pool"}, {maybe(a[3], "k_scale"), "k_scale"},
+// The tensors that the attentions have in common; `a` holds the cache, q and lengths, then what a form has of its own.
+struct Attention {
+    Cache c;
+    Tensor q, out, lse;
+    epq_heads heads;
+    const int64_t* lengths;
+    const int32_t* seq;
+    int64_t batch;
+    double scale;
+    int dtype;
+    Attention(PyObject* const* a, PyObject* seq_, PyObject* scale_, PyObject* out_, PyObject* lse_, const char* call)
+        : c(cache_of(a)), q(tensor(a[5], "q")) {
+        const Tensor& n = tensor(a[6], "lengths");
+        const Tensor *s = maybe(seq_, "seq"), *to = maybe(out_, "out");
+        no_gradient(call, {{&tensor(a[0], "k"), "the k pool"}, {&tensor(a[1], "v"), "the v pool"}, {maybe(a[3], "k_scale"), "k_scale"},
                            {maybe(a[4], "v_scale"), "v_scale"}, {&q, "q"}, {to, "out"}});
-    const at::ScalarType dt = q.scalar_type();
-    if (dt != at::kBFloat16 && dt != at::kHalf)
-        throw TypeProblem(text("paged attention takes float16 or bfloat16 queries, not ", dt));
-    if (c.p.format == EPQ_CACHE_SAME && c.dtype != dt) refuse("queries of ", dt, " for a cache of ", c.dtype);
-    OnDevice on(c.device);
-    epq_heads qh = heads_of(q, "q", c.device, dt, -1, -1, c.p.head_dim);
-    const int64_t B = q.size(0), H = q.size(1), hd = c.p.head_dim;
-    index_of(lengths, "lengths", c.device, at::kLong, B);
-    if (seq) index_of(*seq, "seq", c.device, at::kInt, B);
-    if (((uintptr_t)qh.data | (uintptr_t)(2 * qh.stride_row) | (uintptr_t)(2 * qh.stride_head)) % 4) {
-        q = q.clone(at::MemoryFormat::Contiguous);     // the kernel reads two values at a time
-        qh = heads_of(q, "q", c.device, dt, B, H, hd);
+        const at::ScalarType dt = q.scalar_type();
+        if (dt != at::kBFloat16 && dt != at::kHalf)
+            throw TypeProblem(text("paged attention takes float16 or bfloat16 queries, not ", dt));
+        if (c.p.format == EPQ_CACHE_SAME && c.dtype != dt) refuse("queries of ", dt, " for a cache of ", c.dtype);
+        heads = heads_of(q, "q", c.device, dt, -1, -1, c.p.head_dim);
+        batch = q.size(0);
+        const int64_t H = q.size(1), hd = c.p.head_dim;
+        lengths = index_of(n, "lengths", c.device, at::kLong, batch).const_data_ptr<int64_t>();
+        seq = s ? index_of(*s, "seq", c.device, at::kInt, batch).const_data_ptr<int32_t>() : nullptr;
+        if (to && (to->dim() != 3 || to->size(0) != batch || to->size(1) != H || to->size(2) != hd || to->scalar_type() != dt ||
+                   to->device() != c.device || !to->is_contiguous()))
+            refuse("out must be contiguous [", batch, ", ", H, ", ", hd, "], ", dt, " on ", c.device);
+        scale = scale_ == Py_None ? 1.0 / std::sqrt((double)hd) : number(scale_);
+        dtype = dtype_code(dt);
+        OnDevice on(c.device);
+        if (((uintptr_t)heads.data | (uintptr_t)(2 * heads.stride_row) | (uintptr_t)(2 * heads.stride_head)) % 4) {
+            q = q.clone(at::MemoryFormat::Contiguous);     // the kernel reads two values at a time
+            heads = heads_of(q, "q", c.device, dt, batch, H, hd);
+        }
+        given = to;
+        out = to ? *to : empty({batch, H, hd}, dt, c.device);
+        if (truth(lse_)) lse = empty({batch, H}, at::kFloat, c.device);
     }
-    if (to && (to->dim() != 3 || to->size(0) != B || to->size(1) != H || to->size(2) != hd || to->scalar_type() != dt ||
-               to->device() != c.device || !to->is_contiguous()))
-        refuse("out must be contiguous [", B, ", ", H, ", ", hd, "], ", dt, " on ", c.device);
-    const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)hd) : number(a[8]);
+    float* lse_to() const { return lse.defined() ? lse.data_ptr<float>() : nullptr; }
+    PyObject* results() const {
+        if (given) written(*given);
+        return lse.defined() ? wrap2(out, lse) : wrap(out);
+    }
+
+  private:
+    const Tensor* given;
+};
+
+// attend(k_pool, v_pool, table, k_scale, v_scale, q, lengths, seq | None, scale | None, window, out | None, return_lse,
+//        blocks | None)
+PyObject* attend(PyObject* const* a) {
     const int64_t window = integer(a[9]);
-    const bool with_lse = truth(a[11]);
-    const Tensor out = to ? *to : empty({B, H, hd}, dt, c.device);
-    const Tensor lse = with_lse ? empty({B, H}, at::kFloat, c.device) : Tensor();
-    const int64_t need = lib.attend_bytes(&c.p, B, (int32_t)H);
+    const Tensor* blocks = maybe(a[12], "blocks");
+    const Attention t(a, a[7], a[8], a[10], a[11], "attend");
+    const Cache& c = t.c;
+    if (blocks) {
+        if (blocks->dim() != 3 || blocks->size(0) != t.batch || blocks->size(1) != c.p.kv_heads || blocks->scalar_type() != at::kInt ||
+            blocks->device() != c.device || !blocks->is_contiguous() || blocks->size(2) > INT32_MAX)
+            refuse("blocks must be contiguous int32 [", t.batch, ", ", c.p.kv_heads, ", count] on ", c.device, "; got ",
+                   blocks->sizes(), ", ", blocks->scalar_type(), " on ", blocks->device());
+        if (window) refuse("attention over listed blocks has no window");
+    }
+    OnDevice on(c.device);
+    const int64_t need = lib.attend_bytes(&c.p, t.batch, t.heads.heads);
     if (need < 0) check((int)need, "epq_paged_attend_workspace_bytes");
     const cudaStream_t st = stream_of(c.device);
     const Tensor ws = workspace(c.device, st, need);
-    check(lib.attend(&c.p, &qh, seq ? seq->const_data_ptr<int32_t>() : nullptr, lengths.const_data_ptr<int64_t>(), B, (float)scale,
-                     window, out.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr, dtype_code(dt), ws.data_ptr(), ws.numel(),
-                     st),
-          "epq_paged_attend");
-    if (to) written(*to);
-    return with_lse ? wrap2(out, lse) : wrap(out);
+    if (blocks)
+        check(lib.attend_blocks(&c.p, &t.heads, t.seq, t.lengths, t.batch, blocks->const_data_ptr<int32_t>(),
+                                (int32_t)blocks->size(2), (float)t.scale, t.out.data_ptr(), t.lse_to(), t.dtype, ws.data_ptr(),
+                                ws.numel(), st),
+              "epq_paged_attend_blocks");
+    else
+        check(lib.attend(&c.p, &t.heads, t.seq, t.lengths, t.batch, (float)t.scale, window, t.out.data_ptr(), t.lse_to(), t.dtype,
+                         ws.data_ptr(), ws.numel(), st),
+              "epq_paged_attend");
+    return t.results();
+}
+
+// attend_shared(k_pool, v_pool, table, k_scale, v_scale, q, lengths, starts, prefix, seq | None, scale | None, out | None,
+//               return_lse)
+PyObject* attend_shared(PyObject* const* a) {
+    const Tensor &starts = tensor(a[7], "starts"), &prefix = tensor(a[8], "prefix");
+    const Attention t(a, a[9], a[10], a[11], a[12], "attend_shared");
+    const Cache& c = t.c;
+    const int64_t groups = prefix.dim() == 1 ? prefix.size(0) : -1;
+    index_of(prefix, "prefix", c.device, at::kLong, groups);
+    index_of(starts, "starts", c.device, at::kInt, groups + 1);
+    OnDevice on(c.device);
+    const int64_t need = lib.shared_bytes(&c.p, t.batch, t.heads.heads, groups);
+    if (need < 0) check((int)need, "epq_paged_attend_shared_workspace_bytes");
+    const cudaStream_t st = stream_of(c.device);
+    const Tensor ws = workspace(c.device, st, need);
+    check(lib.attend_shared(&c.p, &t.heads, t.seq, t.lengths, t.batch, starts.const_data_ptr<int32_t>(),
+                            prefix.const_data_ptr<int64_t>(), groups, (float)t.scale, t.out.data_ptr(), t.lse_to(), t.dtype,
+                            ws.data_ptr(), ws.numel(), st),
+          "epq_paged_attend_shared");
+    return t.results();
+}
+
+// The bounds of a cache's pages: [pages, kv_heads, 2, head_dim] of its own type, bfloat16 for 8-bit ones.
+int64_t check_bounds(const Tensor& t, const Cache& c) {
+    const at::ScalarType dt = c.p.format == EPQ_CACHE_SAME ? c.dtype : at::kBFloat16;
+    if (dt == at::kFloat) throw TypeProblem("epure: a float32 cache has no bounds");
+    const int64_t hd = c.p.head_dim, page = c.p.kv_heads * 2 * hd;
+    if (t.dim() != 4 || t.size(0) != c.p.pages || t.size(1) != c.p.kv_heads || t.size(2) != 2 || t.size(3) != hd ||
+        t.scalar_type() != dt || t.device() != c.device || step(t, 3, 1) != 1 || step(t, 2, hd) != hd || step(t, 1, 2 * hd) != 2 * hd)
+        refuse("bounds must be [", c.p.pages, ", ", c.p.kv_heads, ", 2, ", hd, "], ", dt, " on ", c.device,
+               ", the values of a page contiguous; got ", t.sizes(), ", ", t.scalar_type(), " on ", t.device());
+    return step(t, 0, page);
+}
+
+// bounds(k_pool, v_pool, table, k_scale, v_scale, bounds, lengths, seq | None, first | None)
+PyObject* bounds(PyObject* const* a) {
+    const Cache c = cache_of(a);
+    const Tensor &to = tensor(a[5], "bounds"), &lengths = tensor(a[6], "lengths");
+    const Tensor *seq = maybe(a[7], "seq"), *first = maybe(a[8], "first");
+    no_gradient("summarise", {{&tensor(a[0], "k"), "the k pool"}, {&tensor(a[1], "v"), "the v pool"}, {maybe(a[3], "k_scale"), "k_scale"},
+                              {maybe(a[4], "v_scale"), "v_scale"}, {&to, "bounds"}});
+    const int64_t stride = check_bounds(to, c), B = lengths.dim() == 1 ? lengths.size(0) : -1;
+    index_of(lengths, "lengths", c.device, at::kLong, B);
+    if (seq) index_of(*seq, "seq", c.device, at::kInt, B);
+    if (first) index_of(*first, "first", c.device, at::kLong, B);
+    OnDevice on(c.device);
+    check(lib.bounds(&c.p, to.data_ptr(), stride, dtype_code(to.scalar_type()), seq ? seq->const_data_ptr<int32_t>() : nullptr,
+                     first ? first->const_data_ptr<int64_t>() : nullptr, lengths.const_data_ptr<int64_t>(), B, stream_of(c.device)),
+          "epq_paged_bounds");
+    written(to);
+    Py_RETURN_NONE;
+}
+
+// select(k_pool, v_pool, table, k_scale, v_scale, bounds, q, lengths, count, seq | None, sinks, recent)
+PyObject* select(PyObject* const* a) {
+    const Cache c = cache_of(a);
+    const Tensor &from = tensor(a[5], "bounds"), &q = tensor(a[6], "q"), &lengths = tensor(a[7], "lengths");
+    const Tensor* seq = maybe(a[9], "seq");
+    const int64_t count = integer(a[8]), sinks = integer(a[10]), recent = integer(a[11]), most = INT32_MAX;
+    const int64_t stride = check_bounds(from, c);
+    const at::ScalarType dt = q.scalar_type();
+    if (dt != at::kBFloat16 && dt != at::kHalf) throw TypeProblem(text("selection takes float16 or bfloat16 queries, not ", dt));
+    const epq_heads qh = heads_of(q, "q", c.device, dt, -1, -1, c.p.head_dim);
+    const int64_t B = q.size(0);
+    index_of(lengths, "lengths", c.device, at::kLong, B);
+    if (seq) index_of(*seq, "seq", c.device, at::kInt, B);
+    if (count < 1 || sinks < 0 || recent < 0 || sinks > count || recent > count - sinks || count > most)
+        refuse("count=", count, " blocks with sinks=", sinks, " and recent=", recent, " (sinks + recent <= count)");
+    OnDevice on(c.device);
+    const int64_t need = lib.select_bytes(&c.p, B);
+    if (need < 0) check((int)need, "epq_paged_select_workspace_bytes");
+    const Tensor chosen = empty({B, c.p.kv_heads, count}, at::kInt, c.device);
+    const cudaStream_t st = stream_of(c.device);
+    const Tensor ws = workspace(c.device, st, need);
+    check(lib.select(&c.p, from.data_ptr(), stride, dtype_code(from.scalar_type()), &qh, dtype_code(dt),
+                     seq ? seq->const_data_ptr<int32_t>() : nullptr, lengths.const_data_ptr<int64_t>(), B, (int32_t)count,
+                     (int32_t)sinks, (int32_t)recent, chosen.data_ptr<int32_t>(), ws.data_ptr(), ws.numel(), st),
+          "epq_paged_select");
+    return wrap(chosen);
+}
+
+// verify(target, draft | None, tokens, uniforms)
+PyObject* verify(PyObject* const* a) {
+    const Tensor &p = tensor(a[0], "target"), &tokens = tensor(a[2], "tokens"), &u = tensor(a[3], "uniforms");
+    const Tensor* q = maybe(a[1], "draft");
+    if (!p.is_cuda()) refuse("verify needs CUDA tensors");
+    const at::Device dev = p.device();
+    const at::ScalarType dt = p.scalar_type();
+    const int code = dtype_code(dt);
+    if (p.dim() != 3 || p.size(1) < 1 || p.size(2) < 1 || step(p, 2, 1) != 1)
+        refuse("target must be [batch, drafts + 1, vocab] with contiguous rows; got ", p.sizes(), ", strides ", p.strides());
+    const int64_t B = p.size(0), K = p.size(1) - 1, V = p.size(2);
+    if (K > INT32_MAX) refuse(K, " drafts");
+    if (q && (q->dim() != 3 || q->size(0) != B || q->size(1) != K || q->size(2) != V || q->scalar_type() != dt || q->device() != dev ||
+              (q->numel() && step(*q, 2, 1) != 1)))
+        refuse("draft must be [", B, ", ", K, ", ", V, "] with contiguous rows, ", dt, " on ", dev, "; got ", q->sizes(), ", ",
+               q->scalar_type(), " on ", q->device());
+    if (tokens.dim() != 2 || tokens.size(0) != B || tokens.size(1) != K || tokens.scalar_type() != at::kLong || tokens.device() != dev ||
+        step(tokens, 1, 1) != 1)
+        refuse("tokens must be int64 [", B, ", ", K, "] on ", dev, ", rows contiguous; got ", tokens.sizes(), ", ",
+               tokens.scalar_type(), " on ", tokens.device());
+    if (u.dim() != 2 || u.size(0) != B || u.size(1) != K + 1 || u.scalar_type() != at::kFloat || u.device() != dev || step(u, 1, 1) != 1)
+        refuse("uniforms must be float32 [", B, ", ", K + 1, "] on ", dev, ", rows contiguous; got ", u.sizes(), ", ",
+               u.scalar_type(), " on ", u.device());
+    OnDevice on(dev);
+    const Tensor out = empty({B, K + 1}, at::kLong, dev), n = empty({B}, at::kLong, dev);
+    const epq_probs target = {p.data_ptr(), step(p, 0, 0), step(p, 1, 0)};
+    const epq_probs draft = q ? epq_probs{q->data_ptr(), step(*q, 0, 0), step(*q, 1, 0)} : epq_probs{};
+    check(lib.verify(&target, q ? &draft : nullptr, tokens.const_data_ptr<int64_t>(), step(tokens, 0, 0), u.const_data_ptr<float>(),
+                     step(u, 0, 0), B, (int32_t)K, V, code, out.data_ptr<int64_t>(), n.data_ptr<int64_t>(), stream_of(dev)),
+          "epq_verify_drafts");
+    return wrap2(out, n);
 }
 
 PyObject* out_of_memory = nullptr;         // torch.OutOfMemoryError
@@ -420,6 +580,13 @@ PyObject* bind(PyObject* const* a) {
     find(h, "epq_paged_read", lib.read);
     find(h, "epq_paged_attend", lib.attend);
     find(h, "epq_paged_attend_workspace_bytes", lib.attend_bytes);
+    find(h, "epq_paged_attend_blocks", lib.attend_blocks);
+    find(h, "epq_paged_attend_shared", lib.attend_shared);
+    find(h, "epq_paged_attend_shared_workspace_bytes", lib.shared_bytes);
+    find(h, "epq_paged_bounds", lib.bounds);
+    find(h, "epq_paged_select", lib.select);
+    find(h, "epq_paged_select_workspace_bytes", lib.select_bytes);
+    find(h, "epq_verify_drafts", lib.verify);
     Py_INCREF(a[1]);
     Py_XSETREF(out_of_memory, a[1]);
     Py_RETURN_NONE;
@@ -446,8 +613,10 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 #define EPQ_METHOD(name, n) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&call<name, n>)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {EPQ_METHOD(bind, 2),   EPQ_METHOD(rope, 9),    EPQ_METHOD(write, 16),
-                         EPQ_METHOD(read, 8),   EPQ_METHOD(attend, 12), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {EPQ_METHOD(bind, 2),    EPQ_METHOD(rope, 9),           EPQ_METHOD(write, 16),
+                         EPQ_METHOD(read, 8),    EPQ_METHOD(attend, 13),        EPQ_METHOD(attend_shared, 13),
+                         EPQ_METHOD(bounds, 9),  EPQ_METHOD(select, 12),        EPQ_METHOD(verify, 4),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_epq_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

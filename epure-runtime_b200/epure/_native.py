@@ -78,6 +78,10 @@ class EpqPages(ctypes.Structure):
     ]
 
 
+class EpqProbs(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_row", ctypes.c_int64), ("stride_step", ctypes.c_int64)]
+
+
 EXPORTS = (
     "epq_abi_version", "epq_last_error", "epq_device_error", "epq_layout_bytes",
     "epq_relayout", "epq_linear_workspace_bytes", "epq_linear_multi", "epq_linear",
@@ -88,7 +92,9 @@ EXPORTS = (
     "epq_embedding", "epq_decode_linear", "epq_decode_linear_max_rows", "epq_program_create", "epq_program_add_linear",
     "epq_program_add_attention", "epq_program_workspace_bytes", "epq_program_finalize", "epq_program_run",
     "epq_program_destroy", "epq_rope", "epq_paged_write", "epq_paged_read", "epq_paged_attend",
-    "epq_paged_attend_workspace_bytes",
+    "epq_paged_attend_workspace_bytes", "epq_paged_attend_blocks", "epq_paged_attend_shared",
+    "epq_paged_attend_shared_workspace_bytes", "epq_paged_bounds", "epq_paged_select",
+    "epq_paged_select_workspace_bytes", "epq_verify_drafts",
 )
 
 _lib = None
@@ -159,6 +165,16 @@ def load_library(path=None):
         lib.epq_paged_attend.argtypes = [PP, HP, P, P, I64, F32, I64, P, P, I32, P, I64, P]
         lib.epq_paged_attend_workspace_bytes.restype = I64
         lib.epq_paged_attend_workspace_bytes.argtypes = [PP, I64, I32]
+        lib.epq_paged_attend_blocks.argtypes = [PP, HP, P, P, I64, P, I32, F32, P, P, I32, P, I64, P]
+        lib.epq_paged_attend_shared.argtypes = [PP, HP, P, P, I64, P, P, I64, F32, P, P, I32, P, I64, P]
+        lib.epq_paged_attend_shared_workspace_bytes.restype = I64
+        lib.epq_paged_attend_shared_workspace_bytes.argtypes = [PP, I64, I32, I64]
+        lib.epq_paged_bounds.argtypes = [PP, P, I64, I32, P, P, P, I64, P]
+        lib.epq_paged_select.argtypes = [PP, P, I64, I32, HP, I32, P, P, I64, I32, I32, I32, P, P, I64, P]
+        lib.epq_paged_select_workspace_bytes.restype = I64
+        lib.epq_paged_select_workspace_bytes.argtypes = [PP, I64]
+        RP = ctypes.POINTER(EpqProbs)
+        lib.epq_verify_drafts.argtypes = [RP, RP, P, I64, P, I64, I64, I32, I64, I32, P, P, P]
         for name in EXPORTS:
             getattr(lib, name)          # every declared entry point must be exported
         if lib.epq_abi_version() != 1:
@@ -600,10 +616,10 @@ class DecodeProgram:
             _check(self.lib.epq_program_run(self._h, _stream_ptr(self.device)), "epq_program_run")
 
 
-# -- rotary positions, the paged cache and its attention (include/epq_paged.h) ---------------
+# -- rotary positions, the paged cache and its attention (include/epq_paged.h), drafts (include/epq_sampling.h) --
 # The calls of a batched decode step: module _epq_torch (csrc_torch/epq_torch.cpp) checks the
 # tensors and makes the C calls, because a call through ctypes costs more host time than the
-# kernels of a small step take.  epure.rotary and epure.paged are its callers.
+# kernels of a small step take.  epure.rotary, epure.paged and epure.sampling are its callers.
 
 tensor_calls = None
 

@@ -1,13 +1,14 @@
 """A paged key-value cache shared by several sequences, quantised as it is written, and the attention of one new
-token a sequence over it (include/epq_paged.h).
+token a row over it (include/epq_paged.h): over all of a row's tokens, over those of selected blocks, and for rows
+that share a prefix, which is then read once for all of them.
 
 The reference decodes one sequence through the Hugging Face model's own dense cache.  Here the keys and values of
 all sequences live in pools of pages; a page table maps token ``t`` of sequence ``s`` to slot ``t % page_size`` of
 page ``table[s, t // page_size]``.  A pool holds the activations' type, int8 or 8-bit floats (e4m3) with one
 float32 scale a token and head.
 
-``KVPages`` names the tensors of one layer; ``write``, ``read`` and ``attend`` are the operators on it.
-``PagedKVCache`` owns the pools of all layers and hands pages out.  The operators have no gradient: with grad mode
+``KVPages`` names the tensors of one layer; ``write``, ``read``, ``attend``, ``attend_shared``, ``summarise`` and
+``select`` are the operators on it.  ``PagedKVCache`` owns the pools of all layers and hands pages out.  The operators have no gradient: with grad mode
 on they refuse tensors that require one."""
 from typing import NamedTuple, Optional
 
@@ -46,14 +47,48 @@ def read(pages, seq, pos, dtype=None):
     return (_native.tensor_calls or _native.load_tensor_calls()).read(*pages, seq, pos, dtype)
 
 
-def attend(pages, q, lengths, seq=None, scale=None, window=0, out=None, return_lse=False):
+def attend(pages, q, lengths, seq=None, scale=None, window=0, out=None, return_lse=False, blocks=None):
     """Attention of one new token a sequence: q [batch, heads, head_dim] over the first ``lengths`` (int64 [batch])
     tokens of sequences ``seq`` (int32 [batch], default 0..batch-1), the last ``window`` of them where window > 0;
     ``scale`` defaults to head_dim ** -0.5.  Query head h reads key head h // (heads / kv_heads).  A length of 0
     gives zeros.  Returns out, or ``(out, lse)`` with the float32 log-sum-exp [batch, heads] of the scores
-    (-inf for an empty row), with which results over disjoint sets of tokens can be joined."""
+    (-inf for an empty row), with which results over disjoint sets of tokens can be joined.
+
+    ``blocks`` (int32 [batch, kv_heads, count], as ``select`` returns it) attends over the tokens of the listed pages
+    of a row's sequence alone, those below its length: page ``j`` holds tokens ``j * page_size`` on.  A list names
+    each page at most once and -1 for none; its first ``ceil(length / page_size)`` entries are looked at."""
     return (_native.tensor_calls or _native.load_tensor_calls()).attend(*pages, q, lengths, seq, scale, window, out,
-                                                                        return_lse)
+                                                                        return_lse, blocks)
+
+
+def attend_shared(pages, q, lengths, starts, prefix, seq=None, scale=None, out=None, return_lse=False):
+    """``attend`` where rows share their first tokens, which are read once for all of them.
+
+    Rows ``starts[g] .. starts[g + 1) - 1`` (int32 [groups + 1], ascending) have the same first ``prefix[g]`` (int64
+    [groups]) tokens: either their page tables name the same pages there (``PagedKVCache.share``), or they are rows of
+    one sequence (drafted tokens, a prompt's chunk) with lengths of their own.  The shared tokens are found through
+    the table of a group's first row.  A row shorter than its group's prefix attends over its own length, rows in no
+    group share nothing."""
+    return (_native.tensor_calls or _native.load_tensor_calls()).attend_shared(*pages, q, lengths, starts, prefix, seq,
+                                                                               scale, out, return_lse)
+
+
+def summarise(pages, bounds, lengths, seq=None, first=None):
+    """Brings ``bounds`` [pages, kv_heads, 2, head_dim] (of the pool's 16-bit type, bfloat16 for 8-bit pools) up to date:
+    the least and the largest of every value of the keys of each page that holds one of the new tokens ``first[b] ..
+    lengths[b] - 1`` (int64 [batch]; first None: from 0) of sequence ``seq[b]``, over the page's tokens below
+    ``lengths[b]``.  After a decode step ``first = lengths - 1``.  Rows with a page in common must agree about its
+    tokens."""
+    (_native.tensor_calls or _native.load_tensor_calls()).bounds(*pages, bounds, lengths, seq, first)
+
+
+def select(pages, bounds, q, lengths, count, seq=None, sinks=1, recent=1):
+    """The ``count`` blocks (pages) of each row and key head to attend over, int32 [batch, kv_heads, count] in ascending
+    order, -1 behind the last: the first ``sinks``, the last ``recent`` and those of the others in which a query head of
+    the key head may find the largest score, ``sum_d max(q_d lo_d, q_d hi_d)`` by their ``bounds`` (ties to the lowest
+    block).  q [batch, heads, head_dim] is what ``attend`` will be given."""
+    return (_native.tensor_calls or _native.load_tensor_calls()).select(*pages, bounds, q, lengths, count, seq, sinks,
+                                                                        recent)
 
 
 class PagedKVCache:
@@ -62,10 +97,11 @@ class PagedKVCache:
     ``format``: "same" (the activations' ``dtype``; a float32 cache can be written and read, but not attended
     over), "int8" or "fp8".  Pages are handed out by ``reserve(seq,
     tokens)`` and given back by ``release(seq)``; both change the table on the device in the current stream's
-    order, so a captured step sees them at its next replay."""
+    order, so a captured step sees them at its next replay.  ``share(seq, source, tokens)`` lets a sequence begin with
+    another's pages.  ``bounds=True`` holds room for ``summarise`` (``bounds[layer]``)."""
 
     def __init__(self, layers, pages, page_size, kv_heads, head_dim, seqs, max_tokens, format="same",
-                 dtype=torch.bfloat16, device="cuda"):
+                 dtype=torch.bfloat16, device="cuda", bounds=False):
         if format not in FORMATS:
             raise ValueError(f"epure: format must be one of {tuple(FORMATS)} (got {format!r})")
         if min(layers, pages, page_size, kv_heads, seqs, max_tokens) < 1:
@@ -82,9 +118,12 @@ class PagedKVCache:
         scales = format != "same"
         self.k_scale = torch.zeros(shape[:4], device=self.device) if scales else None
         self.v_scale = torch.zeros(shape[:4], device=self.device) if scales else None
+        self.bounds = torch.zeros(layers, pages, kv_heads, 2, head_dim, dtype=torch.bfloat16 if scales else dtype,
+                                  device=self.device) if bounds else None
         self.table = torch.full((seqs, -(-max_tokens // page_size)), -1, dtype=torch.int32, device=self.device)
         self._free = list(range(pages - 1, -1, -1))
         self._held = [[] for _ in range(seqs)]
+        self._users = [0] * pages                      # sequences that hold a page
 
     def layer(self, i):
         """Layer ``i``'s ``KVPages``."""
@@ -115,10 +154,34 @@ class PagedKVCache:
         self.table[seq, first:first + more] = torch.tensor(got, dtype=torch.int32).to(self.device)
         held += got                                    # behind the copy: where it raises, no page is lost
         del self._free[-more:]
+        for p in got:
+            self._users[p] = 1
+
+    def share(self, seq, source, tokens):
+        """Lets the empty sequence ``seq`` begin with the whole pages of the first ``tokens`` tokens of sequence
+        ``source``; returns how many tokens these are (a multiple of the page size).  They are not copied: neither
+        sequence may write them any more.  The others are ``seq``'s own to reserve and write."""
+        self._check(seq)
+        self._check(source)
+        if self._held[seq]:
+            raise ValueError(f"epure: sequence {seq} has pages; release it first")
+        if tokens < 0 or tokens > len(self._held[source]) * self.page_size:
+            raise ValueError(f"epure: {tokens} tokens of sequence {source}, which has room for "
+                             f"{len(self._held[source]) * self.page_size}")
+        whole = tokens // self.page_size
+        if whole:
+            self.table[seq, :whole] = self.table[source, :whole]
+            self._held[seq] = self._held[source][:whole]
+            for p in self._held[seq]:
+                self._users[p] += 1
+        return whole * self.page_size
 
     def release(self, seq):
-        """Gives sequence ``seq``'s pages back."""
+        """Gives sequence ``seq``'s pages back; one that others share stays theirs."""
         self._check(seq)
-        self._free += reversed(self._held[seq])
+        for p in reversed(self._held[seq]):
+            self._users[p] -= 1
+            if not self._users[p]:
+                self._free.append(p)
         self._held[seq] = []
         self.table[seq].fill_(-1)

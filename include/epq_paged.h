@@ -115,6 +115,56 @@ int epq_paged_attend(const epq_pages* pages, const epq_heads* q, const int32_t* 
                      int64_t batch, float scale, int64_t window, void* out, float* lse, int32_t dtype,
                      void* workspace, int64_t workspace_bytes, void* stream);
 
+/* epq_paged_attend where rows share their first tokens, which are read once for all of them:
+ * rows starts[g] .. starts[g + 1) - 1 (int32, groups + 1 of them, ascending) have the same
+ * prefix[g] first tokens, found through the page table of the first of these rows' sequences
+ * (the other rows' entries for them are not read, and have to name pages with the same tokens).
+ * A row whose length is below prefix[g] attends over its own length.  The rows may be sequences
+ * behind a common prompt or several new tokens of one sequence (rows of one seq with growing
+ * lengths).  Rows of no group share nothing.  Groups that are not ascending, or outside the
+ * batch, are reported (bit 4) and share nothing.  A workspace of its own bytes, with
+ * epq_paged_attend's rules. */
+int64_t epq_paged_attend_shared_workspace_bytes(const epq_pages* pages, int64_t batch, int32_t heads, int64_t groups);
+int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const int32_t* seq, const int64_t* lengths,
+                            int64_t batch, const int32_t* starts, const int64_t* prefix, int64_t groups, float scale, void* out,
+                            float* lse, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The bounds of a page's keys: bounds [pages][kv_heads][2][head_dim] hold, of every value of a
+ * head, the least and the largest over the page's tokens, in the cache's own 16-bit type or,
+ * for 8-bit caches (code * scale in float32), rounded to bf16; infinities are held as the
+ * largest finite value and NaN stays.  bounds_stride values lie between pages (a multiple of 8,
+ * 16-byte aligned).  For row b, tokens first[b] (NULL: 0) to lengths[b] - 1 of sequence
+ * s = seq ? seq[b] : b are new: every page that holds one of them gets the bounds of all its
+ * tokens below lengths[b].  Nothing is done where lengths[b] <= first[b].  Two rows with a page
+ * in common must agree about its tokens. */
+int epq_paged_bounds(const epq_pages* pages, void* bounds, int64_t bounds_stride, int32_t dtype, const int32_t* seq,
+                     const int64_t* first, const int64_t* lengths, int64_t batch, void* stream);
+
+/* The blocks (pages) to attend over, by a score that no q . K[t] of a block's tokens passes:
+ *     score(j) = max over the query heads h of key head g of
+ *                sum_d max(q[b, h, d] lo_j[d], q[b, h, d] hi_j[d])
+ * in float32, products first, then neighbouring dims' sums, then neighbours of those (head_dim
+ * padded with zeros to a power of two).  Of the n = ceil(lengths[b] / page_size) blocks of a row
+ * chosen[b, g, 0..count) receives, in ascending order, the first `sinks`, the last `recent` and
+ * those of the others with the largest scores (NaN first), the lowest of equal ones; all of them
+ * where n <= count, and -1 behind the last.  A block whose page is outside the pool comes last.
+ * The workspace is epq_paged_attend's in its rules, and the two may share one on a stream.
+ * batch * kv_heads <= 65536. */
+int64_t epq_paged_select_workspace_bytes(const epq_pages* pages, int64_t batch);
+int epq_paged_select(const epq_pages* pages, const void* bounds, int64_t bounds_stride, int32_t bounds_dtype,
+                     const epq_heads* q, int32_t dtype, const int32_t* seq, const int64_t* lengths, int64_t batch,
+                     int32_t count, int32_t sinks, int32_t recent, int32_t* chosen, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+
+/* epq_paged_attend over the tokens of listed blocks: blocks [batch, kv_heads, count] names pages
+ * of the row's sequence for each key head (token t is in block t / page_size), each at most
+ * once, -1 for none; of a list the first min(count, ceil(lengths[b] / page_size)) entries are
+ * looked at.  Tokens at lengths[b] and behind are not attended over.  A block at or past
+ * max_pages is skipped and reported (bit 4).  No window. */
+int epq_paged_attend_blocks(const epq_pages* pages, const epq_heads* q, const int32_t* seq, const int64_t* lengths,
+                            int64_t batch, const int32_t* blocks, int32_t count, float scale, void* out, float* lse,
+                            int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
