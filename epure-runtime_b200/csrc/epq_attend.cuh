@@ -1,11 +1,13 @@
 // The attention kernel of one new token a row over a paged cache, for every form of it: all
-// tokens of a row's sequence (k_paged_attn.cu, which holds the description), or those of
-// selected blocks (k_paged_attn_blocks.cu).  Each file instantiates its own form.
+// tokens of a row's sequence (k_paged_attn.cu, which holds the description), those of selected
+// blocks (k_paged_attn_blocks.cu), or those behind a shared prefix (k_paged_attn_shared.cu).
+// Each file instantiates its own form.
 #pragma once
 
 #include <cfloat>
 
 #include "epq_paged.cuh"
+#include "epq_shared.cuh"
 
 namespace epq {
 namespace paged {
@@ -23,6 +25,7 @@ struct AttendArgs {
     int64_t window;
     const int32_t* blocks;   // kListed: [batch][kv_heads][count] pages of the sequence, -1: none
     int count;
+    SharedD shared;          // kBehindShared
     int batch, heads, group, chunks, dtype;
     float scale_log2;
 };
@@ -30,7 +33,8 @@ struct AttendArgs {
 // Which tokens a row attends over.
 enum Mode {
     kAllTokens = 0,      // the first lengths[b] of its sequence (the last `window` of them)
-    kListed = 1          // those of the blocks (pages) that a list of each row and key head names
+    kListed = 1,         // those of the blocks (pages) that a list of each row and key head names
+    kBehindShared = 2    // those from row_from[b] on; the others' sums are joined from records
 };
 
 namespace {
@@ -156,6 +160,7 @@ template <int kMode, int kTok> __device__ __forceinline__ Span span_of(const Att
     s.limit = s.n = (int)n;
     s.lo = 0;
     if (kMode == kAllTokens && A.window > 0 && n > A.window) s.lo = (int)(n - A.window);
+    if (kMode == kBehindShared) s.lo = min(A.shared.row_from[b], s.n);
     if (kMode == kListed && s.n > 0) s.n = min(A.count, A.pages.page_of(s.n - 1) + 1) * A.pages.page_size;
     s.first = s.lo & ~(kTok - 1);
     s.blocks = (s.n - s.first + kTok - 1) / kTok;
@@ -219,6 +224,75 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
     return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
+// Four values of a row's head: sums `val` of weights relative to 2^at and their sum `sum` relative to 2^to, divided
+// and written; sum = 0: every score was -inf.
+template <int kMode, bool kQuant>
+__device__ __forceinline__ void emit_row(const AttendArgs& A, int b, int h, int d, const float (&val)[4], float at, float to,
+                                         float sum) {
+    float v[4] = {val[0], val[1], val[2], val[3]};
+    float gain;
+    if (kMode == kBehindShared) {
+        const int tile = A.shared.row_tile[b];
+        if (kQuant && sum != 0.f) {
+            const float turn = ex2(at - to);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] *= turn;
+        }
+        if (sum == 0.f) to = -FLT_MAX;
+        if (tile >= 0 && A.shared.row_from[b] > 0) {   // the records of the pieces of the row's unit
+            const SharedTile T = A.shared.tiles[tile];
+            const int head = h / A.group, row = (b - T.row0) * A.group + h - head * A.group;
+            const int64_t first = T.first + (int64_t)head * T.blocks, run = A.shared.head->run;
+            const int64_t c0 = quotient(first, run), c1 = quotient(first + T.blocks - 1, run);
+            const int two = shared_alternates(T.rows * A.group, A.shared.slots) ? 2 : 1, pieces = (int)(c1 - c0 + 1) * two;
+            const int pitch = A.shared.pitch;
+            const int64_t own = ((int64_t)b * A.heads + h) * pitch;
+            auto record = [&](int p) {
+                const int64_t c = c0 + (two == 2 ? p >> 1 : p);
+                const int slot = two == 2 ? p & 1 : row / kSharedLanes, lane = two == 2 ? row : row % kSharedLanes;
+                return c == c0 ? A.shared.own + (two == 2 ? slot * A.shared.own_records * pitch : 0) + own
+                               : A.shared.cut + ((c * 2 + slot) * kSharedLanes + lane) * pitch;
+            };
+            constexpr int kAtOnce = 4;
+            for (int p0 = 0; p0 < pieces; p0 += kAtOnce) {
+                float2 ml[kAtOnce];
+                float4 a[kAtOnce];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const float* rec = record(min(p0 + i, pieces - 1));
+                    ml[i] = __ldcg(reinterpret_cast<const float2*>(rec + pitch - 4));
+                    a[i] = __ldcg(reinterpret_cast<const float4*>(rec + d));
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    if (p0 + i >= pieces || ml[i].x == -FLT_MAX) continue;     // a piece without a score above -inf
+                    const float top = fmaxf(to, ml[i].x), f = to == top ? 1.f : ex2(to - top);
+                    const float g = ml[i].x == top ? 1.f : ex2(ml[i].x - top);
+                    sum = sum * f + ml[i].y * g;
+                    v[0] = v[0] * f + a[i].x * g;
+                    v[1] = v[1] * f + a[i].y * g;
+                    v[2] = v[2] * f + a[i].z * g;
+                    v[3] = v[3] * f + a[i].w * g;
+                    to = top;
+                }
+            }
+        }
+        gain = sum == 0.f ? 0.f : 1.f / sum;
+    } else {
+        gain = sum == 0.f ? 0.f : 1.f / sum;
+        if (kQuant) gain *= ex2(at - to);
+    }
+    uint2 o;
+    if (A.dtype == EPQ_BF16) {
+        o = make_uint2(pack<true>(v[0] * gain, v[1] * gain), pack<true>(v[2] * gain, v[3] * gain));
+    } else {
+        o = make_uint2(pack<false>(v[0] * gain, v[1] * gain), pack<false>(v[2] * gain, v[3] * gain));
+    }
+    const int64_t place = (int64_t)b * A.heads + h;
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(A.out) + place * A.pages.head_dim + d) = o;
+    if (A.lse && d == 0) A.lse[place] = sum == 0.f ? -INFINITY : (to + log2f(sum)) / kLog2e;
+}
+
 template <int kMode, int kKind, int kDim, int kCols>
 __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) attend_kernel(const AttendArgs A) {
     using S = Shape<kKind, kDim, kCols>;
@@ -272,6 +346,12 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     some_empty = __any_sync(kAll, some_empty);
     for (int b = blockIdx.x; some_empty && b < A.batch; b += gridDim.x) {
         if (span_of<kMode, kTok>(A, b, false).blocks) continue;
+        if (kMode == kBehindShared) {                  // nothing but the shared tokens, if any
+            const float none[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int e = tid; e < A.heads * (hd / 4); e += kThreads)
+                emit_row<kMode, kQuant>(A, b, e / (hd / 4), e % (hd / 4) * 4, none, -FLT_MAX, -FLT_MAX, 0.f);
+            continue;
+        }
         for (int e = tid; e < A.heads * hd; e += kThreads)
             static_cast<uint16_t*>(A.out)[(int64_t)b * A.heads * hd + e] = 0;
         if (A.lse)
@@ -725,18 +805,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         float* const merge = reinterpret_cast<float*>(smem + kWarps * S::kRing);
         constexpr int kQuads = kDim / 4;               // of a head's dims
         auto emit = [&](int h, int d, const float (&val)[4], float mx, float Mx, float sum) {
-            // sum = 0: every score was -inf.  16-bit caches: M = m, and sum is lifted as the weights are.
-            float gain = sum == 0.f ? 0.f : 1.f / sum;
-            if (kQuant) gain *= ex2(Mx - kLift - mx);
-            uint2 o;
-            if (A.dtype == EPQ_BF16) {
-                o = make_uint2(pack<true>(val[0] * gain, val[1] * gain), pack<true>(val[2] * gain, val[3] * gain));
-            } else {
-                o = make_uint2(pack<false>(val[0] * gain, val[1] * gain), pack<false>(val[2] * gain, val[3] * gain));
-            }
-            const int64_t to = (int64_t)seq_b * A.heads + h_first + h;
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(A.out) + to * hd + d) = o;
-            if (A.lse && d == 0) A.lse[to] = sum == 0.f ? -INFINITY : (mx - kSumLift + log2f(sum)) / kLog2e;
+            emit_row<kMode, kQuant>(A, seq_b, h_first + h, d, val, kQuant ? Mx - kLift : mx - kSumLift, mx - kSumLift, sum);
         };
         // none where the unit is whole; else where the piece's record goes
         float* const record = !cut ? nullptr
@@ -907,6 +976,8 @@ int read_attend_error(int* flag) {
 int make_attend(const char* who, const epq_pages* pages, const epq_heads* q, const int32_t* seq, const int64_t* lengths,
                 int64_t batch, float scale, void* out, float* lse, int32_t dtype, void* workspace, int64_t workspace_bytes,
                 AttendArgs* A, int* cols, bool* ready);
+// The form over all of a row's tokens (k_paged_attn.cu).
+int launch_attend_plain(const AttendArgs& A, int cols, cudaStream_t st);
 // Bytes of an attention's workspace: counters and records.
 int64_t attend_bytes(const char* who, const epq_pages* pages, int64_t batch, int32_t heads);
 

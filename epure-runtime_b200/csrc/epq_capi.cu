@@ -119,6 +119,7 @@ int cache_read_device_error(int* flag);
 int attend_read_device_error(int* flag);
 int attend_blocks_read_device_error(int* flag);
 int shared_read_device_error(int* flag);
+int shared_read_timeout(int* flag);
 int sparse_read_device_error(int* flag);
 }  // namespace paged
 namespace sampling {
@@ -171,10 +172,15 @@ int epq_device_error(int* flag) {
         if (rc) return rc;
         paged_bad |= found;
     }
+    int shared_wait = 0;
+    rc = paged::shared_read_timeout(&shared_wait);
+    if (rc) return rc;
+    bwd = bwd || shared_wait;
     int draft = 0;
     rc = sampling::verify_read_device_error(&draft);
     if (rc) return rc;
-    // bit 0: LUT placement check; bit 1: a bounded wait gave up (GEMV, GEMM, backward or chain);
+    // bit 0: LUT placement check; bit 1: a bounded wait gave up (GEMV, GEMM, backward, chain or
+    // attention behind a shared prefix);
     // bit 2: the chain kernel's placement or grid check failed; bit 3: an embedding id was
     // outside the store's rows, or a drafted token outside the vocabulary; bit 4: a decode position was at or past the KV cache's capacity
     // (or, for the paged cache, a position, length or sequence outside it); bit 5: a page

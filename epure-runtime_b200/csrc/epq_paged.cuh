@@ -305,6 +305,7 @@ int cache_read_device_error(int* flag);
 int attend_read_device_error(int* flag);
 int attend_blocks_read_device_error(int* flag);
 int shared_read_device_error(int* flag);
+int shared_read_timeout(int* flag);
 int sparse_read_device_error(int* flag);
 
 }  // namespace paged

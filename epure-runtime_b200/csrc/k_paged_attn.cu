@@ -51,6 +51,8 @@ int64_t records_bytes(int hd, int group) {
 
 int attend_read_device_error(int* flag) { return read_attend_error(flag); }
 
+int launch_attend_plain(const AttendArgs& A, int cols, cudaStream_t st) { return launch_attend_mode<kAllTokens>(A, cols, st); }
+
 int64_t attend_bytes(const char* who, const epq_pages* pages, int64_t batch, int32_t heads) {
     PagesD P;
     const int rc = make_pages(pages, &P, who);
@@ -132,7 +134,7 @@ int epq_paged_attend(const epq_pages* pages, const epq_heads* q, const int32_t* 
                                workspace_bytes, &A, &cols, &ready);
     if (rc != EPQ_OK || !ready) return rc;
     A.window = window;
-    return launch_attend_mode<kAllTokens>(A, cols, static_cast<cudaStream_t>(stream));
+    return launch_attend_plain(A, cols, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -66,8 +66,8 @@ def attend_shared(pages, q, lengths, starts, prefix, seq=None, scale=None, out=N
 
     Rows ``starts[g] .. starts[g + 1) - 1`` (int32 [groups + 1], ascending) have the same first ``prefix[g]`` (int64
     [groups]) tokens: either their page tables name the same pages there (``PagedKVCache.share``), or they are rows of
-    one sequence (drafted tokens, a prompt's chunk) with lengths of their own.  The shared tokens are found through
-    the table of a group's first row.  A row shorter than its group's prefix attends over its own length, rows in no
+    one sequence (drafted tokens, a prompt's chunk) with lengths of their own.  The shared tokens are
+    read through the table of one of the rows.  A row shorter than its group's prefix attends over its own length, rows in no
     group share nothing."""
     return (_native.tensor_calls or _native.load_tensor_calls()).attend_shared(*pages, q, lengths, starts, prefix, seq,
                                                                                scale, out, return_lse)

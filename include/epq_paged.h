@@ -117,13 +117,14 @@ int epq_paged_attend(const epq_pages* pages, const epq_heads* q, const int32_t* 
 
 /* epq_paged_attend where rows share their first tokens, which are read once for all of them:
  * rows starts[g] .. starts[g + 1) - 1 (int32, groups + 1 of them, ascending) have the same
- * prefix[g] first tokens, found through the page table of the first of these rows' sequences
- * (the other rows' entries for them are not read, and have to name pages with the same tokens).
- * A row whose length is below prefix[g] attends over its own length.  The rows may be sequences
+ * prefix[g] first tokens: their sequences' tables name pages that hold the same values there,
+ * and those of one of the rows are read for all.  A row whose length is below prefix[g] attends over its own length.  The rows may be sequences
  * behind a common prompt or several new tokens of one sequence (rows of one seq with growing
- * lengths).  Rows of no group share nothing.  Groups that are not ascending, or outside the
- * batch, are reported (bit 4) and share nothing.  A workspace of its own bytes, with
- * epq_paged_attend's rules. */
+ * lengths).  Rows of no group share nothing; where starts are not ascending or outside the batch,
+ * or a prefix is not in 0..max_pages * page_size, that is reported (bit 4) and none does.  Which
+ * rows are taken together, and whether any are, follows from sizes and lengths alone.
+ * batch <= 65536; a workspace of its own bytes, with epq_paged_attend's rules.
+ * epq_device_error bit 1: a wait of the kernel's own gave up. */
 int64_t epq_paged_attend_shared_workspace_bytes(const epq_pages* pages, int64_t batch, int32_t heads, int64_t groups);
 int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const int32_t* seq, const int64_t* lengths,
                             int64_t batch, const int32_t* starts, const int64_t* prefix, int64_t groups, float scale, void* out,
