@@ -241,15 +241,16 @@ __device__ __forceinline__ void emit_row(const AttendArgs& A, int b, int h, int 
         if (sum == 0.f) to = -FLT_MAX;
         if (tile >= 0 && A.shared.row_from[b] > 0) {   // the records of the pieces of the row's unit
             const SharedTile T = A.shared.tiles[tile];
-            const int head = h / A.group, row = (b - T.row0) * A.group + h - head * A.group;
+            const int head = h / A.group, rows = A.shared.lane_rows;
+            const int part = (b - T.row0) / rows, lane = (b - T.row0 - part * rows) * A.group + h - head * A.group;
             const int64_t first = T.first + (int64_t)head * T.blocks, run = A.shared.head->run;
             const int64_t c0 = quotient(first, run), c1 = quotient(first + T.blocks - 1, run);
-            const int two = shared_alternates(T.rows * A.group, A.shared.slots) ? 2 : 1, pieces = (int)(c1 - c0 + 1) * two;
+            const int two = shared_alternates(T.rows, rows, A.shared.slots) ? 2 : 1, pieces = (int)(c1 - c0 + 1) * two;
             const int pitch = A.shared.pitch;
             const int64_t own = ((int64_t)b * A.heads + h) * pitch;
             auto record = [&](int p) {
                 const int64_t c = c0 + (two == 2 ? p >> 1 : p);
-                const int slot = two == 2 ? p & 1 : row / kSharedLanes, lane = two == 2 ? row : row % kSharedLanes;
+                const int slot = two == 2 ? p & 1 : part;
                 return c == c0 ? A.shared.own + (two == 2 ? slot * A.shared.own_records * pitch : 0) + own
                                : A.shared.cut + ((c * 2 + slot) * kSharedLanes + lane) * pitch;
             };

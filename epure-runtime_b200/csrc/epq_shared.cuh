@@ -14,7 +14,7 @@ constexpr int kSharedLanes = 128;          // query rows (row, head of the group
 // Rows [row0, row0 + rows) of the batch, all of which (but the empty ones) see tokens [0, tokens) of sequence seq.
 // A unit is a tile and a key head; its blocks are dealt out from place first + head * blocks on.
 struct SharedTile {
-    int row0, rows, seq, tokens, blocks, group;
+    int row0, rows, seq, tokens, blocks, reserved0;
     int64_t first;
 };
 struct SharedHead {
@@ -34,11 +34,11 @@ struct SharedD {
     float* own;
     float* cut;
     int64_t own_records;                   // batch * heads
-    int pitch, slots;                      // slots: tensor-core tiles of a unit
+    int pitch, slots, lane_rows;           // slots: tensor-core tiles of a unit; lane_rows: rows that one holds
 };
 
 // Whether a unit's blocks go to two accumulators in turn (its rows fill one tensor-core tile at most).
-__host__ __device__ inline bool shared_alternates(int query_rows, int slots) { return slots == 2 && query_rows <= kSharedLanes; }
+__host__ __device__ inline bool shared_alternates(int rows, int lane_rows, int slots) { return slots == 2 && rows <= lane_rows; }
 
 }  // namespace paged
 }  // namespace epq

@@ -429,6 +429,21 @@ int make_tmap_2d_plain(CUtensorMap* map, const void* base, int elem_bytes, int64
     return EPQ_OK;
 }
 
+int make_tmap_3d(CUtensorMap* map, const void* base, int elem_bytes, const int64_t (&dims)[3], int64_t ld1, int64_t ld2,
+                 const int (&box)[3], bool swizzle, const char* who) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
+    if (!enc) return set_error(EPQ_EUNSUPPORTED, "%s: cuTensorMapEncodeTiled is unavailable", who);
+    const cuuint64_t gdim[3] = {(cuuint64_t)dims[0], (cuuint64_t)dims[1], (cuuint64_t)dims[2]};
+    const cuuint64_t gstride[2] = {(cuuint64_t)ld1 * elem_bytes, (cuuint64_t)ld2 * elem_bytes};
+    const cuuint32_t b[3] = {(cuuint32_t)box[0], (cuuint32_t)box[1], (cuuint32_t)box[2]}, estride[3] = {1, 1, 1};
+    const CUresult cr = enc(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
+                            const_cast<void*>(base), gdim, gstride, b, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS) return set_error(EPQ_EINVAL, "%s: tensor map (error %d)", who, (int)cr);
+    return EPQ_OK;
+}
+
 namespace {
 
 

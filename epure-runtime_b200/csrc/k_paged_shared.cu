@@ -14,9 +14,9 @@
 //
 // Shared part.  Blocks of 128 tokens of all units (tile, key head) are dealt out to the CTAs in
 // equal runs, one CTA an SM, and each piece of a unit leaves its sums as records.  In a CTA:
-//   * 4 loader warps look up pages and bring rows of K and V into a ring of shared-memory stages
-//     in the 128-byte swizzle, 16-bit rows by cp.async, codes of 8-bit caches through registers
-//     to 16 bits (exact);
+//   * one warp looks up pages and copies Q and the rows of K and V (TMA boxes of up to 128 rows
+//     of a page, a lane a box) into shared memory in the 128-byte swizzle; rows of 8-bit caches
+//     pass through four more warps that widen them to 16 bits (exact);
 //   * one thread issues the products: S = Q K^T (Q, K in shared memory) and O += P V (P in tensor
 //     memory, V as the MN-major operand);
 //   * 4 warps a slot take a row a thread: maximum, weights, sum; P goes back in place of S.
@@ -31,6 +31,7 @@
 // The running maximum moves only when a score passes it by 2^8.
 #include "epq_attend.cuh"
 #include "epq_sm100.cuh"
+#include <cuda.h>
 
 namespace epq {
 namespace paged {
@@ -44,7 +45,8 @@ __device__ int g_shared_error = 0;         // kBadPosition, kBadPage
 __device__ int g_shared_timeout = 0;       // a bounded wait gave up
 
 constexpr unsigned kWarpAll = 0xffffffffu;
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 512;
+constexpr int kHeldTiles = 512;            // tiles that the plan keeps in shared memory
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr int kSmemLimit = 232448;         // 227 KB a CTA
 // Bytes of reading that sharing has to save: the plan and the shared part's launch cost about as
@@ -54,15 +56,16 @@ constexpr int64_t kWorth = 32 << 20;
 struct SharedArgs {
     PagesD pages;
     SharedD s;
-    const void* q;
-    int64_t q_row, q_head;
     const int32_t* seq;
     const int64_t* lengths;
     const int32_t* starts;
     const int64_t* prefix;
     int64_t token_bytes;                   // of one cached token: keys, values, scales
-    int batch, groups, heads, group, tile_rows, max_tiles, grid, q_aligned;
+    int batch, groups, heads, group, max_tiles, grid, box_rows;
     float scale_log2;
+};
+struct Maps {                              // q [batch][heads][head_dim], the pools [pages][heads, slots][head_dim]
+    CUtensorMap q, k, v;
 };
 
 // ---------------------------------------------------------------- plan
@@ -76,7 +79,7 @@ __device__ int64_t block_scan(int64_t v, int64_t* shared, int64_t* total) {
     }
     if (lane == 31) shared[warp] = v;
     __syncthreads();
-    int64_t w = shared[lane];
+    int64_t w = lane < kPlanThreads / 32 ? shared[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int64_t u = __shfl_up_sync(kWarpAll, w, o);
@@ -90,10 +93,13 @@ __device__ int64_t block_scan(int64_t v, int64_t* shared, int64_t* total) {
 
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const SharedArgs A) {
     __shared__ int64_t scratch[32];
+    __shared__ SharedTile held[kHeldTiles];
     pdl_enter();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const PagesD& P = A.pages;
     const int64_t cap = (int64_t)P.max_pages * P.page_size;
+    const int tile_rows = A.s.slots * A.s.lane_rows;
+    SharedTile* const tile = A.max_tiles <= kHeldTiles ? held : A.s.tiles;     // (written out at the end)
     // rows that are neither empty nor bad (which the last launch reports)
     auto counts = [&](int b) {
         const int64_t n = A.lengths[b];
@@ -106,24 +112,26 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const SharedArgs A) 
     }
     // groups to tiles
     bool good = true;
-    for (int g = tid; g < A.groups; g += kPlanThreads)
-        good = good && A.starts[g] >= 0 && A.starts[g] <= A.starts[g + 1] && A.starts[g + 1] <= A.batch && A.prefix[g] >= 0 &&
-               A.prefix[g] <= cap;
+    for (int g = tid; g < A.groups; g += kPlanThreads) {
+        const int from = A.starts[g], to = A.starts[g + 1];
+        const int64_t p = A.prefix[g];
+        good = good && from >= 0 && from <= to && to <= A.batch && p >= 0 && p <= cap;
+    }
     good = __syncthreads_and(good);
     if (!good && tid == 0) atomicOr(&g_shared_error, kBadPosition);
     int64_t tiles = 0;
     for (int g0 = 0; good && g0 < A.groups; g0 += kPlanThreads) {
         const int g = g0 + tid;
         const int from = g < A.groups ? A.starts[g] : 0, rows = g < A.groups ? A.starts[g + 1] - from : 0;
-        const int count = rows >= 2 ? (rows + A.tile_rows - 1) / A.tile_rows : 0;
+        const int count = rows >= 2 ? (rows + tile_rows - 1) / tile_rows : 0;
         int64_t all;
         int64_t at = tiles + block_scan(count, scratch, &all) - count;
         for (int i = 0; i < count && at < A.max_tiles; ++i, ++at) {
             SharedTile T = {};
-            T.row0 = from + i * A.tile_rows;
-            T.rows = min(A.tile_rows, from + rows - T.row0);
-            T.group = g;
-            A.s.tiles[at] = T;
+            T.row0 = from + i * tile_rows;
+            T.rows = min(tile_rows, from + rows - T.row0);
+            T.tokens = (int)A.prefix[g];
+            tile[at] = T;
         }
         tiles += all;
     }
@@ -132,25 +140,22 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const SharedArgs A) 
     // what each tile's rows share
     int64_t saved = 0;
     for (int t = warp; t < tiles; t += kPlanThreads / 32) {
-        SharedTile T = A.s.tiles[t];
-        int active = 0, first = INT32_MAX;
-        int64_t least = A.prefix[T.group];
+        const SharedTile T = tile[t];
+        int active = 0, first = INT32_MAX, least = T.tokens;
         for (int r = lane; r < T.rows; r += 32) {
             if (!counts(T.row0 + r)) continue;
             ++active;
             first = min(first, r);
-            least = min(least, A.lengths[T.row0 + r]);
+            least = (int)min((int64_t)least, A.lengths[T.row0 + r]);
         }
         active = __reduce_add_sync(kWarpAll, active);
         first = __reduce_min_sync(kWarpAll, first);
-        least = __reduce_min_sync(kWarpAll, (int)least);
+        least = active < 2 ? 0 : __reduce_min_sync(kWarpAll, least);
         if (lane == 0) {
             const int b = T.row0 + first;
-            T.seq = active < 2 ? 0 : A.seq ? A.seq[b] : b;
-            T.tokens = active < 2 ? 0 : (int)least;
-            T.blocks = (T.tokens + kSharedTokens - 1) / kSharedTokens;
-            A.s.tiles[t] = T;
-            saved += (int64_t)(active - 1) * T.tokens;
+            tile[t].seq = active < 2 ? 0 : A.seq ? A.seq[b] : b;
+            tile[t].tokens = least;
+            saved += (int64_t)(active - 1) * least;
         }
     }
     int64_t all_saved;
@@ -160,23 +165,24 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const SharedArgs A) 
     int64_t total = 0;
     for (int t0 = 0; t0 < tiles; t0 += kPlanThreads) {
         const int t = t0 + tid;
-        const int64_t mine = worth && t < tiles ? (int64_t)A.s.tiles[t].blocks * P.kv_heads : 0;
+        const int blocks = worth && t < tiles ? (tile[t].tokens + kSharedTokens - 1) / kSharedTokens : 0;
+        const int64_t mine = (int64_t)blocks * P.kv_heads;
         int64_t all;
         const int64_t at = total + block_scan(mine, scratch, &all) - mine;
         if (t < tiles) {
-            A.s.tiles[t].first = at;
-            if (!worth) A.s.tiles[t].blocks = 0;
+            SharedTile T = tile[t];
+            T.blocks = blocks;
+            T.first = at;
+            A.s.tiles[t] = T;
         }
         total += all;
     }
     if (tid == 0) *A.s.head = {total, (int)max((int64_t)1, (total + A.grid - 1) / A.grid), (int)tiles};
-    __syncthreads();
     for (int t = warp; worth && t < tiles; t += kPlanThreads / 32) {
-        const SharedTile T = A.s.tiles[t];
-        for (int r = lane; T.blocks && r < T.rows; r += 32) {
-            const int b = T.row0 + r;
-            A.s.row_tile[b] = t;
-            A.s.row_from[b] = counts(b) ? T.tokens : 0;
+        const SharedTile T = tile[t];                                  // (what it needs of T is there since the first part)
+        for (int r = lane; T.tokens && r < T.rows; r += 32) {
+            A.s.row_tile[T.row0 + r] = t;
+            A.s.row_from[T.row0 + r] = counts(T.row0 + r) ? T.tokens : 0;
         }
     }
 }
@@ -186,20 +192,25 @@ enum Codes { kNone = 0, kInts = 1, kFloats = 2 };
 
 template <int kCodes, int kDim> struct Cfg {
     static constexpr int kSlots = kDim == 256 ? 1 : 2;
-    static constexpr int kLoaderWarps = 4;
-    static constexpr int kMmaWarp = kSlots * 4;
-    static constexpr int kThreads = (kMmaWarp + 1 + kLoaderWarps) * 32;
+    static constexpr int kConvertWarps = kCodes ? 4 : 0;
+    static constexpr int kMmaWarp = kSlots * 4 + kConvertWarps, kLoadWarp = kMmaWarp + 1;
+    static constexpr int kThreads = (kLoadWarp + 1) * 32;
     static constexpr int kBuf = kSharedTokens * kDim * 2;              // K or V of a block
     static constexpr int kSlab = kSharedTokens * 128;                  // 64 values of each of its rows
     static constexpr int kQ = kSlots * kSharedLanes * kDim * 2;
-    static constexpr int kRing = 8;                                    // blocks whose masks and scales are kept
+    static constexpr int kRaw = kCodes ? kSharedTokens * kDim : 0;     // codes of K or V of a block
+    static constexpr int kRawStages = kCodes ? 3 : 0;
+    // Blocks whose masks and scales are kept: a block's are written once its K has a stage, when the items that are
+    // kStages stages back have been multiplied, and so the softmax of all before them is done.
+    static constexpr int kRing = kCodes ? 4 : 8;
     static constexpr int kScales = kCodes ? kRing * 2 * kSharedTokens * 4 : 0;
-    static constexpr int kPagesAt = kScales, kMasksAt = kPagesAt + 2 * kSharedTokens * 4, kBarsAt = kMasksAt + kRing * 16;
-    static constexpr int kMisc = kBarsAt + 224;
-    static constexpr int kFit = (kSmemLimit - 1024 - kMisc - kQ) / kBuf;
-    static constexpr int kStages = kFit > 8 ? 8 : kFit;
-    static constexpr int kQAt = kStages * kBuf, kMiscAt = kQAt + kQ, kSmem = 1024 + kMiscAt + kMisc;
-    static_assert(kStages >= 2 && kSmem <= kSmemLimit, "shared memory");
+    static constexpr int kMasksAt = kScales, kBarsAt = kMasksAt + kRing * 16;
+    static constexpr int kMisc = kBarsAt + 304;
+    static constexpr int kFit = (kSmemLimit - 1024 - kMisc - kQ - kRawStages * kRaw) / kBuf, kMost = kCodes ? 4 : 8;
+    static constexpr int kStages = kFit > kMost ? kMost : kFit;
+    static constexpr int kQAt = kStages * kBuf, kRawAt = kQAt + kQ, kMiscAt = kRawAt + kRawStages * kRaw;
+    static constexpr int kSmem = 1024 + kMiscAt + kMisc;
+    static_assert(kStages >= (kSlots == 2 ? 3 : 2) && kSmem <= kSmemLimit, "shared memory");
 };
 
 // A unit's piece in this CTA: blocks [i, i + n) of tile T for key head h.
@@ -225,71 +236,114 @@ __device__ __forceinline__ void next_piece(const SharedArgs& A, Piece& p) {
     }
 }
 
-__device__ __forceinline__ void cp_wait_all_but(int left) {            // groups that may still be on their way
-    switch (left) {
-        case 0: cp_wait<0>(); break;
-        case 1: cp_wait<1>(); break;
-        case 2: cp_wait<2>(); break;
-        default: cp_wait<3>(); break;
+// Codes of 8-bit caches as 16-bit values, exactly: four of them as two pairs.
+template <int kCodes, bool kBf> __device__ __forceinline__ void widen(uint32_t x, uint32_t& p0, uint32_t& p1) {
+    if constexpr (kCodes == kInts && kBf) {
+        // 0x43 above a byte is 128 + its low 7 bits, or 256 + them; taking off 128, or 256 where the byte's top bit is
+        // set, leaves its low 7 bits, less 128 where it is
+        const uint32_t w0 = __byte_perm(x, 0x43434343u, 0x4140), w1 = __byte_perm(x, 0x43434343u, 0x4342);
+        auto value = [](uint32_t w) {
+            const uint32_t a = w & 0xff7fff7fu, b = w & 0xff80ff80u;
+            const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+            return *reinterpret_cast<const uint32_t*>(&r);
+        };
+        p0 = value(w0);
+        p1 = value(w1);
+    } else {
+        codes_f16<kCodes == kInts ? kInt8 : kFp8, false>(x, p0, p1);
+        if (kBf) {
+            const float2 a = unpack2<__half>(p0), b = unpack2<__half>(p1);
+            p0 = pack2<__nv_bfloat16>(a.x, a.y);
+            p1 = pack2<__nv_bfloat16>(b.x, b.y);
+        }
+    }
+}
+
+// Weights as pairs of 16-bit values and of what these leave.  bf16: the upper half of a float32 is one, without its lower
+// bits, and no conversion is needed; two such parts keep 16 bits or more (the second is rounded down too: at most 2^-15).
+template <bool kBf> __device__ __forceinline__ void split(const float (&w)[32], uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float a = w[2 * i], b = w[2 * i + 1];
+        if (kBf) {
+            const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+            hi[i] = __byte_perm(x, y, 0x7632);
+            const float c = a - __uint_as_float(x & 0xffff0000u), d = b - __uint_as_float(y & 0xffff0000u);
+            lo[i] = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x7632);
+        } else {
+            hi[i] = pack2<__half>(a, b);
+            const float2 back = unpack2<__half>(hi[i]);
+            lo[i] = pack2<__half>(a - back.x, b - back.y);
+        }
     }
 }
 
 // kBfQ: S in bf16 (else f16); kBfV: P and V in bf16 (else f16).
 template <int kCodes, bool kBfQ, bool kBfV, int kDim>
-__global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1) shared_kernel(const SharedArgs A) {
+__global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
+    shared_kernel(const SharedArgs A, const __grid_constant__ Maps maps) {
     using C = Cfg<kCodes, kDim>;
     using namespace sm100;
-    using TQ = typename Half<kBfQ>::type;
-    using TV = typename Half<kBfV>::type;
     constexpr int S_ = C::kStages, kSlots = C::kSlots;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const PagesD& P = A.pages;
     const int hd = P.head_dim, gh = A.group, ps = P.page_size;
-
-    const SharedHead head = *A.s.head;
-    Piece first;
-    first.at = (int64_t)blockIdx.x * head.run;
-    first.end = min(head.total, first.at + head.run);
-    if (first.at >= head.total) return;
 
     const uint32_t raw = sm100::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* const gen = smem_raw + (base - raw);
     uint8_t* const misc = gen + C::kMiscAt;
     float* const scales = reinterpret_cast<float*>(misc);              // [kRing][2][128]: of keys, of values
-    int32_t* const page_of_row = reinterpret_cast<int32_t*>(misc + C::kPagesAt);       // [2][128], -1: no token
     uint32_t* const masks = reinterpret_cast<uint32_t*>(misc + C::kMasksAt);           // [kRing][4]
     const uint32_t bars = base + C::kMiscAt + C::kBarsAt;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 64u + 8u * s; };
-    auto s_full = [&](int s) { return bars + 128u + 8u * s; };
-    auto p_full = [&](int s) { return bars + 144u + 8u * s; };
-    auto o_done = [&](int s) { return bars + 160u + 8u * s; };
-    const uint32_t q_free = bars + 176u, over = bars + 184u, tslot = bars + 192u, looked_up = bars + 208u;
-    volatile int* const abortp = reinterpret_cast<volatile int*>(misc + C::kBarsAt + 196);
-    volatile int* const where = reinterpret_cast<volatile int*>(misc + C::kBarsAt + 200);
+    auto raw_full = [&](int s) { return bars + 128u + 8u * s; };
+    auto raw_empty = [&](int s) { return bars + 160u + 8u * s; };
+    auto s_full = [&](int s) { return bars + 192u + 8u * s; };
+    auto p_full = [&](int s) { return bars + 208u + 8u * s; };
+    auto o_done = [&](int s) { return bars + 224u + 8u * s; };
+    const uint32_t q_full = bars + 240u, q_free = bars + 248u, over = bars + 256u, part_full = bars + 264u, tslot = bars + 272u;
+    volatile int* const abortp = reinterpret_cast<volatile int*>(misc + C::kBarsAt + 280);
+    volatile int* const where = reinterpret_cast<volatile int*>(misc + C::kBarsAt + 284);
     auto wait = [&](uint32_t bar, uint32_t parity) {
         return mbar_wait_bounded(bar, parity & 1u, abortp, &g_shared_timeout, kWaitLimit);
     };
+    // every lane, or none
+    auto wait_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(kWarpAll, wait(bar, parity)); };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S_; ++s) {
-            mbar_init(full(s), C::kLoaderWarps * 32);
+            mbar_init(full(s), kCodes ? C::kConvertWarps * 32 : 1);
             mbar_init(empty(s), 1);
+        }
+        for (int s = 0; s < C::kRawStages; ++s) {
+            mbar_init(raw_full(s), 1);
+            mbar_init(raw_empty(s), C::kConvertWarps * 32);
         }
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(s_full(s), 2);                                   // the products' end, and the issuing thread
             mbar_init(p_full(s), 128);
             mbar_init(o_done(s), 1);
         }
+        mbar_init(q_full, 1);
         mbar_init(q_free, 1);
         mbar_init(over, 1);
-        mbar_init(looked_up, C::kLoaderWarps * 32);
+        mbar_init(part_full, 1);
         *abortp = 0;
         mbar_init_fence();
     }
+    if (warp == C::kLoadWarp && lane == 0) {
+        tma_prefetch_desc(&maps.q);
+        tma_prefetch_desc(&maps.k);
+        tma_prefetch_desc(&maps.v);
+    }
     if (warp == C::kMmaWarp) tmem_alloc(tslot, 512);
+    pdl_enter();                                                       // (nothing above reads what the plan writes)
+    const SharedHead head = *A.s.head;
+    Piece first;
+    first.at = (int64_t)blockIdx.x * head.run;
+    first.end = min(head.total, first.at + head.run);
     if (warp == 0) {                                                   // the tile of the first piece
         int t = 0;
         for (int t0 = 0; t0 < head.tiles; t0 += 32) {
@@ -303,215 +357,143 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1) shared_kernel(
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(misc + C::kBarsAt + 192);
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(misc + C::kBarsAt + 272);
     first.t = *where;
     first.c = 0;
-    {
+    first.h = 0;
+    if (first.at < first.end) {
         const SharedTile T = A.s.tiles[first.t];
         first.h = (int)((first.at - T.first) / T.blocks);
     }
     const uint32_t q_at = base + C::kQAt;
     constexpr uint32_t kOCol = kSlots * 128u;                          // S and P of slot s in columns 128 s, O behind them
+    auto alternates = [&](const SharedTile& T) { return kSlots == 1 || shared_alternates(T.rows, A.s.lane_rows, kSlots); };
 
-    if (warp > C::kMmaWarp) {
-        // ------------------------------------------------------------ loaders
-        const int tid = threadIdx.x - (C::kMmaWarp + 1) * 32;          // 0..127
-        // a thread's chunks (16 bytes of a row of the cache): chunk ch of rows row0, row0 + kStep, ...
-        constexpr int kChunks = kDim * (kCodes ? 1 : 2) / 16, kStep = 128 / kChunks, kEach = 128 / kStep;
-        const int ch = tid % kChunks, row0 = tid / kChunks;
-        const bool on = ch * 16 < hd * (kCodes ? 1 : 2);
-        int filled = 0, arrived = 0;                                   // stages
-        constexpr int kLag = S_ - 2 < 3 ? S_ - 2 : 3;
-        bool ok = true;
-        auto arrive_to = [&](int most) {                               // all but `most` of the filled stages are there
-            if (filled - arrived <= most) return;
-            cp_wait_all_but(most);
-            fence_async_smem();
-            while (filled - arrived > most) mbar_arrive(full(arrived++ % S_));
-        };
-        auto open = [&]() {                                            // the next stage, once it is free
-            const int s = filled % S_;
-            bool got = true;
-            if (filled >= S_ && !mbar_try_wait(empty(s), ((filled / S_) - 1) & 1)) {
-                if (!kCodes) arrive_to(0);                             // (the one that frees it may wait for them)
-                got = wait(empty(s), (filled / S_) - 1);
-            }
-            ok = __all_sync(kWarpAll, got);
-            return base + s * C::kBuf;
-        };
-        // this thread's row of the next block: its page's number is on its way
-        int32_t next_page = -1;
-        auto look_up = [&](const SharedTile& T, int block) {
-            const int t = block * kSharedTokens + tid;
-            next_page = t < T.tokens ? P.table[(int64_t)T.seq * P.table_stride + P.page_of(t)] : -1;
-            return t < T.tokens;
-        };
-        bool next_on = false;
-        Piece p = first;
-        int blocks = 0;                                                // before this piece
-        for (; ok && piece_at(A, p); next_piece(A, p)) {
-            const int q_rows = p.T.rows * gh;
-            if (p.c) {
-                if (!kCodes) arrive_to(0);
-                ok = __all_sync(kWarpAll, wait(q_free, p.c - 1));
-                if (!ok) break;
-            }
-            // q, with the first keys: rows (row of the batch, head of the group)
-            {
-                constexpr int kQChunks = kDim / 8, kQStep = 128 / kQChunks;
-                const int qc = tid % kQChunks, inv = (65536 + gh - 1) / gh;
-                const int rows = kSlots == 2 && !shared_alternates(q_rows, kSlots) ? 256 : 128;
-                const bool dims = qc * 8 < hd;
-                for (int r = tid / kQChunks; r < rows; r += kQStep) {
-                    const int b = (r * inv) >> 16, j = r - b * gh;
-                    const bool there = dims && r < q_rows;
-                    const uint16_t* from = static_cast<const uint16_t*>(A.q) +
-                                           (there ? (p.T.row0 + b) * A.q_row + (p.h * gh + j) * A.q_head + qc * 8 : 0);
-                    const uint32_t to = q_at + (r / 128) * (128 * kDim * 2) + (qc / 8) * C::kSlab + (r % 128) * 128 +
-                                        (((qc % 8) ^ (r & 7)) * 16);
-                    if (A.q_aligned) {
-                        cp16(to, from, there ? 16 : 0);
-                    } else {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = there ? reinterpret_cast<const uint32_t*>(from)[i] : 0u;
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                                     : "memory");
-                    }
-                }
-                if (kCodes) {
-                    cp_commit();
-                    cp_wait<0>();
-                }
-            }
-            next_on = look_up(p.T, p.i);
-            for (int k = 0; ok && k < p.n; ++k) {
-                const int block = p.i + k, entry = (blocks + k) % C::kRing;
-                // pages of the block's rows for all loaders; which rows are tokens for the softmax
-                int32_t page = next_page;
-                if (next_on && (page < 0 || page >= P.pages)) {
-                    atomicOr(&g_shared_error, kBadPage);
-                    page = -1;
-                }
-                int32_t* const table = page_of_row + ((blocks + k) & 1) * kSharedTokens;
-                table[tid] = page;
-                const unsigned seen = __ballot_sync(kWarpAll, page >= 0);
-                float ks = 0.f, vs = 0.f;
-                if (kCodes && page >= 0) {
-                    const int t = block * kSharedTokens + tid, slot = t - P.page_of(t) * ps;
-                    const int64_t at = page * P.scale_stride + (int64_t)p.h * ps + slot;
-                    ks = P.k_scale[at];
-                    vs = P.v_scale[at];
-                }
-                mbar_arrive(looked_up);
-                ok = __all_sync(kWarpAll, wait(looked_up, blocks + k));
-                if (!ok) break;
-                if (k + 1 < p.n) next_on = look_up(p.T, block + 1);
-                auto row_at = [&](int r, bool& there) -> int64_t {     // first value of row r of this head
-                    const int32_t pg = table[r];
-                    const int t = block * kSharedTokens + r, slot = t - P.page_of(t) * ps;
-                    there = pg >= 0 && on;
-                    return there ? pg * P.page_stride + ((int64_t)p.h * ps + slot) * hd : 0;
-                };
-                if constexpr (kCodes == kNone) {
-                    uint32_t to[2];
-                    to[0] = open();
-                    if (!ok) break;
-                    if (lane == 0) masks[entry * 4 + tid / 32] = seen;
+    if (warp >= kSlots * 4 + C::kConvertWarps) {
+        if (warp == C::kLoadWarp) {
+            // -------------------------------------------------------- loads: a lane a box of rows of one page
+            const int R = A.box_rows, boxes = kSharedTokens / R;
+            constexpr int kSlabs = kDim / 64;
+            const bool mine = lane < boxes;
+            int fills = 0, parts = 0;                                  // stages filled; blocks that end inside
+            bool ok = true;
+            int32_t next_page = -1;
+            auto look_up = [&](const SharedTile& T, int block) {       // the page of this lane's box; it is on its way
+                const int t = block * kSharedTokens + lane * R;
+                next_page = mine && t < T.tokens ? P.table[(int64_t)T.seq * P.table_stride + P.page_of(t)] : -1;
+            };
+            auto open = [&](uint32_t bar, int f, int ring) {           // fill f's stage of a ring, once it is free
+                ok = f < ring || wait_all(bar, f / ring - 1);
+                return ok;
+            };
+            Piece p = first;
+            for (; ok && piece_at(A, p); next_piece(A, p)) {
+                look_up(p.T, p.i);
+                for (int k = 0; ok && k < p.n; ++k) {
+                    const int block = p.i + k, t0 = block * kSharedTokens + lane * R;
+                    const bool inside = mine && t0 < p.T.tokens;
+                    const int32_t page = next_page;
+                    const bool there = inside && page >= 0 && page < P.pages;
+                    if (inside && !there) atomicOr(&g_shared_error, kBadPage);
+                    if (k + 1 < p.n) look_up(p.T, block + 1);
+                    const int y = there ? p.h * ps + t0 - P.page_of(t0) * ps : 0;
+                    const int count = __popc(__ballot_sync(kWarpAll, there));
+                    // (an 8-bit block's rows that are no tokens are zeroed where the codes are widened)
+                    const bool whole = kCodes || (count == boxes && (block + 1) * kSharedTokens <= p.T.tokens);
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
-                        if (kv) to[1] = open();
-                        if (!ok) break;
-                        const uint8_t* const pool = kv ? P.v : P.k;
-#pragma unroll 4
-                        for (int e = 0; e < kEach; ++e) {
-                            const int r = row0 + e * kStep;
-                            bool there;
-                            const int64_t at = row_at(r, there);
-                            if (on)
-                                cp16(to[kv] + (ch / 8) * C::kSlab + r * 128 + (((ch % 8) ^ (r & 7)) * 16), pool + at * 2 + (there ? ch * 16 : 0),
-                                     there ? 16 : 0);
-                        }
-                        cp_commit();
-                        ++filled;
-                        arrive_to(kLag);
-                    }
-                } else {
-                    constexpr int kHalf = kEach > 8 ? 8 : kEach;       // chunks in registers at once
-                    uint4 x[2][kHalf];
-                    auto fetch = [&](int kv, int e0) {
-                        const uint8_t* const pool = kv ? P.v : P.k;
-#pragma unroll
-                        for (int e = 0; e < kHalf; ++e) {
-                            bool there;
-                            const int64_t at = row_at(row0 + (e0 + e) * kStep, there);
-                            x[kv][e] = there ? __ldg(reinterpret_cast<const uint4*>(pool + at) + ch) : make_uint4(0, 0, 0, 0);
-                        }
-                    };
-                    auto put = [&](int kv, int e0, uint32_t to) {
-#pragma unroll
-                        for (int e = 0; e < kHalf; ++e) {
-                            const int r = row0 + (e0 + e) * kStep;
-                            const uint32_t w[4] = {x[kv][e].x, x[kv][e].y, x[kv][e].z, x[kv][e].w};
-                            uint32_t o[8];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                codes_f16<kCodes == kInts ? kInt8 : kFp8, false>(w[i], o[2 * i], o[2 * i + 1]);
-                                if (kv ? kBfV : kBfQ) {                // exact: codes have at most 8 significant bits
-#pragma unroll
-                                    for (int j = 0; j < 2; ++j) {
-                                        const float2 f = unpack2<__half>(o[2 * i + j]);
-                                        o[2 * i + j] = pack2<__nv_bfloat16>(f.x, f.y);
+                        const CUtensorMap* const map = kv ? &maps.v : &maps.k;
+                        if constexpr (kCodes) {
+                            const int s = fills % C::kRawStages;
+                            if (!open(raw_empty(s), fills, C::kRawStages)) break;
+                            if (lane == 0) mbar_expect_tx(raw_full(s), count * R * hd);
+                            __syncwarp();
+                            if (there) tma_load_3d(base + C::kRawAt + s * C::kRaw + lane * R * hd, map, raw_full(s), 0, y, page);
+                        } else {
+                            const int s = fills % S_;
+                            if (!open(empty(s), fills, S_)) break;
+                            const uint32_t to = base + s * C::kBuf;
+                            if (kv == 0) {                             // which rows are tokens
+                                const int seen = there ? min(R, p.T.tokens - t0) : 0;
+                                if (whole) {
+                                    if (lane < 4) masks[(fills / 2 % C::kRing) * 4 + lane] = kWarpAll;
+                                } else {
+                                    for (int w = 0; w < 4; ++w) {      // (boxes of 8 to 128 rows)
+                                        uint32_t bits = 0;
+                                        const int r0 = lane * R - 32 * w, r1 = r0 + seen;
+                                        if (seen && r1 > 0 && r0 < 32) {
+                                            bits = r1 >= 32 ? kWarpAll : (1u << r1) - 1;
+                                            if (r0 > 0) bits &= ~((1u << r0) - 1);
+                                        }
+                                        bits = __reduce_or_sync(kWarpAll, bits);
+                                        if (lane == 0) masks[(fills / 2 % C::kRing) * 4 + w] = bits;
                                     }
                                 }
                             }
-                            if (on) {
-                                const uint32_t row = to + (ch / 4) * C::kSlab + r * 128;
+                            // a value of a row that is no token must be finite: such a block's V is patched first
+                            const uint32_t bar = kv && !whole ? part_full : full(s);
+                            __syncwarp();
+                            if (lane == 0) mbar_expect_tx(bar, count * R * 128 * kSlabs);
+                            __syncwarp();
+                            if (there)
 #pragma unroll
-                                for (int i = 0; i < 2; ++i)
-                                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + ((((2 * ch + i) % 8) ^ (r & 7)) * 16)),
-                                                 "r"(o[4 * i]), "r"(o[4 * i + 1]), "r"(o[4 * i + 2]), "r"(o[4 * i + 3]) : "memory");
+                                for (int x = 0; x < kSlabs; ++x)
+                                    tma_load_3d(to + x * C::kSlab + lane * R * 128, map, bar, 64 * x, y, page);
+                            if (kv && !whole) {
+                                ok = wait_all(part_full, parts++);
+                                if (!ok) break;
+                                const unsigned good = __ballot_sync(kWarpAll, there);
+                                for (int r = lane; r < kSharedTokens; r += 32)
+                                    if (!(good >> (r / R) & 1) || block * kSharedTokens + r >= p.T.tokens)
+                                        for (int x = 0; x < kSlabs * 8; ++x)
+                                            *reinterpret_cast<uint4*>(gen + s * C::kBuf + (x / 8) * C::kSlab + r * 128 + (x % 8) * 16) =
+                                                make_uint4(0, 0, 0, 0);
+                                fence_async_smem();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(full(s));
                             }
                         }
-                    };
-                    fetch(0, 0);
-                    if (kEach == kHalf) fetch(1, 0);
-#pragma unroll
-                    for (int kv = 0; kv < 2; ++kv) {
-                        const uint32_t to = open();
-                        if (!ok) break;
-                        if (kv == 0) {
-                            if (lane == 0) masks[entry * 4 + tid / 32] = seen;
-                            scales[(entry * 2) * kSharedTokens + tid] = ks;
-                            scales[(entry * 2 + 1) * kSharedTokens + tid] = vs;
+                        ++fills;
+                        if (k == 0 && kv == 0) {                       // q, behind the first keys
+                            if (p.c) {
+                                ok = wait_all(q_free, p.c - 1);
+                                if (!ok) break;
+                            }
+                            const int tiles = alternates(p.T) ? 1 : kSlots;
+                            if (lane == 0) {
+                                mbar_expect_tx(q_full, tiles * kSlabs * A.s.lane_rows * gh * 128);
+                                for (int t = 0; t < tiles; ++t)
+                                    for (int x = 0; x < kSlabs; ++x)
+                                        tma_load_3d(q_at + t * (128 * kDim * 2) + x * C::kSlab, &maps.q, q_full, 64 * x, p.h * gh,
+                                                    p.T.row0 + t * A.s.lane_rows);
+                            }
                         }
-#pragma unroll
-                        for (int e0 = 0; e0 < kEach; e0 += kHalf) {
-                            if (kEach != kHalf && (kv || e0)) fetch(kv, e0);
-                            put(kv, e0, to);
-                        }
-                        fence_async_smem();
-                        mbar_arrive(full(filled % S_));
-                        ++filled;
                     }
                 }
             }
-            blocks += p.n;
-        }
-        if (!kCodes) arrive_to(0);
-        asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp == C::kMmaWarp) {
-        // ------------------------------------------------------------ products
-        if (lane == 0) {
-            constexpr uint32_t s_desc = idesc_f16<kBfQ, 128, kSharedTokens>();
-            constexpr uint32_t o_desc = idesc_f16<kBfV, 128, kDim, false, true>();
+            // the copies in flight land before the CTA ends (their barriers are those that the others wait for; after
+            // a wait that gave up nobody may have)
+            if (!ok) {
+                for (int s = 0; s < (kCodes ? C::kRawStages : S_); ++s)
+                    for (int f = fills - 1; f >= 0 && f >= fills - (kCodes ? C::kRawStages : S_); --f)
+                        if (f % (kCodes ? C::kRawStages : S_) == s)
+                            for (uint32_t i = 0; i < kWaitLimit; ++i)
+                                if (mbar_try_wait(kCodes ? raw_full(s) : full(s), (f / (kCodes ? C::kRawStages : S_)) & 1)) break;
+            }
+        } else if (warp == C::kMmaWarp && lane == 0) {
+            // -------------------------------------------------------- products
+            constexpr uint32_t s_idesc = idesc_f16<kBfQ, 128, kSharedTokens>();
+            constexpr uint32_t o_idesc = idesc_f16<kBfV, 128, kDim, false, true>();
+            const uint64_t q_desc = desc_kmajor_sw128(q_at), k_desc = desc_kmajor_sw128(base);
+            const uint64_t v_desc = desc_mnmajor_sw128(base, C::kSlab, 1024);
             int count[2] = {0, 0};                                     // products with P that a slot has had
             int fills = 0;                                             // stages before this piece
             bool ok = true;
             Piece p = first;
             for (; ok && piece_at(A, p); next_piece(A, p)) {
-                const bool alternate = kSlots == 1 || shared_alternates(p.T.rows * gh, kSlots);
+                const bool alternate = alternates(p.T);
                 const int items = alternate ? p.n : 2 * p.n;
+                ok = wait(q_full, p.c);
                 // item w is block w (alternate) or w / 2, of slot w % kSlots
                 auto scores = [&](int w) {
                     const int slot = w % kSlots, block = alternate ? w : w >> 1, f = fills + 2 * block, s = f % S_;
@@ -520,10 +502,18 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1) shared_kernel(
                     if (count[slot]) ok = ok && wait(o_done(slot), count[slot] - 1);
                     if (!ok) return;
                     tc_fence_after();
-                    const uint32_t q = q_at + (alternate ? 0 : slot * 128 * kDim * 2), k = base + s * C::kBuf;
-                    for (int d = 0; d < hd / 16; ++d)
-                        mma_f16_ss(tmem + slot * 128, desc_kmajor_sw128(q + (d / 4) * C::kSlab) + 2 * (d % 4),
-                                   desc_kmajor_sw128(k + (d / 4) * C::kSlab) + 2 * (d % 4), s_desc, d != 0);
+                    const uint64_t q = q_desc + (alternate ? 0 : slot * (128 * kDim * 2 / 16)), k = k_desc + s * (C::kBuf / 16);
+                    auto step = [&](int d) {                           // 16 dims
+                        const uint32_t off = (d / 4) * (C::kSlab / 16) + 2 * (d % 4);
+                        mma_f16_ss(tmem + slot * 128, q + off, k + off, s_idesc, d != 0);
+                    };
+                    if (hd == kDim) {
+#pragma unroll
+                        for (int d = 0; d < kDim / 16; ++d) step(d);
+                    } else {
+#pragma unroll 1
+                        for (int d = 0; d < hd / 16; ++d) step(d);
+                    }
                     mma_commit(s_full(slot));
                     mbar_arrive(s_full(slot));
                     if (alternate || slot == 1) mma_commit(empty(s));
@@ -534,12 +524,13 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1) shared_kernel(
                     ok = ok && wait(full(s), f / S_) && wait(p_full(slot), count[slot]);
                     if (!ok) return;
                     tc_fence_after();
-                    const uint32_t v = base + s * C::kBuf, o = tmem + kOCol + slot * kDim;
+                    const uint64_t v = v_desc + s * (C::kBuf / 16);
+                    const uint32_t o = tmem + kOCol + slot * kDim, p_at = tmem + slot * 128;
+#pragma unroll
                     for (int t = 0; t < kSharedTokens / 16; ++t) {     // 16 tokens: 8 columns of each part of P
-                        const uint32_t at = tmem + slot * 128 + 32 * (t / 2) + 8 * (t % 2);
-                        const uint64_t d = desc_mnmajor_sw128(v + t * 2048, C::kSlab, 1024);
-                        mma_f16_ts(o, at, d, o_desc, w >= kSlots || t != 0);
-                        mma_f16_ts(o, at + 16, d, o_desc, 1);
+                        const uint32_t at = p_at + 32 * (t / 2) + 8 * (t % 2);
+                        mma_f16_ts(o, at, v + t * (2048 / 16), o_idesc, w >= kSlots || t != 0);
+                        mma_f16_ts(o, at + 16, v + t * (2048 / 16), o_idesc, 1);
                     }
                     mma_commit(o_done(slot));
                     ++count[slot];
@@ -558,69 +549,143 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1) shared_kernel(
                 if (mbar_try_wait(over, 0)) break;
         }
         __syncwarp();
+    } else if (kCodes && warp >= kSlots * 4) {
+        // ------------------------------------------------------------ 8-bit rows to 16 bits: a thread a row
+        if constexpr (kCodes != kNone) {
+            const int row = threadIdx.x - kSlots * 128, chunks = hd / 16;
+            const int ch0 = row % chunks;                              // lanes begin at different chunks: no bank conflicts
+            int fills = 0;
+            bool ok = true;
+            int32_t next_page = -1;
+            auto look_up = [&](const SharedTile& T, int block) {
+                const int t = block * kSharedTokens + row;
+                next_page = t < T.tokens ? P.table[(int64_t)T.seq * P.table_stride + P.page_of(t)] : -1;
+            };
+            Piece p = first;
+            for (; ok && piece_at(A, p); next_piece(A, p)) {
+                look_up(p.T, p.i);
+                for (int k = 0; ok && k < p.n; ++k) {
+                    const int block = p.i + k, entry = fills / 2 % C::kRing;
+                    const int32_t page = next_page;
+                    const bool there = page >= 0 && page < P.pages;    // (others are reported by the loads)
+                    float ks = 0.f, vs = 0.f;
+                    if (there) {
+                        const int t = block * kSharedTokens + row;
+                        const int64_t at = page * P.scale_stride + (int64_t)p.h * ps + t - P.page_of(t) * ps;
+                        ks = P.k_scale[at];
+                        vs = P.v_scale[at];
+                    }
+                    if (k + 1 < p.n) look_up(p.T, block + 1);
+                    const unsigned seen = __ballot_sync(kWarpAll, there);
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const int s = fills % S_, rs = fills % C::kRawStages;
+                        ok = wait_all(raw_full(rs), fills / C::kRawStages) && (fills < S_ || wait_all(empty(s), fills / S_ - 1));
+                        if (!ok) break;
+                        if (kv == 0) {
+                            if (lane == 0) masks[entry * 4 + row / 32] = seen;
+                            scales[entry * 2 * kSharedTokens + row] = ks;
+                            scales[(entry * 2 + 1) * kSharedTokens + row] = vs;
+                        }
+                        const uint4* const from = reinterpret_cast<const uint4*>(gen + C::kRawAt + rs * C::kRaw + row * hd);
+                        uint8_t* const to = gen + s * C::kBuf + row * 128;
+                        int ch = ch0;
+#pragma unroll 4
+                        for (int c = 0; c < chunks; ++c) {
+                            const uint4 x = there ? from[ch] : make_uint4(0, 0, 0, 0);
+                            uint32_t o[8];
+                            if (kv) {
+                                widen<kCodes, kBfV>(x.x, o[0], o[1]);
+                                widen<kCodes, kBfV>(x.y, o[2], o[3]);
+                                widen<kCodes, kBfV>(x.z, o[4], o[5]);
+                                widen<kCodes, kBfV>(x.w, o[6], o[7]);
+                            } else {
+                                widen<kCodes, kBfQ>(x.x, o[0], o[1]);
+                                widen<kCodes, kBfQ>(x.y, o[2], o[3]);
+                                widen<kCodes, kBfQ>(x.z, o[4], o[5]);
+                                widen<kCodes, kBfQ>(x.w, o[6], o[7]);
+                            }
+                            uint8_t* const slab = to + (ch / 4) * C::kSlab;
+                            const int place = 2 * (ch % 4);
+                            *reinterpret_cast<uint4*>(slab + ((place ^ (row & 7)) * 16)) = make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4*>(slab + (((place + 1) ^ (row & 7)) * 16)) = make_uint4(o[4], o[5], o[6], o[7]);
+                            if (++ch == chunks) ch = 0;
+                        }
+                        fence_async_smem();
+                        mbar_arrive(full(s));
+                        mbar_arrive(raw_empty(rs));
+                        ++fills;
+                    }
+                }
+            }
+        }
     } else {
         // ------------------------------------------------------------ softmax: thread = query row = TMEM lane
-        const int slot = warp / 4, part = warp & 3, row = part * 32 + lane;
-        const uint32_t lane_at = tmem + ((uint32_t)(part * 32) << 16);
+        const int slot = warp / 4, quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t s_at = lane_at + slot * 128, o_at = lane_at + kOCol + slot * kDim;
         constexpr float kRowLift = kBfV ? 0.f : kLift;
         const bool down = A.scale_log2 < 0.f;
+        const int my_b = row / gh, my_j = row - my_b * gh;             // row of the tile's part, head of the group
         int count = 0, blocks = 0;
         bool ok = true;
         Piece p = first;
         for (; ok && piece_at(A, p); next_piece(A, p)) {
-            const int q_rows = p.T.rows * gh;
-            const bool alternate = kSlots == 1 || shared_alternates(q_rows, kSlots);
+            const bool alternate = alternates(p.T);
             const int step = alternate ? kSlots : 1;
             float m = -FLT_MAX, l = 0.f;
             bool begun = false;
             for (int k = alternate ? slot : 0; k < p.n; k += step) {
                 const int entry = (blocks + k) % C::kRing;
-                ok = __all_sync(kWarpAll, wait(s_full(slot), count));
+                ok = wait_all(s_full(slot), count);
                 if (!ok) break;
                 tc_fence_after();
+                const uint4 mask = *reinterpret_cast<const uint4*>(masks + entry * 4);
+                const bool part = (mask.x & mask.y & mask.z & mask.w) != kWarpAll;     // some rows are no tokens
                 const float* const ks = scales + entry * 2 * kSharedTokens;
                 const float* const vs = ks + kSharedTokens;
-                // the scores of 32 tokens, without the softmax's scale; those that are no tokens are -inf
+                // the scores of 32 tokens, times the sign of the scale
                 auto scores = [&](int c, float (&v)[32]) {
                     uint32_t x[32];
                     tmem_ld_32x32b_x32(s_at + 32 * c, x);
-                    const uint32_t mask = masks[entry * 4 + c];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
-                        if (kCodes) f = *reinterpret_cast<const float4*>(ks + 32 * c + i);
-                        v[i] = __uint_as_float(x[i]) * f.x;
-                        v[i + 1] = __uint_as_float(x[i + 1]) * f.y;
-                        v[i + 2] = __uint_as_float(x[i + 2]) * f.z;
-                        v[i + 3] = __uint_as_float(x[i + 3]) * f.w;
+                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(x[i]);
+                    if (kCodes) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(ks + 32 * c + i);
+                            mul2(v[i], v[i + 1], v[i], v[i + 1], f.x, f.y);
+                            mul2(v[i + 2], v[i + 3], v[i + 2], v[i + 3], f.z, f.w);
+                        }
                     }
-                    return mask;
+                    if (down) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = -v[i];
+                    }
+                    return masks[entry * 4 + c];
                 };
-                float top = -INFINITY;                                 // fmaxf passes over NaN, which reaches the sums
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // fmaxf passes over NaN, which reaches the sums
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     float v[32];
-                    const uint32_t mask = scores(c, v);
-                    if (mask == kWarpAll && !down) {
-                        float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) t0 = fmaxf(t0, v[i]), t1 = fmaxf(t1, v[i + 1]);
-                        top = fmaxf(top, fmaxf(t0, t1));
-                    } else {
+                    const uint32_t tokens = scores(c, v);
+                    if (part) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (mask >> i & 1) top = fmaxf(top, down ? -v[i] : v[i]);
+                            if (!(tokens >> i & 1)) v[i] = -INFINITY;
                     }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) tops[i & 3] = fmaxf(tops[i & 3], v[i]);
                 }
-                top *= fabsf(A.scale_log2);
+                const float scale = fabsf(A.scale_log2);
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale;
                 const bool moved = top > m + kSlack;
                 if (!begun) {
                     if (moved) m = top;
                     begun = true;
                 } else if (__any_sync(kWarpAll, moved)) {
                     // the sums so far come down; the last products with P are complete
-                    ok = __all_sync(kWarpAll, wait(o_done(slot), count - 1));
+                    ok = wait_all(o_done(slot), count - 1);
                     if (!ok) break;
                     tc_fence_after();
                     const float turn = moved ? ex2(m - top) : 1.f;
@@ -629,55 +694,44 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1) shared_kernel(
                         l *= turn;
                     }
 #pragma unroll 1
-                    for (int d = 0; d < hd; d += 32) {
-                        uint32_t x[32];
-                        tmem_ld_32x32b_x32(o_at + d, x);
+                    for (int d = 0; d < hd; d += 16) {
+                        uint32_t o[16];
+                        tmem_ld_32x32b_x16(o_at + d, o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * turn);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            uint32_t half[16];
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) half[j] = x[16 * i + j];
-                            tmem_st_32x32b_x16(o_at + d + 16 * i, half);
-                        }
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * turn);
+                        tmem_st_32x32b_x16(o_at + d, o);
                     }
                 }
+                // weights, 32 tokens at a time: their first parts and their second ones go where these tokens' scores were
                 const float less = m - kRowLift;
-                float part_l = 0.f;
+                float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
-                    float v[32];
-                    const uint32_t mask = scores(c, v);
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    float w[32];
+                    const uint32_t tokens = scores(c, w);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = ex2(fmaf(v[i], A.scale_log2, -less));
-                    if (mask != kWarpAll) {
+                    for (int i = 0; i < 32; ++i) w[i] = ex2(fmaf(w[i], scale, -less));
+                    if (part) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (!(mask >> i & 1)) v[i] = 0.f;
+                            if (!(tokens >> i & 1)) w[i] = 0.f;
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[i & 3] += v[i];
-                    part_l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    for (int i = 0; i < 32; ++i) sums[i & 3] += w[i];
                     if (kCodes) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
                             const float4 f = *reinterpret_cast<const float4*>(vs + 32 * c + i);
-                            v[i] *= f.x, v[i + 1] *= f.y, v[i + 2] *= f.z, v[i + 3] *= f.w;
+                            mul2(w[i], w[i + 1], w[i], w[i + 1], f.x, f.y);
+                            mul2(w[i + 2], w[i + 3], w[i + 2], w[i + 3], f.z, f.w);
                         }
                     }
                     uint32_t hi[16], lo[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        hi[i] = pack2<TV>(v[2 * i], v[2 * i + 1]);
-                        const float2 back = unpack2<TV>(hi[i]);
-                        lo[i] = pack2<TV>(v[2 * i] - back.x, v[2 * i + 1] - back.y);
-                    }
+                    split<kBfV>(w, hi, lo);
                     tmem_st_32x32b_x16(s_at + 32 * c, hi);
                     tmem_st_32x32b_x16(s_at + 32 * c + 16, lo);
                 }
-                l += part_l;
+                l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(p_full(slot));
@@ -685,28 +739,24 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1) shared_kernel(
             }
             if (!ok) break;
             // ---- the piece's records
-            const int at_row = alternate ? row : slot * kSharedLanes + row;
+            float* rec = nullptr;
+            const int b = (alternate ? 0 : slot * A.s.lane_rows) + my_b;
+            if (my_b < A.s.lane_rows && b < p.T.rows)
+                rec = p.i == 0 ? A.s.own + ((alternate ? slot * A.s.own_records : 0) + (int64_t)(p.T.row0 + b) * A.heads + p.h * gh + my_j) *
+                                               A.s.pitch
+                               : A.s.cut + (((int64_t)blockIdx.x * 2 + slot) * kSharedLanes + row) * A.s.pitch;
             if (begun) {
-                ok = __all_sync(kWarpAll, wait(o_done(slot), count - 1));
+                ok = wait_all(o_done(slot), count - 1);
                 if (!ok) break;
                 tc_fence_after();
-            }
-            float* rec = nullptr;
-            if (at_row < q_rows) {
-                const int b = at_row / gh, h = p.h * gh + at_row - b * gh;
-                rec = p.i == 0 ? A.s.own + ((alternate ? slot * A.s.own_records : 0) + (int64_t)(p.T.row0 + b) * A.heads + h) * A.s.pitch
-                               : A.s.cut + (((int64_t)blockIdx.x * 2 + slot) * kSharedLanes + row) * A.s.pitch;
-            }
-            if (begun) {
 #pragma unroll 1
                 for (int d = 0; d < hd; d += 32) {
-                    uint32_t x[32];
-                    tmem_ld_32x32b_x32(o_at + d, x);
+                    uint32_t o[32];
+                    tmem_ld_32x32b_x32(o_at + d, o);
                     if (rec) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
-                            if (d + i < hd)
-                                *reinterpret_cast<uint4*>(rec + d + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                            if (d + i < hd) *reinterpret_cast<uint4*>(rec + d + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
                 }
             }
@@ -723,23 +773,24 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1) shared_kernel(
     }
 }
 
-template <int kCodes, bool kBfQ, bool kBfV, int kDim> int launch_shared(const SharedArgs& A, cudaStream_t st) {
+template <int kCodes, bool kBfQ, bool kBfV, int kDim> int launch_shared(const SharedArgs& A, const Maps& maps, cudaStream_t st) {
     using C = Cfg<kCodes, kDim>;
     return launch(shared_kernel<kCodes, kBfQ, kBfV, kDim>, dim3((unsigned)A.grid), dim3(C::kThreads), (size_t)C::kSmem, st,
-                  "epq_paged_attend_shared", A);
+                  "epq_paged_attend_shared", A, maps);
 }
-template <int kCodes, bool kBfQ, bool kBfV> int launch_shared_d(const SharedArgs& A, cudaStream_t st) {
+template <int kCodes, bool kBfQ, bool kBfV> int launch_shared_d(const SharedArgs& A, const Maps& maps, cudaStream_t st) {
     const int hd = A.pages.head_dim;
-    if (hd <= 64) return launch_shared<kCodes, kBfQ, kBfV, 64>(A, st);
-    if (hd <= 128) return launch_shared<kCodes, kBfQ, kBfV, 128>(A, st);
-    return launch_shared<kCodes, kBfQ, kBfV, 256>(A, st);
+    if (hd <= 64) return launch_shared<kCodes, kBfQ, kBfV, 64>(A, maps, st);
+    if (hd <= 128) return launch_shared<kCodes, kBfQ, kBfV, 128>(A, maps, st);
+    if constexpr (kCodes == kNone) return launch_shared<kCodes, kBfQ, kBfV, 256>(A, maps, st);
+    return EPQ_EUNSUPPORTED;               // (may_share)
 }
 
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 // Where things lie in the workspace, behind the attention's own part.
 struct Layout {
-    int tile_rows, max_tiles, slots, pitch;
+    int lane_rows, max_tiles, slots, pitch;
     int64_t head, tiles, row_tile, row_from, own, cut, bytes;
 };
 Layout layout_of(const PagesD& P, int64_t batch, int heads, int64_t groups, int64_t behind) {
@@ -747,9 +798,9 @@ Layout layout_of(const PagesD& P, int64_t batch, int heads, int64_t groups, int6
     const int dim = P.head_dim <= 64 ? 64 : P.head_dim <= 128 ? 128 : 256, group = heads / P.kv_heads;
     L.slots = dim == 256 ? 1 : 2;
     L.pitch = dim + 4;
-    L.tile_rows = L.slots * kSharedLanes / group;
+    L.lane_rows = kSharedLanes / group;
     const int64_t some = groups < batch / 2 ? groups : batch / 2;      // groups of two rows or more
-    L.max_tiles = (int)(batch / (L.tile_rows ? L.tile_rows : 1) + some + 1);
+    L.max_tiles = (int)(batch / (L.slots * L.lane_rows) + some + 1);
     L.head = behind;
     L.tiles = L.head + 256;
     L.row_tile = align256(L.tiles + L.max_tiles * (int64_t)sizeof(SharedTile));
@@ -760,14 +811,21 @@ Layout layout_of(const PagesD& P, int64_t batch, int heads, int64_t groups, int6
     return L;
 }
 
-// Whether a batch can share anything that is worth it: groups of two rows or more whose query heads fit a tile, and
-// enough tokens that the tables could hold.
+// Whether a batch can share anything that is worth it: groups of two rows or more whose query heads fit a tile, enough
+// tokens that the tables could hold, and pages that the copies of rows take: boxes of 8 rows or more, which lie side by
+// side in the 128-byte swizzle.  8-bit heads above 128 have no room for their 16-bit form.
 bool may_share(const PagesD& P, int64_t batch, int heads, int64_t groups, int64_t token_bytes) {
     const int64_t most = (int64_t)P.max_pages * P.page_size;
     const int64_t pool = P.pages > (1LL << 40) / P.page_size ? 1LL << 40 : P.pages * P.page_size;   // (all tables together)
     const int64_t tokens = most < pool ? most : pool;
-    return groups > 0 && batch > 1 && heads / P.kv_heads <= kSharedLanes &&
+    return groups > 0 && batch > 1 && heads / P.kv_heads <= kSharedLanes && P.page_size % 8 == 0 &&
+           (P.format == EPQ_CACHE_SAME || P.head_dim <= 128) &&
            (double)(batch - 1) * (double)tokens * (double)token_bytes >= (double)kWorth;
+}
+// Whether rows of q can be copied as boxes (other views take the plain form).
+bool boxes_of(const epq_heads& q, int64_t batch) {
+    auto good = [](int64_t stride) { return stride > 0 && stride % 8 == 0 && stride < (1LL << 36); };
+    return (uintptr_t)q.data % 16 == 0 && good(q.stride_row) && (q.heads == 1 || good(q.stride_head));
 }
 int64_t bytes_of_token(const PagesD& P, int dtype_bytes) {
     return 2LL * P.kv_heads * (P.format == EPQ_CACHE_SAME ? P.head_dim * dtype_bytes : P.head_dim + 4);
@@ -824,7 +882,7 @@ int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const in
     const PagesD& P = A.pages;
     const int64_t token_bytes = bytes_of_token(P, 2);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!may_share(P, batch, A.heads, groups, token_bytes)) return launch_attend_plain(A, cols, st);
+    if (!may_share(P, batch, A.heads, groups, token_bytes) || !boxes_of(*q, batch)) return launch_attend_plain(A, cols, st);
     const int64_t behind = align256(attend_bytes(who, pages, batch, A.heads));
     const Layout L = layout_of(P, batch, A.heads, groups, behind);
     if (workspace_bytes < L.bytes)
@@ -842,10 +900,7 @@ int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const in
     S.s.own_records = batch * A.heads;
     S.s.pitch = L.pitch;
     S.s.slots = L.slots;
-    S.q = q->data;
-    S.q_row = q->stride_row;
-    S.q_head = q->stride_head;
-    S.q_aligned = heads_aligned(*q, 2, 16);
+    S.s.lane_rows = L.lane_rows;
     S.seq = seq;
     S.lengths = lengths;
     S.starts = starts;
@@ -855,19 +910,29 @@ int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const in
     S.groups = (int)groups;
     S.heads = A.heads;
     S.group = A.group;
-    S.tile_rows = L.tile_rows;
     S.max_tiles = L.max_tiles;
     S.grid = device_sms();
     S.scale_log2 = A.scale_log2;
-    int e = launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, who, S);
+    S.box_rows = kSharedTokens;
+    while (P.page_size % S.box_rows) S.box_rows /= 2;
+    Maps maps;
+    const bool codes = P.format != EPQ_CACHE_SAME;
+    int e = make_tmap_3d(&maps.q, q->data, 2, {P.head_dim, q->heads, batch}, q->heads > 1 ? q->stride_head : P.head_dim,
+                         q->stride_row, {64, A.group, L.lane_rows}, true, who);
+    for (int i = 0; e == EPQ_OK && i < 2; ++i)
+        e = make_tmap_3d(i ? &maps.v : &maps.k, i ? P.v : P.k, codes ? 1 : 2,
+                         {P.head_dim, (int64_t)P.kv_heads * P.page_size, P.pages}, P.head_dim, P.page_stride,
+                         {codes ? P.head_dim : 64, S.box_rows, 1}, !codes, who);
+    if (e != EPQ_OK) return e;
+    e = launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, who, S);
     if (e != EPQ_OK) return e;
     const bool bf = dtype == EPQ_BF16;
     if (P.format == EPQ_CACHE_INT8)
-        e = bf ? launch_shared_d<kInts, true, true>(S, st) : launch_shared_d<kInts, false, true>(S, st);
+        e = bf ? launch_shared_d<kInts, true, true>(S, maps, st) : launch_shared_d<kInts, false, true>(S, maps, st);
     else if (P.format == EPQ_CACHE_FP8)
-        e = bf ? launch_shared_d<kFloats, true, true>(S, st) : launch_shared_d<kFloats, false, true>(S, st);
+        e = bf ? launch_shared_d<kFloats, true, true>(S, maps, st) : launch_shared_d<kFloats, false, true>(S, maps, st);
     else
-        e = bf ? launch_shared_d<kNone, true, true>(S, st) : launch_shared_d<kNone, false, false>(S, st);
+        e = bf ? launch_shared_d<kNone, true, true>(S, maps, st) : launch_shared_d<kNone, false, false>(S, maps, st);
     if (e != EPQ_OK) return e;
     A.shared = S.s;
     return attend_behind_shared(A, cols, st);

@@ -380,7 +380,8 @@ struct Attention {
     int64_t batch;
     double scale;
     int dtype;
-    Attention(PyObject* const* a, PyObject* seq_, PyObject* scale_, PyObject* out_, PyObject* lse_, const char* call)
+    // `align`: bytes that q is read at once; another q is copied
+    Attention(PyObject* const* a, PyObject* seq_, PyObject* scale_, PyObject* out_, PyObject* lse_, const char* call, int align)
         : c(cache_of(a)), q(tensor(a[5], "q")) {
         const Tensor& n = tensor(a[6], "lengths");
         const Tensor *s = maybe(seq_, "seq"), *to = maybe(out_, "out");
@@ -401,8 +402,10 @@ struct Attention {
         scale = scale_ == Py_None ? 1.0 / std::sqrt((double)hd) : number(scale_);
         dtype = dtype_code(dt);
         OnDevice on(c.device);
-        if (((uintptr_t)heads.data | (uintptr_t)(2 * heads.stride_row) | (uintptr_t)(2 * heads.stride_head)) % 4) {
-            q = q.clone(at::MemoryFormat::Contiguous);     // the kernel reads two values at a time
+        const bool expanded = (batch > 1 && heads.stride_row == 0) || (H > 1 && heads.stride_head == 0);
+        if (((uintptr_t)heads.data | (uintptr_t)(2 * heads.stride_row) | (uintptr_t)(2 * heads.stride_head)) % align ||
+            (expanded && align == 16)) {
+            q = q.clone(at::MemoryFormat::Contiguous);
             heads = heads_of(q, "q", c.device, dt, batch, H, hd);
         }
         given = to;
@@ -424,7 +427,7 @@ struct Attention {
 PyObject* attend(PyObject* const* a) {
     const int64_t window = integer(a[9]);
     const Tensor* blocks = maybe(a[12], "blocks");
-    const Attention t(a, a[7], a[8], a[10], a[11], "attend");
+    const Attention t(a, a[7], a[8], a[10], a[11], "attend", 4);
     const Cache& c = t.c;
     if (blocks) {
         if (blocks->dim() != 3 || blocks->size(0) != t.batch || blocks->size(1) != c.p.kv_heads || blocks->scalar_type() != at::kInt ||
@@ -454,7 +457,7 @@ PyObject* attend(PyObject* const* a) {
 //               return_lse)
 PyObject* attend_shared(PyObject* const* a) {
     const Tensor &starts = tensor(a[7], "starts"), &prefix = tensor(a[8], "prefix");
-    const Attention t(a, a[9], a[10], a[11], a[12], "attend_shared");
+    const Attention t(a, a[9], a[10], a[11], a[12], "attend_shared", 16);
     const Cache& c = t.c;
     const int64_t groups = prefix.dim() == 1 ? prefix.size(0) : -1;
     index_of(prefix, "prefix", c.device, at::kLong, groups);
