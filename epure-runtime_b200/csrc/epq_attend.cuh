@@ -256,12 +256,12 @@ __device__ __forceinline__ void emit_row(const AttendArgs& A, int b, int h, int 
             };
             constexpr int kAtOnce = 4;
             for (int p0 = 0; p0 < pieces; p0 += kAtOnce) {
-                float2 ml[kAtOnce];
+                float4 ml[kAtOnce];
                 float4 a[kAtOnce];
 #pragma unroll
                 for (int i = 0; i < kAtOnce; ++i) {
                     const float* rec = record(min(p0 + i, pieces - 1));
-                    ml[i] = __ldcg(reinterpret_cast<const float2*>(rec + pitch - 4));
+                    ml[i] = __ldcg(reinterpret_cast<const float4*>(rec + pitch - 4));
                     a[i] = __ldcg(reinterpret_cast<const float4*>(rec + d));
                 }
 #pragma unroll
@@ -269,7 +269,7 @@ __device__ __forceinline__ void emit_row(const AttendArgs& A, int b, int h, int 
                     if (p0 + i >= pieces || ml[i].x == -FLT_MAX) continue;     // a piece without a score above -inf
                     const float top = fmaxf(to, ml[i].x), f = to == top ? 1.f : ex2(to - top);
                     const float g = ml[i].x == top ? 1.f : ex2(ml[i].x - top);
-                    sum = sum * f + ml[i].y * g;
+                    sum = sum * f + (ml[i].y + ml[i].z) * g;
                     v[0] = v[0] * f + a[i].x * g;
                     v[1] = v[1] * f + a[i].y * g;
                     v[2] = v[2] * f + a[i].z * g;

@@ -24,7 +24,7 @@ struct SharedHead {
 };
 
 // Where they lie.  A record is a query row's sums over a part of the shared tokens, pitch floats: head_dim values
-// (in the kernels' own dimension dim), then the maximum m (log2) and the sum l of 2^(score - m).  A unit's first piece
+// (in the kernels' own dimension dim), then the maximum m (log2) and the sum of 2^(score - m) in two parts.  A unit's first piece
 // leaves its records in `own` [2][batch * heads]; one that goes on into another CTA in that CTA's `cut` [grid][2][128].
 struct SharedD {
     SharedHead* head;

@@ -19,6 +19,15 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// One lane of a converged warp, the same each time.  Products are issued under it rather than by a lane of
+// the program's own choice: their operands are registers of the warp, and only so does the compiler know
+// that it need not bring them together from the lanes first.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t on;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(on));
+    return on != 0;
+}
+
 // ---------------------------------------------------------------- mbarriers
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");

@@ -19,7 +19,7 @@
 //     pass through four more warps that widen them to 16 bits (exact);
 //   * one thread issues the products: S = Q K^T (Q, K in shared memory) and O += P V (P in tensor
 //     memory, V as the MN-major operand);
-//   * 4 warps a slot take a row a thread: maximum, weights, sum; P goes back in place of S.
+//   * 8 warps a slot take half a row a thread: maximum, weights, sum; P goes back in place of S.
 // Two slots (S and O in tensor memory: all of its 512 columns) keep the products of one under
 // the softmax of the other: two tiles of 128 rows over the same block, or, for units of up to
 // 128 rows, one tile whose blocks alternate.
@@ -193,7 +193,7 @@ enum Codes { kNone = 0, kInts = 1, kFloats = 2 };
 template <int kCodes, int kDim> struct Cfg {
     static constexpr int kSlots = kDim == 256 ? 1 : 2;
     static constexpr int kConvertWarps = kCodes ? 4 : 0;
-    static constexpr int kMmaWarp = kSlots * 4 + kConvertWarps, kLoadWarp = kMmaWarp + 1;
+    static constexpr int kSoftmaxWarps = kSlots * 8, kMmaWarp = kSoftmaxWarps + kConvertWarps, kLoadWarp = kMmaWarp + 1;
     static constexpr int kThreads = (kLoadWarp + 1) * 32;
     static constexpr int kBuf = kSharedTokens * kDim * 2;              // K or V of a block
     static constexpr int kSlab = kSharedTokens * 128;                  // 64 values of each of its rows
@@ -204,8 +204,8 @@ template <int kCodes, int kDim> struct Cfg {
     // kStages stages back have been multiplied, and so the softmax of all before them is done.
     static constexpr int kRing = kCodes ? 4 : 8;
     static constexpr int kScales = kCodes ? kRing * 2 * kSharedTokens * 4 : 0;
-    static constexpr int kMasksAt = kScales, kBarsAt = kMasksAt + kRing * 16;
-    static constexpr int kMisc = kBarsAt + 304;
+    static constexpr int kMasksAt = kScales, kTopsAt = kMasksAt + kRing * 16, kBarsAt = kTopsAt + kSlots * 2 * kSharedLanes * 4;
+    static constexpr int kMisc = kBarsAt + 352;
     static constexpr int kFit = (kSmemLimit - 1024 - kMisc - kQ - kRawStages * kRaw) / kBuf, kMost = kCodes ? 4 : 8;
     static constexpr int kStages = kFit > kMost ? kMost : kFit;
     static constexpr int kQAt = kStages * kBuf, kRawAt = kQAt + kQ, kMiscAt = kRawAt + kRawStages * kRaw;
@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
     uint8_t* const misc = gen + C::kMiscAt;
     float* const scales = reinterpret_cast<float*>(misc);              // [kRing][2][128]: of keys, of values
     uint32_t* const masks = reinterpret_cast<uint32_t*>(misc + C::kMasksAt);           // [kRing][4]
+    float* const tops = reinterpret_cast<float*>(misc + C::kTopsAt);   // [slots][halves][128]
     const uint32_t bars = base + C::kMiscAt + C::kBarsAt;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 64u + 8u * s; };
@@ -304,6 +305,7 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
     auto p_full = [&](int s) { return bars + 208u + 8u * s; };
     auto o_done = [&](int s) { return bars + 224u + 8u * s; };
     const uint32_t q_full = bars + 240u, q_free = bars + 248u, over = bars + 256u, part_full = bars + 264u, tslot = bars + 272u;
+    auto pair_full = [&](int i) { return bars + 288u + 8u * i; };
     volatile int* const abortp = reinterpret_cast<volatile int*>(misc + C::kBarsAt + 280);
     volatile int* const where = reinterpret_cast<volatile int*>(misc + C::kBarsAt + 284);
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -323,7 +325,8 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
         }
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(s_full(s), 2);                                   // the products' end, and the issuing thread
-            mbar_init(p_full(s), 128);
+            mbar_init(p_full(s), 256);
+            for (int i = 0; i < 4; ++i) mbar_init(pair_full(4 * s + i), 64);
             mbar_init(o_done(s), 1);
         }
         mbar_init(q_full, 1);
@@ -357,7 +360,7 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(misc + C::kBarsAt + 272);
+    const uint32_t tmem = __shfl_sync(kWarpAll, *reinterpret_cast<volatile uint32_t*>(misc + C::kBarsAt + 272), 0);
     first.t = *where;
     first.c = 0;
     first.h = 0;
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
     constexpr uint32_t kOCol = kSlots * 128u;                          // S and P of slot s in columns 128 s, O behind them
     auto alternates = [&](const SharedTile& T) { return kSlots == 1 || shared_alternates(T.rows, A.s.lane_rows, kSlots); };
 
-    if (warp >= kSlots * 4 + C::kConvertWarps) {
+    if (warp >= C::kMmaWarp) {
         if (warp == C::kLoadWarp) {
             // -------------------------------------------------------- loads: a lane a box of rows of one page
             const int R = A.box_rows, boxes = kSharedTokens / R;
@@ -480,28 +483,30 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
                             for (uint32_t i = 0; i < kWaitLimit; ++i)
                                 if (mbar_try_wait(kCodes ? raw_full(s) : full(s), (f / (kCodes ? C::kRawStages : S_)) & 1)) break;
             }
-        } else if (warp == C::kMmaWarp && lane == 0) {
+        } else {
             // -------------------------------------------------------- products
             constexpr uint32_t s_idesc = idesc_f16<kBfQ, 128, kSharedTokens>();
             constexpr uint32_t o_idesc = idesc_f16<kBfV, 128, kDim, false, true>();
             const uint64_t q_desc = desc_kmajor_sw128(q_at), k_desc = desc_kmajor_sw128(base);
             const uint64_t v_desc = desc_mnmajor_sw128(base, C::kSlab, 1024);
-            int count[2] = {0, 0};                                     // products with P that a slot has had
+            int count0 = 0, count1 = 0;                                // products with P that the slots have had
             int fills = 0;                                             // stages before this piece
             bool ok = true;
             Piece p = first;
             for (; ok && piece_at(A, p); next_piece(A, p)) {
                 const bool alternate = alternates(p.T);
                 const int items = alternate ? p.n : 2 * p.n;
-                ok = wait(q_full, p.c);
+                ok = wait_all(q_full, p.c);
                 // item w is block w (alternate) or w / 2, of slot w % kSlots
                 auto scores = [&](int w) {
                     const int slot = w % kSlots, block = alternate ? w : w >> 1, f = fills + 2 * block, s = f % S_;
-                    ok = ok && wait(full(s), f / S_);
+                    ok = ok && wait_all(full(s), f / S_);
                     // P of the slot's last item lies where S goes
-                    if (count[slot]) ok = ok && wait(o_done(slot), count[slot] - 1);
+                    const int had = slot ? count1 : count0;
+                    if (had) ok = ok && wait_all(o_done(slot), had - 1);
                     if (!ok) return;
                     tc_fence_after();
+                    if (!elect_one()) return;
                     const uint64_t q = q_desc + (alternate ? 0 : slot * (128 * kDim * 2 / 16)), k = k_desc + s * (C::kBuf / 16);
                     auto step = [&](int d) {                           // 16 dims
                         const uint32_t off = (d / 4) * (C::kSlab / 16) + 2 * (d % 4);
@@ -521,9 +526,12 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
                 };
                 auto sums = [&](int w) {
                     const int slot = w % kSlots, block = alternate ? w : w >> 1, f = fills + 2 * block + 1, s = f % S_;
-                    ok = ok && wait(full(s), f / S_) && wait(p_full(slot), count[slot]);
+                    const int had = slot ? count1 : count0;
+                    ok = ok && wait_all(full(s), f / S_) && wait_all(p_full(slot), had);
+                    (slot ? count1 : count0) = had + 1;
                     if (!ok) return;
                     tc_fence_after();
+                    if (!elect_one()) return;
                     const uint64_t v = v_desc + s * (C::kBuf / 16);
                     const uint32_t o = tmem + kOCol + slot * kDim, p_at = tmem + slot * 128;
 #pragma unroll
@@ -533,26 +541,30 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
                         mma_f16_ts(o, at + 16, v + t * (2048 / 16), o_idesc, 1);
                     }
                     mma_commit(o_done(slot));
-                    ++count[slot];
                     if (alternate || slot == 1) mma_commit(empty(s));
                 };
-                for (int w = 0; w < kSlots && w < items && ok; ++w) scores(w);
+                for (int w = 0; w < kSlots && w < items && ok; ++w) {
+                    scores(w);
+                    __syncwarp();
+                }
                 for (int w = 0; w < items && ok; ++w) {
                     sums(w);
+                    __syncwarp();
                     if (ok && w + kSlots < items) scores(w + kSlots);
+                    __syncwarp();
                 }
                 fills += 2 * p.n;
             }
             // every product is complete before tensor memory is released
-            mma_commit(over);
+            if (elect_one()) mma_commit(over);
             for (uint32_t i = 0; i < kWaitLimit; ++i)
                 if (mbar_try_wait(over, 0)) break;
         }
         __syncwarp();
-    } else if (kCodes && warp >= kSlots * 4) {
+    } else if (kCodes && warp >= C::kSoftmaxWarps) {
         // ------------------------------------------------------------ 8-bit rows to 16 bits: a thread a row
         if constexpr (kCodes != kNone) {
-            const int row = threadIdx.x - kSlots * 128, chunks = hd / 16;
+            const int row = threadIdx.x - C::kSoftmaxWarps * 32, chunks = hd / 16;
             const int ch0 = row % chunks;                              // lanes begin at different chunks: no bank conflicts
             int fills = 0;
             bool ok = true;
@@ -620,8 +632,10 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
             }
         }
     } else {
-        // ------------------------------------------------------------ softmax: thread = query row = TMEM lane
-        const int slot = warp / 4, quarter = warp & 3, row = quarter * 32 + lane;
+        // ------------------------------------------------------------ softmax: two threads a query row (TMEM lane), each
+        // with half of a block's tokens
+        const int slot = warp / 8, half = warp / 4 % 2, quarter = warp % 4, row = quarter * 32 + lane;
+        const uint32_t both = pair_full(4 * slot + quarter);
         const uint32_t lane_at = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t s_at = lane_at + slot * 128, o_at = lane_at + kOCol + slot * kDim;
         constexpr float kRowLift = kBfV ? 0.f : kLift;
@@ -664,9 +678,9 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
                     }
                     return masks[entry * 4 + c];
                 };
-                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // fmaxf passes over NaN, which reaches the sums
+                float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // fmaxf passes over NaN, which reaches the sums
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 2 * half; c < 2 * half + 2; ++c) {
                     float v[32];
                     const uint32_t tokens = scores(c, v);
                     if (part) {
@@ -675,10 +689,15 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
                             if (!(tokens >> i & 1)) v[i] = -INFINITY;
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) tops[i & 3] = fmaxf(tops[i & 3], v[i]);
+                    for (int i = 0; i < 32; ++i) most[i & 3] = fmaxf(most[i & 3], v[i]);
                 }
                 const float scale = fabsf(A.scale_log2);
-                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale;
+                const float mine = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+                tops[(2 * slot + half) * kSharedLanes + row] = mine;
+                mbar_arrive(both);
+                ok = wait_all(both, count);
+                if (!ok) break;
+                const float top = fmaxf(mine, tops[(2 * slot + 1 - half) * kSharedLanes + row]) * scale;
                 const bool moved = top > m + kSlack;
                 if (!begun) {
                     if (moved) m = top;
@@ -694,7 +713,7 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
                         l *= turn;
                     }
 #pragma unroll 1
-                    for (int d = 0; d < hd; d += 16) {
+                    for (int d = 16 * half; d < hd; d += 32) {
                         uint32_t o[16];
                         tmem_ld_32x32b_x16(o_at + d, o);
 #pragma unroll
@@ -706,7 +725,7 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
                 const float less = m - kRowLift;
                 float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 2 * half; c < 2 * half + 2; ++c) {
                     float w[32];
                     const uint32_t tokens = scores(c, w);
 #pragma unroll
@@ -750,7 +769,7 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll 1
-                for (int d = 0; d < hd; d += 32) {
+                for (int d = 32 * half; d < hd; d += 64) {
                     uint32_t o[32];
                     tmem_ld_32x32b_x32(o_at + d, o);
                     if (rec) {
@@ -761,7 +780,10 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
                 }
             }
             tc_fence_before();
-            if (rec) *reinterpret_cast<float2*>(rec + A.s.pitch - 4) = make_float2(m == -FLT_MAX ? m : m - kRowLift, l);
+            if (rec) {
+                if (half == 0) rec[A.s.pitch - 4] = m == -FLT_MAX ? m : m - kRowLift;
+                rec[A.s.pitch - 3 + half] = l;
+            }
             blocks += p.n;
         }
     }
