@@ -34,7 +34,7 @@ struct AttendArgs {
 enum Mode {
     kAllTokens = 0,      // the first lengths[b] of its sequence (the last `window` of them)
     kListed = 1,         // those of the blocks (pages) that a list of each row and key head names
-    kBehindShared = 2    // those from row_from[b] on; the others' sums are joined from records
+    kBehindShared = 2    // those from row_from[b] on, left as sums
 };
 
 namespace {
@@ -164,6 +164,7 @@ template <int kMode, int kTok> __device__ __forceinline__ Span span_of(const Att
     if (kMode == kListed && s.n > 0) s.n = min(A.count, A.pages.page_of(s.n - 1) + 1) * A.pages.page_size;
     s.first = s.lo & ~(kTok - 1);
     s.blocks = (s.n - s.first + kTok - 1) / kTok;
+    if (kMode == kBehindShared && s.lo == s.n) s.blocks = 0;
     return s;
 }
 
@@ -225,71 +226,26 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 }
 
 // Four values of a row's head: sums `val` of weights relative to 2^at and their sum `sum` relative to 2^to, divided
-// and written; sum = 0: every score was -inf.
+// and written; sum = 0: every score was -inf.  Behind a shared prefix the sums go to the join as they are.
 template <int kMode, bool kQuant>
 __device__ __forceinline__ void emit_row(const AttendArgs& A, int b, int h, int d, const float (&val)[4], float at, float to,
                                          float sum) {
-    float v[4] = {val[0], val[1], val[2], val[3]};
-    float gain;
+    const int64_t place = (int64_t)b * A.heads + h;
     if (kMode == kBehindShared) {
-        const int tile = A.shared.row_tile[b];
-        if (kQuant && sum != 0.f) {
-            const float turn = ex2(at - to);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] *= turn;
-        }
-        if (sum == 0.f) to = -FLT_MAX;
-        if (tile >= 0 && A.shared.row_from[b] > 0) {   // the records of the pieces of the row's unit
-            const SharedTile T = A.shared.tiles[tile];
-            const int head = h / A.group, rows = A.shared.lane_rows;
-            const int part = (b - T.row0) / rows, lane = (b - T.row0 - part * rows) * A.group + h - head * A.group;
-            const int64_t first = T.first + (int64_t)head * T.blocks, run = A.shared.head->run;
-            const int64_t c0 = quotient(first, run), c1 = quotient(first + T.blocks - 1, run);
-            const int two = shared_alternates(T.rows, rows, A.shared.slots) ? 2 : 1, pieces = (int)(c1 - c0 + 1) * two;
-            const int pitch = A.shared.pitch;
-            const int64_t own = ((int64_t)b * A.heads + h) * pitch;
-            auto record = [&](int p) {
-                const int64_t c = c0 + (two == 2 ? p >> 1 : p);
-                const int slot = two == 2 ? p & 1 : part;
-                return c == c0 ? A.shared.own + (two == 2 ? slot * A.shared.own_records * pitch : 0) + own
-                               : A.shared.cut + ((c * 2 + slot) * kSharedLanes + lane) * pitch;
-            };
-            constexpr int kAtOnce = 4;
-            for (int p0 = 0; p0 < pieces; p0 += kAtOnce) {
-                float4 ml[kAtOnce];
-                float4 a[kAtOnce];
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    const float* rec = record(min(p0 + i, pieces - 1));
-                    ml[i] = __ldcg(reinterpret_cast<const float4*>(rec + pitch - 4));
-                    a[i] = __ldcg(reinterpret_cast<const float4*>(rec + d));
-                }
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    if (p0 + i >= pieces || ml[i].x == -FLT_MAX) continue;     // a piece without a score above -inf
-                    const float top = fmaxf(to, ml[i].x), f = to == top ? 1.f : ex2(to - top);
-                    const float g = ml[i].x == top ? 1.f : ex2(ml[i].x - top);
-                    sum = sum * f + (ml[i].y + ml[i].z) * g;
-                    v[0] = v[0] * f + a[i].x * g;
-                    v[1] = v[1] * f + a[i].y * g;
-                    v[2] = v[2] * f + a[i].z * g;
-                    v[3] = v[3] * f + a[i].w * g;
-                    to = top;
-                }
-            }
-        }
-        gain = sum == 0.f ? 0.f : 1.f / sum;
-    } else {
-        gain = sum == 0.f ? 0.f : 1.f / sum;
-        if (kQuant) gain *= ex2(at - to);
+        const float turn = kQuant && sum != 0.f ? ex2(at - to) : 1.f;
+        float* const rec = A.shared.rest + place * A.shared.pitch;
+        *reinterpret_cast<float4*>(rec + d) = make_float4(val[0] * turn, val[1] * turn, val[2] * turn, val[3] * turn);
+        if (d == 0) *reinterpret_cast<float4*>(rec + A.shared.pitch - 4) = make_float4(sum == 0.f ? -FLT_MAX : to, sum, 0.f, 0.f);
+        return;
     }
+    float gain = sum == 0.f ? 0.f : 1.f / sum;
+    if (kQuant) gain *= ex2(at - to);
     uint2 o;
     if (A.dtype == EPQ_BF16) {
-        o = make_uint2(pack<true>(v[0] * gain, v[1] * gain), pack<true>(v[2] * gain, v[3] * gain));
+        o = make_uint2(pack<true>(val[0] * gain, val[1] * gain), pack<true>(val[2] * gain, val[3] * gain));
     } else {
-        o = make_uint2(pack<false>(v[0] * gain, v[1] * gain), pack<false>(v[2] * gain, v[3] * gain));
+        o = make_uint2(pack<false>(val[0] * gain, val[1] * gain), pack<false>(val[2] * gain, val[3] * gain));
     }
-    const int64_t place = (int64_t)b * A.heads + h;
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(A.out) + place * A.pages.head_dim + d) = o;
     if (A.lse && d == 0) A.lse[place] = sum == 0.f ? -INFINITY : (to + log2f(sum)) / kLog2e;
 }
@@ -348,9 +304,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     for (int b = blockIdx.x; some_empty && b < A.batch; b += gridDim.x) {
         if (span_of<kMode, kTok>(A, b, false).blocks) continue;
         if (kMode == kBehindShared) {                  // nothing but the shared tokens, if any
-            const float none[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int e = tid; e < A.heads * (hd / 4); e += kThreads)
-                emit_row<kMode, kQuant>(A, b, e / (hd / 4), e % (hd / 4) * 4, none, -FLT_MAX, -FLT_MAX, 0.f);
+            for (int h = tid; h < A.heads; h += kThreads)
+                *reinterpret_cast<float4*>(A.shared.rest + ((int64_t)b * A.heads + h + 1) * A.shared.pitch - 4) =
+                    make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
             continue;
         }
         for (int e = tid; e < A.heads * hd; e += kThreads)

@@ -1,6 +1,6 @@
-// Attention of rows that share a prefix, in three launches: a plan (which tokens are shared by
-// which rows), the shared tokens (k_paged_shared.cu), and each row's other tokens, joined with
-// what the rows found over the shared ones (k_paged_attn_shared.cu).  What they hand on.
+// Attention of rows that share a prefix, in four launches: a plan (which tokens are shared by
+// which rows) and the shared tokens (k_paged_shared.cu), each row's other tokens
+// (k_paged_attn_shared.cu), and the join of both (k_paged_shared.cu).  What they hand on.
 #pragma once
 
 #include "epq_paged.cuh"
@@ -26,6 +26,7 @@ struct SharedHead {
 // Where they lie.  A record is a query row's sums over a part of the shared tokens, pitch floats: head_dim values
 // (in the kernels' own dimension dim), then the maximum m (log2) and the sum of 2^(score - m) in two parts.  A unit's first piece
 // leaves its records in `own` [2][batch * heads]; one that goes on into another CTA in that CTA's `cut` [grid][2][128].
+// `rest` [batch * heads] holds the sums over the rows' other tokens.
 struct SharedD {
     SharedHead* head;
     SharedTile* tiles;
@@ -33,6 +34,7 @@ struct SharedD {
     int32_t* row_from;                     // [batch]: tokens that the row's tile took care of
     float* own;
     float* cut;
+    float* rest;
     int64_t own_records;                   // batch * heads
     int pitch, slots, lane_rows;           // slots: tensor-core tiles of a unit; lane_rows: rows that one holds
 };

@@ -1,7 +1,5 @@
-// The last launch of epq_paged_attend_shared: each row's own tokens, behind those that it shares
-// (epq_shared.cuh), by the kernel of k_paged_attn.cu.  Where a row's result is written its sums
-// are joined with the records that the shared part left, in the order of the pieces, so results
-// do not depend on timing.
+// Of epq_paged_attend_shared: each row's own tokens, behind those that it shares (epq_shared.cuh),
+// by the kernel of k_paged_attn.cu.  Its sums are joined with those over the shared tokens.
 #include "epq_attend.cuh"
 
 namespace epq {

@@ -1,5 +1,5 @@
-// Attention of one new token a row where rows share a prefix (epq_paged_attend_shared): the plan
-// and the shared tokens.  (The rest: k_paged_attn_shared.cu; what they hand on: epq_shared.cuh.)
+// Attention of one new token a row where rows share a prefix (epq_paged_attend_shared): the plan,
+// the shared tokens and the join.  (The rest: k_paged_attn_shared.cu; what they hand on: epq_shared.cuh.)
 //
 // Rows of a group that see tokens [0, L) all alike are one attention of many query rows over one
 // set of keys: with r rows and g query heads a key head, r g rows over L tokens, 4 r g flops a
@@ -795,6 +795,90 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
     }
 }
 
+// ---------------------------------------------------------------- the join
+// A warp a row's head: the records of its unit's pieces and of its other tokens, in the order of the pieces, so that
+// results do not depend on timing.  Bound: the records' bytes (from L2), all asked for at once.
+constexpr int kJoinWarps = 8;
+
+template <bool kBf> __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const AttendArgs A) {
+    pdl_enter();
+    const SharedD& S = A.shared;
+    const int lane = threadIdx.x & 31, hd = A.pages.head_dim, pitch = S.pitch;
+    const int64_t place = (int64_t)blockIdx.x * kJoinWarps + threadIdx.x / 32;
+    if (place >= S.own_records) return;
+    const int b = (int)(place / A.heads), h = (int)(place - (int64_t)b * A.heads);
+    const int tile = S.row_tile[b], from = S.row_from[b];
+    const float* const rest = S.rest + place * pitch;
+    int64_t c0 = 0;
+    int pieces = 0, two = 1, part = 0, at = 0;
+    if (tile >= 0 && from > 0) {
+        const SharedTile T = S.tiles[tile];
+        const int head = h / A.group;
+        part = (b - T.row0) / S.lane_rows;
+        at = (b - T.row0 - part * S.lane_rows) * A.group + h - head * A.group;
+        const int64_t first = T.first + (int64_t)head * T.blocks, run = S.head->run;
+        c0 = first / run;
+        two = shared_alternates(T.rows, S.lane_rows, S.slots) ? 2 : 1;
+        pieces = (int)((first + T.blocks - 1) / run - c0 + 1) * two;
+    }
+    auto record = [&](int p) -> const float* {                          // p = pieces: the rest
+        if (p >= pieces) return rest;
+        const int64_t c = c0 + (two == 2 ? p >> 1 : p);
+        const int slot = two == 2 ? p & 1 : part;
+        return c == c0 ? S.own + ((two == 2 ? slot * S.own_records : 0) + place) * pitch
+                       : S.cut + ((c * 2 + slot) * kSharedLanes + at) * pitch;
+    };
+    const bool two_rows = lane * 4 + 128 < hd;                         // (head_dim above 128: a lane's second four values)
+    float top = -FLT_MAX, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int p0 = 0; p0 <= pieces; p0 += 32) {
+        // a lane a record: its maximum and sum; one without a score above -inf holds no values
+        const int p = p0 + lane;
+        float4 ml = make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
+        if (p <= pieces) ml = __ldcg(reinterpret_cast<const float4*>(record(p) + pitch - 4));
+        float m = ml.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kWarpAll, m, o));
+        const float now = fmaxf(top, m), turn = now == top ? 1.f : ex2(top - now);
+        const bool empty = ml.x == -FLT_MAX && ml.y + ml.z == 0.f;     // (a sum can be NaN without a maximum)
+        const float weight = empty ? 0.f : ex2(ml.x - now);
+        float l = empty ? 0.f : (ml.y + ml.z) * weight;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(kWarpAll, l, o);
+        sum = sum * turn + l;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= turn;
+        top = now;
+        const unsigned there = __ballot_sync(kWarpAll, !empty);
+        const int count = min(32, pieces + 1 - p0);
+        constexpr int kAtOnce = 8;
+        for (int q0 = 0; q0 < count; q0 += kAtOnce) {
+            float4 x[kAtOnce], y[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                x[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (q0 + i < count && there >> (q0 + i) & 1 && lane * 4 < hd) {
+                    const float* rec = record(p0 + q0 + i);
+                    x[i] = __ldcg(reinterpret_cast<const float4*>(rec) + lane);
+                    if (two_rows) y[i] = __ldcg(reinterpret_cast<const float4*>(rec + 128) + lane);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                const float w = __shfl_sync(kWarpAll, weight, q0 + i);
+                v[0] += x[i].x * w, v[1] += x[i].y * w, v[2] += x[i].z * w, v[3] += x[i].w * w;
+                v[4] += y[i].x * w, v[5] += y[i].y * w, v[6] += y[i].z * w, v[7] += y[i].w * w;
+            }
+        }
+    }
+    using T = typename Half<kBf>::type;
+    const float gain = sum == 0.f ? 0.f : 1.f / sum;
+    uint16_t* const out = static_cast<uint16_t*>(A.out) + place * hd + lane * 4;
+    if (lane * 4 < hd) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0] * gain, v[1] * gain), pack2<T>(v[2] * gain, v[3] * gain));
+    if (two_rows)
+        *reinterpret_cast<uint2*>(out + 128) = make_uint2(pack2<T>(v[4] * gain, v[5] * gain), pack2<T>(v[6] * gain, v[7] * gain));
+    if (A.lse && lane == 0) A.lse[place] = sum == 0.f ? -INFINITY : (top + log2f(sum)) / kLog2e;
+}
+
 template <int kCodes, bool kBfQ, bool kBfV, int kDim> int launch_shared(const SharedArgs& A, const Maps& maps, cudaStream_t st) {
     using C = Cfg<kCodes, kDim>;
     return launch(shared_kernel<kCodes, kBfQ, kBfV, kDim>, dim3((unsigned)A.grid), dim3(C::kThreads), (size_t)C::kSmem, st,
@@ -813,7 +897,7 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 // Where things lie in the workspace, behind the attention's own part.
 struct Layout {
     int lane_rows, max_tiles, slots, pitch;
-    int64_t head, tiles, row_tile, row_from, own, cut, bytes;
+    int64_t head, tiles, row_tile, row_from, rest, own, cut, bytes;
 };
 Layout layout_of(const PagesD& P, int64_t batch, int heads, int64_t groups, int64_t behind) {
     Layout L;
@@ -827,7 +911,8 @@ Layout layout_of(const PagesD& P, int64_t batch, int heads, int64_t groups, int6
     L.tiles = L.head + 256;
     L.row_tile = align256(L.tiles + L.max_tiles * (int64_t)sizeof(SharedTile));
     L.row_from = align256(L.row_tile + batch * 4);
-    L.own = align256(L.row_from + batch * 4);
+    L.rest = align256(L.row_from + batch * 4);
+    L.own = align256(L.rest + batch * heads * L.pitch * 4);
     L.cut = align256(L.own + 2 * batch * heads * L.pitch * 4);
     L.bytes = L.cut + (int64_t)device_sms() * 2 * kSharedLanes * L.pitch * 4;
     return L;
@@ -917,6 +1002,7 @@ int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const in
     S.s.tiles = reinterpret_cast<SharedTile*>(ws + L.tiles);
     S.s.row_tile = reinterpret_cast<int32_t*>(ws + L.row_tile);
     S.s.row_from = reinterpret_cast<int32_t*>(ws + L.row_from);
+    S.s.rest = reinterpret_cast<float*>(ws + L.rest);
     S.s.own = reinterpret_cast<float*>(ws + L.own);
     S.s.cut = reinterpret_cast<float*>(ws + L.cut);
     S.s.own_records = batch * A.heads;
@@ -957,7 +1043,10 @@ int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const in
         e = bf ? launch_shared_d<kNone, true, true>(S, maps, st) : launch_shared_d<kNone, false, false>(S, maps, st);
     if (e != EPQ_OK) return e;
     A.shared = S.s;
-    return attend_behind_shared(A, cols, st);
+    e = attend_behind_shared(A, cols, st);
+    if (e != EPQ_OK) return e;
+    const dim3 grid((unsigned)cdiv(S.s.own_records, kJoinWarps)), threads(kJoinWarps * 32);
+    return bf ? launch(join_kernel<true>, grid, threads, 0, st, who, A) : launch(join_kernel<false>, grid, threads, 0, st, who, A);
 }
 
 }  // extern "C"
