@@ -641,18 +641,25 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
         constexpr float kRowLift = kBfV ? 0.f : kLift;
         const bool down = A.scale_log2 < 0.f;
         const int my_b = row / gh, my_j = row - my_b * gh;             // row of the tile's part, head of the group
-        int count = 0, blocks = 0;
+        int count = 0, blocks = 0, met = 0;                            // blocks of the slot, of all; with the pair's maximum
         bool ok = true;
         Piece p = first;
         for (; ok && piece_at(A, p); next_piece(A, p)) {
             const bool alternate = alternates(p.T);
             const int step = alternate ? kSlots : 1;
+            // warps whose rows are none pass on at once: what is in their lanes stays in their lanes
+            const bool active = quarter * 32 < min(A.s.lane_rows, p.T.rows - (alternate ? 0 : slot * A.s.lane_rows)) * gh;
             float m = -FLT_MAX, l = 0.f;
             bool begun = false;
             for (int k = alternate ? slot : 0; k < p.n; k += step) {
                 const int entry = (blocks + k) % C::kRing;
                 ok = wait_all(s_full(slot), count);
                 if (!ok) break;
+                if (!active) {
+                    mbar_arrive(p_full(slot));
+                    ++count;
+                    continue;
+                }
                 tc_fence_after();
                 const uint4 mask = *reinterpret_cast<const uint4*>(masks + entry * 4);
                 const bool part = (mask.x & mask.y & mask.z & mask.w) != kWarpAll;     // some rows are no tokens
@@ -695,7 +702,7 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
                 const float mine = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
                 tops[(2 * slot + half) * kSharedLanes + row] = mine;
                 mbar_arrive(both);
-                ok = wait_all(both, count);
+                ok = wait_all(both, met++);
                 if (!ok) break;
                 const float top = fmaxf(mine, tops[(2 * slot + 1 - half) * kSharedLanes + row]) * scale;
                 const bool moved = top > m + kSlack;

@@ -9,16 +9,17 @@
 // and the sum's order is fixed (neighbours, then neighbours of their sums), so which blocks
 // are chosen is the same wherever it is computed in float32.
 //
-// Bounds.  Bound: HBM, one read of the keys.  A warp takes one head of one page; its lanes
-// hold 16 bytes of a row each, the rows of an access side by side, and are joined at the end.
+// Bounds.  Bound: HBM, one read of the keys; for the pages of a decode step the chain of length,
+// page and keys.  Up to 8 warps share one head of one page, so that a page is two accesses deep;
+// a warp's lanes hold 16 bytes of a row each, the rows of an access side by side.
 //
 // Selection.  Bound: HBM, 4 head_dim bytes a block and head; next to it the issue rate, about
-// 1.5 instructions a dim, block and query head.  A lane holds 8 dims of q, split as
-// max(q, 0) and min(q, 0), so that max(q lo, q hi) = max(q, 0) hi + min(q, 0) lo is a product
-// and a fused product of two dims at once (one of the two is zero: nothing is rounded).  The
-// lanes of a block then add up all its heads together: each step halves the heads a lane
-// holds.  The CTAs of a unit (row, key head) leave its scores as integers in the order of the
-// floats; the last of them finds the count-th largest bit by bit and writes the list.
+// 1.5 instructions a dim, block and query head.  A lane holds 8 dims of two blocks; q lies in
+// shared memory as max(q, 0) and min(q, 0), so that max(q lo, q hi) = max(q, 0) hi + min(q, 0) lo
+// is a product and a fused product of two dims at once (one of the two is zero: nothing is
+// rounded).  The lanes of a block then add up all its heads together: each step halves the heads
+// a lane holds.  The CTAs of a unit (row, key head) leave its scores as integers in the order of
+// the floats; the last of them finds the count-th largest, two bits at a time, and writes the list.
 #include "epq_paged.cuh"
 
 namespace epq {
@@ -31,6 +32,7 @@ constexpr unsigned kAll = 0xffffffffu;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxUnits = 65536;               // counters in the workspace
+constexpr int kMaxBlocks = (1 << 21) - 1;      // of a sequence, in a selection
 
 // ---------------------------------------------------------------- bounds
 struct BoundsArgs {
@@ -41,6 +43,7 @@ struct BoundsArgs {
     uint16_t* bounds;
     int64_t stride;                            // values between pages
     int parts;                                 // CTAs a row
+    int team;                                  // warps a head of a page
 };
 
 enum Kind { kBf16 = 0, kF16 = 1, kInt8 = 2, kFp8 = 3 };
@@ -79,12 +82,11 @@ template <int kKind> struct Chunk {
 #pragma unroll
         for (int i = 0; i < 4; ++i) lo[i] = min2<T2>(lo[i], w[i]), hi[i] = max2<T2>(hi[i], w[i]);
     }
-    __device__ __forceinline__ void join(int from, bool on) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t l = __shfl_sync(kAll, lo[i], from), h = __shfl_sync(kAll, hi[i], from);
-            if (on) lo[i] = min2<T2>(lo[i], l), hi[i] = max2<T2>(hi[i], h);
-        }
+    static constexpr int kWords = 8;
+    __device__ __forceinline__ uint32_t word(int i) const { return i < 4 ? lo[i] : hi[i - 4]; }
+    __device__ __forceinline__ void join(int i, uint32_t x) {          // word i of another
+        if (i < 4) lo[i] = min2<T2>(lo[i], x);
+        else hi[i - 4] = max2<T2>(hi[i - 4], x);
     }
     // infinities as the largest finite value
     __device__ __forceinline__ void store(uint16_t* to_lo, uint16_t* to_hi) const {
@@ -130,12 +132,11 @@ template <int kKind> struct Codes {
             }
         }
     }
-    __device__ __forceinline__ void join(int from, bool on) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float l = __shfl_sync(kAll, lo[i], from), h = __shfl_sync(kAll, hi[i], from);
-            if (on) lo[i] = min_nan(lo[i], l), hi[i] = max_nan(hi[i], h);
-        }
+    static constexpr int kWords = 32;
+    __device__ __forceinline__ uint32_t word(int i) const { return __float_as_uint(i < 16 ? lo[i] : hi[i - 16]); }
+    __device__ __forceinline__ void join(int i, uint32_t x) {
+        if (i < 16) lo[i] = min_nan(lo[i], __uint_as_float(x));
+        else hi[i - 16] = max_nan(hi[i - 16], __uint_as_float(x));
     }
     __device__ __forceinline__ void store(uint16_t* to_lo, uint16_t* to_hi) const {
         constexpr uint32_t top = 0x7f7f7f7fu, bottom = top | 0x80008000u;
@@ -167,6 +168,7 @@ __device__ __forceinline__ int row_length(const PagesD& P, const int32_t* seq, c
 template <int kKind>
 __global__ void __launch_bounds__(kThreads) bounds_kernel(const BoundsArgs A) {
     using C = typename std::conditional<kKind <= kF16, Chunk<kKind>, Codes<kKind>>::type;
+    __shared__ uint32_t shared[C::kWords][kWarps][32];
     pdl_enter();
     const PagesD& P = A.pages;
     const int b = blockIdx.x / A.parts, part = blockIdx.x - b * A.parts;
@@ -179,17 +181,21 @@ __global__ void __launch_bounds__(kThreads) bounds_kernel(const BoundsArgs A) {
         return;
     }
     if (n == 0 || from >= n) return;
-    const int ps = P.page_size, hd = P.head_dim;
+    const int ps = P.page_size, hd = P.head_dim, team = A.team, teams = kWarps / team;
+    const int member = warp % team, first = part * teams + warp / team;        // the team's first item
     const int c0 = P.page_of((int)from), cols = P.page_of(n - 1) + 1 - c0;
     const int chunks = hd * C::kBytes / 16, rows = 32 / chunks;        // of a row; rows an access
     const int row = lane / chunks, ch = lane - row * chunks;
     const bool on = row < rows;
     const int items = cols * P.kv_heads;                               // (below 2^31: a page has at least its heads' tokens)
-    for (int i = part * kWarps + warp; i < items; i += A.parts * kWarps) {
+    auto together = [&]() {                                            // the team's warps
+        if (team > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / team), "r"(team * 32) : "memory");
+    };
+    for (int i = first; i < items; i += A.parts * teams) {
         const int col = c0 + i / P.kv_heads, head = i % P.kv_heads;
         const int64_t page = P.table[(int64_t)s * P.table_stride + col];
         if (page < 0 || page >= P.pages) {
-            if (lane == 0) atomicOr(&g_sparse_error, kBadPage);
+            if (lane == 0 && member == 0) atomicOr(&g_sparse_error, kBadPage);
             continue;
         }
         const int tokens = min(ps, n - col * ps);
@@ -199,12 +205,12 @@ __global__ void __launch_bounds__(kThreads) bounds_kernel(const BoundsArgs A) {
         C c;
         c.clear();
         constexpr int kAtOnce = 8;
-        for (int t = on ? row : tokens; t < tokens; t += kAtOnce * rows) {
+        for (int t = on ? member * rows + row : tokens; t < tokens; t += kAtOnce * team * rows) {
             uint4 x[kAtOnce];
             float f[kAtOnce];
 #pragma unroll
             for (int e = 0; e < kAtOnce; ++e) {
-                const int u = min(t + e * rows, tokens - 1);           // (a row twice changes no bound)
+                const int u = min(t + e * team * rows, tokens - 1);    // (a row twice changes no bound)
                 x[e] = __ldg(k + (int64_t)u * chunks);
                 f[e] = kKind >= kInt8 ? __ldg(scale + u) : 1.f;
             }
@@ -213,14 +219,30 @@ __global__ void __launch_bounds__(kThreads) bounds_kernel(const BoundsArgs A) {
         }
         __syncwarp();
         for (int r = rows; r > 1;) {                                   // the upper rows' lanes into the lower ones'
-            const int half = (r + 1) / 2;
-            c.join((lane + half * chunks) & 31, row + half < r);
+            const int half = (r + 1) / 2, other = (lane + half * chunks) & 31;
+            const bool take = row + half < r;
+#pragma unroll
+            for (int w = 0; w < C::kWords; ++w) {
+                const uint32_t x = __shfl_sync(kAll, c.word(w), other);
+                if (take) c.join(w, x);
+            }
             r = half;
         }
-        if (row == 0) {
+        if (team > 1) {                                                // the other warps into the first
+            if (member && row == 0)
+#pragma unroll
+                for (int w = 0; w < C::kWords; ++w) shared[w][warp][lane] = c.word(w);
+            together();
+            if (!member && row == 0)
+                for (int m = 1; m < team; ++m)
+#pragma unroll
+                    for (int w = 0; w < C::kWords; ++w) c.join(w, shared[w][warp + m][lane]);
+        }
+        if (row == 0 && !member) {
             uint16_t* to = A.bounds + page * A.stride + (int64_t)head * 2 * hd + ch * (16 / C::kBytes);
             c.store(to, to + hd);
         }
+        together();                                                    // (the words are read)
     }
 }
 
@@ -276,7 +298,7 @@ __device__ __forceinline__ uint32_t key_of(float s) {
 // the others, ties to the lowest block, in ascending order.
 __device__ void choose(const SelectArgs& A, const uint32_t* keys, int n, int32_t* out) {
     constexpr int kHeld = 16;                                          // keys of a thread that stay in registers
-    __shared__ int sums[2][kWarps];
+    __shared__ int64_t sums[2][kWarps];
     __shared__ int before[kWarps][3];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int each = (n + kThreads - 1) / kThreads, j0 = min(n, tid * each), j1 = min(n, j0 + each);
@@ -287,24 +309,30 @@ __device__ void choose(const SelectArgs& A, const uint32_t* keys, int n, int32_t
     const bool in_registers = each <= kHeld;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) held[i] = in_registers && j0 + i < j1 ? free_key(j0 + i) : 0u;
-    // the largest value that at least `need` keys reach
+    // the largest value that at least `need` keys reach, two bits at a time: of the three next values the largest that
+    // so many reach (their counts in 21 bits each; a unit has below 2^21 blocks)
     uint32_t at = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t to = at | 1u << bit;
-        int have = 0;
+    for (int bit = 30; bit >= 0; bit -= 2) {
+        const uint32_t to1 = at | 1u << bit, to2 = at | 2u << bit, to3 = at | 3u << bit;
+        int have1 = 0, have2 = 0, have3 = 0;
+        auto count = [&](uint32_t key) { have1 += key >= to1, have2 += key >= to2, have3 += key >= to3; };
         if (in_registers) {
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) have += held[i] >= to;
+            for (int i = 0; i < kHeld; ++i) count(held[i]);
         } else {
-            for (int j = j0; j < j1; ++j) have += free_key(j) >= to;
+            for (int j = j0; j < j1; ++j) count(free_key(j));
         }
-        have = __reduce_add_sync(kAll, have);
-        if (lane == 0) sums[bit & 1][warp] = have;
+        const int h1 = __reduce_add_sync(kAll, have1), h2 = __reduce_add_sync(kAll, have2), h3 = __reduce_add_sync(kAll, have3);
+        int64_t* const mine = sums[bit / 2 & 1];
+        if (lane == 0) mine[warp] = h1 | (int64_t)h2 << 21 | (int64_t)h3 << 42;
         __syncthreads();
-        int total = 0;
+        int64_t total = 0;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) total += sums[bit & 1][w];
-        if (total >= need) at = to;
+        for (int w = 0; w < kWarps; ++w) total += mine[w];
+        constexpr int kMask = (1 << 21) - 1;
+        if ((int)(total >> 42) >= need) at = to3;
+        else if ((int)(total >> 21 & kMask) >= need) at = to2;
+        else if ((int)(total & kMask) >= need) at = to1;
     }
     // sure ones and ties before this thread's blocks
     int sure = 0, ties = 0, above = 0;
@@ -347,8 +375,10 @@ __device__ void choose(const SelectArgs& A, const uint32_t* keys, int n, int32_t
 
 // kLanes lanes a block, 8 dims each; kHeads query heads at once.
 template <bool kIsBf16, int kLanes, int kHeads>
-__global__ void __launch_bounds__(kThreads) select_kernel(const SelectArgs A) {
+__global__ void __launch_bounds__(kThreads, 2) select_kernel(const SelectArgs A) {
     using T = typename std::conditional<kIsBf16, __nv_bfloat16, __half>::type;   // of the bounds
+    // of a head and a lane's dims (i, i + 4): max(q, 0) of i = 0, 1 and 2, 3, min(q, 0) of the same
+    __shared__ float4 split[kHeads][4][kLanes];
     __shared__ bool last;
     pdl_enter();
     const PagesD& P = A.pages;
@@ -366,45 +396,48 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectArgs A) {
         return;
     }
     uint32_t* keys = A.keys + (int64_t)unit * P.max_pages;
-    constexpr int kAtOnce = 32 / kLanes;                               // blocks of a warp's step
-    const int sub = lane / kLanes, dim = (lane % kLanes) * 8;
+    constexpr int kGroups = 32 / kLanes, kEach = 2, kStep = kGroups * kEach;   // blocks of a warp's step
+    const int sub = lane / kLanes, mine = lane % kLanes, dim = mine * 8;
     const bool on = dim < hd;
     const int per = (n + A.parts - 1) / A.parts, end = min(n, (part + 1) * per);
     const int32_t* table = P.table + (int64_t)s * P.table_stride;
     for (int h0 = 0; h0 < A.group; h0 += kHeads) {
-        uint64_t up[kHeads][4], down[kHeads][4];                       // max(q, 0) and min(q, 0) of dims (i, i + 4)
-#pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
+        if (h0) __syncthreads();
+        for (int e = threadIdx.x; e < kHeads * kLanes; e += kThreads) {
+            const int h = e / kLanes, l = e % kLanes;
             float f[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = 0.f;
-            if (on && h0 + h < A.group) {
-                const uint16_t* q = static_cast<const uint16_t*>(A.q) + b * A.q_row + (head * A.group + h0 + h) * A.q_head + dim;
+            if (8 * l < hd && h0 + h < A.group) {
+                const uint16_t* q = static_cast<const uint16_t*>(A.q) + b * A.q_row + (head * A.group + h0 + h) * A.q_head + 8 * l;
                 if (A.dtype == EPQ_BF16) {
-                    Eight<__nv_bfloat16> e;
-                    e.load(reinterpret_cast<const __nv_bfloat16*>(q), A.q_aligned);
-                    e.get(f);
+                    Eight<__nv_bfloat16> x;
+                    x.load(reinterpret_cast<const __nv_bfloat16*>(q), A.q_aligned);
+                    x.get(f);
                 } else {
-                    Eight<__half> e;
-                    e.load(reinterpret_cast<const __half*>(q), A.q_aligned);
-                    e.get(f);
+                    Eight<__half> x;
+                    x.load(reinterpret_cast<const __half*>(q), A.q_aligned);
+                    x.get(f);
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                up[h][i] = pair(max_nan(f[i], 0.f), max_nan(f[i + 4], 0.f));
-                down[h][i] = pair(min_nan(f[i], 0.f), min_nan(f[i + 4], 0.f));
+            for (int i = 0; i < 2; ++i) {
+                split[h][i][l] = make_float4(max_nan(f[2 * i], 0.f), max_nan(f[2 * i + 4], 0.f), max_nan(f[2 * i + 1], 0.f),
+                                             max_nan(f[2 * i + 5], 0.f));
+                split[h][2 + i][l] = make_float4(min_nan(f[2 * i], 0.f), min_nan(f[2 * i + 4], 0.f), min_nan(f[2 * i + 1], 0.f),
+                                                 min_nan(f[2 * i + 5], 0.f));
             }
         }
+        __syncthreads();
         // the head that this lane is left with, and whether there is one
-        int mine = 0;
+        int left = 0;
 #pragma unroll
-        for (int o = 1, half = kHeads / 2; half > 0; o <<= 1, half >>= 1) mine += lane & o ? half : 0;
-        const bool is_head = h0 + mine < A.group;
+        for (int o = 1, half = kHeads / 2; half > 0; o <<= 1, half >>= 1) left += lane & o ? half : 0;
+        const bool is_head = h0 + left < A.group;
 
         const uint4 none = make_uint4(0, 0, 0, 0);
-        constexpr int kStep = kWarps * kAtOnce;
-        int j = part * per + warp * kAtOnce + sub;
+        const int stride = kWarps * kStep;
+        int j = part * per + warp * kStep + sub;                       // this lane's first block of the step; the others kGroups apart
         auto page_at = [&](int i) { return i < end ? table[i] : 0; };
         auto fetch = [&](int i, int page, uint4& l, uint4& h) {        // a block's bounds, zeros where there are none
             l = h = none;
@@ -415,63 +448,84 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectArgs A) {
             }
         };
         // bounds one step ahead, page numbers two
-        int page = page_at(j), next_page = page_at(j + kStep);
-        uint4 lo, hi;
-        fetch(j, page, lo, hi);
-        for (; __any_sync(kAll, j < end); j += kStep) {
-            const int after = page_at(j + 2 * kStep);
-            uint4 next_lo, next_hi;
-            fetch(j + kStep, next_page, next_lo, next_hi);
-            uint64_t l[4], h[4];
-            {
-                const uint32_t lw[4] = {lo.x, lo.y, lo.z, lo.w}, hw[4] = {hi.x, hi.y, hi.z, hi.w};
+        int page[kEach], next_page[kEach];
+        uint4 lo[kEach], hi[kEach];
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            page[x] = page_at(j + x * kGroups);
+            next_page[x] = page_at(j + stride + x * kGroups);
+        }
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) fetch(j + x * kGroups, page[x], lo[x], hi[x]);
+        for (; __any_sync(kAll, j < end); j += stride) {
+            uint64_t l[kEach][4], h[kEach][4];
+            int now[kEach];
+#pragma unroll
+            for (int x = 0; x < kEach; ++x) {
+                const uint32_t lw[4] = {lo[x].x, lo[x].y, lo[x].z, lo[x].w}, hw[4] = {hi[x].x, hi[x].y, hi[x].z, hi[x].w};
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float2 a = unpack2<T>(lw[i]), c = unpack2<T>(lw[i + 2]);
-                    l[2 * i] = pair(a.x, c.x);
-                    l[2 * i + 1] = pair(a.y, c.y);
+                    l[x][2 * i] = pair(a.x, c.x);
+                    l[x][2 * i + 1] = pair(a.y, c.y);
                     const float2 d = unpack2<T>(hw[i]), e = unpack2<T>(hw[i + 2]);
-                    h[2 * i] = pair(d.x, e.x);
-                    h[2 * i + 1] = pair(d.y, e.y);
+                    h[x][2 * i] = pair(d.x, e.x);
+                    h[x][2 * i + 1] = pair(d.y, e.y);
                 }
+                now[x] = page[x];
+                page[x] = next_page[x];
+                next_page[x] = page_at(j + 2 * stride + x * kGroups);
+                fetch(j + stride + x * kGroups, page[x], lo[x], hi[x]);
             }
-            float v[kHeads];
+            float v[kEach][kHeads];
 #pragma unroll
             for (int e = 0; e < kHeads; ++e) {
-                uint64_t t[4];
+                uint64_t up[4], down[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) t[i] = fma_pair(up[e][i], h[i], mul_pair(down[e][i], l[i]));
-                v[e] = add_halves(add_pair(add_pair(t[0], t[1]), add_pair(t[2], t[3])));
-            }
-            // each step joins two lanes' sums; while a lane holds several heads it passes on half of them
-            int held = kHeads;
+                for (int i = 0; i < 2; ++i) {
+                    const float4 a = split[e][i][mine], c = split[e][2 + i][mine];
+                    up[2 * i] = pair(a.x, a.y);
+                    up[2 * i + 1] = pair(a.z, a.w);
+                    down[2 * i] = pair(c.x, c.y);
+                    down[2 * i + 1] = pair(c.z, c.w);
+                }
 #pragma unroll
-            for (int o = 1; o < kLanes; o <<= 1) {
-                if (held > 1) {
-                    held /= 2;
+                for (int x = 0; x < kEach; ++x) {
+                    uint64_t t[4];
 #pragma unroll
-                    for (int e = 0; e < kHeads / 2; ++e)
-                        if (e < held) {
-                            const float give = lane & o ? v[e] : v[e + held], keep = lane & o ? v[e + held] : v[e];
-                            v[e] = keep + __shfl_xor_sync(kAll, give, o);
-                        }
-                } else {
-                    v[0] += __shfl_xor_sync(kAll, v[0], o);
+                    for (int i = 0; i < 4; ++i) t[i] = fma_pair(up[i], h[x][i], mul_pair(down[i], l[x][i]));
+                    v[x][e] = add_halves(add_pair(add_pair(t[0], t[1]), add_pair(t[2], t[3])));
                 }
             }
-            float score = is_head ? v[0] : -INFINITY;
 #pragma unroll
-            for (int o = 1; o < kHeads; o <<= 1) score = max_nan(score, __shfl_xor_sync(kAll, score, o));
-            if (lane % kLanes == 0 && j < end) {
-                const bool good = page >= 0 && page < P.pages;
-                if (!good) atomicOr(&g_sparse_error, kBadPage);
-                const uint32_t key = good ? key_of(score) : 0u;
-                keys[j] = h0 ? max(keys[j], key) : key;
+            for (int x = 0; x < kEach; ++x) {
+                // each step joins two lanes' sums; while a lane holds several heads it passes on half of them
+                int held = kHeads;
+#pragma unroll
+                for (int o = 1; o < kLanes; o <<= 1) {
+                    if (held > 1) {
+                        held /= 2;
+#pragma unroll
+                        for (int e = 0; e < kHeads / 2; ++e)
+                            if (e < held) {
+                                const float give = lane & o ? v[x][e] : v[x][e + held], keep = lane & o ? v[x][e + held] : v[x][e];
+                                v[x][e] = keep + __shfl_xor_sync(kAll, give, o);
+                            }
+                    } else {
+                        v[x][0] += __shfl_xor_sync(kAll, v[x][0], o);
+                    }
+                }
+                float score = is_head ? v[x][0] : -INFINITY;
+#pragma unroll
+                for (int o = 1; o < kHeads; o <<= 1) score = max_nan(score, __shfl_xor_sync(kAll, score, o));
+                const int i = j + x * kGroups;
+                if (mine == 0 && i < end) {
+                    const bool good = now[x] >= 0 && now[x] < P.pages;
+                    if (!good) atomicOr(&g_sparse_error, kBadPage);
+                    const uint32_t key = good ? key_of(score) : 0u;
+                    keys[i] = h0 ? max(keys[i], key) : key;
+                }
             }
-            page = next_page;
-            next_page = after;
-            lo = next_lo;
-            hi = next_hi;
         }
     }
     __syncthreads();
@@ -550,8 +604,12 @@ int epq_paged_bounds(const epq_pages* pages, void* bounds, int64_t bounds_stride
     A.lengths = lengths;
     A.bounds = static_cast<uint16_t*>(bounds);
     A.stride = bounds_stride;
+    // warps a head of a page: 8 accesses of 512 bytes each
+    const int64_t bytes = (int64_t)P.page_size * P.head_dim * (P.format == EPQ_CACHE_SAME ? 2 : 1);
+    A.team = 1;
+    while (A.team < kWarps && A.team * 4096 < bytes) A.team *= 2;
     // enough CTAs a row to fill the card where all of its pages are new
-    const int64_t most = cdiv((int64_t)P.max_pages * P.kv_heads, kWarps), fill = cdiv(8LL * device_sms(), batch);
+    const int64_t most = cdiv((int64_t)P.max_pages * P.kv_heads * A.team, kWarps), fill = cdiv(8LL * device_sms(), batch);
     A.parts = (int)(most < fill ? most : fill);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto go = [&](auto kern) {
@@ -566,6 +624,8 @@ int64_t epq_paged_select_workspace_bytes(const epq_pages* pages, int64_t batch) 
     PagesD P;
     const int rc = make_pages(pages, &P, "epq_paged_select_workspace_bytes");
     if (rc != EPQ_OK) return rc;
+    if (P.max_pages > kMaxBlocks)
+        return set_error(EPQ_EUNSUPPORTED, "epq_paged_select: %d pages a sequence (at most %d)", P.max_pages, kMaxBlocks);
     if (batch < 0 || batch * P.kv_heads > kMaxUnits)
         return set_error(EPQ_EUNSUPPORTED, "epq_paged_select: batch=%lld of %d key heads (at most %d units)", (long long)batch,
                          P.kv_heads, kMaxUnits);
@@ -613,8 +673,8 @@ int epq_paged_select(const epq_pages* pages, const void* bounds, int64_t bounds_
     A.count = count;
     A.sinks = sinks;
     A.recent = recent;
-    // CTAs a unit: enough to fill the card, each with at least two steps of its warps
-    const int64_t units = batch * P.kv_heads, fill = cdiv(2LL * device_sms(), units), most = cdiv(P.max_pages, 64);
+    // CTAs a unit: enough to fill the card twice (lengths differ), each with at least two steps of its warps
+    const int64_t units = batch * P.kv_heads, fill = cdiv(4LL * device_sms(), units), most = cdiv(P.max_pages, 64);
     A.parts = (int)(fill < most ? fill : most);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const unsigned grid = (unsigned)(units * A.parts);

@@ -5,11 +5,16 @@
 // probabilities, the weights, the place of the drawn token).
 //
 // Split.  A row is a thread-block cluster; each of its warps sums the weights of one run of the
-// vocabulary in 64 bits.  The sums of all warps are scanned in distributed shared memory by
-// every CTA alike, and the one warp whose run holds the drawn token goes through it a second
-// time (from L2).  So results depend neither on timing nor on another row.
-// 64 bits, because the drawn token is where a cumulative sum passes a number: float32 sums of
-// 128k weights would move it in about one draw of a hundred.
+// vocabulary.  The runs' sums are scanned in distributed shared memory by every CTA alike; the
+// CTA whose run holds the drawn token goes through that run a second time (from L2), a part of it
+// a warp, and the warp whose part holds it a third time.  So results depend neither on timing nor
+// on another row.
+//
+// Precision.  The drawn token is where a cumulative sum passes a number: float32 sums of 128k
+// weights would move it in about one draw of a hundred.  64-bit additions, and above all the
+// conversions to 64 bits, are what the first pass would spend its time on, so it sums in pairs of
+// float32: each sum and difference with what its rounding left over, which keeps about 46 bits.
+// All that follows is 64-bit.
 #include "epq_common.cuh"
 #include "epq_paged.cuh"
 #include "epq_sampling.h"
@@ -21,11 +26,10 @@ namespace {
 __device__ int g_verify_error = 0;
 
 constexpr unsigned kAll = 0xffffffffu;
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
-constexpr int kRuns = kCluster * kWarps;       // runs of the vocabulary
-static_assert(kRuns % 32 == 0, "a warp scans the runs");
+// Threads a CTA: few rows have the most warps on each of them, many rows all CTAs of a row of 64
+// sequences on the card at once (4 an SM).
+constexpr int kFew = 1024, kMany = 256;
 
 struct VerifyArgs {
     epq_probs p, q;                            // q.data NULL: drafts of probability 1
@@ -51,7 +55,7 @@ __device__ __forceinline__ double cluster_load(const double* mine, unsigned rank
 
 // kV values of a row from element e on, as they count: those of [0, n) and 0 outside.  With
 // kV > 1 the address of element e is a multiple of their size.
-template <typename T, int kV> __device__ __forceinline__ void fetch(float (&f)[kV], const T* row, int64_t e, int64_t n) {
+template <typename T, int kV> __device__ __forceinline__ void fetch(float (&f)[kV], const T* row, int e, int n) {
     if (kV > 1 && e >= 0 && e + kV <= n) {
         paged::load_v<T, kV>(f, row + e);
     } else {
@@ -70,10 +74,23 @@ __device__ __forceinline__ double scan(double v, int lane) {
     return v;
 }
 
-template <typename T, int kV>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
+// A sum in two floats: values that were added, and what the additions' roundings left over.
+struct Sum {
+    float s = 0.f, rest = 0.f;
+    __device__ __forceinline__ void add(float x, float left) {
+        const float t = s + x, z = t - s;
+        rest += (s - (t - z)) + (x - z) + left;
+        s = t;
+    }
+    __device__ __forceinline__ double value() const { return isinf(s) ? (double)s : (double)s + (double)rest; }
+};
+
+template <typename T, int kV, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads == kMany ? 4 : 1) verify_kernel(const VerifyArgs A) {
+    constexpr int kWarps = kThreads / 32, kRuns = kCluster * kWarps;   // runs of the vocabulary
+    static_assert(kRuns % 32 == 0, "a warp scans the runs");
     __shared__ int taken_at;                   // accepted drafts, times 2, and whether the next one was refused
-    __shared__ double sums[kWarps];
+    __shared__ double sums[kWarps], parts[kWarps];
     paged::pdl_enter();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t b = blockIdx.x / kCluster;
@@ -83,6 +100,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
     const int64_t* x = A.tokens + b * A.tokens_stride;
     const float* u = A.uniforms + b * A.uniforms_stride;
     const int64_t V = A.vocab;
+    const double draw = (double)u[A.drafts];
 
     // ---- accepted drafts (every CTA finds them alike)
     if (warp == 0) {
@@ -114,52 +132,66 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
     const int n = taken_at >> 1;
     const T* p = p0 + n * A.p.stride_step;
     const T* q = q0 + n * A.q.stride_step;
-    const double draw = (double)u[A.drafts];
 
     // ---- weights; elements are counted from a 16-byte boundary of p's row
-    const int64_t head = kV > 1 ? (int64_t)((uintptr_t)p % 16 / sizeof(T)) : 0;
+    const int head = kV > 1 ? (int)((uintptr_t)p % 16 / sizeof(T)) : 0;
     constexpr int kTile = 32 * kV;
-    const int64_t tiles = (head + V + kTile - 1) / kTile, per = (tiles + kRuns - 1) / kRuns;
-    const int run = rank * kWarps + warp;
-    const int64_t t0 = min(tiles, run * per), t1 = min(tiles, t0 + per);
+    const int vocab = (int)V, tiles = (head + vocab + kTile - 1) / kTile, per = (tiles + kRuns - 1) / kRuns;
     // 0: the whole row; 1: max(p - q, 0); 2: all but the drafted token
     int how = taken_at & 1 ? (A.q.data ? 1 : 2) : 0;
-    const int64_t without = how == 2 ? x[n] : -1;
-    auto weights = [&](int64_t tile, double (&w)[kV]) {
-        const int64_t e = tile * kTile + lane * kV - head;
+    const int without = how == 2 ? (int)x[n] : -1;
+    auto load = [&](int tile, float (&f)[kV], float (&g)[kV]) {
+        const int e = tile * kTile + lane * kV - head;
+        fetch<T, kV>(f, p, e, vocab);
+        if (how == 1) fetch<T, kV>(g, q, e, vocab);
+    };
+    auto weights = [&](int tile, double (&w)[kV]) {
+        const int e = tile * kTile + lane * kV - head;
         float f[kV], g[kV];
-        fetch<T, kV>(f, p, e, V);
-        if (how == 1) fetch<T, kV>(g, q, e, V);
+        load(tile, f, g);
 #pragma unroll
         for (int i = 0; i < kV; ++i) {
-            double v = how == 1 ? (double)f[i] - (double)g[i] : (double)f[i];
-            if (e + i == without) v = 0.0;
-            w[i] = v > 0.0 ? v : 0.0;          // (NaN too)
+            const double v = how == 1 ? (double)f[i] - (double)g[i] : (double)f[i];
+            w[i] = v > 0.0 && e + i != without ? v : 0.0;              // (NaN is none)
         }
     };
-    double total = 0.0, target = 0.0, upto = 0.0, mine = 0.0;
-    int from = -1, last_with = -1;
+    auto added = [&](double v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+        return v;
+    };
+    double target = 0.0, upto = 0.0;
+    int from = -1;
     for (int pass = 0;; ++pass) {              // (all CTAs go through it equally often, whatever they read)
-        mine = 0.0;
-        constexpr int kAtOnce = kV > 1 ? 4 : 8;
-        for (int64_t t = t0; t < t1; t += kAtOnce) {
-            double w[kAtOnce][kV];
+        const int t0 = min(tiles, (rank * kWarps + warp) * per), t1 = min(tiles, t0 + per);
+        Sum lanes[kV];
+        constexpr int kAtOnce = kV > 4 ? 2 : kV > 1 ? 4 : 8;
+        for (int t = t0; t < t1; t += kAtOnce) {
+            float f[kAtOnce][kV], g[kAtOnce][kV];
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) {
-                if (t + i < t1) {
-                    weights(t + i, w[i]);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < kV; ++k) w[i][k] = 0.0;
-                }
-            }
+            for (int i = 0; i < kAtOnce; ++i) load(t + i < t1 ? t + i : tiles, f[i], g[i]);   // (tile `tiles` lies outside)
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
-                for (int k = 0; k < kV; ++k) mine += w[i][k];
+                for (int k = 0; k < kV; ++k) {
+                    const float a = f[i][k];
+                    float d = a, left = 0.f;
+                    if (how == 1) {
+                        const float c = g[i][k];
+                        d = a - c;
+                        const float z = d - a;
+                        left = (a - (d - z)) - (c + z);
+                    } else if (how == 2 && (t + i) * kTile + lane * kV - head + k == without) {
+                        d = 0.f;
+                    }
+                    const bool some = d > 0.f;                         // (NaN is none)
+                    lanes[k].add(some ? d : 0.f, some ? left : 0.f);
+                }
         }
+        double mine = 0.0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(kAll, mine, o);
+        for (int k = 0; k < kV; ++k) mine += lanes[k].value();
+        mine = added(mine);
         if (lane == 0) sums[warp] = mine;
         cluster_sync();
         // every warp scans the runs' sums: lane l those of kRuns / 32 runs
@@ -172,8 +204,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
             own += part[i];
         }
         const double to = scan(own, lane);
-        total = __shfl_sync(kAll, to, 31);
-        target = draw * total;
+        target = draw * __shfl_sync(kAll, to, 31);
         double at = to - own;
         int hit = kRuns, with = -1;            // first run that passes the target, last run with a weight
         double before = 0.0;
@@ -188,8 +219,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
             }
             at += part[i];
         }
-        const int first = __reduce_min_sync(kAll, hit);
-        last_with = __reduce_max_sync(kAll, with);
+        const int first = __reduce_min_sync(kAll, hit), last_with = __reduce_max_sync(kAll, with);
         from = first < kRuns ? first : last_with;
         upto = __shfl_sync(kAll, before, first < kRuns ? first / kEach : 0);
         if (first == kRuns) target = INFINITY;                         // the last token with a weight
@@ -198,42 +228,64 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
         how = 0;                               // nothing is left of the residual: p itself
     }
 
-    // ---- the drawn token, by the warp whose run it is in (-1: by the first)
-    if (run != max(from, 0)) return;
-    int64_t token = -1;
-    if (from >= 0) {
-        for (int64_t t = t0; t < t1; ++t) {
-            double w[kV], own = 0.0;
-            weights(t, w);
-#pragma unroll
-            for (int k = 0; k < kV; ++k) own += w[k];
-            const double to = scan(own, lane);
-            double at = upto + (to - own);
-            int64_t found = -1, with = -1;
-#pragma unroll
-            for (int k = 0; k < kV; ++k) {
-                at += w[k];
-                if (w[k] > 0.0) {
-                    with = t * kTile + lane * kV + k - head;
-                    if (found < 0 && at > target) found = with;
-                }
-            }
-            const unsigned any = __ballot_sync(kAll, found >= 0), some = __ballot_sync(kAll, with >= 0);
-            if (any) {
-                token = __shfl_sync(kAll, found, __ffs(any) - 1);
-                break;
-            }
-            // where the two orders of summing differ in the last bit, the run's last token with a weight
-            if (some) token = __shfl_sync(kAll, with, 31 - __clz(some));
-            upto += __shfl_sync(kAll, to, 31);
-        }
-    }
+    // ---- the drawn token, by the CTA whose run it is in (-1: by the first)
+    if (rank != max(from, 0) / kWarps) return;
     int64_t* out = A.out + b * (A.drafts + 1);
-    for (int i = lane; i <= A.drafts; i += 32) out[i] = i < n ? x[i] : i == n ? token : -1;
-    if (lane == 0) A.accepted[b] = n;
+    auto write = [&](int64_t token) {
+        for (int i = lane; i <= A.drafts; i += 32) out[i] = i < n ? x[i] : i == n ? token : -1;
+        if (lane == 0) A.accepted[b] = n;
+    };
+    if (from < 0) {
+        if (warp == 0) write(-1);
+        return;
+    }
+    const int r0 = min(tiles, from * per), r1 = min(tiles, r0 + per), each = (r1 - r0 + kWarps - 1) / kWarps;
+    const int t0 = min(r1, r0 + warp * each), t1 = min(r1, t0 + each);
+    double mine = 0.0;
+    for (int t = t0; t < t1; ++t) {
+        double w[kV];
+        weights(t, w);
+#pragma unroll
+        for (int k = 0; k < kV; ++k) mine += w[k];
+    }
+    mine = added(mine);
+    if (lane == 0) parts[warp] = mine;
+    __syncthreads();
+    const double own = lane < kWarps ? parts[lane] : 0.0, to = scan(own, lane);
+    const unsigned some = __ballot_sync(kAll, own > 0.0), past = __ballot_sync(kAll, own > 0.0 && upto + to > target);
+    // (where two orders of summing differ in the last bits, the run's last part with a weight)
+    const int chosen = past ? __ffs(past) - 1 : some ? 31 - __clz(some) : 0;
+    if (warp != chosen) return;
+    upto += __shfl_sync(kAll, to - own, chosen);
+    int64_t token = -1;
+    for (int t = t0; t < t1; ++t) {
+        double w[kV], sum = 0.0;
+        weights(t, w);
+#pragma unroll
+        for (int k = 0; k < kV; ++k) sum += w[k];
+        const double end = scan(sum, lane);
+        double at = upto + (end - sum);
+        int found = -1, with = -1;
+#pragma unroll
+        for (int k = 0; k < kV; ++k) {
+            at += w[k];
+            if (w[k] > 0.0) {
+                with = t * kTile + lane * kV + k - head;
+                if (found < 0 && at > target) found = with;
+            }
+        }
+        const unsigned any = __ballot_sync(kAll, found >= 0), weighed = __ballot_sync(kAll, with >= 0);
+        if (any) {
+            token = __shfl_sync(kAll, found, __ffs(any) - 1);
+            break;
+        }
+        if (weighed) token = __shfl_sync(kAll, with, 31 - __clz(weighed));     // (the part's last, as above)
+        upto += __shfl_sync(kAll, end, 31);
+    }
+    write(token);
 }
 
-template <typename T, int kV>
+template <typename T, int kV, int kThreads>
 int launch_verify(const VerifyArgs& A, int64_t batch, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(batch * kCluster));
@@ -247,7 +299,7 @@ int launch_verify(const VerifyArgs& A, int64_t batch, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, verify_kernel<T, kV>, A);
+    cudaLaunchKernelEx(&cfg, verify_kernel<T, kV, kThreads>, A);
     return check_launch("epq_verify_drafts");
 }
 
@@ -257,7 +309,9 @@ template <typename T> int launch_verify_t(const VerifyArgs& A, int64_t batch, cu
     const bool wide = !A.q.data || (((uintptr_t)A.p.data - (uintptr_t)A.q.data) % 16 == 0 &&
                                     (A.p.stride_row - A.q.stride_row) * (int64_t)sizeof(T) % 16 == 0 &&
                                     (A.p.stride_step - A.q.stride_step) * (int64_t)sizeof(T) % 16 == 0);
-    return wide ? launch_verify<T, kV>(A, batch, st) : launch_verify<T, 1>(A, batch, st);
+    const bool few = batch * kCluster <= device_sms();
+    if (wide) return few ? launch_verify<T, kV, kFew>(A, batch, st) : launch_verify<T, kV, kMany>(A, batch, st);
+    return few ? launch_verify<T, 1, kFew>(A, batch, st) : launch_verify<T, 1, kMany>(A, batch, st);
 }
 
 }  // namespace
@@ -281,7 +335,7 @@ extern "C" int epq_verify_drafts(const epq_probs* target, const epq_probs* draft
         return set_error(EPQ_EINVAL, "epq_verify_drafts: batch=%lld, drafts=%d, vocab=%lld", (long long)batch, drafts,
                          (long long)vocab);
     if (!dtype_ok(dtype)) return set_error(EPQ_EDTYPE, "epq_verify_drafts: dtype %d", dtype);
-    if (batch > INT32_MAX / kCluster || drafts > (1 << 20) || vocab > INT32_MAX)
+    if (batch > INT32_MAX / kCluster || drafts > (1 << 20) || vocab > INT32_MAX / 2)
         return set_error(EPQ_EUNSUPPORTED, "epq_verify_drafts: batch=%lld, drafts=%d, vocab=%lld", (long long)batch, drafts,
                          (long long)vocab);
     if (batch == 0) return EPQ_OK;

@@ -150,7 +150,7 @@ int epq_paged_bounds(const epq_pages* pages, void* bounds, int64_t bounds_stride
  * those of the others with the largest scores (NaN first), the lowest of equal ones; all of them
  * where n <= count, and -1 behind the last.  A block whose page is outside the pool comes last.
  * The workspace is epq_paged_attend's in its rules, and the two may share one on a stream.
- * batch * kv_heads <= 65536. */
+ * batch * kv_heads <= 65536, max_pages < 2^21. */
 int64_t epq_paged_select_workspace_bytes(const epq_pages* pages, int64_t batch);
 int epq_paged_select(const epq_pages* pages, const void* bounds, int64_t bounds_stride, int32_t bounds_dtype,
                      const epq_heads* q, int32_t dtype, const int32_t* seq, const int64_t* lengths, int64_t batch,

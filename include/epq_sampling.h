@@ -30,8 +30,9 @@ typedef struct epq_probs {
  * the first v whose weights w_0 .. w_v sum to more than u_drafts times their whole sum, where
  *     w = max(p_n - q_n, 0) at a refused draft (p_n without x_n where draft is NULL, and p_n
  *         itself where nothing is left), else w = p_n.
- * Products and sums are 64-bit.  Weights that are negative or NaN count as 0; where the sum
- * reaches no token (u of 1, say) the last with a weight is taken, and -1 where none has one.
+ * Products are 64-bit, sums keep 45 bits or more of the weights' (whose sum lies in float32's
+ * range).  Weights that are negative or NaN count as 0; where the sum reaches no token (u of 1,
+ * say) the last with a weight is taken, and -1 where none has one.
  * out [batch, drafts + 1] receives the accepted drafts, the drawn token and -1 behind it;
  * accepted [batch] receives n.  A drafted token of vocab or more ends its row's drafts and is
  * reported by epq_device_error (bit 3).  The probabilities need only the alignment of their

@@ -73,7 +73,7 @@ def test_bad_verifications(lib):  # noqa: F811
     assert verify(batch=-1) == -1 and verify(drafts=-1) == -1 and verify(vocab=0) == -1
     assert verify(x=None) == -1 and verify(u=None) == -1 and verify(out=None) == -1 and verify(n=None) == -1
     assert verify(dtype=7) == -3 and verify(p=EpqProbs(4098, 1, 1)) == -4 and verify(q=EpqProbs(4097, 1, 1), dtype=2) == -4
-    assert verify(batch=2 ** 29) == -8 and verify(vocab=2 ** 31) == -8
+    assert verify(batch=2 ** 29) == -8 and verify(vocab=2 ** 30) == -8
     assert verify(batch=0) == 0
 
 
