@@ -318,7 +318,10 @@ __device__ void choose(const SelectArgs& A, const uint32_t* keys, int n, int32_t
         auto count = [&](uint32_t key) { have1 += key >= to1, have2 += key >= to2, have3 += key >= to3; };
         if (in_registers) {
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) count(held[i]);
+            for (int i = 0; i < kHeld; ++i) {
+                if (i >= each) break;
+                count(held[i]);
+            }
         } else {
             for (int j = j0; j < j1; ++j) count(free_key(j));
         }

@@ -90,7 +90,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == kMany ? 4 : 1) verify_ke
     constexpr int kWarps = kThreads / 32, kRuns = kCluster * kWarps;   // runs of the vocabulary
     static_assert(kRuns % 32 == 0, "a warp scans the runs");
     __shared__ int taken_at;                   // accepted drafts, times 2, and whether the next one was refused
-    __shared__ double sums[kWarps], parts[kWarps];
+    __shared__ double sums[kWarps], parts[kWarps], found_target, found_upto;
+    __shared__ int found_run;
     paged::pdl_enter();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t b = blockIdx.x / kCluster;
@@ -194,37 +195,47 @@ __global__ void __launch_bounds__(kThreads, kThreads == kMany ? 4 : 1) verify_ke
         mine = added(mine);
         if (lane == 0) sums[warp] = mine;
         cluster_sync();
-        // every warp scans the runs' sums: lane l those of kRuns / 32 runs
-        constexpr int kEach = kRuns / 32;
-        double part[kEach], own = 0.0;
+        // a warp of each CTA scans the runs' sums: lane l those of kRuns / 32 runs
+        if (warp == 0) {
+            constexpr int kEach = kRuns / 32;
+            double part[kEach], own = 0.0;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int r = lane * kEach + i;
-            part[i] = cluster_load(sums + r % kWarps, r / kWarps);
-            own += part[i];
-        }
-        const double to = scan(own, lane);
-        target = draw * __shfl_sync(kAll, to, 31);
-        double at = to - own;
-        int hit = kRuns, with = -1;            // first run that passes the target, last run with a weight
-        double before = 0.0;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            if (part[i] > 0.0) {
-                with = lane * kEach + i;
-                if (hit == kRuns && at + part[i] > target) {
-                    hit = lane * kEach + i;
-                    before = at;
-                }
+            for (int i = 0; i < kEach; ++i) {
+                const int r = lane * kEach + i;
+                part[i] = cluster_load(sums + r % kWarps, r / kWarps);
             }
-            at += part[i];
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) own += part[i];
+            const double to = scan(own, lane);
+            target = draw * __shfl_sync(kAll, to, 31);
+            double at = to - own;
+            int hit = kRuns, with = -1;        // first run that passes the target, last run with a weight
+            double before = 0.0;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                if (part[i] > 0.0) {
+                    with = lane * kEach + i;
+                    if (hit == kRuns && at + part[i] > target) {
+                        hit = lane * kEach + i;
+                        before = at;
+                    }
+                }
+                at += part[i];
+            }
+            const int first = __reduce_min_sync(kAll, hit), last_with = __reduce_max_sync(kAll, with);
+            upto = __shfl_sync(kAll, before, first < kRuns ? first / kEach : 0);
+            if (lane == 0) {
+                found_run = first < kRuns ? first : last_with;
+                found_target = first < kRuns ? target : INFINITY;      // (else the last token with a weight)
+                found_upto = upto;
+            }
         }
-        const int first = __reduce_min_sync(kAll, hit), last_with = __reduce_max_sync(kAll, with);
-        from = first < kRuns ? first : last_with;
-        upto = __shfl_sync(kAll, before, first < kRuns ? first / kEach : 0);
-        if (first == kRuns) target = INFINITY;                         // the last token with a weight
         cluster_sync();                        // nobody reads the sums any more
-        if (last_with >= 0 || pass) break;
+        from = found_run;
+        target = found_target;
+        upto = found_upto;
+        if (from >= 0 || pass) break;
+        __syncthreads();                       // (the three are read)
         how = 0;                               // nothing is left of the residual: p itself
     }
 

@@ -11,28 +11,39 @@ steps after it will see.
     decoder = PackedDecoder(shapes, max_len=4096)
     batch = BatchDecoder(decoder, seqs=16, format="int8")
     tokens = batch.generate(prompts, n_new=64)        # greedy, one CUDA graph a step
+    tokens = batch.generate(prompts, n_new=64, prefix=system)       # behind a prompt that all have in common
+    tokens, passes = batch.speculate(prompts, n_new=64, drafts=4)   # drafted tokens, judged several at a time
+
+With ``sparse`` a step attends over the blocks that ``epure.paged.select`` chooses, not over the whole cache.
 """
 import math
 
 import torch
 import torch.nn.functional as F
 
-from . import _native, paged
+from . import _native, paged, sampling
 
 
 class BatchDecoder:
     """``decoder``: a ``PackedDecoder`` in mode "ours" (its stores, embedding, lm_head and rotary tables are used, its
     own cache is not).  ``seqs`` sequences of up to the decoder's ``max_len`` tokens; ``pages`` defaults to room for
-    all of them.  ``format``: "same", "int8" or "fp8"."""
+    all of them.  ``format``: "same", "int8" or "fp8".  ``sparse``: (count, sinks, recent) blocks of ``page_size`` tokens
+    that each step's attention reads, as ``paged.select`` takes them; None: all."""
 
-    def __init__(self, decoder, seqs=16, format="same", page_size=64, pages=None):
+    def __init__(self, decoder, seqs=16, format="same", page_size=64, pages=None, sparse=None):
         if decoder.mode != "ours" or decoder.dtype != torch.bfloat16:
             raise ValueError("epure: a BatchDecoder needs a PackedDecoder in linear_mode 'ours'")
         sh = decoder.shapes
         self.decoder, self.shapes, self.device = decoder, sh, decoder.device
         per_seq = -(-decoder.max_len // page_size)
         self.cache = paged.PagedKVCache(decoder.layers, pages or seqs * per_seq, page_size, sh.kv_heads, sh.head_dim,
-                                        seqs, decoder.max_len, format, decoder.dtype, decoder.device)
+                                        seqs, decoder.max_len, format, decoder.dtype, decoder.device,
+                                        bounds=sparse is not None)
+        if sparse is not None:
+            count, sinks, recent = sparse
+            if min(sinks, recent) < 0 or count < max(1, sinks + recent):
+                raise ValueError(f"epure: sparse=(count, sinks, recent) with sinks + recent <= count (got {sparse})")
+        self.sparse = sparse
         self._layers = [self.cache.layer(i) for i in range(decoder.layers)]
         # rows that the fused linears of a block take; larger batches go through linear_multi and separate glue
         rms, none = _native.PRO_RMSNORM, _native.PRO_NONE
@@ -59,25 +70,44 @@ class BatchDecoder:
         return paged.write(pages, k.view(rows, -1, hd), v.view(rows, -1, hd), seq, pos, q=q, q_out=q, cos=d.cos,
                            sin=d.sin, qk_norm=d.qk_norm, eps=d.eps)
 
-    # -- one token a sequence ------------------------------------------------------------------------------------
-    def step(self, tokens, seq, pos):
+    def _attend(self, layer, pages, q, lengths, seq, first, scale, shared):
+        """Attention of a step's rows q [rows, heads, head_dim]."""
+        if shared is not None:
+            return paged.attend_shared(pages, q, lengths, *shared, seq=seq, scale=scale)
+        if self.sparse is None:
+            return paged.attend(pages, q, lengths, seq=seq, scale=scale)
+        count, sinks, recent = self.sparse
+        bounds = self.cache.bounds[layer]
+        paged.summarise(pages, bounds, lengths, seq=seq, first=first)
+        chosen = paged.select(pages, bounds, q, lengths, count, seq=seq, sinks=sinks, recent=recent)
+        return paged.attend(pages, q, lengths, seq=seq, scale=scale, blocks=chosen)
+
+    # -- one token a row -----------------------------------------------------------------------------------------
+    def step(self, tokens, seq, pos, shared=None):
         """Logits [batch, vocab] after feeding token ``tokens[b]`` (int64) as token ``pos[b]`` (int64) of sequence
         ``seq[b]`` (int32), all on the device.  A negative position is an idle row.  The pages must be reserved
-        (``cache.reserve``).  Static shapes: capturable."""
+        (``cache.reserve``).  Static shapes: capturable.
+
+        Several rows may be tokens of one sequence (drafts): each attends over its own position and those before it.
+        ``shared``: ``(starts, prefix)`` as ``paged.attend_shared`` takes them, for rows that have their first tokens in
+        common; not with ``sparse``, where a call has one row a sequence."""
+        if shared is not None and self.sparse is not None:
+            raise ValueError("epure: a sparse step reads selected blocks, not a shared prefix")
         d, sh = self.decoder, self.shapes
         B, scale = tokens.shape[0], 1.0 / math.sqrt(sh.head_dim)
         lengths = (pos + 1).clamp_(min=0)                              # idle rows have no tokens
+        first = pos.clamp(min=0) if self.sparse is not None else None
         h = d.embed[tokens]                                            # residual stream [B, hidden]
         fused = B <= self._fused_rows
         y = None if fused else _native.add_rmsnorm(h, eps=d.eps)
-        for pages, b in zip(self._layers, d.stack.blocks):
+        for layer, (pages, b) in enumerate(zip(self._layers, d.stack.blocks)):
             qkv = [b["q_proj"], b["k_proj"], b["v_proj"]]
             if fused:
                 q, k, v = _native.decode_linear(h, qkv, prologue=_native.PRO_RMSNORM, eps=d.eps)
             else:
                 q, k, v = _native.linear_multi(y, qkv)
             q = self._write(pages, q, k, v, seq, pos)
-            att = paged.attend(pages, q, lengths, seq=seq, scale=scale).view(B, -1)
+            att = self._attend(layer, pages, q, lengths, seq, first, scale, shared).view(B, -1)
             if fused:
                 _native.decode_linear(att, [b["o_proj"]], epilogue=_native.EPI_RESIDUAL, outs=[h])
                 (a,) = _native.decode_linear(h, [b["gate_proj"], b["up_proj"]], prologue=_native.PRO_RMSNORM,
@@ -100,14 +130,19 @@ class BatchDecoder:
         if T < 1:
             raise ValueError("epure: an empty prompt")
         self.cache.reserve(seq, past + T)
+        if self.sparse is not None:                                    # the bounds of the pages that the prompt fills
+            row, till = torch.tensor([seq], dtype=torch.int32, device=dev), torch.tensor([past + T], device=dev)
+            since = torch.tensor([past], device=dev)
         pos = torch.arange(past, past + T, device=dev)
         every = torch.arange(past + T, device=dev)
         ids = torch.full((past + T,), seq, dtype=torch.int32, device=dev)
         seen = None if past == 0 else every[None, :] <= pos[:, None]
         h = d.embed[prompt.to(dev)]
-        for pages, b in zip(self._layers, d.stack.blocks):
+        for layer, (pages, b) in enumerate(zip(self._layers, d.stack.blocks)):
             q, k, v = _native.linear_multi(d._rms(h), [b["q_proj"], b["k_proj"], b["v_proj"]])
             q = self._write(pages, q, k, v, ids[past:], pos)
+            if self.sparse is not None:
+                paged.summarise(pages, self.cache.bounds[layer], till, seq=row, first=since)
             k, v = paged.read(pages, ids, every, dtype=d.dtype)
             att = F.scaled_dot_product_attention(q.transpose(0, 1)[None], k.transpose(0, 1)[None],
                                                  v.transpose(0, 1)[None], attn_mask=seen, is_causal=seen is None,
@@ -119,16 +154,20 @@ class BatchDecoder:
         return self._logits(h[-1:].contiguous())[0]
 
     # -- greedy decoding -----------------------------------------------------------------------------------------
-    def _captured(self, batch):
-        """(graph, tok, seq, pos): one greedy step of ``batch`` rows; writes the argmax into tok, advances pos."""
-        if batch not in self._graphs:
+    def _captured(self, batch, behind=False):
+        """(graph, tok, seq, pos, starts, prefix): one greedy step of ``batch`` rows, all of them behind one prefix where
+        ``behind``; writes the argmax into tok, advances pos."""
+        if (batch, behind) not in self._graphs:
             dev = self.device
             tok = torch.zeros(batch, dtype=torch.long, device=dev)
             seq = torch.arange(batch, dtype=torch.int32, device=dev)
             pos = torch.full((batch,), -1, dtype=torch.long, device=dev)     # idle rows: no cache is touched
+            starts = torch.tensor([0, batch], dtype=torch.int32, device=dev)
+            prefix = torch.zeros(1, dtype=torch.long, device=dev)
+            shared = (starts, prefix) if behind else None
 
             def body():
-                tok.copy_(torch.argmax(self.step(tok, seq, pos), dim=-1))
+                tok.copy_(torch.argmax(self.step(tok, seq, pos, shared), dim=-1))
                 pos.add_(1)
 
             side = torch.cuda.Stream(device=dev)
@@ -141,38 +180,134 @@ class BatchDecoder:
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 body()
-            self._graphs[batch] = (graph, tok, seq, pos)
-        return self._graphs[batch]
+            self._graphs[batch, behind] = (graph, tok, seq, pos, starts, prefix)
+        return self._graphs[batch, behind]
 
-    def generate(self, prompts, n_new, graph=True):
+    def _check(self, prompts):
+        if not 1 <= len(prompts) <= self.cache.seqs:
+            raise ValueError(f"epure: {len(prompts)} prompts for a cache of {self.cache.seqs} sequences")
+
+    def _begin(self, prompts, n_new, prefix):
+        """Reserves and fills the sequences of ``prompts`` (behind the common tokens ``prefix``, if any) with room for
+        ``n_new`` more tokens: (greedy first tokens, lengths, tokens in common), the first a list of tensors."""
+        n = 0 if prefix is None else prefix.shape[0]
+        whole = 0
+        first, lengths = [], []
+        for i, p in enumerate(prompts):
+            if i == 0:
+                self.cache.reserve(0, n + p.shape[0] + n_new)
+                if n:
+                    self.prefill(0, prefix)
+                    whole = n // self.cache.page_size * self.cache.page_size
+            elif n:                                        # the prefix's whole pages are shared, its rest is written again
+                self.cache.share(i, 0, whole)
+            self.cache.reserve(i, n + p.shape[0] + n_new)
+            if n and i and whole < n:
+                self.prefill(i, prefix[whole:], past=whole)
+            first.append(torch.argmax(self.prefill(i, p, past=n)))
+            lengths.append(n + p.shape[0])
+        return first, lengths, n
+
+    def generate(self, prompts, n_new, graph=True, prefix=None):
         """``n_new`` greedy tokens after each of the ``prompts`` (long tensors), a long tensor [len(prompts), n_new].
-        The sequences 0 .. len(prompts) - 1 are used and released."""
+        ``prefix`` (a long tensor) comes before every prompt: it is computed and kept once, and each step's attention
+        reads it once for all rows.  The sequences 0 .. len(prompts) - 1 are used and released."""
+        self._check(prompts)
         B, dev = len(prompts), self.device
-        if not 1 <= B <= self.cache.seqs:
-            raise ValueError(f"epure: {B} prompts for a cache of {self.cache.seqs} sequences")
         out = torch.empty(B, n_new, dtype=torch.long, device=dev)
         try:
-            first = []
-            for i, p in enumerate(prompts):
-                self.cache.reserve(i, p.shape[0] + n_new)
-                first.append(torch.argmax(self.prefill(i, p)))
-            tok, pos = torch.stack(first), torch.tensor([p.shape[0] for p in prompts], device=dev)
+            first, lengths, n = self._begin(prompts, n_new, prefix)
+            tok, pos = torch.stack(first), torch.tensor(lengths, device=dev)
             seq = torch.arange(B, dtype=torch.int32, device=dev)
+            behind = n > 0 and self.sparse is None
             if graph:
-                g, gtok, gseq, gpos = self._captured(B)
+                g, gtok, gseq, gpos, _, gprefix = self._captured(B, behind)
                 gtok.copy_(tok)
                 gseq.copy_(seq)
                 gpos.copy_(pos)
+                gprefix.fill_(n)
                 for t in range(n_new):
                     out[:, t] = gtok
                     if t + 1 < n_new:
                         g.replay()
             else:
+                shared = (torch.tensor([0, B], dtype=torch.int32, device=dev), torch.tensor([n], device=dev)) if behind else None
                 for t in range(n_new):
                     out[:, t] = tok
                     if t + 1 < n_new:
-                        tok = torch.argmax(self.step(tok, seq, pos + t), dim=-1)
+                        tok = torch.argmax(self.step(tok, seq, pos + t, shared), dim=-1)
         finally:
             for i in range(B):
                 self.cache.release(i)
         return out
+
+    # -- drafted tokens ------------------------------------------------------------------------------------------
+    def judge(self, tokens, drafts, seq, pos, uniforms, temperature=1.0, draft_probs=None):
+        """One pass over drafted tokens: ``tokens`` [batch] (the last known token of each sequence, at ``pos``) and
+        ``drafts`` [batch, n] behind it (a row's end at its first negative one) are fed together, n + 1 rows a sequence
+        that share what the sequence holds already, and judged by ``sampling.verify`` with the numbers ``uniforms``
+        [batch, n + 1].  ``temperature`` 0 takes the most likely token.  Returns verify's ``(tokens [batch, n + 1],
+        accepted [batch])``: a row's first ``accepted + 1`` tokens are its next ones.  The cache then holds ``pos +
+        accepted + 1`` of its tokens; the last one returned is the next call's.  The pages must be reserved up to ``pos +
+        n + 1`` tokens.  A negative position is an idle row.  Not with ``sparse``.  Capturable."""
+        if self.sparse is not None:
+            raise ValueError("epure: drafted tokens are judged over the whole cache (sparse=None)")
+        B, n = drafts.shape
+        dev = self.device
+        rows = torch.cat((tokens[:, None], drafts), 1)
+        there = (rows >= 0).to(torch.long).cumprod(1) * (pos >= 0)[:, None]
+        step = torch.arange(n + 1, device=dev)
+        at = torch.where(there > 0, pos[:, None] + step, -1)
+        starts = torch.arange(0, B * (n + 1) + 1, n + 1, dtype=torch.int32, device=dev)
+        logits = self.step(rows.clamp(min=0).reshape(-1), seq.repeat_interleave(n + 1), at.reshape(-1),
+                           (starts, (pos + 1).clamp(min=0)))
+        logits = logits.view(B, n + 1, -1)
+        if temperature > 0:
+            probs = torch.softmax(logits / temperature, -1)
+        else:
+            probs = torch.zeros_like(logits).scatter_(-1, logits.argmax(-1, keepdim=True), 1.0)
+        return sampling.verify(probs, draft_probs, drafts, uniforms)
+
+    def speculate(self, prompts, n_new, drafts=4, temperature=0.0, prefix=None, generator=None):
+        """``n_new`` tokens after each of the ``prompts``, drafted ``drafts`` at a time by looking the last two tokens up
+        in what a sequence holds so far (the tokens behind their last occurrence), and the number of passes it took.
+        ``temperature`` 0 gives ``generate``'s tokens but for near ties; ``generator`` (of the decoder's device) draws
+        the random numbers otherwise.  A sequence needs room for ``drafts + 1`` tokens more."""
+        self._check(prompts)
+        B, dev = len(prompts), self.device
+        if drafts < 0 or self.sparse is not None:
+            raise ValueError(f"epure: drafts={drafts} (at least 0, and judged over the whole cache: sparse=None)")
+        room = n_new + drafts + 1
+        passes = 0
+        try:
+            first, lengths, n = self._begin(prompts, room, prefix)
+            before = [] if prefix is None else prefix.tolist()
+            text = [before + p.tolist() + [int(t)] for p, t in zip(prompts, first)]
+            done = [n + p.shape[0] + n_new for p in prompts]
+            seq = torch.arange(B, dtype=torch.int32, device=dev)
+            while any(len(x) < d for x, d in zip(text, done)):
+                guess = [_look_up(x, drafts) for x in text]
+                pos = [len(x) - 1 if len(x) < d else -1 for x, d in zip(text, done)]
+                u = torch.rand(B, drafts + 1, device=dev, generator=generator)
+                got, kept = self.judge(torch.tensor([x[-1] for x in text], device=dev),
+                                       torch.tensor(guess, dtype=torch.long, device=dev).view(B, drafts), seq,
+                                       torch.tensor(pos, device=dev), u, temperature)
+                passes += 1
+                for x, p, tokens, k in zip(text, pos, got.tolist(), kept.tolist()):
+                    if p >= 0:
+                        x += tokens[:k + 1]
+        finally:
+            for i in range(B):
+                self.cache.release(i)
+        out = torch.tensor([x[d - n_new:d] for x, d in zip(text, done)], device=dev)
+        return out, passes
+
+
+def _look_up(text, count):
+    """Up to ``count`` tokens behind the last earlier occurrence of the text's last two, padded with -1."""
+    last = text[-2:]
+    for i in range(len(text) - 3, -1, -1):
+        if text[i:i + 2] == last:
+            got = text[i + 2:i + 2 + count]
+            return got + [-1] * (count - len(got))
+    return [-1] * count
