@@ -231,7 +231,7 @@ template <int kMode, bool kQuant>
 __device__ __forceinline__ void emit_row(const AttendArgs& A, int b, int h, int d, const float (&val)[4], float at, float to,
                                          float sum) {
     const int64_t place = (int64_t)b * A.heads + h;
-    if (kMode == kBehindShared) {
+    if (kMode == kBehindShared && A.shared.row_from[b] > 0) {
         const float turn = kQuant && sum != 0.f ? ex2(at - to) : 1.f;
         float* const rec = A.shared.rest + place * A.shared.pitch;
         *reinterpret_cast<float4*>(rec + d) = make_float4(val[0] * turn, val[1] * turn, val[2] * turn, val[3] * turn);
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
     some_empty = __any_sync(kAll, some_empty);
     for (int b = blockIdx.x; some_empty && b < A.batch; b += gridDim.x) {
         if (span_of<kMode, kTok>(A, b, false).blocks) continue;
-        if (kMode == kBehindShared) {                  // nothing but the shared tokens, if any
+        if (kMode == kBehindShared && A.shared.row_from[b] > 0) {      // nothing but the shared tokens, if any
             for (int h = tid; h < A.heads; h += kThreads)
                 *reinterpret_cast<float4*>(A.shared.rest + ((int64_t)b * A.heads + h + 1) * A.shared.pitch - 4) =
                     make_float4(-FLT_MAX, 0.f, 0.f, 0.f);

@@ -9,8 +9,8 @@
 // Plan (one CTA): groups are cut into tiles of up to 256 query rows (128 where head_dim > 128);
 // L of a tile is its prefix, or the shortest of its rows' lengths.  No score needs a mask by row
 // then: what a row sees beyond L is its own part, and a value there that is not finite stays in
-// the rows that see it.  Where the whole batch would save less than kWorth bytes of reading,
-// nothing is shared.
+// the rows that see it.  A tile shares where reading its tokens row by row is reckoned to take
+// longer than its blocks here (Reckoning below), a batch where its tiles save more than kFixed.
 //
 // Shared part.  Blocks of 128 tokens of all units (tile, key head) are dealt out to the CTAs in
 // equal runs, one CTA an SM, and each piece of a unit leaves its sums as records.  In a CTA:
@@ -49,9 +49,26 @@ constexpr int kPlanThreads = 512;
 constexpr int kHeldTiles = 512;            // tiles that the plan keeps in shared memory
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr int kSmemLimit = 232448;         // 227 KB a CTA
-// Bytes of reading that sharing has to save: the plan and the shared part's launch cost about as
-// much as these take from HBM.
-constexpr int64_t kWorth = 32 << 20;
+
+// What is reckoned with, in ns, from both sides measured (B200, graphs of calls; 2 to 64 rows a
+// group, 1 to 16 groups, 1024 to 65536 tokens, 32 / 8, 64 / 8 and 8 / 1 heads of 64 and 128,
+// 16 / 4 of 256).  Row by row: 10 us and 9.0 to 10.3 TB/s of 16-bit caches (6.2 for heads of 256), 5.6
+// to 6.9 of 8-bit ones; what several rows read comes from L2.  Shared: 30 to 41 us, and a block of 128
+// tokens and 128 rows 1.65 us (64 dims), 2.0 (128) or 4.1 (256), 8-bit ones 2.6 and 3.1.  So 2
+// rows of 32 / 8 heads do not share before 2 x 16 groups x 16k tokens (222 us for 326; 16 x 4k:
+// 81 for 80), 4 groups of 4 with int8 not at all (354 us for 309 at 64k), and 64 rows always
+// from 4k tokens on.  What the plan then leaves row by row costs its launches, 9 us.
+constexpr float kFixed = 25000.f;
+struct Reckoning {
+    float row_token;                       // a token of all key heads, row by row, on the whole card
+    float block;                           // 128 tokens of 128 rows and a key head, on one SM
+};
+Reckoning reckon(const PagesD& P) {
+    const int64_t token_bytes = 2LL * P.kv_heads * (P.format == EPQ_CACHE_SAME ? P.head_dim * 2 : P.head_dim + 4);
+    if (P.format != EPQ_CACHE_SAME) return {(float)token_bytes / 6900.f, P.head_dim <= 64 ? 2600.f : 3100.f};
+    if (P.head_dim > 128) return {(float)token_bytes / 6200.f, 4100.f};
+    return {(float)token_bytes / 9300.f, P.head_dim <= 64 ? 1650.f : 2050.f};
+}
 
 struct SharedArgs {
     PagesD pages;
@@ -60,7 +77,8 @@ struct SharedArgs {
     const int64_t* lengths;
     const int32_t* starts;
     const int64_t* prefix;
-    int64_t token_bytes;                   // of one cached token: keys, values, scales
+    Reckoning cost;
+    bool always;                           // share whatever can be
     int batch, groups, heads, group, max_tiles, grid, box_rows;
     float scale_log2;
 };
@@ -154,13 +172,18 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const SharedArgs A) 
         if (lane == 0) {
             const int b = T.row0 + first;
             tile[t].seq = active < 2 ? 0 : A.seq ? A.seq[b] : b;
-            tile[t].tokens = least;
-            saved += (int64_t)(active - 1) * least;
+            const int blocks = (least + kSharedTokens - 1) / kSharedTokens;
+            const int tile_slots = T.rows > A.s.lane_rows ? 2 : 1;              // (of up to 128 query rows)
+            const float gain = (float)active * (float)least * A.cost.row_token -
+                               (float)blocks * (float)(P.kv_heads * tile_slots) * A.cost.block / (float)A.grid;
+            const bool shares = A.always || gain > 0.f;
+            tile[t].tokens = shares ? least : 0;
+            saved += shares ? (int64_t)gain : 0;
         }
     }
     int64_t all_saved;
     block_scan(saved, scratch, &all_saved);
-    const bool worth = all_saved * A.token_bytes >= kWorth;
+    const bool worth = A.always || all_saved > (int64_t)kFixed;
     // places of the units
     int64_t total = 0;
     for (int t0 = 0; t0 < tiles; t0 += kPlanThreads) {
@@ -803,31 +826,30 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
 }
 
 // ---------------------------------------------------------------- the join
-// A warp a row's head: the records of its unit's pieces and of its other tokens, in the order of the pieces, so that
-// results do not depend on timing.  Bound: the records' bytes (from L2), all asked for at once.
+// kTeam warps a row's head: the records of its unit's pieces and of its other tokens, in the order of the pieces, so that
+// results do not depend on timing.  Bound: the records' bytes (from L2), 8 records at a time and warp.  Up to
+// 4 query rows an SM, of many pieces each, get a CTA each: 16 rows of 8 heads behind one prefix of 64k
+// 45 us in all, with a warp each 86; 64 rows of 32 heads behind 4k 58 and 42, so they get a warp.
 constexpr int kJoinWarps = 8;
 
-template <bool kBf> __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const AttendArgs A) {
+template <bool kBf, int kTeam> __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const AttendArgs A) {
     pdl_enter();
     const SharedD& S = A.shared;
     const int lane = threadIdx.x & 31, hd = A.pages.head_dim, pitch = S.pitch;
-    const int64_t place = (int64_t)blockIdx.x * kJoinWarps + threadIdx.x / 32;
+    __shared__ float parts[kTeam > 1 ? kTeam : 1][kTeam > 1 ? 10 : 1][32];
+    const int member = threadIdx.x / 32 % kTeam;
+    const int64_t place = (int64_t)blockIdx.x * (kJoinWarps / kTeam) + threadIdx.x / 32 / kTeam;
     if (place >= S.own_records) return;
     const int b = (int)(place / A.heads), h = (int)(place - (int64_t)b * A.heads);
-    const int tile = S.row_tile[b], from = S.row_from[b];
+    const int tile = S.row_tile[b];
+    if (S.row_from[b] == 0) return;                                    // it shares nothing and is written already
     const float* const rest = S.rest + place * pitch;
-    int64_t c0 = 0;
-    int pieces = 0, two = 1, part = 0, at = 0;
-    if (tile >= 0 && from > 0) {
-        const SharedTile T = S.tiles[tile];
-        const int head = h / A.group;
-        part = (b - T.row0) / S.lane_rows;
-        at = (b - T.row0 - part * S.lane_rows) * A.group + h - head * A.group;
-        const int64_t first = T.first + (int64_t)head * T.blocks, run = S.head->run;
-        c0 = first / run;
-        two = shared_alternates(T.rows, S.lane_rows, S.slots) ? 2 : 1;
-        pieces = (int)((first + T.blocks - 1) / run - c0 + 1) * two;
-    }
+    const SharedTile T = S.tiles[tile];
+    const int head = h / A.group, part = (b - T.row0) / S.lane_rows;
+    const int at = (b - T.row0 - part * S.lane_rows) * A.group + h - head * A.group;
+    const int64_t first = T.first + (int64_t)head * T.blocks, run = S.head->run, c0 = first / run;
+    const int two = shared_alternates(T.rows, S.lane_rows, S.slots) ? 2 : 1;
+    const int pieces = (int)((first + T.blocks - 1) / run - c0 + 1) * two;
     auto record = [&](int p) -> const float* {                          // p = pieces: the rest
         if (p >= pieces) return rest;
         const int64_t c = c0 + (two == 2 ? p >> 1 : p);
@@ -837,11 +859,12 @@ template <bool kBf> __global__ void __launch_bounds__(kJoinWarps * 32) join_kern
     };
     const bool two_rows = lane * 4 + 128 < hd;                         // (head_dim above 128: a lane's second four values)
     float top = -FLT_MAX, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int p0 = 0; p0 <= pieces; p0 += 32) {
+    const int per = (pieces + kTeam) / kTeam, end = min(pieces + 1, per * (member + 1));
+    for (int p0 = per * member; p0 < end; p0 += 32) {
         // a lane a record: its maximum and sum; one without a score above -inf holds no values
         const int p = p0 + lane;
         float4 ml = make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
-        if (p <= pieces) ml = __ldcg(reinterpret_cast<const float4*>(record(p) + pitch - 4));
+        if (p < end) ml = __ldcg(reinterpret_cast<const float4*>(record(p) + pitch - 4));
         float m = ml.x;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kWarpAll, m, o));
@@ -856,7 +879,7 @@ template <bool kBf> __global__ void __launch_bounds__(kJoinWarps * 32) join_kern
         for (int i = 0; i < 8; ++i) v[i] *= turn;
         top = now;
         const unsigned there = __ballot_sync(kWarpAll, !empty);
-        const int count = min(32, pieces + 1 - p0);
+        const int count = min(32, end - p0);
         constexpr int kAtOnce = 8;
         for (int q0 = 0; q0 < count; q0 += kAtOnce) {
             float4 x[kAtOnce], y[kAtOnce];
@@ -877,12 +900,32 @@ template <bool kBf> __global__ void __launch_bounds__(kJoinWarps * 32) join_kern
             }
         }
     }
-    using T = typename Half<kBf>::type;
+    if (kTeam > 1) {
+        parts[member][0][lane] = top;
+        parts[member][1][lane] = sum;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) parts[member][2 + i][lane] = v[i];
+        __syncthreads();
+        if (member) return;
+#pragma unroll
+        for (int w = 1; w < kTeam; ++w) top = fmaxf(top, parts[w][0][lane]);
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kTeam; ++w) {                              // (a warp without a score has zeros)
+            const float turn = ex2(parts[w][0][lane] - top);
+            sum += parts[w][1][lane] * turn;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += parts[w][2 + i][lane] * turn;
+        }
+    }
+    using H = typename Half<kBf>::type;
     const float gain = sum == 0.f ? 0.f : 1.f / sum;
     uint16_t* const out = static_cast<uint16_t*>(A.out) + place * hd + lane * 4;
-    if (lane * 4 < hd) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0] * gain, v[1] * gain), pack2<T>(v[2] * gain, v[3] * gain));
+    if (lane * 4 < hd) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<H>(v[0] * gain, v[1] * gain), pack2<H>(v[2] * gain, v[3] * gain));
     if (two_rows)
-        *reinterpret_cast<uint2*>(out + 128) = make_uint2(pack2<T>(v[4] * gain, v[5] * gain), pack2<T>(v[6] * gain, v[7] * gain));
+        *reinterpret_cast<uint2*>(out + 128) = make_uint2(pack2<H>(v[4] * gain, v[5] * gain), pack2<H>(v[6] * gain, v[7] * gain));
     if (A.lse && lane == 0) A.lse[place] = sum == 0.f ? -INFINITY : (top + log2f(sum)) / kLog2e;
 }
 
@@ -925,24 +968,21 @@ Layout layout_of(const PagesD& P, int64_t batch, int heads, int64_t groups, int6
     return L;
 }
 
-// Whether a batch can share anything that is worth it: groups of two rows or more whose query heads fit a tile, enough
+// Whether a batch can share anything (that is worth it): groups of two rows or more whose query heads fit a tile, enough
 // tokens that the tables could hold, and pages that the copies of rows take: boxes of 8 rows or more, which lie side by
 // side in the 128-byte swizzle.  8-bit heads above 128 have no room for their 16-bit form.
-bool may_share(const PagesD& P, int64_t batch, int heads, int64_t groups, int64_t token_bytes) {
+bool may_share(const PagesD& P, int64_t batch, int heads, int64_t groups, bool always) {
     const int64_t most = (int64_t)P.max_pages * P.page_size;
     const int64_t pool = P.pages > (1LL << 40) / P.page_size ? 1LL << 40 : P.pages * P.page_size;   // (all tables together)
     const int64_t tokens = most < pool ? most : pool;
     return groups > 0 && batch > 1 && heads / P.kv_heads <= kSharedLanes && P.page_size % 8 == 0 &&
            (P.format == EPQ_CACHE_SAME || P.head_dim <= 128) &&
-           (double)(batch - 1) * (double)tokens * (double)token_bytes >= (double)kWorth;
+           (always || (double)batch * (double)tokens * (double)reckon(P).row_token > (double)kFixed);
 }
 // Whether rows of q can be copied as boxes (other views take the plain form).
 bool boxes_of(const epq_heads& q, int64_t batch) {
     auto good = [](int64_t stride) { return stride > 0 && stride % 8 == 0 && stride < (1LL << 36); };
     return (uintptr_t)q.data % 16 == 0 && good(q.stride_row) && (q.heads == 1 || good(q.stride_head));
-}
-int64_t bytes_of_token(const PagesD& P, int dtype_bytes) {
-    return 2LL * P.kv_heads * (P.format == EPQ_CACHE_SAME ? P.head_dim * dtype_bytes : P.head_dim + 4);
 }
 
 }  // namespace
@@ -969,7 +1009,8 @@ using namespace epq::paged;
 
 extern "C" {
 
-int64_t epq_paged_attend_shared_workspace_bytes(const epq_pages* pages, int64_t batch, int32_t heads, int64_t groups) {
+int64_t epq_paged_attend_shared_workspace_bytes(const epq_pages* pages, int64_t batch, int32_t heads, int64_t groups,
+                                                int32_t always) {
     const char* const who = "epq_paged_attend_shared_workspace_bytes";
     if (groups < 0) return set_error(EPQ_EINVAL, "%s: groups=%lld", who, (long long)groups);
     const int64_t behind = attend_bytes(who, pages, batch, heads);
@@ -977,13 +1018,13 @@ int64_t epq_paged_attend_shared_workspace_bytes(const epq_pages* pages, int64_t 
     PagesD P;
     make_pages(pages, &P, who);
     if (batch > 65536) return set_error(EPQ_EUNSUPPORTED, "%s: batch=%lld", who, (long long)batch);
-    if (!may_share(P, batch, heads, groups, bytes_of_token(P, 2))) return behind;
+    if (!may_share(P, batch, heads, groups, always != 0)) return behind;
     return layout_of(P, batch, heads, groups, align256(behind)).bytes;
 }
 
 int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const int32_t* seq, const int64_t* lengths,
-                            int64_t batch, const int32_t* starts, const int64_t* prefix, int64_t groups, float scale, void* out,
-                            float* lse, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+                            int64_t batch, const int32_t* starts, const int64_t* prefix, int64_t groups, int32_t always,
+                            float scale, void* out, float* lse, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* const who = "epq_paged_attend_shared";
     if (groups < 0 || groups > INT32_MAX - 1 || (groups && (!starts || !prefix)))
         return set_error(EPQ_EINVAL, "%s: groups=%lld, or NULL starts or prefix", who, (long long)groups);
@@ -994,9 +1035,8 @@ int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const in
                                &ready);
     if (rc != EPQ_OK || !ready) return rc;
     const PagesD& P = A.pages;
-    const int64_t token_bytes = bytes_of_token(P, 2);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!may_share(P, batch, A.heads, groups, token_bytes) || !boxes_of(*q, batch)) return launch_attend_plain(A, cols, st);
+    if (!may_share(P, batch, A.heads, groups, always != 0) || !boxes_of(*q, batch)) return launch_attend_plain(A, cols, st);
     const int64_t behind = align256(attend_bytes(who, pages, batch, A.heads));
     const Layout L = layout_of(P, batch, A.heads, groups, behind);
     if (workspace_bytes < L.bytes)
@@ -1020,7 +1060,8 @@ int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const in
     S.lengths = lengths;
     S.starts = starts;
     S.prefix = prefix;
-    S.token_bytes = token_bytes;
+    S.cost = reckon(P);
+    S.always = always != 0;
     S.batch = (int)batch;
     S.groups = (int)groups;
     S.heads = A.heads;
@@ -1052,8 +1093,11 @@ int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const in
     A.shared = S.s;
     e = attend_behind_shared(A, cols, st);
     if (e != EPQ_OK) return e;
-    const dim3 grid((unsigned)cdiv(S.s.own_records, kJoinWarps)), threads(kJoinWarps * 32);
-    return bf ? launch(join_kernel<true>, grid, threads, 0, st, who, A) : launch(join_kernel<false>, grid, threads, 0, st, who, A);
+    const bool teams = S.s.own_records <= 4LL * S.grid;
+    const dim3 grid((unsigned)cdiv(S.s.own_records, teams ? 1 : kJoinWarps)), threads(kJoinWarps * 32);
+    auto join = [&](auto kern) { return launch(kern, grid, threads, 0, st, who, A); };
+    if (teams) return bf ? join(join_kernel<true, kJoinWarps>) : join(join_kernel<false, kJoinWarps>);
+    return bf ? join(join_kernel<true, 1>) : join(join_kernel<false, 1>);
 }
 
 }  // extern "C"

@@ -454,7 +454,7 @@ PyObject* attend(PyObject* const* a) {
 }
 
 // attend_shared(k_pool, v_pool, table, k_scale, v_scale, q, lengths, starts, prefix, seq | None, scale | None, out | None,
-//               return_lse)
+//               return_lse, always)
 PyObject* attend_shared(PyObject* const* a) {
     const Tensor &starts = tensor(a[7], "starts"), &prefix = tensor(a[8], "prefix");
     const Attention t(a, a[9], a[10], a[11], a[12], "attend_shared", 16);
@@ -463,12 +463,13 @@ PyObject* attend_shared(PyObject* const* a) {
     index_of(prefix, "prefix", c.device, at::kLong, groups);
     index_of(starts, "starts", c.device, at::kInt, groups + 1);
     OnDevice on(c.device);
-    const int64_t need = lib.shared_bytes(&c.p, t.batch, t.heads.heads, groups);
+    const int always = truth(a[13]);
+    const int64_t need = lib.shared_bytes(&c.p, t.batch, t.heads.heads, groups, always);
     if (need < 0) check((int)need, "epq_paged_attend_shared_workspace_bytes");
     const cudaStream_t st = stream_of(c.device);
     const Tensor ws = workspace(c.device, st, need);
     check(lib.attend_shared(&c.p, &t.heads, t.seq, t.lengths, t.batch, starts.const_data_ptr<int32_t>(),
-                            prefix.const_data_ptr<int64_t>(), groups, (float)t.scale, t.out.data_ptr(), t.lse_to(), t.dtype,
+                            prefix.const_data_ptr<int64_t>(), groups, always, (float)t.scale, t.out.data_ptr(), t.lse_to(), t.dtype,
                             ws.data_ptr(), ws.numel(), st),
           "epq_paged_attend_shared");
     return t.results();
@@ -617,7 +618,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define EPQ_METHOD(name, n) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&call<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {EPQ_METHOD(bind, 2),    EPQ_METHOD(rope, 9),           EPQ_METHOD(write, 16),
-                         EPQ_METHOD(read, 8),    EPQ_METHOD(attend, 13),        EPQ_METHOD(attend_shared, 13),
+                         EPQ_METHOD(read, 8),    EPQ_METHOD(attend, 13),        EPQ_METHOD(attend_shared, 14),
                          EPQ_METHOD(bounds, 9),  EPQ_METHOD(select, 12),        EPQ_METHOD(verify, 4),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_epq_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

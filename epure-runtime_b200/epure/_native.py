@@ -166,9 +166,9 @@ def load_library(path=None):
         lib.epq_paged_attend_workspace_bytes.restype = I64
         lib.epq_paged_attend_workspace_bytes.argtypes = [PP, I64, I32]
         lib.epq_paged_attend_blocks.argtypes = [PP, HP, P, P, I64, P, I32, F32, P, P, I32, P, I64, P]
-        lib.epq_paged_attend_shared.argtypes = [PP, HP, P, P, I64, P, P, I64, F32, P, P, I32, P, I64, P]
+        lib.epq_paged_attend_shared.argtypes = [PP, HP, P, P, I64, P, P, I64, I32, F32, P, P, I32, P, I64, P]
         lib.epq_paged_attend_shared_workspace_bytes.restype = I64
-        lib.epq_paged_attend_shared_workspace_bytes.argtypes = [PP, I64, I32, I64]
+        lib.epq_paged_attend_shared_workspace_bytes.argtypes = [PP, I64, I32, I64, I32]
         lib.epq_paged_bounds.argtypes = [PP, P, I64, I32, P, P, P, I64, P]
         lib.epq_paged_select.argtypes = [PP, P, I64, I32, HP, I32, P, P, I64, I32, I32, I32, P, P, I64, P]
         lib.epq_paged_select_workspace_bytes.restype = I64

@@ -61,16 +61,18 @@ def attend(pages, q, lengths, seq=None, scale=None, window=0, out=None, return_l
                                                                         return_lse, blocks)
 
 
-def attend_shared(pages, q, lengths, starts, prefix, seq=None, scale=None, out=None, return_lse=False):
+def attend_shared(pages, q, lengths, starts, prefix, seq=None, scale=None, out=None, return_lse=False,
+                  always=False):
     """``attend`` where rows share their first tokens, which are read once for all of them.
 
     Rows ``starts[g] .. starts[g + 1) - 1`` (int32 [groups + 1], ascending) have the same first ``prefix[g]`` (int64
     [groups]) tokens: either their page tables name the same pages there (``PagedKVCache.share``), or they are rows of
     one sequence (drafted tokens, a prompt's chunk) with lengths of their own.  The shared tokens are
     read through the table of one of the rows.  A row shorter than its group's prefix attends over its own length, rows in no
-    group share nothing."""
+    group share nothing.  Groups for which reading row by row is reckoned to be faster (few rows, short prefixes) are
+    read that way, unless ``always``."""
     return (_native.tensor_calls or _native.load_tensor_calls()).attend_shared(*pages, q, lengths, starts, prefix, seq,
-                                                                               scale, out, return_lse)
+                                                                               scale, out, return_lse, always)
 
 
 def summarise(pages, bounds, lengths, seq=None, first=None):

@@ -122,13 +122,15 @@ int epq_paged_attend(const epq_pages* pages, const epq_heads* q, const int32_t* 
  * behind a common prompt or several new tokens of one sequence (rows of one seq with growing
  * lengths).  Rows of no group share nothing; where starts are not ascending or outside the batch,
  * or a prefix is not in 0..max_pages * page_size, that is reported (bit 4) and none does.  Which
- * rows are taken together, and whether any are, follows from sizes and lengths alone.
+ * rows are taken together, and whether any are, follows from sizes and lengths alone: groups for which reading row
+ * by row is reckoned to be faster are read that way, unless `always` is not 0.
  * batch <= 65536; a workspace of its own bytes, with epq_paged_attend's rules.
  * epq_device_error bit 1: a wait of the kernel's own gave up. */
-int64_t epq_paged_attend_shared_workspace_bytes(const epq_pages* pages, int64_t batch, int32_t heads, int64_t groups);
+int64_t epq_paged_attend_shared_workspace_bytes(const epq_pages* pages, int64_t batch, int32_t heads, int64_t groups,
+                                                int32_t always);
 int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const int32_t* seq, const int64_t* lengths,
-                            int64_t batch, const int32_t* starts, const int64_t* prefix, int64_t groups, float scale, void* out,
-                            float* lse, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+                            int64_t batch, const int32_t* starts, const int64_t* prefix, int64_t groups, int32_t always,
+                            float scale, void* out, float* lse, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The bounds of a page's keys: bounds [pages][kv_heads][2][head_dim] hold, of every value of a
  * head, the least and the largest over the page's tokens, in the cache's own 16-bit type or,

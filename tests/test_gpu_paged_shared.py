@@ -90,8 +90,8 @@ def _check(case, q, scale=None, **kw):
     pages, starts, prefix, seq, lengths, seen = case
     sc = 1 / math.sqrt(q.shape[-1]) if scale is None else scale
     n = torch.tensor(lengths, device=DEV)
-    out, lse = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, scale=scale, return_lse=True, **kw)
-    again = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, scale=scale, return_lse=True)
+    out, lse = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, scale=scale, return_lse=True, **kw, always=True)
+    again = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, scale=scale, return_lse=True, always=True)
     assert torch.equal(out, again[0]) and torch.equal(lse, again[1])           # the order of the pieces is fixed
     k = torch.cat([s[0] for s in seen]).double()
     v = torch.cat([s[1] for s in seen]).double()
@@ -163,7 +163,7 @@ def test_agrees_with_attention_without_sharing():
     q = _q(case, 32, 128, torch.bfloat16)
     n = torch.tensor(lengths, device=DEV)
     a, la = paged.attend(pages, q, n, seq=seq, return_lse=True)
-    b, lb = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, return_lse=True)
+    b, lb = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, return_lse=True, always=True)
     # two results within their own rounding of each other, and float32 sums in another order
     assert float((a.double() - b.double()).abs().max()) <= 2.0 ** -7 * float(a.abs().max())
     some = torch.isfinite(la)
@@ -171,7 +171,7 @@ def test_agrees_with_attention_without_sharing():
     # no group, groups of one row, starts that leave rows out
     for s, p in (([0], []), (list(range(len(lengths) + 1)), [100] * len(lengths)), ([3, 3, 9], [9000, 9000])):
         got = paged.attend_shared(pages, q, n, torch.tensor(s, dtype=torch.int32, device=DEV),
-                                  torch.tensor(p, dtype=torch.long, device=DEV), seq=seq)
+                                  torch.tensor(p, dtype=torch.long, device=DEV), seq=seq, always=True)
         assert float((a.double() - got.double()).abs().max()) <= 2.0 ** -7 * float(a.abs().max())
 
 
@@ -213,12 +213,12 @@ def test_not_finite_values_stay_in_their_row():
     pages, starts, prefix, seq, lengths, seen = case
     q = _q(case, 8, 64, torch.bfloat16, gain=0.5).abs()
     n = torch.tensor(lengths, device=DEV)
-    want = paged.attend_shared(pages, q, n, starts, prefix, seq=seq)
+    want = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, always=True)
     t = torch.tensor([9020], device=DEV)
     bad = torch.full((1, 2, 64), float("nan"), dtype=torch.bfloat16, device=DEV)
     paged.write(pages, bad, bad, seq[4:5], t)
     q[9, 3] = float("nan")
-    got = paged.attend_shared(pages, q, n, starts, prefix, seq=seq)
+    got = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, always=True)
     assert torch.isnan(got[4]).all() and torch.isnan(got[9, 3]).all()
     keep = torch.ones(20, 8, dtype=torch.bool, device=DEV)
     keep[4] = False
@@ -228,7 +228,7 @@ def test_not_finite_values_stay_in_their_row():
     k = torch.full((1, 2, 64), float("-inf"), dtype=torch.bfloat16, device=DEV)
     v = torch.ones(1, 2, 64, dtype=torch.bfloat16, device=DEV)
     paged.write(pages, k, v, seq[:1], torch.tensor([123], device=DEV))
-    out, lse = paged.attend_shared(pages, q.abs() + 0.1, n, starts, prefix, seq=seq, return_lse=True)
+    out, lse = paged.attend_shared(pages, q.abs() + 0.1, n, starts, prefix, seq=seq, return_lse=True, always=True)
     assert torch.isfinite(out[keep]).all() and torch.isfinite(lse[keep]).all()
 
 
@@ -241,7 +241,7 @@ def test_a_value_beyond_a_row_stays_unseen():
     bad = torch.full((1, 2, 128), float("inf"), dtype=torch.bfloat16, device=DEV)
     paged.write(pages, bad, bad, seq[:1], torch.tensor([9003], device=DEV))
     n = torch.tensor(lengths, device=DEV)
-    got = paged.attend_shared(pages, q, n, starts, case[2], seq=seq)
+    got = paged.attend_shared(pages, q, n, starts, case[2], seq=seq, always=True)
     assert torch.isfinite(got[:3]).all() and not torch.isfinite(got[3:]).any()
     case = (pages, starts[:1].new_tensor([0, 3]), case[2], seq[:3], lengths[:3], seen[:3])
     _check(case, q[:3])
@@ -255,15 +255,15 @@ def test_layouts():
     n = torch.tensor(lengths, device=DEV)
     wide = torch.randn(24, 20, 128, generator=_gen(6), device=DEV).to(torch.bfloat16)
     q = wide[:, 2:10]
-    want = paged.attend_shared(pages, q.contiguous(), n, starts, prefix, seq=seq)
+    want = paged.attend_shared(pages, q.contiguous(), n, starts, prefix, seq=seq, always=True)
     odd = torch.empty(24 * 8 * 128 + 2, dtype=q.dtype, device=DEV)[2:].view(24, 8, 128).copy_(q)
     odder = torch.empty(24 * 8 * 128 + 1, dtype=q.dtype, device=DEV)[1:].view(24, 8, 128).copy_(q)
     swap = torch.empty(8, 24, 128, dtype=q.dtype, device=DEV).transpose(0, 1).copy_(q)
     for x in (q, odd, odder, swap):
-        assert torch.equal(paged.attend_shared(pages, x, n, starts, prefix), want)
+        assert torch.equal(paged.attend_shared(pages, x, n, starts, prefix, always=True), want)
     out = torch.empty_like(want)
     version = out._version
-    assert paged.attend_shared(pages, q, n, starts, prefix, out=out) is out and torch.equal(out, want) and out._version > version
+    assert paged.attend_shared(pages, q, n, starts, prefix, out=out, always=True) is out and torch.equal(out, want) and out._version > version
 
 
 def test_captured_and_replayed():
@@ -275,18 +275,18 @@ def test_captured_and_replayed():
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        paged.attend_shared(pages, q, n, starts, prefix, seq=seq)
+        paged.attend_shared(pages, q, n, starts, prefix, seq=seq, always=True)
     torch.cuda.current_stream().wait_stream(side)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        out, lse = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, return_lse=True)
+        out, lse = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, return_lse=True, always=True)
     for change in (lambda: None, lambda: n.sub_(100), lambda: prefix.fill_(4321), lambda: n[5:9].zero_(),
                    lambda: starts.copy_(torch.tensor([2, 20], dtype=torch.int32)), lambda: prefix.fill_(0)):
         change()
         torch.cuda.synchronize()
         graph.replay()
         with torch.cuda.stream(side):
-            want = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, return_lse=True)
+            want = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, return_lse=True, always=True)
         torch.cuda.synchronize()
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
 
@@ -302,7 +302,25 @@ def test_little_to_share_is_not_shared():
     pages, starts, prefix, seq, lengths, _ = case
     q, n = _q(case, 8, 128, torch.bfloat16), torch.tensor(lengths, device=DEV)
     few = torch.tensor([0, 1], dtype=torch.int32, device=DEV)              # known on the device alone
-    assert torch.equal(paged.attend_shared(pages, q, n, few, prefix, seq=seq), paged.attend(pages, q, n, seq=seq))
+    assert torch.equal(paged.attend_shared(pages, q, n, few, prefix, seq=seq, always=True), paged.attend(pages, q, n, seq=seq))
+
+
+@pytest.mark.parametrize("rows,tokens,shares", [(24, 9000, False), (100, 9000, True), (3, 9000, False)])
+def test_shares_where_it_is_reckoned_to_be_faster(rows, tokens, shares):
+    """Told apart by tables that, against the rules, name zeros in all rows but the first."""
+    from epure import paged
+    case = _case([(tokens, [5] * rows)], 2, 128, 64, "same", torch.bfloat16, spare=1)
+    pages, starts, prefix, seq, lengths, _ = case
+    zero = torch.ones(pages.k.shape[0], dtype=torch.bool, device=DEV)
+    zero[pages.table[pages.table >= 0].long()] = False
+    zero = int(zero.nonzero()[0])
+    pages.k[zero], pages.v[zero] = 0, 0
+    pages.table[1:, :tokens // 64] = zero
+    q, n = _q(case, 8, 128, torch.bfloat16), torch.tensor(lengths, device=DEV)
+    alone = paged.attend(pages, q, n)
+    together = paged.attend_shared(pages, q, n, starts, prefix, always=True)
+    assert not torch.equal(alone, together)
+    assert torch.equal(paged.attend_shared(pages, q, n, starts, prefix), together if shares else alone)
 
 
 def test_refusals():
@@ -315,14 +333,14 @@ def test_refusals():
                 dict(out=torch.empty(3, 4, 32, device=DEV)), dict(out=torch.empty(4, 3, 64, dtype=q.dtype, device=DEV).transpose(0, 1))):
         kw = {**dict(lengths=n, starts=starts, prefix=prefix, seq=seq), **bad}
         with pytest.raises(RuntimeError, match="must be"):
-            paged.attend_shared(pages, q, **kw)
+            paged.attend_shared(pages, q, **kw, always=True)
     with pytest.raises(TypeError, match="queries"):
-        paged.attend_shared(pages, q.float(), n, starts, prefix)
+        paged.attend_shared(pages, q.float(), n, starts, prefix, always=True)
     with pytest.raises(RuntimeError, match="query heads"):
-        paged.attend_shared(pages, q[:, :3], n, starts, prefix)
+        paged.attend_shared(pages, q[:, :3], n, starts, prefix, always=True)
     with pytest.raises(RuntimeError, match="gradient"):
-        paged.attend_shared(pages, q.clone().requires_grad_(), n, starts, prefix)
-    empty = paged.attend_shared(pages, q[:0], n[:0], starts[:1], prefix[:0], return_lse=True)
+        paged.attend_shared(pages, q.clone().requires_grad_(), n, starts, prefix, always=True)
+    empty = paged.attend_shared(pages, q[:0], n[:0], starts[:1], prefix[:0], return_lse=True, always=True)
     assert empty[0].shape == (0, 4, 64) and empty[1].shape == (0, 4)
 
 
@@ -343,13 +361,13 @@ assert _native.device_error() == 0
 want = paged.attend(pages, q, n)
 if kind == "starts":
     for bad in (t(0, 25).int(), t(-1, 24).int(), t(20, 4).int()):
-        assert torch.equal(paged.attend_shared(pages, q, n, bad, prefix), want)
+        assert torch.equal(paged.attend_shared(pages, q, n, bad, prefix, always=True), want)
 elif kind == "prefix":
     for bad in (-1, 10241):
-        assert torch.equal(paged.attend_shared(pages, q, n, starts, t(bad)), want)
+        assert torch.equal(paged.attend_shared(pages, q, n, starts, t(bad), always=True), want)
 elif kind == "length":                                 # bad rows are empty, the others go on
     n[3], n[7] = -5, 10241
-    out = paged.attend_shared(pages, q, n, starts, prefix)
+    out = paged.attend_shared(pages, q, n, starts, prefix, always=True)
     keep = torch.ones(24, dtype=torch.bool, device=dev)
     keep[3] = keep[7] = False
     assert not out[~keep].any()
@@ -357,14 +375,14 @@ elif kind == "length":                                 # bad rows are empty, the
 elif kind == "page":                                   # the tokens of a bad page are left out
     table[:, 5] = 200
     table[:, 6] = -3
-    out, lse = paged.attend_shared(pages, q, n, starts, prefix, return_lse=True)
+    out, lse = paged.attend_shared(pages, q, n, starts, prefix, return_lse=True, always=True)
     a, la = paged.attend(pages, q, n, return_lse=True)
     assert float((out.double() - a.double()).abs().max()) <= 2 ** -7 * float(a.abs().max())
     assert float((lse - la).abs().max()) <= 1e-4
 elif kind == "seq":
     seq = torch.arange(24, dtype=torch.int32, device=dev)
     seq[0], seq[9] = -1, 24
-    out = paged.attend_shared(pages, q, n, starts, prefix, seq=seq)
+    out = paged.attend_shared(pages, q, n, starts, prefix, seq=seq, always=True)
     assert not out[[0, 9]].any() and out[1:9].any(-1).all()
 torch.cuda.synchronize()
 print("FLAG", _native.device_error())

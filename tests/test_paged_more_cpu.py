@@ -26,7 +26,7 @@ def _blocks(lib, p=None, q=None, batch=1, blocks=P, count=4, dtype=2, ws=1 << 30
 
 
 def _shared(lib, p=None, q=None, batch=1, starts=P, prefix=P, groups=1, dtype=2, ws=1 << 34, work=4096, lengths=P):
-    return lib.epq_paged_attend_shared(ref(p or _pages()), ref(q or _heads(4)), None, lengths, batch, starts, prefix, groups, 1.0, P,
+    return lib.epq_paged_attend_shared(ref(p or _pages()), ref(q or _heads(4)), None, lengths, batch, starts, prefix, groups, 0, 1.0, P,
                                        None, dtype, ctypes.c_void_p(work), ws, None)
 
 
@@ -35,7 +35,7 @@ def test_bad_pages(lib, field, value, code):  # noqa: F811
     p = _pages(**{field: value})
     assert _bounds(lib, p) == code and _select(lib, p) == code and _blocks(lib, p) == code and _shared(lib, p) == code
     assert lib.epq_paged_select_workspace_bytes(ref(p), 1) == code
-    assert lib.epq_paged_attend_shared_workspace_bytes(ref(p), 1, 4, 1) == code
+    assert lib.epq_paged_attend_shared_workspace_bytes(ref(p), 1, 4, 1, 0) == code
 
 
 def test_bad_bounds_and_selections(lib):  # noqa: F811
@@ -60,7 +60,7 @@ def test_bad_lists_and_groups(lib):  # noqa: F811
         assert call(lib, batch=0) == 0 and call(lib, _pages(seqs=40000), batch=40000) == -8
     assert _blocks(lib, count=-1) == -1 and _blocks(lib, blocks=None) == -1
     assert _shared(lib, groups=-1) == -1 and _shared(lib, starts=None) == -1 and _shared(lib, prefix=None) == -1
-    assert lib.epq_paged_attend_shared_workspace_bytes(ref(_pages()), 1, 4, -1) == -1
+    assert lib.epq_paged_attend_shared_workspace_bytes(ref(_pages()), 1, 4, -1, 0) == -1
 
 
 def test_bad_verifications(lib):  # noqa: F811
