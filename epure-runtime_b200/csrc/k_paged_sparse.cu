@@ -13,14 +13,20 @@
 // page and keys.  Up to 8 warps share one head of one page, so that a page is two accesses deep;
 // a warp's lanes hold 16 bytes of a row each, the rows of an access side by side.
 //
-// Selection.  Bound: HBM, 4 head_dim bytes a block and head; next to it the issue rate, about
-// 1.5 instructions a dim, block and query head.  A lane holds 8 dims of two blocks; q lies in
-// shared memory as max(q, 0) and min(q, 0), so that max(q lo, q hi) = max(q, 0) hi + min(q, 0) lo
-// is a product and a fused product of two dims at once (one of the two is zero: nothing is
-// rounded).  The lanes of a block then add up all its heads together: each step halves the heads
-// a lane holds.  The CTAs of a unit (row, key head) leave its scores as integers in the order of
-// the floats; the last of them finds the count-th largest, two bits at a time, and writes the list.
+// Selection.  Bound: HBM, 4 head_dim bytes a block and head.  The defined sums would be bound by the
+// issue rate (185 instructions a block of 8 heads of 128: 64 x 32k took 104 us for 21 us of bytes),
+// so they are formed for few blocks only.  As max(q lo, q hi) = max(q, 0) hi + min(q, 0) lo (lo <= hi)
+// the scores of 16 blocks and 8 heads are a product on the tensor cores (m16n8k16: a group's heads are
+// its 8 columns; tcgen05's tiles of 128 rows would be read from shared memory, where these operands
+// come from HBM straight into the registers that multiply them).  Its float32 sums have another
+// order than the defined ones.  Together they are off by less than E = (1.5 head_dim + 8) 2^-23 |q|_1
+// max|bounds|: head_dim additions, each off by at most 2^-23 of the sum of all |q_d bound_d|, in the
+// one, log2 of that in the other.  The CTAs of a unit (row, key head) leave their scores as integers in the order of the floats;
+// the last of them finds the count-th largest, T, two bits at a time.  A block more than 2 E above T
+// is chosen and one more than 2 E below is not, whatever the order; where those between are more
+// than are still wanted, their defined scores decide.
 #include "epq_paged.cuh"
+#include <cfloat>
 
 namespace epq {
 namespace paged {
@@ -257,35 +263,10 @@ struct SelectArgs {
     const int64_t* lengths;
     int32_t* chosen;
     uint32_t* keys;                            // [units][max_pages]
+    float* largest;                            // [units][parts]: max|bounds|
     unsigned* counters;
     int heads, group, dtype, q_aligned, count, sinks, recent, parts;
 };
-
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ float add_halves(uint64_t a) {
-    float x, y;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a));
-    return x + y;
-}
 
 // Integers in the order of the floats; -0 is 0 and NaN the largest.
 __device__ __forceinline__ uint32_t key_of(float s) {
@@ -293,246 +274,423 @@ __device__ __forceinline__ uint32_t key_of(float s) {
     const uint32_t u = __float_as_uint(s + 0.f);
     return u >> 31 ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float score_of(uint32_t key) { return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key); }
 
-// The unit's list: the first `sinks` and last `recent` of its n > count blocks and the best of
-// the others, ties to the lowest block, in ascending order.
-__device__ void choose(const SelectArgs& A, const uint32_t* keys, int n, int32_t* out) {
-    constexpr int kHeld = 16;                                          // keys of a thread that stay in registers
-    __shared__ int64_t sums[2][kWarps];
-    __shared__ int before[kWarps][3];
+// Where the `need`-th largest of some keys lies (1 <= need <= their number): in [low, high], with `above` of them past high.
+// Counted in 1024 bins of the range, then in 1024 of the bin it is in, until `stop` or fewer keys are left or low = high.
+constexpr int kBins = 1024;
+struct Place {
+    uint32_t low, high;
+    int above;
+};
+template <typename F> __device__ Place find_place(int need, int stop, int j0, int j1, const F& key_at) {
+    __shared__ int bins[kBins], sums[kWarps], found[3];
+    __shared__ uint32_t ends[2][kWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int each = (n + kThreads - 1) / kThreads, j0 = min(n, tid * each), j1 = min(n, j0 + each);
-    const int past = n - A.recent;
-    const int need = A.count - A.sinks - A.recent;                     // n > count: the two do not meet
-    auto free_key = [&](int j) { return j < A.sinks || j >= past ? 0u : __ldcg(keys + j); };
-    uint32_t held[kHeld];
-    const bool in_registers = each <= kHeld;
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) held[i] = in_registers && j0 + i < j1 ? free_key(j0 + i) : 0u;
-    // the largest value that at least `need` keys reach, two bits at a time: of the three next values the largest that
-    // so many reach (their counts in 21 bits each; a unit has below 2^21 blocks)
-    uint32_t at = 0;
-    for (int bit = 30; bit >= 0; bit -= 2) {
-        const uint32_t to1 = at | 1u << bit, to2 = at | 2u << bit, to3 = at | 3u << bit;
-        int have1 = 0, have2 = 0, have3 = 0;
-        auto count = [&](uint32_t key) { have1 += key >= to1, have2 += key >= to2, have3 += key >= to3; };
-        if (in_registers) {
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
-                if (i >= each) break;
-                count(held[i]);
-            }
-        } else {
-            for (int j = j0; j < j1; ++j) count(free_key(j));
-        }
-        const int h1 = __reduce_add_sync(kAll, have1), h2 = __reduce_add_sync(kAll, have2), h3 = __reduce_add_sync(kAll, have3);
-        int64_t* const mine = sums[bit / 2 & 1];
-        if (lane == 0) mine[warp] = h1 | (int64_t)h2 << 21 | (int64_t)h3 << 42;
-        __syncthreads();
-        int64_t total = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) total += mine[w];
-        constexpr int kMask = (1 << 21) - 1;
-        if ((int)(total >> 42) >= need) at = to3;
-        else if ((int)(total >> 21 & kMask) >= need) at = to2;
-        else if ((int)(total & kMask) >= need) at = to1;
+    Place at = {kAll, 0u, 0};
+    for (int j = j0 + tid; j < j1; j += kThreads) {
+        const uint32_t key = key_at(j);
+        at.low = min(at.low, key);
+        at.high = max(at.high, key);
     }
-    // sure ones and ties before this thread's blocks
-    int sure = 0, ties = 0, above = 0;
-    for (int j = j0; j < j1; ++j) {
-        const bool forced = j < A.sinks || j >= past;
-        const uint32_t key = free_key(j);
-        above += !forced && key > at;
-        sure += forced || key > at;
-        ties += !forced && key == at;
-    }
-    int sure_to = sure, ties_to = ties;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(kAll, sure_to, o), c = __shfl_up_sync(kAll, ties_to, o);
-        if (lane >= o) sure_to += a, ties_to += c;
-    }
-    above = __reduce_add_sync(kAll, above);
-    if (lane == 31) before[warp][0] = sure_to, before[warp][1] = ties_to, before[warp][2] = above;
+    at.low = __reduce_min_sync(kAll, at.low);
+    at.high = __reduce_max_sync(kAll, at.high);
+    __syncthreads();                                                   // (an earlier call's are read)
+    if (lane == 0) ends[0][warp] = at.low, ends[1][warp] = at.high;
     __syncthreads();
-    int all_above = 0;
-    sure_to -= sure;
-    ties_to -= ties;
-    for (int w = 0; w < kWarps; ++w) {
-        all_above += before[w][2];
-        if (w < warp) sure_to += before[w][0], ties_to += before[w][1];
-    }
-    const int take = need - all_above;                                 // ties that are chosen
-    for (int j = j0; j < j1; ++j) {
-        const bool forced = j < A.sinks || j >= past;
-        const uint32_t key = free_key(j);
-        if (forced || key > at) {
-            out[sure_to + min(ties_to, take)] = j;
-            ++sure_to;
-        } else if (key == at) {
-            if (ties_to < take) out[sure_to + ties_to] = j;
-            ++ties_to;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) at.low = min(at.low, ends[0][w]), at.high = max(at.high, ends[1][w]);
+    while (true) {
+        const int shift = max(0, 22 - __clz(at.high - at.low));        // (the range's bits less 10)
+        constexpr int kMine = kBins / kThreads;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) bins[tid + i * kThreads] = 0;
+        __syncthreads();
+        for (int j = j0 + tid; j < j1; j += kThreads) {
+            const uint32_t key = key_at(j);
+            if (key >= at.low && key <= at.high) atomicAdd(&bins[(key - at.low) >> shift], 1);
         }
+        __syncthreads();
+        // thread 0 has the last bins
+        int have[kMine], all = 0;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) all += have[i] = bins[kBins - 1 - tid * kMine - i];
+        int upto = all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(kAll, upto, o);
+            if (lane >= o) upto += u;
+        }
+        if (lane == 31) sums[warp] = upto;
+        __syncthreads();
+        int before = at.above + upto - all;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) before += w < warp ? sums[w] : 0;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            if (before < need && before + have[i] >= need) found[0] = kBins - 1 - tid * kMine - i, found[1] = before, found[2] = have[i];
+            before += have[i];
+        }
+        __syncthreads();
+        at.low += (uint32_t)found[0] << shift;
+        at.high = min(at.high, at.low + ((1u << shift) - 1u));
+        at.above = found[1];
+        if (found[2] <= stop || shift == 0) return at;
+        __syncthreads();                                               // (found and sums are read)
     }
 }
 
-// kLanes lanes a block, 8 dims each; kHeads query heads at once.
-template <bool kIsBf16, int kLanes, int kHeads>
+// 8 values of a row of q from dim on.
+__device__ __forceinline__ void load_q(const SelectArgs& A, int b, int h, int dim, float (&f)[8]) {
+    const uint16_t* q = static_cast<const uint16_t*>(A.q) + b * A.q_row + h * A.q_head + dim;
+    if (A.dtype == EPQ_BF16) {
+        Eight<__nv_bfloat16> x;
+        x.load(reinterpret_cast<const __nv_bfloat16*>(q), A.q_aligned);
+        x.get(f);
+    } else {
+        Eight<__half> x;
+        x.load(reinterpret_cast<const __half*>(q), A.q_aligned);
+        x.get(f);
+    }
+}
+
+// The defined score of a block of row b's key head, by a warp: as many lanes a query head as hold its dims, 8 each;
+// neighbours' sums first.
+template <typename T> __device__ float defined_score(const SelectArgs& A, int b, int head, const T* bounds) {
+    const int lane = threadIdx.x & 31, hd = A.pages.head_dim;
+    int lanes = 2;
+    while (lanes * 8 < hd) lanes *= 2;
+    const int dim = lane % lanes * 8;
+    float lo[8], hi[8], score = -INFINITY;
+    const bool on = dim < hd;
+    if (on) {
+        load_v<T, 8>(lo, bounds + dim);
+        load_v<T, 8>(hi, bounds + hd + dim);
+    }
+#pragma unroll 4
+    for (int h0 = 0; h0 < A.group; h0 += 32 / lanes) {
+        const int h = h0 + lane / lanes;
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = 0.f;
+        if (on && h < A.group) {
+            load_q(A, b, head * A.group + h, dim, t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = max_nan(__fmul_rn(t[i], lo[i]), __fmul_rn(t[i], hi[i]));
+        }
+        float v = __fadd_rn(__fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3])),
+                            __fadd_rn(__fadd_rn(t[4], t[5]), __fadd_rn(t[6], t[7])));
+        for (int o = 1; o < lanes; o <<= 1) v = __fadd_rn(v, __shfl_xor_sync(kAll, v, o));
+        if (h < A.group) score = max_nan(score, v);
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) score = max_nan(score, __shfl_xor_sync(kAll, score, o));
+    return score;
+}
+
+// The unit's list: the first `sinks` and last `recent` of its n > count blocks and the best of
+// the others, ties to the lowest block, in ascending order.  The keys' scores are off by at most `err`;
+// NaN: by any amount.
+constexpr int kLocal = 4096;                                           // keys that shared memory holds
+template <typename T>
+__device__ void choose(const SelectArgs& A, uint32_t* keys, int n, int b, int head, const int32_t* table, float err, int32_t* out) {
+    constexpr int kListed = 1024, kFew = 8;
+    __shared__ int before[kWarps][3];
+    __shared__ uint32_t local[kLocal];
+    __shared__ int list[kListed], listed;
+    __shared__ uint32_t defined[kListed];
+    const PagesD& P = A.pages;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int first = A.sinks, past = n - A.recent;
+    const int need = A.count - A.sinks - A.recent;                     // n > count: the two do not meet
+    const bool here = n <= kLocal;
+    if (here)
+        for (int j = tid; j < n; j += kThreads) local[j] = __ldcg(keys + j);
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    auto key_at = [&](int j) { return here ? local[j] : __ldcg(keys + j); };
+    auto set_key = [&](int j, uint32_t key) { (here ? local : keys)[j] = key; };
+    auto defined_key = [&](int j) {                                    // (of a block with a page: its key is not 0)
+        const T* bounds = reinterpret_cast<const T*>(A.bounds) + table[j] * A.stride + (int64_t)head * 2 * P.head_dim;
+        return key_of(defined_score<T>(A, b, head, bounds));
+    };
+    // chosen: keys above `over`, and of those that equal it as many as are still wanted
+    uint32_t over = kAll;
+    if (need > 0) {
+        Place at = find_place(need, kFew, first, past, key_at);
+        bool few = false;
+        for (int attempt = 0; attempt < 2; ++attempt) {
+            // those that are in the place, or that the error may bring there
+            const float from = score_of(at.low) - 2.f * err, to = score_of(at.high) + 2.f * err;
+            const bool sure = from > -FLT_MAX && to < FLT_MAX;         // (false with NaN)
+            const uint32_t low = key_of(from), high = key_of(to);
+            if (!sure && err != 0.f) break;
+            if (attempt == 0 && err == 0.f) {                          // scores of no error: nothing to look up
+                at = find_place(need, 0, first, past, key_at);
+                break;
+            }
+            int above = 0;
+            for (int j = first + tid; j < past; j += kThreads) {
+                const uint32_t key = key_at(j);
+                above += key > high;
+                if (key >= low && key <= high) {
+                    const int i = atomicAdd(&listed, 1);               // (in any order: they are ranked below)
+                    if (i < kListed) list[i] = j;
+                }
+            }
+            above = __reduce_add_sync(kAll, above);
+            if (lane == 0) before[warp][0] = above;
+            __syncthreads();
+            int all_above = 0;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) all_above += before[w][0];
+            const int count = listed, wanted = need - all_above;       // (1 <= wanted <= count)
+            few = count <= kListed;
+            if (few) {
+                over = high;
+                for (int i = warp; i < count && count > wanted; i += kWarps) {
+                    const uint32_t key = defined_key(list[i]);
+                    if (lane == 0) defined[i] = key;
+                }
+                __syncthreads();
+                for (int i = tid; i < count; i += kThreads) {
+                    int better = 0;
+                    for (int e = 0; e < count && count > wanted; ++e)
+                        better += defined[e] > defined[i] || (defined[e] == defined[i] && list[e] < list[i]);
+                    set_key(list[i], better < wanted ? kAll : 0u);
+                }
+                __syncthreads();
+                break;
+            }
+            __syncthreads();
+            if (tid == 0) listed = 0;
+            at = find_place(need, 0, first, past, key_at);
+        }
+        if (!few) {
+            if (err != 0.f) {                                          // every score anew
+                __syncthreads();
+                for (int j = first + warp; j < past; j += kWarps) {
+                    if (key_at(j) == 0u) continue;                     // (no page)
+                    const uint32_t key = defined_key(j);
+                    __syncwarp();
+                    if (lane == 0) set_key(j, key);
+                }
+                __syncthreads();
+                at = find_place(need, 0, first, past, key_at);
+            }
+            over = at.low;
+        }
+    }
+    // a warp an eighth of the blocks: how many are above, how many equal
+    const int each = (n + kThreads - 1) / kThreads * 32, w0 = min(n, warp * each), w1 = min(n, w0 + each);
+    int sure = 0, ties = 0, forced = 0;
+    auto look = [&](int j0, unsigned* above, unsigned* equal) {
+        const int j = j0 + lane;
+        const bool edge = j < w1 && (j < first || j >= past), in = j < w1 && !edge && need > 0;
+        const uint32_t key = in ? key_at(j) : 0u;
+        *above = __ballot_sync(kAll, edge || (in && key > over));
+        *equal = __ballot_sync(kAll, in && key == over);
+        return __popc(__ballot_sync(kAll, edge));
+    };
+    for (int j0 = w0; j0 < w1; j0 += 32) {
+        unsigned above, equal;
+        forced += look(j0, &above, &equal);
+        sure += __popc(above);
+        ties += __popc(equal);
+    }
+    __syncthreads();
+    if (lane == 0) before[warp][0] = sure, before[warp][1] = ties, before[warp][2] = forced;
+    __syncthreads();
+    int all_sure = 0, all_forced = 0, sure_to = 0, ties_to = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        all_sure += before[w][0];
+        all_forced += before[w][2];
+        if (w < warp) sure_to += before[w][0], ties_to += before[w][1];
+    }
+    const int take = need - (all_sure - all_forced);                   // ties that are chosen
+    for (int j0 = w0; j0 < w1; j0 += 32) {
+        unsigned above, equal;
+        look(j0, &above, &equal);
+        const unsigned below = (1u << lane) - 1u;
+        const int s = sure_to + __popc(above & below), t = ties_to + __popc(equal & below);
+        if (above >> lane & 1) out[s + min(t, take)] = j0 + lane;
+        else if ((equal >> lane & 1) && t < take) out[s + t] = j0 + lane;
+        sure_to += __popc(above);
+        ties_to += __popc(equal);
+    }
+}
+
+template <bool kIsBf16>
+__device__ __forceinline__ void multiply(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (kIsBf16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Heads of up to 32 kSteps.  Lane 4 g + c holds 8 dims from 32 i + 8 c on of rows g and g + 8 (blocks) and of column g (a
+// head): any order of the dims is one, if it is the same in both.
+constexpr int kRows = 16, kColumns = 8;
+
+template <bool kIsBf16, int kSteps>
 __global__ void __launch_bounds__(kThreads, 2) select_kernel(const SelectArgs A) {
     using T = typename std::conditional<kIsBf16, __nv_bfloat16, __half>::type;   // of the bounds
-    // of a head and a lane's dims (i, i + 4): max(q, 0) of i = 0, 1 and 2, 3, min(q, 0) of the same
-    __shared__ float4 split[kHeads][4][kLanes];
+    using T2 = typename std::conditional<kIsBf16, __nv_bfloat162, __half2>::type;
+    constexpr int kAtOnce = kSteps < 4 ? kSteps : 4;                   // steps whose loads are under way together
+    // max(q, 0) and min(q, 0) as T, and what that leaves of an f16 q over bf16 bounds (as bf16, exact)
+    __shared__ uint4 columns[2][2][kSteps][32];
+    __shared__ float norms[kColumns], peaks[kColumns], largest[kWarps];
     __shared__ bool last;
     pdl_enter();
     const PagesD& P = A.pages;
     const int unit = blockIdx.x / A.parts, part = blockIdx.x - unit * A.parts;
     const int b = unit / P.kv_heads, head = unit - b * P.kv_heads;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int hd = P.head_dim;
     int s;
-    const int length = row_length(P, A.seq, A.lengths, b, &s, threadIdx.x == 0 && part == 0 && head == 0);
+    const int length = row_length(P, A.seq, A.lengths, b, &s, tid == 0 && part == 0 && head == 0);
     const int n = length ? P.page_of(length - 1) + 1 : 0;
     int32_t* out = A.chosen + (int64_t)unit * A.count;
     if (n <= A.count) {
         if (part == 0)
-            for (int j = threadIdx.x; j < A.count; j += kThreads) out[j] = j < n ? j : -1;
+            for (int j = tid; j < A.count; j += kThreads) out[j] = j < n ? j : -1;
         return;
     }
     uint32_t* keys = A.keys + (int64_t)unit * P.max_pages;
-    constexpr int kGroups = 32 / kLanes, kEach = 2, kStep = kGroups * kEach;   // blocks of a warp's step
-    const int sub = lane / kLanes, mine = lane % kLanes, dim = mine * 8;
-    const bool on = dim < hd;
-    const int per = (n + A.parts - 1) / A.parts, end = min(n, (part + 1) * per);
+    const int per = (n + A.parts - 1) / A.parts, begin = min(n, part * per), end = min(n, begin + per);
     const int32_t* table = P.table + (int64_t)s * P.table_stride;
-    for (int h0 = 0; h0 < A.group; h0 += kHeads) {
-        if (h0) __syncthreads();
-        for (int e = threadIdx.x; e < kHeads * kLanes; e += kThreads) {
-            const int h = e / kLanes, l = e % kLanes;
+    const bool two = kIsBf16 && A.dtype == EPQ_F16;
+    float norm = 0.f;                                                  // the largest head's |q|_1
+    T2 most;                                                           // of |bounds|
+    most.x = most.y = T(0.f);
+    for (int h0 = 0; h0 < A.group; h0 += kColumns) {
+        __syncthreads();                                               // (the last heads' columns are read)
+        {                                                              // a warp a head: |q|_1, max|q|
+            float sum = 0.f, top = 0.f;
+            if (h0 + warp < A.group)
+                for (int d = lane * 8; d < hd; d += 256) {
+                    float f[8];
+                    load_q(A, b, head * A.group + h0 + warp, d, f);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum += fabsf(f[i]), top = max_nan(top, fabsf(f[i]));
+                }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                sum += __shfl_xor_sync(kAll, sum, o);
+                top = max_nan(top, __shfl_xor_sync(kAll, top, o));
+            }
+            if (lane == 0) norms[warp] = sum, peaks[warp] = top;
+        }
+        __syncthreads();
+        // a bf16 q over f16 bounds is brought to f16 by a power of two
+        auto lift_of = [&](int h) {
+            const float top = peaks[h];
+            return !kIsBf16 && A.dtype == EPQ_BF16 && top >= 1e-33f && top < INFINITY ? ldexpf(1.f, -ilogbf(top)) : 1.f;
+        };
+#pragma unroll
+        for (int h = 0; h < kColumns; ++h) norm = max_nan(norm, norms[h]);
+        for (int e = tid; e < kSteps * 32; e += kThreads) {
+            const int i = e / 32, h = e % 32 >> 2, dim = 32 * i + 8 * (e & 3);
             float f[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = 0.f;
-            if (8 * l < hd && h0 + h < A.group) {
-                const uint16_t* q = static_cast<const uint16_t*>(A.q) + b * A.q_row + (head * A.group + h0 + h) * A.q_head + 8 * l;
-                if (A.dtype == EPQ_BF16) {
-                    Eight<__nv_bfloat16> x;
-                    x.load(reinterpret_cast<const __nv_bfloat16*>(q), A.q_aligned);
-                    x.get(f);
-                } else {
-                    Eight<__half> x;
-                    x.load(reinterpret_cast<const __half*>(q), A.q_aligned);
-                    x.get(f);
-                }
-            }
+            for (int x = 0; x < 8; ++x) f[x] = 0.f;
+            if (dim < hd && h0 + h < A.group) load_q(A, b, head * A.group + h0 + h, dim, f);
+            const float lift = lift_of(h);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                split[h][i][l] = make_float4(max_nan(f[2 * i], 0.f), max_nan(f[2 * i + 4], 0.f), max_nan(f[2 * i + 1], 0.f),
-                                             max_nan(f[2 * i + 5], 0.f));
-                split[h][2 + i][l] = make_float4(min_nan(f[2 * i], 0.f), min_nan(f[2 * i + 4], 0.f), min_nan(f[2 * i + 1], 0.f),
-                                                 min_nan(f[2 * i + 5], 0.f));
+            for (int half = 0; half < 2; ++half) {
+                uint32_t w[2][4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    float v[2], rest[2];
+                    T2 near, left;
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) v[y] = half ? min_nan(f[2 * x + y] * lift, 0.f) : max_nan(f[2 * x + y] * lift, 0.f);
+                    near.x = T(v[0]), near.y = T(v[1]);
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) rest[y] = v[y] - (float)(y ? near.y : near.x);
+                    left.x = T(rest[0]), left.y = T(rest[1]);
+                    w[0][x] = *reinterpret_cast<uint32_t*>(&near);
+                    w[1][x] = *reinterpret_cast<uint32_t*>(&left);
+                }
+                columns[0][half][i][e % 32] = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+                columns[1][half][i][e % 32] = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
             }
         }
         __syncthreads();
-        // the head that this lane is left with, and whether there is one
-        int left = 0;
+        const bool is0 = h0 + 2 * c < A.group, is1 = h0 + 2 * c + 1 < A.group;
+        const float back0 = 1.f / lift_of(2 * c), back1 = 1.f / lift_of(2 * c + 1);
+        const int stride = kWarps * kRows;
+        auto page_at = [&](int j) { return j < end ? table[j] : -1; };
+        int next0 = page_at(begin + warp * kRows + g), next1 = page_at(begin + warp * kRows + g + 8);
+        for (int j = begin + warp * kRows; j < end; j += stride) {
+            const int page0 = next0, page1 = next1;
+            const bool good0 = page0 >= 0 && page0 < P.pages, good1 = page1 >= 0 && page1 < P.pages;
+            next0 = page_at(j + stride + g);
+            next1 = page_at(j + stride + g + 8);
+            const uint16_t* from0 = A.bounds + (good0 ? page0 : 0) * A.stride + (int64_t)head * 2 * hd + 8 * c;
+            const uint16_t* from1 = A.bounds + (good1 ? page1 : 0) * A.stride + (int64_t)head * 2 * hd + 8 * c;
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int o = 1, half = kHeads / 2; half > 0; o <<= 1, half >>= 1) left += lane & o ? half : 0;
-        const bool is_head = h0 + left < A.group;
-
-        const uint4 none = make_uint4(0, 0, 0, 0);
-        const int stride = kWarps * kStep;
-        int j = part * per + warp * kStep + sub;                       // this lane's first block of the step; the others kGroups apart
-        auto page_at = [&](int i) { return i < end ? table[i] : 0; };
-        auto fetch = [&](int i, int page, uint4& l, uint4& h) {        // a block's bounds, zeros where there are none
-            l = h = none;
-            if (i < end && page >= 0 && page < P.pages && on) {
-                const uint16_t* from = A.bounds + page * A.stride + (int64_t)head * 2 * hd + dim;
-                l = __ldg(reinterpret_cast<const uint4*>(from));
-                h = __ldg(reinterpret_cast<const uint4*>(from + hd));
-            }
-        };
-        // bounds one step ahead, page numbers two
-        int page[kEach], next_page[kEach];
-        uint4 lo[kEach], hi[kEach];
+            for (int i0 = 0; i0 < kSteps; i0 += kAtOnce) {
+                uint4 x[2][kAtOnce], y[2][kAtOnce];                    // rows g and g + 8; hi, lo
 #pragma unroll
-        for (int x = 0; x < kEach; ++x) {
-            page[x] = page_at(j + x * kGroups);
-            next_page[x] = page_at(j + stride + x * kGroups);
-        }
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int x = 0; x < kEach; ++x) fetch(j + x * kGroups, page[x], lo[x], hi[x]);
-        for (; __any_sync(kAll, j < end); j += stride) {
-            uint64_t l[kEach][4], h[kEach][4];
-            int now[kEach];
-#pragma unroll
-            for (int x = 0; x < kEach; ++x) {
-                const uint32_t lw[4] = {lo[x].x, lo[x].y, lo[x].z, lo[x].w}, hw[4] = {hi[x].x, hi[x].y, hi[x].z, hi[x].w};
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float2 a = unpack2<T>(lw[i]), c = unpack2<T>(lw[i + 2]);
-                    l[x][2 * i] = pair(a.x, c.x);
-                    l[x][2 * i + 1] = pair(a.y, c.y);
-                    const float2 d = unpack2<T>(hw[i]), e = unpack2<T>(hw[i + 2]);
-                    h[x][2 * i] = pair(d.x, e.x);
-                    h[x][2 * i + 1] = pair(d.y, e.y);
-                }
-                now[x] = page[x];
-                page[x] = next_page[x];
-                next_page[x] = page_at(j + 2 * stride + x * kGroups);
-                fetch(j + stride + x * kGroups, page[x], lo[x], hi[x]);
-            }
-            float v[kEach][kHeads];
-#pragma unroll
-            for (int e = 0; e < kHeads; ++e) {
-                uint64_t up[4], down[4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float4 a = split[e][i][mine], c = split[e][2 + i][mine];
-                    up[2 * i] = pair(a.x, a.y);
-                    up[2 * i + 1] = pair(a.z, a.w);
-                    down[2 * i] = pair(c.x, c.y);
-                    down[2 * i + 1] = pair(c.z, c.w);
-                }
-#pragma unroll
-                for (int x = 0; x < kEach; ++x) {
-                    uint64_t t[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) t[i] = fma_pair(up[i], h[x][i], mul_pair(down[i], l[x][i]));
-                    v[x][e] = add_halves(add_pair(add_pair(t[0], t[1]), add_pair(t[2], t[3])));
-                }
-            }
-#pragma unroll
-            for (int x = 0; x < kEach; ++x) {
-                // each step joins two lanes' sums; while a lane holds several heads it passes on half of them
-                int held = kHeads;
-#pragma unroll
-                for (int o = 1; o < kLanes; o <<= 1) {
-                    if (held > 1) {
-                        held /= 2;
-#pragma unroll
-                        for (int e = 0; e < kHeads / 2; ++e)
-                            if (e < held) {
-                                const float give = lane & o ? v[x][e] : v[x][e + held], keep = lane & o ? v[x][e + held] : v[x][e];
-                                v[x][e] = keep + __shfl_xor_sync(kAll, give, o);
-                            }
-                    } else {
-                        v[x][0] += __shfl_xor_sync(kAll, v[x][0], o);
+                    for (int i = 0; i < kAtOnce; ++i) {
+                        const int dim = 32 * (i0 + i), at = (half ? 0 : hd) + dim;
+                        x[half][i] = y[half][i] = make_uint4(0, 0, 0, 0);
+                        if (good0 && dim + 8 * c < hd) x[half][i] = __ldg(reinterpret_cast<const uint4*>(from0 + at));
+                        if (good1 && dim + 8 * c < hd) y[half][i] = __ldg(reinterpret_cast<const uint4*>(from1 + at));
                     }
-                }
-                float score = is_head ? v[x][0] : -INFINITY;
 #pragma unroll
-                for (int o = 1; o < kHeads; o <<= 1) score = max_nan(score, __shfl_xor_sync(kAll, score, o));
-                const int i = j + x * kGroups;
-                if (mine == 0 && i < end) {
-                    const bool good = now[x] >= 0 && now[x] < P.pages;
-                    if (!good) atomicOr(&g_sparse_error, kBadPage);
-                    const uint32_t key = good ? key_of(score) : 0u;
-                    keys[i] = h0 ? max(keys[i], key) : key;
-                }
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i) {
+                        const uint4 u = x[half][i], v = y[half][i], w = columns[0][half][i0 + i][lane];
+                        multiply<kIsBf16>(d, u.x, v.x, u.y, v.y, w.x, w.y);
+                        multiply<kIsBf16>(d, u.z, v.z, u.w, v.w, w.z, w.w);
+                        if (two) {
+                            const uint4 z = columns[1][half][i0 + i][lane];
+                            multiply<kIsBf16>(d, u.x, v.x, u.y, v.y, z.x, z.y);
+                            multiply<kIsBf16>(d, u.z, v.z, u.w, v.w, z.z, z.w);
+                        }
+                        if (h0 == 0) {
+                            const uint32_t words[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) most = __hmax2_nan(most, __habs2(*reinterpret_cast<const T2*>(&words[e])));
+                        }
+                    }
+            }
+            float score0 = max_nan(is0 ? d[0] * back0 : -INFINITY, is1 ? d[1] * back1 : -INFINITY);
+            float score1 = max_nan(is0 ? d[2] * back0 : -INFINITY, is1 ? d[3] * back1 : -INFINITY);
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                score0 = max_nan(score0, __shfl_xor_sync(kAll, score0, o));
+                score1 = max_nan(score1, __shfl_xor_sync(kAll, score1, o));
+            }
+            const int mine = j + g + 8 * c;                            // lanes c = 0 and 1 write
+            if (c < 2 && mine < end) {
+                const bool good = c ? good1 : good0;
+                if (!good) atomicOr(&g_sparse_error, kBadPage);
+                const uint32_t key = good ? key_of(c ? score1 : score0) : 0u;
+                keys[mine] = h0 ? max(keys[mine], key) : key;
             }
         }
     }
+    {
+        float top = max_nan((float)most.x, (float)most.y);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kAll, top, o));
+        if (lane == 0) largest[warp] = top;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
+        float top = 0.f;
+        for (int w = 0; w < kWarps; ++w) top = max_nan(top, largest[w]);
+        A.largest[blockIdx.x] = top;
         // releases the CTA's keys (complete at the barrier above), acquires the others'
         unsigned done;
         asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(done) : "l"(A.counters + unit) : "memory");
@@ -540,22 +698,29 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const SelectArgs A)
         if (last) A.counters[unit] = 0u;
     }
     __syncthreads();
-    if (last) choose(A, keys, n, out);
+    if (!last) return;
+    float top = 0.f;
+    for (int p = lane; p < A.parts; p += 32) top = max_nan(top, __ldcg(A.largest + unit * A.parts + p));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kAll, top, o));
+    // Exact where all is zero; values that the tensor cores may take for zeros are nothing beside 1e-30.  Each product is
+    // cut off once and each of the head_dim / 8 sums twice; an f16 q over bf16 bounds has two parts, a lifted bf16 q is off by 2^-25 of
+    // its largest value.
+    float err = NAN;
+    if (top < INFINITY && norm < INFINITY) {
+        const float steps = (two || !kIsBf16 ? 3.f : 1.5f) * (float)hd + 8.f;
+        if (top == 0.f || norm == 0.f) err = 0.f;
+        else if (top >= 1e-30f && norm >= 1e-30f && norm * top < 1e37f) err = steps * 0x1p-23f * 1.05f * (norm * top) + 1e-35f;
+    }
+    choose<T>(A, keys, n, b, head, table, err, out);
 }
 
-template <bool kIsBf16, int kLanes>
-int launch_select_h(const SelectArgs& A, unsigned grid, cudaStream_t st) {
-    auto go = [&](auto kern) { return launch(kern, dim3(grid), dim3(kThreads), 0, st, "epq_paged_select", A); };
-    if (A.group == 1) return go(select_kernel<kIsBf16, kLanes, 1>);
-    if (A.group == 2) return go(select_kernel<kIsBf16, kLanes, 2>);
-    if (A.group <= 4) return go(select_kernel<kIsBf16, kLanes, 4>);
-    return go(select_kernel<kIsBf16, kLanes, 8>);
-}
 template <bool kIsBf16> int launch_select(const SelectArgs& A, unsigned grid, cudaStream_t st) {
+    auto go = [&](auto kern) { return launch(kern, dim3(grid), dim3(kThreads), 0, st, "epq_paged_select", A); };
     const int hd = A.pages.head_dim;
-    if (hd <= 64) return launch_select_h<kIsBf16, 8>(A, grid, st);
-    if (hd <= 128) return launch_select_h<kIsBf16, 16>(A, grid, st);
-    return launch_select_h<kIsBf16, 32>(A, grid, st);
+    if (hd <= 64) return go(select_kernel<kIsBf16, 2>);
+    if (hd <= 128) return go(select_kernel<kIsBf16, 4>);
+    return go(select_kernel<kIsBf16, 8>);
 }
 
 // Bounds are held in the cache's own 16-bit type, or in bf16 for 8-bit caches.
@@ -632,7 +797,8 @@ int64_t epq_paged_select_workspace_bytes(const epq_pages* pages, int64_t batch) 
     if (batch < 0 || batch * P.kv_heads > kMaxUnits)
         return set_error(EPQ_EUNSUPPORTED, "epq_paged_select: batch=%lld of %d key heads (at most %d units)", (long long)batch,
                          P.kv_heads, kMaxUnits);
-    return (int64_t)kMaxUnits * 4 + batch * P.kv_heads * P.max_pages * 4;
+    // counters, keys, the parts' largest bounds
+    return (int64_t)kMaxUnits * 4 + batch * P.kv_heads * ((int64_t)P.max_pages + cdiv(P.max_pages, kRows * kWarps)) * 4;
 }
 
 int epq_paged_select(const epq_pages* pages, const void* bounds, int64_t bounds_stride, int32_t bounds_dtype,
@@ -676,9 +842,10 @@ int epq_paged_select(const epq_pages* pages, const void* bounds, int64_t bounds_
     A.count = count;
     A.sinks = sinks;
     A.recent = recent;
-    // CTAs a unit: enough to fill the card twice (lengths differ), each with at least two steps of its warps
-    const int64_t units = batch * P.kv_heads, fill = cdiv(4LL * device_sms(), units), most = cdiv(P.max_pages, 64);
+    // CTAs a unit: enough to fill the card twice (lengths differ), each with a step of its warps
+    const int64_t units = batch * P.kv_heads, fill = cdiv(4LL * device_sms(), units), most = cdiv(P.max_pages, kRows * kWarps);
     A.parts = (int)(fill < most ? fill : most);
+    A.largest = reinterpret_cast<float*>(A.keys + units * P.max_pages);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const unsigned grid = (unsigned)(units * A.parts);
     return bounds_dtype == EPQ_BF16 ? launch_select<true>(A, grid, st) : launch_select<false>(A, grid, st);

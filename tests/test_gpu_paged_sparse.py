@@ -187,6 +187,41 @@ def test_select_ties_and_not_finite_scores():
     assert got[0, 0].tolist() == list(range(9)) + [199] and got[1, 1].tolist() == list(range(9)) + [129]
 
 
+@pytest.mark.parametrize("fmt,cache,dtype", [("same", torch.bfloat16, torch.bfloat16), ("same", torch.float16, torch.float16),
+                                             ("int8", torch.bfloat16, torch.float16), ("same", torch.float16, torch.bfloat16)])
+@pytest.mark.parametrize("heads,kv,hd,blocks", [(8, 1, 128, 300), (24, 2, 64, 900), (6, 2, 256, 130), (4, 4, 80, 3000)])
+def test_select_scores_apart_by_their_rounding(fmt, cache, dtype, heads, kv, hd, blocks):
+    """Blocks that differ in the last bits of their sums, of up to 1024 and of more: the defined order of summing decides."""
+    from epure import paged
+    pages, bounds, q, lengths = _selection_case(heads, kv, hd, [blocks, 40], fmt, cache, ps=1)
+    q = q.to(dtype)
+    bounds[:, :, :, 1:] = bounds[:1, :, :, 1:]                                 # all alike...
+    bounds[:, :, :, 0] = 100.0
+    small = torch.rand(bounds.shape[0], kv, 2, hd // 4, generator=_gen(8), device=DEV) * 2e-3
+    bounds[..., hd // 2:hd // 2 + hd // 4] = (small.sort(2).values + 1e-3).to(bounds.dtype)    # ... but for these
+    for count in (2, 33, 120):
+        got = paged.select(pages, bounds, q, lengths, count)
+        assert torch.equal(got, _expected(q, bounds, pages.table, [blocks, 40], count, 1, 1, kv)), count
+
+
+@pytest.mark.parametrize("fmt,cache,dtype", [("same", torch.bfloat16, torch.bfloat16), ("int8", torch.bfloat16, torch.float16),
+                                             ("same", torch.float16, torch.bfloat16)])
+def test_select_queries_of_any_size(fmt, cache, dtype):
+    """Queries near both ends of their type's range, and of both in one row."""
+    from epure import paged
+    pages, bounds, q, lengths = _selection_case(8, 2, 64, [90] * 6, fmt, cache)
+    q = q.to(dtype)
+    large, small = (3e4, 1e-7) if dtype == torch.float16 else (1e37, 1e-39)
+    q[0] *= large / 8
+    q[1] *= small
+    q[2, :, ::3] *= large / 8
+    q[3, ::2] *= small
+    q[4, 1] = 0
+    q[5, :, 5:] *= 0
+    got = paged.select(pages, bounds, q, lengths, 12)
+    assert torch.equal(got, _expected(q, bounds, pages.table, [90] * 6, 12, 1, 1, 2))
+
+
 def test_select_other_layouts():
     """Rows of a projection, rows that are not aligned, a subset of the sequences, several rows of one."""
     from epure import paged
