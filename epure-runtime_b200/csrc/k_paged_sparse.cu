@@ -562,6 +562,9 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const SelectArgs A)
     uint32_t* keys = A.keys + (int64_t)unit * P.max_pages;
     const int per = (n + A.parts - 1) / A.parts, begin = min(n, part * per), end = min(n, begin + per);
     const int32_t* table = P.table + (int64_t)s * P.table_stride;
+    // the first blocks' pages: on their way while q is read
+    auto page_at = [&](int j) { return j < end ? table[j] : -1; };
+    const int first0 = page_at(begin + warp * kRows + g), first1 = page_at(begin + warp * kRows + g + 8);
     const bool two = kIsBf16 && A.dtype == EPQ_F16;
     float norm = 0.f;                                                  // the largest head's |q|_1
     T2 most;                                                           // of |bounds|
@@ -623,8 +626,7 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const SelectArgs A)
         const bool is0 = h0 + 2 * c < A.group, is1 = h0 + 2 * c + 1 < A.group;
         const float back0 = 1.f / lift_of(2 * c), back1 = 1.f / lift_of(2 * c + 1);
         const int stride = kWarps * kRows;
-        auto page_at = [&](int j) { return j < end ? table[j] : -1; };
-        int next0 = page_at(begin + warp * kRows + g), next1 = page_at(begin + warp * kRows + g + 8);
+        int next0 = first0, next1 = first1;
         for (int j = begin + warp * kRows; j < end; j += stride) {
             const int page0 = next0, page1 = next1;
             const bool good0 = page0 >= 0 && page0 < P.pages, good1 = page1 >= 0 && page1 < P.pages;

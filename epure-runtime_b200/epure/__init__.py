@@ -7,8 +7,9 @@ Drop-in for the public API of epure-runtime v0.2.4 (epure/__init__.py:11-37):
 On a GPU every packed linear runs libepq.so, hand-written sm_100a kernels
 behind a C ABI (include/epq.h); indices are decoded inside the matmul and the
 dense weight is never written.  ``epure.model`` and ``epure.serving`` are decoders
-over them (one sequence; a batch over a paged cache), ``epure.paged`` and
-``epure.rotary`` the cache, attention and rotary operators by themselves.
+over them (one sequence; a batch over a paged cache), ``epure.paged``,
+``epure.rotary`` and ``epure.sampling`` the cache, attention, rotary and draft
+verification operators by themselves.
 """
 from .container import describe, extras, read_header
 from .finetune import (

@@ -17,6 +17,6 @@ def verify(target, draft, tokens, uniforms):
 
     Draft i is accepted while ``u_i q_i(x_i) < p_i(x_i)``.  Behind the accepted ones one token is drawn with the row's last
     number: at a refused draft from ``max(p - q, 0)`` (without a draft's probabilities: p without the token), else from p.
-    The result holds a row's accepted drafts, the drawn token, and -1 behind it.  Sums are 64-bit, so the drawn token is the
-    definition's; without drafts (``tokens`` [batch, 0]) this samples from the target."""
+    The result holds a row's accepted drafts, the drawn token, and -1 behind it.  Products are 64-bit and sums keep 45 bits or more, so
+    the drawn token is the definition's (but where the number lies that near a token's edge); without drafts (``tokens`` [batch, 0]) this samples from the target."""
     return (_native.tensor_calls or _native.load_tensor_calls()).verify(target, draft, tokens, uniforms)

@@ -299,7 +299,7 @@ class BatchDecoder:
         finally:
             for i in range(B):
                 self.cache.release(i)
-        out = torch.tensor([x[d - n_new:d] for x, d in zip(text, done)], device=dev)
+        out = torch.tensor([x[d - n_new:d] for x, d in zip(text, done)], dtype=torch.long, device=dev).view(B, n_new)
         return out, passes
 
 

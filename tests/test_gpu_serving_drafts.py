@@ -137,6 +137,18 @@ def test_speculate(kw):
     assert b.cache.free_pages() == free
 
 
+def test_speculate_no_or_one_token():
+    """Nothing to generate, and the token that the prompts themselves give."""
+    from epure.serving import BatchDecoder
+    b = BatchDecoder(_decoder(), seqs=2, page_size=16)
+    prompts = _prompts([5, 9])
+    got, passes = b.speculate(prompts, 0)
+    assert got.shape == (2, 0) and got.dtype == torch.long and passes == 0
+    got, passes = b.speculate(prompts, 1)
+    assert got.shape == (2, 1) and passes == 0
+    assert torch.equal(got, b.generate(prompts, 1))
+
+
 @pytest.mark.parametrize("fmt", ["same", "int8", "fp8"])
 def test_sparse_steps(fmt):
     """A selection that covers every block gives the dense steps' logits; a small one runs, in a graph as well, and its bounds
