@@ -832,11 +832,13 @@ __global__ void __launch_bounds__(Cfg<kCodes, kDim>::kThreads, 1)
 // 45 us in all, with a warp each 86; 64 rows of 32 heads behind 4k 58 and 42, so they get a warp.
 constexpr int kJoinWarps = 8;
 
-template <bool kBf, int kTeam> __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const AttendArgs A) {
+template <bool kBf, int kTeam, bool kWide>
+__global__ void __launch_bounds__(kJoinWarps * 32, kWide ? 2 : 3) join_kernel(const AttendArgs A) {
+    constexpr int kVals = kWide ? 8 : 4;                               // a lane's: dims 4 lane on, and with kWide 128 + 4 lane on
     pdl_enter();
     const SharedD& S = A.shared;
     const int lane = threadIdx.x & 31, hd = A.pages.head_dim, pitch = S.pitch;
-    __shared__ float parts[kTeam > 1 ? kTeam : 1][kTeam > 1 ? 10 : 1][32];
+    __shared__ float parts[kTeam > 1 ? kTeam : 1][kTeam > 1 ? 2 + kVals : 1][32];
     const int member = threadIdx.x / 32 % kTeam;
     const int64_t place = (int64_t)blockIdx.x * (kJoinWarps / kTeam) + threadIdx.x / 32 / kTeam;
     if (place >= S.own_records) return;
@@ -857,8 +859,10 @@ template <bool kBf, int kTeam> __global__ void __launch_bounds__(kJoinWarps * 32
         return c == c0 ? S.own + ((two == 2 ? slot * S.own_records : 0) + place) * pitch
                        : S.cut + ((c * 2 + slot) * kSharedLanes + at) * pitch;
     };
-    const bool two_rows = lane * 4 + 128 < hd;                         // (head_dim above 128: a lane's second four values)
-    float top = -FLT_MAX, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const bool second = kWide && lane * 4 + 128 < hd;
+    float top = -FLT_MAX, sum = 0.f, v[kVals];
+#pragma unroll
+    for (int i = 0; i < kVals; ++i) v[i] = 0.f;
     const int per = (pieces + kTeam) / kTeam, end = min(pieces + 1, per * (member + 1));
     for (int p0 = per * member; p0 < end; p0 += 32) {
         // a lane a record: its maximum and sum; one without a score above -inf holds no values
@@ -876,27 +880,30 @@ template <bool kBf, int kTeam> __global__ void __launch_bounds__(kJoinWarps * 32
         for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(kWarpAll, l, o);
         sum = sum * turn + l;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= turn;
+        for (int i = 0; i < kVals; ++i) v[i] *= turn;
         top = now;
         const unsigned there = __ballot_sync(kWarpAll, !empty);
         const int count = min(32, end - p0);
         constexpr int kAtOnce = 8;
         for (int q0 = 0; q0 < count; q0 += kAtOnce) {
-            float4 x[kAtOnce], y[kAtOnce];
+            float4 x[kAtOnce], y[kWide ? kAtOnce : 1];
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i) {
-                x[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                x[i] = y[kWide ? i : 0] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (q0 + i < count && there >> (q0 + i) & 1 && lane * 4 < hd) {
                     const float* rec = record(p0 + q0 + i);
                     x[i] = __ldcg(reinterpret_cast<const float4*>(rec) + lane);
-                    if (two_rows) y[i] = __ldcg(reinterpret_cast<const float4*>(rec + 128) + lane);
+                    if (second) y[kWide ? i : 0] = __ldcg(reinterpret_cast<const float4*>(rec + 128) + lane);
                 }
             }
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i) {
                 const float w = __shfl_sync(kWarpAll, weight, q0 + i);
                 v[0] += x[i].x * w, v[1] += x[i].y * w, v[2] += x[i].z * w, v[3] += x[i].w * w;
-                v[4] += y[i].x * w, v[5] += y[i].y * w, v[6] += y[i].z * w, v[7] += y[i].w * w;
+                if (kWide) {
+                    const float4 z = y[kWide ? i : 0];
+                    v[kVals - 4] += z.x * w, v[kVals - 3] += z.y * w, v[kVals - 2] += z.z * w, v[kVals - 1] += z.w * w;
+                }
             }
         }
     }
@@ -904,28 +911,29 @@ template <bool kBf, int kTeam> __global__ void __launch_bounds__(kJoinWarps * 32
         parts[member][0][lane] = top;
         parts[member][1][lane] = sum;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) parts[member][2 + i][lane] = v[i];
+        for (int i = 0; i < kVals; ++i) parts[member][2 + i][lane] = v[i];
         __syncthreads();
         if (member) return;
 #pragma unroll
         for (int w = 1; w < kTeam; ++w) top = fmaxf(top, parts[w][0][lane]);
         sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        for (int i = 0; i < kVals; ++i) v[i] = 0.f;
 #pragma unroll
         for (int w = 0; w < kTeam; ++w) {                              // (a warp without a score has zeros)
             const float turn = ex2(parts[w][0][lane] - top);
             sum += parts[w][1][lane] * turn;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += parts[w][2 + i][lane] * turn;
+            for (int i = 0; i < kVals; ++i) v[i] += parts[w][2 + i][lane] * turn;
         }
     }
     using H = typename Half<kBf>::type;
     const float gain = sum == 0.f ? 0.f : 1.f / sum;
     uint16_t* const out = static_cast<uint16_t*>(A.out) + place * hd + lane * 4;
     if (lane * 4 < hd) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<H>(v[0] * gain, v[1] * gain), pack2<H>(v[2] * gain, v[3] * gain));
-    if (two_rows)
-        *reinterpret_cast<uint2*>(out + 128) = make_uint2(pack2<H>(v[4] * gain, v[5] * gain), pack2<H>(v[6] * gain, v[7] * gain));
+    if (second)
+        *reinterpret_cast<uint2*>(out + 128) =
+            make_uint2(pack2<H>(v[kVals - 4] * gain, v[kVals - 3] * gain), pack2<H>(v[kVals - 2] * gain, v[kVals - 1] * gain));
     if (A.lse && lane == 0) A.lse[place] = sum == 0.f ? -INFINITY : (top + log2f(sum)) / kLog2e;
 }
 
@@ -1096,8 +1104,12 @@ int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const in
     const bool teams = S.s.own_records <= 4LL * S.grid;
     const dim3 grid((unsigned)cdiv(S.s.own_records, teams ? 1 : kJoinWarps)), threads(kJoinWarps * 32);
     auto join = [&](auto kern) { return launch(kern, grid, threads, 0, st, who, A); };
-    if (teams) return bf ? join(join_kernel<true, kJoinWarps>) : join(join_kernel<false, kJoinWarps>);
-    return bf ? join(join_kernel<true, 1>) : join(join_kernel<false, 1>);
+    if (P.head_dim > 128) {
+        if (teams) return bf ? join(join_kernel<true, kJoinWarps, true>) : join(join_kernel<false, kJoinWarps, true>);
+        return bf ? join(join_kernel<true, 1, true>) : join(join_kernel<false, 1, true>);
+    }
+    if (teams) return bf ? join(join_kernel<true, kJoinWarps, false>) : join(join_kernel<false, kJoinWarps, false>);
+    return bf ? join(join_kernel<true, 1, false>) : join(join_kernel<false, 1, false>);
 }
 
 }  // extern "C"
