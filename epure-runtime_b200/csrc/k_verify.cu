@@ -15,6 +15,9 @@
 // conversions to 64 bits, are what the first pass would spend its time on, so it sums in pairs of
 // float32: each sum and difference with what its rounding left over, which keeps about 46 bits.
 // All that follows is 64-bit.
+//
+// Measured (B200, graphs of calls): 64 x 4 drafts over 128,256 tokens, float32: 16.8 us (10.2 at the copy rate); 1 x 4 over
+// 151,936: 9.9 us; 33 x 7 looked up over 32,001, bf16: 6.9 us.  With 64-bit sums in the first pass 1 x 4 took 21 us.
 #include "epq_common.cuh"
 #include "epq_paged.cuh"
 #include "epq_sampling.h"

@@ -50,7 +50,7 @@ def test_bad_bounds_and_selections(lib):  # noqa: F811
     assert _select(lib, q=_heads(3)) == -2 and _select(lib, chosen=None) == -1
     assert _select(lib, ws=65536 * 4) == -6 and _select(lib, work=4100) == -6
     assert _select(lib, _pages(seqs=40000), batch=40000) == -8
-    assert lib.epq_paged_select_workspace_bytes(ref(_pages()), 2) == 65536 * 4 + 2 * 2 * 4 * 4
+    assert lib.epq_paged_select_workspace_bytes(ref(_pages()), 2) == 65536 * 4 + 2 * 2 * (4 + 1) * 4        # counters, keys, largest bounds
 
 
 def test_bad_lists_and_groups(lib):  # noqa: F811
