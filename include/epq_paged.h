@@ -147,7 +147,7 @@ int epq_paged_bounds(const epq_pages* pages, void* bounds, int64_t bounds_stride
  *     score(j) = max over the query heads h of key head g of
  *                sum_d max(q[b, h, d] lo_j[d], q[b, h, d] hi_j[d])
  * in float32, products first, then neighbouring dims' sums, then neighbours of those (head_dim
- * padded with zeros to a power of two).  Of the n = ceil(lengths[b] / page_size) blocks of a row
+ * padded with zeros to a power of two; lo <= hi, as epq_paged_bounds leaves them).  Of the n = ceil(lengths[b] / page_size) blocks of a row
  * chosen[b, g, 0..count) receives, in ascending order, the first `sinks`, the last `recent` and
  * those of the others with the largest scores (NaN first), the lowest of equal ones; all of them
  * where n <= count, and -1 behind the last.  A block whose page is outside the pool comes last.
