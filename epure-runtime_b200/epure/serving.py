@@ -189,10 +189,10 @@ class BatchDecoder:
 
     def _begin(self, prompts, n_new, prefix):
         """Reserves and fills the sequences of ``prompts`` (behind the common tokens ``prefix``, if any) with room for
-        ``n_new`` more tokens: (greedy first tokens, lengths, tokens in common), the first a list of tensors."""
+        ``n_new`` more tokens: (logits behind each, lengths, tokens in common), the first a list of tensors."""
         n = 0 if prefix is None else prefix.shape[0]
         whole = 0
-        first, lengths = [], []
+        logits, lengths = [], []
         for i, p in enumerate(prompts):
             if i == 0:
                 self.cache.reserve(0, n + p.shape[0] + n_new)
@@ -204,9 +204,9 @@ class BatchDecoder:
             self.cache.reserve(i, n + p.shape[0] + n_new)
             if n and i and whole < n:
                 self.prefill(i, prefix[whole:], past=whole)
-            first.append(torch.argmax(self.prefill(i, p, past=n)))
+            logits.append(self.prefill(i, p, past=n))
             lengths.append(n + p.shape[0])
-        return first, lengths, n
+        return logits, lengths, n
 
     def generate(self, prompts, n_new, graph=True, prefix=None):
         """``n_new`` greedy tokens after each of the ``prompts`` (long tensors), a long tensor [len(prompts), n_new].
@@ -216,8 +216,8 @@ class BatchDecoder:
         B, dev = len(prompts), self.device
         out = torch.empty(B, n_new, dtype=torch.long, device=dev)
         try:
-            first, lengths, n = self._begin(prompts, n_new, prefix)
-            tok, pos = torch.stack(first), torch.tensor(lengths, device=dev)
+            logits, lengths, n = self._begin(prompts, n_new, prefix)
+            tok, pos = torch.stack([torch.argmax(x) for x in logits]), torch.tensor(lengths, device=dev)
             seq = torch.arange(B, dtype=torch.int32, device=dev)
             behind = n > 0 and self.sparse is None
             if graph:
@@ -244,8 +244,8 @@ class BatchDecoder:
     # -- drafted tokens ------------------------------------------------------------------------------------------
     def judge(self, tokens, drafts, seq, pos, uniforms, temperature=1.0, draft_probs=None):
         """One pass over drafted tokens: ``tokens`` [batch] (the last known token of each sequence, at ``pos``) and
-        ``drafts`` [batch, n] behind it (a row's end at its first negative one) are fed together, n + 1 rows a sequence
-        that share what the sequence holds already, and judged by ``sampling.verify`` with the numbers ``uniforms``
+        ``drafts`` [batch, n] behind it (a row's end at its first one outside the vocabulary) are fed together, n + 1 rows
+        a sequence that share what the sequence holds already, and judged by ``sampling.verify`` with the numbers ``uniforms``
         [batch, n + 1].  ``temperature`` 0 takes the most likely token.  Returns verify's ``(tokens [batch, n + 1],
         accepted [batch])``: a row's first ``accepted + 1`` tokens are its next ones.  The cache then holds ``pos +
         accepted + 1`` of its tokens; the last one returned is the next call's.  The pages must be reserved up to ``pos +
@@ -254,6 +254,7 @@ class BatchDecoder:
             raise ValueError("epure: drafted tokens are judged over the whole cache (sparse=None)")
         B, n = drafts.shape
         dev = self.device
+        drafts = drafts.masked_fill(drafts >= self.decoder.embed.shape[0], -1)
         rows = torch.cat((tokens[:, None], drafts), 1)
         there = (rows >= 0).to(torch.long).cumprod(1) * (pos >= 0)[:, None]
         step = torch.arange(n + 1, device=dev)
@@ -261,12 +262,7 @@ class BatchDecoder:
         starts = torch.arange(0, B * (n + 1) + 1, n + 1, dtype=torch.int32, device=dev)
         logits = self.step(rows.clamp(min=0).reshape(-1), seq.repeat_interleave(n + 1), at.reshape(-1),
                            (starts, (pos + 1).clamp(min=0)))
-        logits = logits.view(B, n + 1, -1)
-        if temperature > 0:
-            probs = torch.softmax(logits / temperature, -1)
-        else:
-            probs = torch.zeros_like(logits).scatter_(-1, logits.argmax(-1, keepdim=True), 1.0)
-        return sampling.verify(probs, draft_probs, drafts, uniforms)
+        return sampling.verify(_probabilities(logits.view(B, n + 1, -1), temperature), draft_probs, drafts, uniforms)
 
     def speculate(self, prompts, n_new, drafts=4, temperature=0.0, prefix=None, generator=None):
         """``n_new`` tokens after each of the ``prompts``, drafted ``drafts`` at a time by looking the last two tokens up
@@ -280,9 +276,12 @@ class BatchDecoder:
         room = n_new + drafts + 1
         passes = 0
         try:
-            first, lengths, n = self._begin(prompts, room, prefix)
+            logits, _, n = self._begin(prompts, room, prefix)
+            u = torch.rand(B, 1, device=dev, generator=generator)
+            none = torch.empty(B, 0, dtype=torch.long, device=dev)
+            first, _ = sampling.verify(_probabilities(torch.stack(logits)[:, None], temperature), None, none, u)
             before = [] if prefix is None else prefix.tolist()
-            text = [before + p.tolist() + [int(t)] for p, t in zip(prompts, first)]
+            text = [before + p.tolist() + [t] for p, t in zip(prompts, first[:, 0].tolist())]
             done = [n + p.shape[0] + n_new for p in prompts]
             seq = torch.arange(B, dtype=torch.int32, device=dev)
             while any(len(x) < d for x, d in zip(text, done)):
@@ -301,6 +300,13 @@ class BatchDecoder:
                 self.cache.release(i)
         out = torch.tensor([x[d - n_new:d] for x, d in zip(text, done)], dtype=torch.long, device=dev).view(B, n_new)
         return out, passes
+
+
+def _probabilities(logits, temperature):
+    """What tokens are drawn with; a temperature of 0 takes the most likely one."""
+    if temperature > 0:
+        return torch.softmax(logits / temperature, -1)
+    return torch.zeros_like(logits).scatter_(-1, logits.argmax(-1, keepdim=True), 1.0)
 
 
 def _look_up(text, count):

@@ -107,6 +107,23 @@ def test_judge_agrees_with_single_steps(fmt):
     assert bool((kept >= 0).all()) and bool((got[:3, 0] >= 0).all())
 
 
+def test_judge_ends_at_a_draft_outside_the_vocabulary():
+    """Such a draft is not looked up in the embedding: the row is judged as one that ends there."""
+    from epure.serving import BatchDecoder
+    b = BatchDecoder(_decoder(), seqs=2, page_size=16)
+    prompts = _prompts([5, 9])
+    for i, p in enumerate(prompts):
+        b.cache.reserve(i, len(p) + 4)
+        b.prefill(i, p)
+    seq, pos = torch.arange(2, dtype=torch.int32, device=DEV), torch.tensor([5, 9], device=DEV)
+    tok, u = torch.tensor([1, 2], device=DEV), torch.full((2, 4), 0.25, device=DEV)
+    want = b.judge(tok, torch.tensor([[3, -1, -1], [-1, 4, 4]], device=DEV), seq, pos, u, temperature=1.0)
+    for bad in (1000, 2 ** 40):
+        got = b.judge(tok, torch.tensor([[3, bad, 4], [bad, 4, 4]], device=DEV), seq, pos, u, temperature=1.0)
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
 def test_judge_behind_long_sequences():
     """Drafts of sequences long enough for the shared form: the logits' choice equals that of rows by themselves."""
     from epure.serving import BatchDecoder
@@ -135,6 +152,25 @@ def test_speculate(kw):
     out, passes = b.speculate(prompts, 10, generator=gen, **kw)
     assert out.shape == (3, 10) and bool((out >= 0).all()) and bool((out < 1000).all()) and 1 <= passes <= 10
     assert b.cache.free_pages() == free
+
+
+def test_speculate_draws_its_first_token_too():
+    """With a temperature the token behind each prompt is drawn like the others, not the most likely one."""
+    from epure import sampling
+    from epure.serving import BatchDecoder
+    b = BatchDecoder(_decoder(), seqs=3, page_size=16)
+    prompts = _prompts([5, 9, 17])
+    logits = []
+    for i, p in enumerate(prompts):
+        b.cache.reserve(i, len(p))
+        logits.append(b.prefill(i, p))
+        b.cache.release(i)
+    logits = torch.stack(logits)
+    u = torch.rand(3, 1, device=DEV, generator=torch.Generator(device=DEV).manual_seed(8))
+    want, _ = sampling.verify(torch.softmax(logits / 5.0, -1)[:, None], None, torch.empty(3, 0, dtype=torch.long, device=DEV), u)
+    got, _ = b.speculate(prompts, 1, temperature=5.0, generator=torch.Generator(device=DEV).manual_seed(8))
+    assert torch.equal(got, want)
+    assert not torch.equal(got[:, 0], logits.argmax(-1))
 
 
 def test_speculate_no_or_one_token():
