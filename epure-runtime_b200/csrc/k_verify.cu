@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kMany ? 4 : 1) verify_ke
     const int vocab = (int)V, tiles = (head + vocab + kTile - 1) / kTile, per = (tiles + kRuns - 1) / kRuns;
     // 0: the whole row; 1: max(p - q, 0); 2: all but the drafted token
     int how = taken_at & 1 ? (A.q.data ? 1 : 2) : 0;
-    const int without = how == 2 ? (int)x[n] : -1;
+    int without = how == 2 ? (int)x[n] : -1;
     auto load = [&](int tile, float (&f)[kV], float (&g)[kV]) {
         const int e = tile * kTile + lane * kV - head;
         fetch<T, kV>(f, p, e, vocab);
@@ -239,7 +239,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == kMany ? 4 : 1) verify_ke
         upto = found_upto;
         if (from >= 0 || pass) break;
         __syncthreads();                       // (the three are read)
-        how = 0;                               // nothing is left of the residual: p itself
+        how = 0;                               // nothing is left of the residual: p itself, the drafted token too
+        without = -1;
     }
 
     // ---- the drawn token, by the CTA whose run it is in (-1: by the first)

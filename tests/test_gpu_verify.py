@@ -144,6 +144,30 @@ def test_weights_that_are_not_ordinary():
     _check(tiny, None, torch.zeros(1, 0, dtype=torch.long, device=DEV), torch.tensor([[0.7]], device=DEV))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("V", [1, 4, 999, 32001, 150000])
+def test_nothing_left_but_the_draft(dtype, V):
+    """Drafts without probabilities whose target gives a weight to nothing else: a refused one leaves nothing, so the target
+    itself is drawn from, which is the drafted token.  (Filtered probabilities that were not normalised again, or a
+    float16 row whose others went to 0.)"""
+    g = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.randint(0, V, (8, 3), generator=g, device=DEV)
+    x[0], x[1] = 0, V - 1
+    p = torch.zeros(8, 4, V, dtype=dtype, device=DEV)
+    p[:, :3].scatter_(2, x[:, :, None], 0.5)
+    p[:, 3, V // 2] = 0.25
+    p[4] *= -1                                         # no weight at all
+    p[5, 0] = torch.where(p[5, 0] == 0, math.nan, p[5, 0].float()).to(dtype)
+    u = torch.full((8, 4), 0.7, device=DEV)
+    u[2, 0], u[3, :2] = 0.3, 0.3                       # refused at the second and the third draft
+    u[:, 3] = torch.tensor([0.3, 0.999, 0.3, 0.001, 0.3, 0.3, 0.6, 0.9], device=DEV)
+    got, n = _check(p, None, x, u)
+    assert n.tolist() == [0, 0, 1, 2, 0, 0, 0, 0]
+    for b in (0, 1, 2, 3, 5, 6, 7):
+        assert int(got[b, n[b]]) == int(x[b, n[b]])
+    assert got[4].tolist() == [-1] * 4
+
+
 def test_close_weights_need_64_bits():
     """A uniform row of 2^18 tokens: every number's token is where it says, not where float32 sums would put it."""
     from epure import sampling
