@@ -337,7 +337,7 @@ template <typename F> __device__ Place find_place(int need, int stop, int j0, in
         }
         __syncthreads();
         at.low += (uint32_t)found[0] << shift;
-        at.high = min(at.high, at.low + ((1u << shift) - 1u));
+        at.high = at.low + min(at.high - at.low, (1u << shift) - 1u);  // (a bin of NaN's key may end past 2^32)
         at.above = found[1];
         if (found[2] <= stop || shift == 0) return at;
         __syncthreads();                                               // (found and sums are read)

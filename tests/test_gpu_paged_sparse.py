@@ -187,6 +187,22 @@ def test_select_ties_and_not_finite_scores():
     assert got[0, 0].tolist() == list(range(9)) + [199] and got[1, 1].tolist() == list(range(9)) + [129]
 
 
+@pytest.mark.parametrize("blocks,nans", [(60, 20), (300, 12), (300, 299), (5000, 20), (9000, 1500)])
+@pytest.mark.parametrize("fmt,dtype", [("same", torch.bfloat16), ("same", torch.float16), ("int8", torch.float16)])
+def test_select_as_many_nan_as_are_wanted(blocks, nans, fmt, dtype):
+    """Blocks with NaN come first, the lowest of them, be there more than are wanted, as many or fewer."""
+    from epure import paged
+    n = [blocks, 40, blocks]
+    pages, bounds, q, lengths = _selection_case(4, 2, 64, n, fmt, dtype, ps=1)
+    pick = torch.randperm(blocks - 2, generator=torch.Generator().manual_seed(blocks))[:nans] + 1
+    for h, d in ((0, 5), (1, 63)):
+        bounds[pages.table[0, pick.to(DEV)].long(), h, h, d] = math.nan
+    q[2, 1, 7] = math.nan                              # all scores of a key head
+    for count in sorted({2, nans // 2 + 3, nans + 2, min(blocks - 1, nans + 9)}):
+        got = paged.select(pages, bounds, q, lengths, count)
+        assert torch.equal(got, _expected(q, bounds, pages.table, n, count, 1, 1, 2)), count
+
+
 @pytest.mark.parametrize("fmt,cache,dtype", [("same", torch.bfloat16, torch.bfloat16), ("same", torch.float16, torch.float16),
                                              ("int8", torch.bfloat16, torch.float16), ("same", torch.float16, torch.bfloat16)])
 @pytest.mark.parametrize("heads,kv,hd,blocks", [(8, 1, 128, 300), (24, 2, 64, 900), (6, 2, 256, 130), (4, 4, 80, 3000)])
