@@ -247,6 +247,31 @@ def test_a_value_beyond_a_row_stays_unseen():
     _check(case, q[:3])
 
 
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_weights_are_not_too_small_on_average(fmt):
+    """The mean of the results' relative errors, over 2^20 of them behind one block of 128 positive values.
+
+    Each result is rounded to float16: an error of mean 0 and at most 2^-11, so the mean of all of them has a standard
+    deviation below 2^-11 / sqrt(3) / 2^10 < 2^-21.7.  A block's 16 products add to float32 sums that lose at most 2^-23 of
+    their value each time, half of it on average: below 2^-20 in all.  A second part of a weight rounded to the nearest is off
+    by 2^-16 at most and by nothing on average; one that is cut off is too small by 2^-17.1 on average (weights 2^-6 to 1).
+    Four standard deviations and the sums: 2^-20 + 2^-19.7 < 2^-18.8."""
+    from epure import paged
+    B, H, hd = 1024, 8, 128
+    pages, starts, prefix, seq, lengths, _ = _case([(128, [0] * B)], 1, hd, 64, fmt, torch.float16)
+    g = _gen(21)
+    at, pos = torch.zeros(128, dtype=torch.int32, device=DEV), torch.arange(128, device=DEV)
+    k = torch.randn(128, 1, hd, generator=g, device=DEV).half()
+    v = (0.5 + 0.5 * torch.rand(128, 1, hd, generator=g, device=DEV)).half()
+    paged.write(pages, k, v, at, pos)
+    k, v = (x[:, 0].double() for x in paged.read(pages, at, pos, torch.float32))
+    q = torch.randn(B, H, hd, generator=g, device=DEV).half()
+    out = paged.attend_shared(pages, q, torch.tensor(lengths, device=DEV), starts, prefix, seq=seq, always=True)
+    want = torch.softmax(q.double() @ k.T / math.sqrt(hd), -1) @ v
+    mean = float(((out.double() - want) / want).mean())
+    assert abs(mean) <= 2.0 ** -18.8, math.log2(abs(mean))
+
+
 def test_layouts():
     """Rows of a projection, unaligned rows, heads by rows, an output that is given, the default sequences."""
     from epure import paged
