@@ -114,7 +114,6 @@ __global__ void __launch_bounds__(kThreads, kThreads == kMany ? 4 : 1) verify_ke
             bool keep = false, there = false;
             if (i < A.drafts) {
                 const int64_t t = x[i];
-                if (t >= V && rank == 0) atomicOr(&g_verify_error, 1);
                 there = t >= 0 && t < V;
                 if (there) {
                     const double px = paged::to_f<T>(p0[i * A.p.stride_step + t]);
@@ -131,6 +130,15 @@ __global__ void __launch_bounds__(kThreads, kThreads == kMany ? 4 : 1) verify_ke
             }
         }
         if (lane == 0) taken_at = 2 * n + refused;
+    } else if (warp == 1 && rank == 0) {       // what ends the row's drafts: a negative token, or one to report
+        for (int i0 = 0; i0 < A.drafts; i0 += 32) {
+            const int64_t t = i0 + lane < A.drafts ? x[i0 + lane] : 0;
+            const unsigned past = __ballot_sync(kAll, t >= V), ends = __ballot_sync(kAll, t < 0) | past;
+            if (ends) {
+                if (lane == 0 && past >> (__ffs(ends) - 1) & 1) atomicOr(&g_verify_error, 1);
+                break;
+            }
+        }
     }
     __syncthreads();
     const int n = taken_at >> 1;

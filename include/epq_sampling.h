@@ -35,7 +35,8 @@ typedef struct epq_probs {
  * say) the last with a weight is taken, and -1 where none has one.
  * out [batch, drafts + 1] receives the accepted drafts, the drawn token and -1 behind it;
  * accepted [batch] receives n.  A drafted token of vocab or more ends its row's drafts and is
- * reported by epq_device_error (bit 3).  The probabilities need only the alignment of their
+ * reported by epq_device_error (bit 3); what lies behind the end of a row's drafts is not looked
+ * at.  The probabilities need only the alignment of their
  * type. */
 int epq_verify_drafts(const epq_probs* target, const epq_probs* draft, const int64_t* tokens, int64_t tokens_stride,
                       const float* uniforms, int64_t uniforms_stride, int64_t batch, int32_t drafts, int64_t vocab,

@@ -271,3 +271,34 @@ def test_tokens_outside_the_vocabulary_are_reported():
     r = subprocess.run([sys.executable, "-c", _CHILD, PKG], capture_output=True, text=True, timeout=300, env=dict(os.environ))
     assert r.returncode == 0, r.stderr[-2000:]
     assert "FLAG 8" in r.stdout
+
+
+_BEHIND = r"""
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from epure import _native, sampling
+p = torch.full((3, 41, 10), 0.1, device="cuda:0")
+u = torch.full((3, 41), 0.35, device="cuda:0")
+x = torch.full((3, 40), 4, device="cuda:0")
+x[0, 2], x[0, 3] = -1, 10                              # behind a row's end
+x[1, 39], x[1, 7:39] = 2 ** 40, -1
+x[2, 0] = -5
+x[2, 1:] = 77
+u[0, :2] = 0.0
+got, n = sampling.verify(p, None, x, u)
+assert n.tolist() == [2, 0, 0]
+assert _native.device_error() == 0
+x[1] = 4                                               # refused at once, far before the one outside
+x[1, 38] = 10
+sampling.verify(p, None, x, u)
+torch.cuda.synchronize()
+print("FLAG", _native.device_error())
+"""
+
+
+def test_what_lies_behind_a_rows_drafts_is_not_reported():
+    """Tokens behind a row's end are no drafts, whatever they hold; one of the row's drafts that is outside the vocabulary is
+    reported wherever it lies and whatever was refused before it."""
+    r = subprocess.run([sys.executable, "-c", _BEHIND, PKG], capture_output=True, text=True, timeout=300, env=dict(os.environ))
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert "FLAG 8" in r.stdout
