@@ -26,6 +26,9 @@ struct AttendArgs {
     const int32_t* blocks;   // kListed: [batch][kv_heads][count] pages of the sequence, -1: none
     int count;
     SharedD shared;          // kBehindShared
+    const int32_t* starts;   // kAllTokens, for a batch that could share but does not: its groups, which are looked
+    const int64_t* prefix;   // at for their errors alone
+    int groups;
     int batch, heads, group, chunks, dtype;
     float scale_log2;
 };
@@ -281,12 +284,31 @@ __global__ void __launch_bounds__(kThreads, Shape<kKind, kDim, kCols>::kCtas) at
         }
         return v;
     };
+    const bool looks = kMode == kAllTokens && A.groups > 0 && blockIdx.x == gridDim.x - 1;
+    int from = 0, to = 0;                              // a thread's first group, on its way with the lengths
+    int64_t prefix = 0;
+    if (looks && tid < A.groups) {
+        from = A.starts[tid];
+        to = A.starts[tid + 1];
+        prefix = A.prefix[tid];
+    }
     const int first_blocks = b0 < b1 ? span_of<kMode, kTok>(A, b0, blockIdx.x == 0).blocks : 0;
     int mine = weight(first_blocks), some_empty = b0 < b1 && first_blocks == 0;
     for (int b = b0 + 1; b < b1; ++b) {
         const int blocks = span_of<kMode, kTok>(A, b, blockIdx.x == 0).blocks;
         mine += weight(blocks);
         some_empty |= blocks == 0;
+    }
+    if (looks) {
+        auto bad_group = [&]() { return from < 0 || from > to || to > A.batch || prefix < 0 || prefix > (int64_t)P.max_pages * P.page_size; };
+        bool bad = bad_group();
+        for (int g = tid + kThreads; g < A.groups; g += kThreads) {
+            from = A.starts[g];
+            to = A.starts[g + 1];
+            prefix = A.prefix[g];
+            bad |= bad_group();
+        }
+        if (bad) atomicOr(&g_attend_error, kBadPosition);
     }
     const int64_t total = (int64_t)__reduce_add_sync(kAll, mine) * units;
     const int run = max(kMinBlocks, (int)quotient(total + gridDim.x - 1, gridDim.x));

@@ -1051,7 +1051,12 @@ int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const in
     if (rc != EPQ_OK || !ready) return rc;
     const PagesD& P = A.pages;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!may_share(P, batch, A.heads, groups, always != 0) || !boxes_of(*q, batch)) return launch_attend_plain(A, cols, st);
+    if (!may_share(P, batch, A.heads, groups, always != 0) || !boxes_of(*q, batch)) {
+        A.starts = starts;
+        A.prefix = prefix;
+        A.groups = (int)groups;
+        return launch_attend_plain(A, cols, st);
+    }
     const int64_t behind = align256(attend_bytes(who, pages, batch, A.heads));
     const Layout L = layout_of(P, batch, A.heads, groups, behind);
     if (workspace_bytes < L.bytes)

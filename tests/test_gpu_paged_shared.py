@@ -421,3 +421,47 @@ def test_bad_groups_lengths_and_pages_are_reported(kind, flag):
                        env=dict(os.environ))
     assert r.returncode == 0, r.stderr[-2000:]
     assert f"FLAG {flag}" in r.stdout
+
+
+_SMALL = r"""
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from epure import _native, paged
+dev, kind = "cuda:0", sys.argv[2]
+t = lambda *v: torch.tensor(v, device=dev)
+ps, always = (7, True) if kind == "pages" else (16, False)
+k = torch.randn(12, 2, ps, 64, device=dev).to(torch.bfloat16)
+pages = paged.KVPages(k, k.flip(0), torch.arange(12, dtype=torch.int32, device=dev).view(3, 4))
+q = torch.randn(3, 4, 64, device=dev).to(torch.bfloat16)
+n = t(20, 4, 28)
+want = paged.attend(pages, q, n)
+call = lambda starts, prefix: paged.attend_shared(pages, q, n, starts, prefix, always=always)
+groups = 700 if kind == "last" else 1
+good = t(*[0] * groups, 3).int(), t(*[4] * groups)
+assert torch.equal(call(*good), want)
+assert torch.equal(call(t(0).int(), t(0)[:0]), want)
+assert _native.device_error() == 0
+if kind == "prefix":
+    bad = t(0, 3).int(), t(4 * ps + 1)
+elif kind == "negative":
+    bad = t(0, 3).int(), t(-1)
+elif kind == "descending":
+    bad = t(2, 1).int(), t(4)
+elif kind == "last":
+    bad = t(*[0] * 700, 4).int(), good[1]
+else:
+    bad = t(0, 4).int(), t(4)
+assert torch.equal(call(*bad), want)
+torch.cuda.synchronize()
+print("FLAG", _native.device_error())
+"""
+
+
+@pytest.mark.parametrize("kind", ["starts", "prefix", "negative", "descending", "last", "pages"])
+def test_bad_groups_are_reported_where_nothing_is_shared(kind):
+    """Also where a batch is read row by row from the start: too little to share, or pages that cannot be (in a child process:
+    the flag stays set)."""
+    r = subprocess.run([sys.executable, "-c", _SMALL, PKG, kind], capture_output=True, text=True, timeout=300,
+                       env=dict(os.environ))
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert "FLAG 16" in r.stdout
