@@ -272,6 +272,22 @@ def test_weights_are_not_too_small_on_average(fmt):
     assert abs(mean) <= 2.0 ** -18.8, math.log2(abs(mean))
 
 
+def test_many_groups():
+    """More tiles than a warp looks at together, of two to five rows, with empty groups and groups of one row between."""
+    groups = [(37 + 61 * (i % 17), [[3, 0], [1, 9, -1, 4], [5], [], [2, 2, 7], [0, 1, 2, 3, 4]][i % 6]) for i in range(90)]
+    for fmt in ("same", "int8"):
+        case = _case(groups, 2, 64, 16, fmt, torch.bfloat16)
+        _check(case, _q(case, 8, 64, torch.bfloat16))
+
+
+@pytest.mark.parametrize("fmt,hd", [("same", 16), ("int8", 16), ("same", 48)])
+def test_more_groups_than_the_plan_holds(fmt, hd):
+    """More groups and tiles than the plan's threads and shared memory hold (512 each), of small heads."""
+    groups = [(5 + 13 * (i % 29), [1, 2] if i % 7 else [1, 2, 3]) for i in range(1100)]
+    case = _case(groups, 1, hd, 8, fmt, torch.bfloat16, same=True)
+    _check(case, _q(case, 2, hd, torch.bfloat16))
+
+
 def test_layouts():
     """Rows of a projection, unaligned rows, heads by rows, an output that is given, the default sequences."""
     from epure import paged
