@@ -31,9 +31,12 @@
 // The running maximum moves only when a score passes it by 2^8.
 //
 // Measured (B200, device time in a graph of calls, all four launches): 64 rows behind 8,192 tokens, 32 / 8
-// heads of 128, bf16: 67 us (row by row 211); 256 rows behind 32,768, 64 / 8 heads, e4m3: 622 us, 553 of
+// heads of 128, bf16: 67 us (row by row 211); 256 rows behind 32,768, 64 / 8 heads, e4m3: 628 us, 552 of
 // them the shared tokens (row by row 2,152).  What bounds it is a slot's chain of product, softmax and product, about
-// 4 us a block of 128 tokens for 1.7 us of tensor time with two slots.
+// 4 us a block of 128 tokens for 1.7 us of tensor time with two slots: a softmax thread reads its half row of S from
+// tensor memory twice, 32 columns at a time and each time to the end, and the 8-bit forms, built for 22 warps at 80
+// registers, spill (88 to 92 bytes stored, 300 to 308 loaded a thread).  A tile whose shortest row is of 5 tokens goes row by
+// row: 64 rows behind 8,192 take 211 us with one such row.
 #include "epq_attend.cuh"
 #include "epq_sm100.cuh"
 #include <cuda.h>

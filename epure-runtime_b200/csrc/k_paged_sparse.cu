@@ -5,7 +5,8 @@
 //   lo[d], hi[d] = min, max over the page's tokens of K[t, d]
 //   score = max over the key head's query heads of  sum_d max(q_d lo_d, q_d hi_d)
 //
-// which no q . K[t] of the page passes.  A product of two 16-bit values is exact in float32
+// which no q . K[t] of the page passes (16-bit caches, finite keys, up to the sums' rounding; the
+// bounds of 8-bit ones are rounded to the nearest bf16).  A product of two 16-bit values is exact in float32
 // and the sum's order is fixed (neighbours, then neighbours of their sums), so which blocks
 // are chosen is the same wherever it is computed in float32.
 //
@@ -19,12 +20,15 @@
 // the scores of 16 blocks and 8 heads are a product on the tensor cores (m16n8k16: a group's heads are
 // its 8 columns; tcgen05's tiles of 128 rows would be read from shared memory, where these operands
 // come from HBM straight into the registers that multiply them).  Its float32 sums have another
-// order than the defined ones.  Together they are off by less than E = (1.5 head_dim + 8) 2^-23 |q|_1
-// max|bounds|: head_dim additions, each off by at most 2^-23 of the sum of all |q_d bound_d|, in the
-// one, log2 of that in the other.  The CTAs of a unit (row, key head) leave their scores as integers in the order of the floats;
-// the last of them finds the count-th largest, T, two bits at a time.  A block more than 2 E above T
-// is chosen and one more than 2 E below is not, whatever the order; where those between are more
-// than are still wanted, their defined scores decide.
+// order than the defined ones.  Together they are taken to be off by less than E = (1.5 head_dim + 8) 2^-23 |q|_1
+// max|bounds| (3 head_dim over f16 bounds, and for an f16 q over bf16 bounds, which has two parts): head_dim
+// products and twice head_dim / 8 sums of them, each off by at most 2^-23 of the sum of all |q_d bound_d|, in
+// the one, log2 of that in the other.  That assumes of the tensor cores, whose sums no document specifies, that
+// addends keep 24 bits from the largest of their sum's values on.
+// The CTAs of a unit (row, key head) leave their scores as integers in the order of the floats;
+// the last of them finds the count-th largest, T, by counting in 1,024 bins of the scores' range and then
+// of the bin that it is in.  A block more than 2 E above T is chosen and one more than 2 E below is not,
+// whatever the order; where those between are more than are still wanted, their defined scores decide.
 //
 // Measured (B200, graphs of calls): selection of 64 rows of up to 32,768 tokens in pages of 32, 64 / 8 heads: 51 us for 137 MB
 // (3 CTAs an SM with half the loads: 48, but 1 us more for small calls); 1 x 131,072 in pages of 64: 14.4 us, a chain

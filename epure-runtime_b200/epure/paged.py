@@ -70,7 +70,12 @@ def attend_shared(pages, q, lengths, starts, prefix, seq=None, scale=None, out=N
     one sequence (drafted tokens, a prompt's chunk) with lengths of their own.  The shared tokens are
     read through the table of one of the rows.  A row shorter than its group's prefix attends over its own length, rows in no
     group share nothing.  Groups for which reading row by row is reckoned to be faster (few rows, short prefixes) are
-    read that way, unless ``always``."""
+    read that way, unless ``always``.
+
+    Nothing is shared, with ``always`` either, in pages whose size is no multiple of 8, by 8-bit heads above 128, and with
+    more than 128 query heads a key head.  Rows are taken together in tiles of a group's consecutive rows, as far as the shortest
+    row of a tile that is not empty: put rows that are much shorter than their prefix into no group.  Where a batch could
+    share and then does not, the call takes about 10 us longer than ``attend``."""
     return (_native.tensor_calls or _native.load_tensor_calls()).attend_shared(*pages, q, lengths, starts, prefix, seq,
                                                                                scale, out, return_lse, always)
 
@@ -88,7 +93,7 @@ def select(pages, bounds, q, lengths, count, seq=None, sinks=1, recent=1):
     """The ``count`` blocks (pages) of each row and key head to attend over, int32 [batch, kv_heads, count] in ascending
     order, -1 behind the last: the first ``sinks``, the last ``recent`` and those of the others in which a query head of
     the key head may find the largest score, ``sum_d max(q_d lo_d, q_d hi_d)`` by their ``bounds`` (ties to the lowest
-    block).  q [batch, heads, head_dim] is what ``attend`` will be given."""
+    block; 8-bit caches have theirs rounded to bfloat16, so a token's score may pass its block's there).  q [batch, heads, head_dim] is what ``attend`` will be given."""
     return (_native.tensor_calls or _native.load_tensor_calls()).select(*pages, bounds, q, lengths, count, seq, sinks,
                                                                         recent)
 

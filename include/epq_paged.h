@@ -123,7 +123,11 @@ int epq_paged_attend(const epq_pages* pages, const epq_heads* q, const int32_t* 
  * lengths).  Rows of no group share nothing; where starts are not ascending or outside the batch,
  * or a prefix is not in 0..max_pages * page_size, that is reported (bit 4) and none does.  Which
  * rows are taken together, and whether any are, follows from sizes and lengths alone: groups for which reading row
- * by row is reckoned to be faster are read that way, unless `always` is not 0.
+ * by row is reckoned to be faster are read that way, unless `always` is not 0.  With `always` too nothing is shared
+ * in pages whose size is no multiple of 8, by 8-bit heads above 128, with more than 128 query heads a key head, and where q
+ * is not 16-byte aligned with positive strides of a multiple of 8 values.  Rows are taken together in tiles of a group's
+ * consecutive rows, up to 256 query rows each (128 for heads above 128), as far as the shortest of a tile's lengths
+ * (empty rows aside): one row of 5 tokens among 64 that share 8192 leaves all of them row by row (67 us, with it 211).
  * batch <= 65536; a workspace of its own bytes, with epq_paged_attend's rules.
  * epq_device_error bit 1: a wait of the kernel's own gave up. */
 int64_t epq_paged_attend_shared_workspace_bytes(const epq_pages* pages, int64_t batch, int32_t heads, int64_t groups,
@@ -143,11 +147,13 @@ int epq_paged_attend_shared(const epq_pages* pages, const epq_heads* q, const in
 int epq_paged_bounds(const epq_pages* pages, void* bounds, int64_t bounds_stride, int32_t dtype, const int32_t* seq,
                      const int64_t* first, const int64_t* lengths, int64_t batch, void* stream);
 
-/* The blocks (pages) to attend over, by a score that no q . K[t] of a block's tokens passes:
+/* The blocks (pages) to attend over, by a score that bounds q . K[t] for a block's tokens:
  *     score(j) = max over the query heads h of key head g of
  *                sum_d max(q[b, h, d] lo_j[d], q[b, h, d] hi_j[d])
  * in float32, products first, then neighbouring dims' sums, then neighbours of those (head_dim
- * padded with zeros to a power of two; lo <= hi, as epq_paged_bounds leaves them).  Of the n = ceil(lengths[b] / page_size) blocks of a row
+ * padded with zeros to a power of two; lo <= hi, as epq_paged_bounds leaves them).  No q . K[t] passes it, up to float32's
+ * rounding of the sums, over a 16-bit cache with finite keys; the bounds of an 8-bit one are rounded to the nearest bf16, by up
+ * to 2^-8 of their value, and infinite keys are held as finite ones, so there a product can.  Of the n = ceil(lengths[b] / page_size) blocks of a row
  * chosen[b, g, 0..count) receives, in ascending order, the first `sinks`, the last `recent` and
  * those of the others with the largest scores (NaN first), the lowest of equal ones; all of them
  * where n <= count, and -1 behind the last.  A block whose page is outside the pool comes last.
